@@ -246,6 +246,61 @@ int moeb_probe_tc_issue(int n, int issuers, int per_stage, int wait, int data, i
                         double *cycles_per_mma, double *tflops, double *side_cycles_per_op);
 int moeb_probe_mma_sync(int warps_per_sm, int iters, double *tflops);
 
+/* --- 4-bit KV cache, and attention over it. The cache of one layer holds pages of page_size tokens (a power of two,
+ * 16 to 4096) that sequences take through page tables; K and V rows (one token, one KV head, head_dim = 64 or 128 values)
+ * are quantized as they are written, in the weights' two formats: int4 affine in groups of 64 (value = scale * code +
+ * bias, bf16 scale and bias; codes, scales and biases equal moeb_quantize_q4's) or MXFP4 in groups of 32. A group that
+ * holds a NaN or an infinity, or (int4) spans more than fp32 can hold, reads back as NaN everywhere and touches no other
+ * group. No counterpart in the reference (its decode keeps mlx-lm's 16-bit cache); the int4 format is that of mlx-lm's
+ * quantized cache.
+ *   kq, vq  uint32 [pages][kv_heads][page_size][head_dim / 8]   codes, the word order of csrc/kv.cuh
+ *   ks, vs  int4: uint32 [pages][kv_heads][page_size][head_dim / 64] (scale | bias << 16)
+ *           MXFP4: uint8 [pages][kv_heads][page_size][head_dim / 32] (E8M0)
+ *   err     uint32, zero at first: the sticky error word (MOEB_DEVERR_PAGE)
+ * All arrays are device memory, 16-byte aligned; their first contents do not matter (rows that were never written read
+ * back as what they hold). The struct itself is host memory and read during the call only.
+ *
+ * Rows of a call: T rows, B sequences. Sequence b has rows cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1], not decreasing),
+ * or T / B rows each where cu is NULL. They are its newest tokens: row i of n sits at position lens[b] - n + i (lens
+ * int32 [B] counts them in). Position p is in page table[b * table_row + p / page_size] (int32, P entries per sequence).
+ * Rows behind the last sequence, and rows whose position is negative, are passed over. A position outside the table, or
+ * a page id outside [0, pages), sets MOEB_DEVERR_PAGE: nothing is written there and nothing is read from there. */
+#define MOEB_KV_Q4 0
+#define MOEB_KV_MXFP4 1
+#define MOEB_DEVERR_PAGE 4u
+typedef struct {
+    void *kq, *ks, *vq, *vs;
+    unsigned *err;
+    int pages, page_size, kv_heads, head_dim, format;
+} moeb_kv_cache;
+
+/* Quantizes k and v (bf16, row t head h at t * k_row + h * k_head elements, head_dim contiguous; 16-byte aligned, strides
+ * multiples of 8) into the pages of their tokens. Two rows of one call must not name the same place of the cache (two
+ * sequences may share pages that neither writes): the words of such a row come from either. */
+int moeb_kv_write(const moeb_kv_cache *cache, const void *k, long k_row, long k_head, const void *v, long v_row,
+                  long v_head, int T, const int *cu, const int *lens, const int *table, long table_row, int B, int P,
+                  cudaStream_t stream);
+/* Reads rows back as bf16 [T][kv_heads][head_dim] (the value rounded once): row i of sequence b is position first[b] + i
+ * (first int32 [B]; NULL: 0). A row without a valid page is zero and sets MOEB_DEVERR_PAGE; rows behind the last
+ * sequence keep what they held. */
+int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *first, const int *table, long table_row,
+                 int B, int P, void *k, void *v, cudaStream_t stream);
+/* y[t][h] = softmax(scale * q . k) v over the keys that row t sees, KV head h / (H / kv_heads): for a row at position p,
+ * keys j <= p with window == 0 or j > p - window or j < sinks (a sliding window of `window` keys, the first `sinks` tokens
+ * staying visible). sink_logits (fp32 [H] or NULL): exp(sink_logits[h]) joins the softmax's sum without a value. A row
+ * that sees nothing gives zeros (lse -inf, or the sink logit). Pages that no row of the call sees are not read: their
+ * table entries may be anything. q: bf16, strides as moeb_kv_write's k; y: bf16 [T][H][head_dim]; lse: fp32 [T][H], the
+ * natural logarithm of the softmax's sum, or NULL. max_q: the most rows that a sequence has in this call (a larger bound
+ * costs time only; a sequence with more rows than max_q is passed over). Scores, statistics and sums are fp32. ws: scratch
+ * of moeb_kv_attention_workspace_bytes, with no first contents and none kept, 16-byte aligned: one call at a time. */
+size_t moeb_kv_attention_workspace_bytes(int T, int B, int H, int kv_heads, int head_dim, int max_q);
+int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, long q_head, int T, int H, const int *cu,
+                      const int *lens, const int *table, long table_row, int B, int P, int max_q, float scale, int window,
+                      int sinks, const float *sink_logits, void *y, float *lse, void *ws, size_t ws_bytes,
+                      cudaStream_t stream);
+/* Copies the cache's sticky error word to *out (host) and clears it. Synchronises `stream`. */
+int moeb_kv_read_error(const moeb_kv_cache *cache, unsigned *out, cudaStream_t stream);
+
 /* --- moeb_experts_q4 for callers that cannot allocate device memory. No counterpart in the reference (moe-lab
  * always lets the variant allocate its scratch). The scratch lives in a static 16 MiB device array inside the
  * library (held by every GPU that loads it until exit), so the caller passes only inputs and the output. T is

@@ -14,13 +14,22 @@ POLICY_AUTO, POLICY_SLOTS, POLICY_TILES8, POLICY_TILES16, POLICY_TILES8_RING, PO
 POLICY_TC = 6
 POLICY_DECODE = 7
 POLICY_TILES24_RING = 8
-DEVERR_EXPERT_ID, DEVERR_TIMEOUT = 1, 2
+DEVERR_EXPERT_ID, DEVERR_TIMEOUT, DEVERR_PAGE = 1, 2, 4
+KV_Q4, KV_MXFP4 = 0, 1
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_long
 _F = ctypes.c_float
 _S = ctypes.c_size_t
+
+
+class KvCacheStruct(ctypes.Structure):  # moeb_kv_cache
+    _fields_ = [(n, _P) for n in ("kq", "ks", "vq", "vs", "err")] + \
+        [(n, _I) for n in ("pages", "page_size", "kv_heads", "head_dim", "format")]
+
+
+_C = ctypes.POINTER(KvCacheStruct)
 
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
@@ -61,6 +70,11 @@ SIGNATURES = {
     "moeb_ep_p2p_combine": (_I, [_P, _P] + [_I] * 5 + [_P, _P, _P]),
     "moeb_ep_p2p_set_wait_limit": (_I, [_P, _I, _I, _I, ctypes.c_double, _P]),
     "moeb_ep_p2p_read_error": (_I, [_P, _I, _I, _I, ctypes.POINTER(ctypes.c_uint), _P]),
+    "moeb_kv_write": (_I, [_C, _P, _L, _L, _P, _L, _L, _I, _P, _P, _P, _L, _I, _I, _P]),
+    "moeb_kv_read": (_I, [_C, _I, _P, _P, _P, _L, _I, _I, _P, _P, _P]),
+    "moeb_kv_attention_workspace_bytes": (_S, [_I] * 6),
+    "moeb_kv_attention": (_I, [_C, _P, _L, _L, _I, _I, _P, _P, _P, _L, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P, _S, _P]),
+    "moeb_kv_read_error": (_I, [_C, ctypes.POINTER(ctypes.c_uint), _P]),
     "moeb_probe_tc_issue": (_I, [_I] * 7 + [ctypes.POINTER(ctypes.c_double)] * 3),
     "moeb_probe_mma_sync": (_I, [_I, _I, ctypes.POINTER(ctypes.c_double)]),
 }

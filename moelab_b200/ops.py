@@ -342,3 +342,166 @@ def ep_p2p_combine(xch, slot_pos, T, k, d, residual=None, device=None):
     _lib.call("moeb_ep_p2p_combine", ctypes.c_void_p(xch.base), _p(slot_pos), xch.P, xch.C, T, d, k,
               _p(residual), _p(y), _stream())
     return y
+
+
+# ------------------------------------------------------------------ 4-bit KV cache and attention over it
+class KVCache:
+    """One layer's paged K / V cache in 4 bits (include/moelab_b200.h: moeb_kv_cache). `pages` pages of `page_size` tokens
+    (a power of two, 16 to 4096), `kv_heads` heads of 64 or 128 values, fmt "q4" (int4 affine, groups of 64: 4.5 bits a
+    value) or "mxfp4" (groups of 32: 4.25 bits). The arrays are plain tensors; what page a token of a sequence is in is the
+    caller's page table."""
+
+    def __init__(self, pages, kv_heads, head_dim, page_size=64, fmt="q4", device=None):
+        if fmt not in ("q4", "mxfp4"):
+            raise ValueError(f"unknown format {fmt!r} (q4 or mxfp4)")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+        if not 16 <= page_size <= 4096 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 4096, got {page_size}")
+        if pages <= 0 or not 0 < kv_heads <= 1024:
+            raise ValueError("pages and kv_heads must be positive, kv_heads at most 1024")
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ValueError("the cache must be on a CUDA device (moelab_b200 has no CPU path)")
+        self.pages, self.page_size, self.kv_heads, self.head_dim, self.fmt = pages, page_size, kv_heads, head_dim, fmt
+        rows = (pages, kv_heads, page_size)
+        par = (head_dim // 64, torch.int32) if fmt == "q4" else (head_dim // 32, torch.uint8)
+        self.kq, self.vq = (torch.zeros(*rows, head_dim // 8, dtype=torch.int32, device=device) for _ in range(2))
+        self.ks, self.vs = (torch.zeros(*rows, par[0], dtype=par[1], device=device) for _ in range(2))
+        self.err = torch.zeros(1, dtype=torch.int32, device=device)
+        self.device = self.kq.device
+        self._c = ctypes.pointer(_lib.KvCacheStruct(
+            *(t.data_ptr() for t in (self.kq, self.ks, self.vq, self.vs, self.err)), pages, page_size, kv_heads, head_dim,
+            _lib.KV_Q4 if fmt == "q4" else _lib.KV_MXFP4))
+
+    def read_error(self):
+        """Sticky device error bits (DEVERR_PAGE); synchronises the current stream and clears them."""
+        out = ctypes.c_uint(0)
+        with torch.cuda.device(self.device):
+            _lib.call("moeb_kv_read_error", self._c, ctypes.byref(out), _stream())
+        return out.value
+
+
+def _kv_ints(t, name, cache, size=None):
+    if t is None:
+        return None
+    _need(t, torch.int32, name)
+    if t.device != cache.device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+    if t.dim() != 1 or (size is not None and t.shape[0] != size):
+        raise ValueError(f"{name} must be int32 [{size}], got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _kv_table(table, cache):
+    if not table.is_cuda or table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be a CUDA int32 [sequences, pages] tensor with contiguous rows")
+    if table.device != cache.device:
+        raise ValueError(f"table is on {table.device}, the cache on {cache.device}")
+    B, P = table.shape
+    if B > 1 and table.stride(0) < P:
+        raise ValueError("table rows overlap")
+    return table.data_ptr(), max(table.stride(0), P), B, P
+
+
+def _kv_rows(t, name, cache, heads=None):
+    if not t.is_cuda or t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != cache.head_dim:
+        raise ValueError(f"{name} must be a CUDA bfloat16 [rows, heads, {cache.head_dim}] tensor, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    if t.device != cache.device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+    if heads is not None and t.shape[1] != heads:
+        raise ValueError(f"{name} has {t.shape[1]} heads, the cache {heads}")
+    r, h, one = t.stride()
+    if one != 1 or r % 8 or h % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name} must have contiguous values, row and head strides that are multiples of 8, and a 16-byte "
+                         f"aligned start")
+    return t.data_ptr(), r, h
+
+
+def _kv_out(t, name, shape, dtype, device):
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"{name} must be a contiguous, 16-byte aligned {dtype} {tuple(shape)} tensor on {device}")
+    return t
+
+
+def _kv_call(cache, name, *args):
+    """The call on the cache's device and that device's current stream."""
+    if cache.device.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(cache.device):
+            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _kv_cu(cu, T, B, cache):
+    if cu is None and B and T % B:
+        raise ValueError(f"{T} rows for {B} sequences: give cu, or the same number of rows for each")
+    return _kv_ints(cu, "cu", cache, B + 1)
+
+
+def kv_write(cache, k, v, table, lens, cu=None):
+    """Quantize the newest tokens' k and v (bf16 [T, kv_heads, head_dim], any row and head strides that are multiples of 8)
+    into the cache. table int32 [B, P]: page ids of each sequence; lens int32 [B]: its tokens, these included; cu int32
+    [B + 1]: sequence b has rows cu[b] .. cu[b + 1] - 1 (None: T / B rows each), its last ones. Rows behind the last
+    sequence are passed over; a token without a valid page is dropped and sets DEVERR_PAGE (cache.read_error())."""
+    kp, vp = _kv_rows(k, "k", cache, cache.kv_heads), _kv_rows(v, "v", cache, cache.kv_heads)
+    T = k.shape[0]
+    if v.shape[0] != T:
+        raise ValueError(f"k has {T} rows, v {v.shape[0]}")
+    tp, trow, B, P = _kv_table(table, cache)
+    _kv_call(cache, "moeb_kv_write", cache._c, *kp, *vp, T, _kv_cu(cu, T, B, cache), _kv_ints(lens, "lens", cache, B), tp,
+             trow, B, P)
+
+
+def kv_read(cache, table, cu, rows, first=None, out=None):
+    """Read rows back as bf16: (k, v), each [rows, kv_heads, head_dim]. Row i of sequence b (rows cu[b] .. cu[b + 1] - 1;
+    cu None: rows / B each) is its position first[b] + i (first None: i). out: (k, v) to fill, whose rows behind the last
+    sequence are left as they were; without it those rows are zero."""
+    tp, trow, B, P = _kv_table(table, cache)
+    cp, fp = _kv_cu(cu, rows, B, cache), _kv_ints(first, "first", cache, B)
+    shape = (rows, cache.kv_heads, cache.head_dim)
+    if out is None:
+        new = torch.empty if cu is None else torch.zeros
+        k, v = (new(shape, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+    else:
+        k, v = (_kv_out(t, "out", shape, torch.bfloat16, cache.device) for t in out)
+    _kv_call(cache, "moeb_kv_read", cache._c, rows, cp, fp, tp, trow, B, P, k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=0, sinks=0, sink_logits=None, out=None,
+                 return_lse=False):
+    """Causal attention of the newest tokens' queries (bf16 [T, H, head_dim], H a multiple of the cache's heads) over the
+    cache, after kv_write: single tokens and prompts. table, lens and cu as in kv_write. A row at position p sees the keys
+    j <= p; with window > 0 only the last `window` of them and the first `sinks` tokens. sink_logits fp32 [H]: a logit per
+    head that joins the softmax without a value. max_q: the most rows that a sequence has in the call (None: T; a tight
+    bound picks the better kernels). scale: of the scores (None: head_dim ** -0.5). out: y to fill, whose rows behind the
+    last sequence are left as they were; without it those rows are zero. Returns y bf16 [T, H, head_dim] (and, with
+    return_lse, the fp32 [T, H] logarithm of each softmax's sum). A row that sees nothing is zero (lse -inf)."""
+    qp = _kv_rows(q, "q", cache)
+    T, H, D = q.shape
+    tp, trow, B, P = _kv_table(table, cache)
+    cp, lp = _kv_cu(cu, T, B, cache), _kv_ints(lens, "lens", cache, B)
+    if H == 0 or H % cache.kv_heads:
+        raise ValueError(f"{H} query heads over {cache.kv_heads} KV heads")
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    if sink_logits is not None:
+        _need(sink_logits, torch.float32, "sink_logits")
+        if sink_logits.shape != (H,) or sink_logits.device != cache.device:
+            raise ValueError(f"sink_logits must be float32 [{H}] on {cache.device}")
+    max_q = T // max(B, 1) if cu is None else T if max_q is None else min(int(max_q), T)
+    if T and max_q <= 0:
+        raise ValueError("max_q must be positive")
+    new = torch.empty if cu is None else torch.zeros
+    y = new((T, H, D), dtype=torch.bfloat16, device=cache.device) if out is None else \
+        _kv_out(out, "out", (T, H, D), torch.bfloat16, cache.device)
+    lse = torch.full((T, H), -float("inf"), device=cache.device) if return_lse else None
+    nbytes = _lib.load().moeb_kv_attention_workspace_bytes(T, B, H, cache.kv_heads, D, max_q)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
+    _kv_call(cache, "moeb_kv_attention", cache._c, *qp, T, H, cp, lp, tp, trow, B, P, max_q,
+             D ** -0.5 if scale is None else float(scale), int(window), int(sinks),
+             None if sink_logits is None else sink_logits.data_ptr(), y.data_ptr(), None if lse is None else lse.data_ptr(),
+             None if ws is None else ws.data_ptr(), nbytes)
+    return (y, lse) if return_lse else y
