@@ -249,14 +249,15 @@ int moeb_probe_mma_sync(int warps_per_sm, int iters, double *tflops);
 /* --- 4-bit KV cache, and attention over it. The cache of one layer holds pages of page_size tokens (a power of two,
  * 16 to 4096) that sequences take through page tables; K and V rows (one token, one KV head, head_dim = 64 or 128 values)
  * are quantized as they are written, in the weights' two formats: int4 affine in groups of 64 (value = scale * code +
- * bias, bf16 scale and bias; codes, scales and biases equal moeb_quantize_q4's) or MXFP4 in groups of 32. A group that
+ * bias, bf16 scale and bias; codes, scales and biases equal moeb_quantize_q4's, but that a group of zeros has scale 0) or
+ * MXFP4 in groups of 32. A group that
  * holds a NaN or an infinity, or (int4) spans more than fp32 can hold, reads back as NaN everywhere and touches no other
  * group. No counterpart in the reference (its decode keeps mlx-lm's 16-bit cache); the int4 format is that of mlx-lm's
  * quantized cache.
  *   kq, vq  uint32 [pages][kv_heads][page_size][head_dim / 8]   codes, the word order of csrc/kv.cuh
  *   ks, vs  int4: uint32 [pages][kv_heads][page_size][head_dim / 64] (scale | bias << 16)
  *           MXFP4: uint8 [pages][kv_heads][page_size][head_dim / 32] (E8M0)
- *   err     uint32, zero at first: the sticky error word (MOEB_DEVERR_PAGE)
+ *   err     uint32, zero at first: the sticky error word (MOEB_DEVERR_PAGE, MOEB_DEVERR_ROWS)
  * All arrays are device memory, 16-byte aligned; their first contents do not matter (rows that were never written read
  * back as what they hold). The struct itself is host memory and read during the call only.
  *
@@ -268,6 +269,7 @@ int moeb_probe_mma_sync(int warps_per_sm, int iters, double *tflops);
 #define MOEB_KV_Q4 0
 #define MOEB_KV_MXFP4 1
 #define MOEB_DEVERR_PAGE 4u
+#define MOEB_DEVERR_ROWS 8u /* a sequence had more rows than max_q: they were passed over */
 typedef struct {
     void *kq, *ks, *vq, *vs;
     unsigned *err;
@@ -291,7 +293,7 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
  * that sees nothing gives zeros (lse -inf, or the sink logit). Pages that no row of the call sees are not read: their
  * table entries may be anything. q: bf16, strides as moeb_kv_write's k; y: bf16 [T][H][head_dim]; lse: fp32 [T][H], the
  * natural logarithm of the softmax's sum, or NULL. max_q: the most rows that a sequence has in this call (a larger bound
- * costs time only; a sequence with more rows than max_q is passed over). Scores, statistics and sums are fp32. ws: scratch
+ * costs time only; a sequence with more rows may be passed over, which sets MOEB_DEVERR_ROWS). Scores, statistics and sums are fp32. ws: scratch
  * of moeb_kv_attention_workspace_bytes, with no first contents and none kept, 16-byte aligned: one call at a time. */
 size_t moeb_kv_attention_workspace_bytes(int T, int B, int H, int kv_heads, int head_dim, int max_q);
 int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, long q_head, int T, int H, const int *cu,

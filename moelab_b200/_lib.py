@@ -14,7 +14,7 @@ POLICY_AUTO, POLICY_SLOTS, POLICY_TILES8, POLICY_TILES16, POLICY_TILES8_RING, PO
 POLICY_TC = 6
 POLICY_DECODE = 7
 POLICY_TILES24_RING = 8
-DEVERR_EXPERT_ID, DEVERR_TIMEOUT, DEVERR_PAGE = 1, 2, 4
+DEVERR_EXPERT_ID, DEVERR_TIMEOUT, DEVERR_PAGE, DEVERR_ROWS = 1, 2, 4, 8
 KV_Q4, KV_MXFP4 = 0, 1
 
 _P = ctypes.c_void_p

@@ -43,7 +43,9 @@ MOEB_DEV uint32_t kv_quant_q4(const float (&v)[8], uint32_t &par) {
         q = fminf(fmaxf(q, 0.0f), 15.0f);
         word |= (uint32_t)q << (4 * ((i >> 1) + 4 * (i & 1)));
     }
-    par = bad ? 0x7fff7fffu : (uint32_t)f2bf(scale) | ((uint32_t)f2bf(bias) << 16);
+    // q0 = 0: the largest magnitude is below half the smallest scale, every code is 0 and the values are zeros. The weight
+    // quantizer keeps that scale; here it is 0, so that attention, which takes codes less 8, meets nothing to cancel.
+    par = bad ? 0x7fff7fffu : q0 == 0.0f ? 0u : (uint32_t)f2bf(scale) | ((uint32_t)f2bf(bias) << 16);
     return bad ? 0u : word;
 }
 MOEB_DEV uint32_t kv_quant_fp4(const float (&v)[8], uint32_t &par) {
@@ -73,7 +75,7 @@ MOEB_DEV uint32_t kv_quant_fp4(const float (&v)[8], uint32_t &par) {
 
 template <int FMT, int D>
 __global__ void __launch_bounds__(128) k_kv_write(KvWriteArgs a) {
-    constexpr int W = D / 8, G = D / 64;
+    constexpr int W = D / 8;
     pdl_wait();
     const long gid = (long)blockIdx.x * blockDim.x + threadIdx.x;
     const int w = (int)(gid % W);
@@ -111,10 +113,18 @@ __global__ void __launch_bounds__(128) k_kv_write(KvWriteArgs a) {
     const uint32_t word = FMT == FMT_Q4 ? kv_quant_q4(x, par) : kv_quant_fp4(x, par);
     if (page < 0) return;
     const size_t row = kv_row(a.c, page, h, p);
-    (isv ? a.c.vq : a.c.kq)[row * W + (isv ? kv_vpos(w, G) : kv_kpos(w, G))] = word;
+    if (!isv) {
+        a.c.kq[row * W + kv_kpos<FMT, D>(w)] = word;
+    } else if (FMT == FMT_Q4) {
+        a.c.vq[row * W + kv_vpos_q4<D>(w)] = word;
+    } else {
+        uint16_t *dst = reinterpret_cast<uint16_t *>(a.c.vq) + row * (D / 4);
+        dst[kv_vpos_fp4<D>(2 * w)] = (uint16_t)word;
+        dst[kv_vpos_fp4<D>(2 * w + 1)] = (uint16_t)(word >> 16);
+    }
     void *ps = isv ? a.c.vs : a.c.ks;
     if (FMT == FMT_Q4) {
-        if ((w & 7) == 0) static_cast<uint32_t *>(ps)[row * G + (w >> 3)] = par;
+        if ((w & 7) == 0) static_cast<uint32_t *>(ps)[row * (D / 64) + (w >> 3)] = par;
     } else if ((w & 3) == 0) {
         static_cast<uint8_t *>(ps)[row * (D / 32) + (w >> 2)] = (uint8_t)par;
     }
@@ -122,7 +132,7 @@ __global__ void __launch_bounds__(128) k_kv_write(KvWriteArgs a) {
 
 template <int FMT, int D>
 __global__ void __launch_bounds__(128) k_kv_read(KvReadArgs a) {
-    constexpr int W = D / 8, G = D / 64;
+    constexpr int W = D / 8;
     pdl_wait();
     const long gid = (long)blockIdx.x * blockDim.x + threadIdx.x;
     const int w = (int)(gid % W);
@@ -140,7 +150,7 @@ __global__ void __launch_bounds__(128) k_kv_read(KvReadArgs a) {
     uint4 o = make_uint4(0, 0, 0, 0);
     if (page >= 0) {
         const size_t row = kv_row(a.c, page, h, (int)p);
-        const uint32_t word = (isv ? a.c.vq : a.c.kq)[row * W + (isv ? kv_vpos(w, G) : kv_kpos(w, G))];
+        const uint32_t word = isv ? kv_vword<FMT, D>(a.c.vq, row, w) : a.c.kq[row * W + kv_kpos<FMT, D>(w)];
         float x[8];
         kv_word_values<FMT>(word, kv_par<FMT>(isv ? a.c.vs : a.c.ks, row, w, D), x);
         o = make_uint4(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7]));
@@ -153,13 +163,13 @@ __global__ void __launch_bounds__(128) k_kv_read(KvReadArgs a) {
 // One CTA per (row, query head), a warp per key in turn: every case, nothing shared between rows.
 template <int FMT, int D>
 __global__ void __launch_bounds__(128) k_kv_attn_rows(KvAttnArgs a) {
-    constexpr int E = D / 32, W = D / 8, G = D / 64, NW = 4;
+    constexpr int E = D / 32, W = D / 8, NW = 4;
     __shared__ float sm[NW], sl[NW], so[NW][D];
     pdl_wait();
     const int t = blockIdx.x, h = blockIdx.y, hk = h / a.Gq, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int r0, r1;
     const int b = kv_seq_of(a.s, t, r0, r1);
-    if (b < 0) return;
+    if (b < 0 || (r1 - r0) * a.Gq <= a.few) return;
     const int p = a.s.lens[b] - (r1 - t);
     float q[E], o[E], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -177,13 +187,13 @@ __global__ void __launch_bounds__(128) k_kv_attn_rows(KvAttnArgs a) {
         }
         const size_t row = kv_row(a.c, page, hk, j);
         float x[8], d = 0.f;
-        kv_word_values<FMT>(a.c.kq[row * W + kv_kpos(w, G)], kv_par<FMT>(a.c.ks, row, w, D), x);
+        kv_word_values<FMT>(a.c.kq[row * W + kv_kpos<FMT, D>(w)], kv_par<FMT>(a.c.ks, row, w, D), x);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i >= e0 && i < e0 + E) d += q[i - e0 < 0 ? 0 : (i - e0) % E] * x[i];
         const float s = warp_sum(d) * a.scale, mn = fmaxf(m, s);
         const float f = m == -INFINITY ? 0.f : exp2f(m - mn), pr = exp2f(s - mn);
-        kv_word_values<FMT>(a.c.vq[row * W + kv_vpos(w, G)], kv_par<FMT>(a.c.vs, row, w, D), x);
+        kv_word_values<FMT>(kv_vword<FMT, D>(a.c.vq, row, w), kv_par<FMT>(a.c.vs, row, w, D), x);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i >= e0 && i < e0 + E) o[(i - e0) % E] = o[(i - e0) % E] * f + pr * x[i];

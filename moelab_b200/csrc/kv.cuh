@@ -7,18 +7,22 @@
 //   MXFP4 parameters  uint8  [pages][Hkv][page][D / 32]  (E8M0; value = E2M1(code) * 2^(byte - 127))
 // so a page's tokens of one head are one contiguous block, and 16 tokens (a tensor-core tile's rows) are D * 8 bytes in a
 // row. The order inside a row is the one the decode kernel's registers want (kv_attn.cu):
-//   K: word w of group g (64 values) at (w / 2) * 2 * G + 2 * g + w % 2, G = D / 64: a lane's words (2 c, 2 c + 1 of every
-//      group) are one 8- or 16-byte load
-//   V: word w of group g at w * G + g: a lane's words (w of every group) are one 4- or 8-byte load
-//   int4 word: element 2 p at nibble p, element 2 p + 1 at nibble p + 4 (as in the expert weights);
-//   MXFP4 word: element i at nibble i (a byte is a pair for the E2M1 -> fp16 conversion)
+//   int4 word: 8 values, element 2 p at nibble p, element 2 p + 1 at nibble p + 4 (as in the expert weights), w = 0 .. 7 in
+//     its group g of 64, G = D / 64;  K: at (w / 2) * 2 G + 2 g + w % 2,  V: at w * G + g
+//   MXFP4: groups of 32, H = D / 32;  K: words of 8 values, element i at nibble i, word w = 0 .. 3 of group g at w * H + g,
+//     V: half-words of 4 values, element i at nibble i, half-word u = 0 .. 7 of group g at half-word u * H + g
+// With it a lane's codes of one key (K: 1 / 4 of the row, V: 1 / 8) are one load of 4 to 16 bytes, and hold the same part of
+// every group.
 #pragma once
 #include "common.cuh"
 #include "kernels.h"
 
 namespace moeb {
 
-enum : uint32_t { ERR_PAGE = 4u };  // a visible token's page is outside the table or the cache
+enum : uint32_t {
+    ERR_PAGE = 4u,  // a token's page is outside the table or the cache
+    ERR_ROWS = 8u,  // a sequence has more rows than the call's max_q: they were passed over
+};
 
 struct KvCache {
     uint32_t *kq, *vq;
@@ -34,8 +38,15 @@ struct KvSeqs {
     int B, P, T, each;
 };
 
-__host__ __device__ __forceinline__ int kv_kpos(int w, int G) { return ((w & 7) >> 1) * 2 * G + 2 * (w >> 3) + (w & 1); }
-__host__ __device__ __forceinline__ int kv_vpos(int w, int G) { return (w & 7) * G + (w >> 3); }
+// place in its row of K's word w (values 8 w ..), of V's word w (int4), of V's half-word u (values 4 u .., MXFP4)
+template <int FMT, int D>
+MOEB_DEV int kv_kpos(int w) {
+    return FMT == FMT_Q4 ? ((w & 7) >> 1) * (D / 32) + 2 * (w >> 3) + (w & 1) : (w & 3) * (D / 32) + (w >> 2);
+}
+template <int D>
+MOEB_DEV int kv_vpos_q4(int w) { return (w & 7) * (D / 64) + (w >> 3); }
+template <int D>
+MOEB_DEV int kv_vpos_fp4(int u) { return (u & 7) * (D / 32) + (u >> 3); }
 
 MOEB_DEV int kv_clamp_row(int v, int T) { return v < 0 ? 0 : (v > T ? T : v); }
 // rows [r0, r1) of sequence b, inside [0, T)
@@ -102,6 +113,14 @@ MOEB_DEV uint32_t kv_par(const void *ps, size_t row, int w, int D) {
     return static_cast<const uint8_t *>(ps)[row * (D / 32) + (w >> 2)];
 }
 
+// V's word w of a row in natural order of its values
+template <int FMT, int D>
+MOEB_DEV uint32_t kv_vword(const uint32_t *vq, size_t row, int w) {
+    if (FMT == FMT_Q4) return vq[row * (D / 8) + kv_vpos_q4<D>(w)];
+    const uint16_t *p = reinterpret_cast<const uint16_t *>(vq) + row * (D / 4);
+    return p[kv_vpos_fp4<D>(2 * w)] | (uint32_t)p[kv_vpos_fp4<D>(2 * w + 1)] << 16;
+}
+
 struct KvWriteArgs {
     KvCache c;
     KvSeqs s;
@@ -122,15 +141,41 @@ struct KvAttnArgs {
     int H, Gq;         // query heads, query heads per KV head
     float scale;       // of the scores, times log2(e)
     int window, sinks;
+    int few;           // sequences of at most this many (row, head) columns are another kernel's
+    int only;          // the kernel for few rows has the call to itself (longer sequences are an error)
     const float *sink_logits;  // [H] or null
     uint16_t *y;       // [T][H][D]
     float *lse;        // [T][H] or null
 };
+// Four values of one row's result: v is the sum of weights 2^(score - M) times values, L the sum of the weights.
+template <int D>
+MOEB_DEV void kv_finish(const KvAttnArgs &a, int t, int head, int d4, float4 v, float M, float L) {
+    if (a.sink_logits) {
+        const float s = a.sink_logits[head] * 1.4426950408889634f, N = fmaxf(M, s), use = N == -INFINITY ? 0.f : N;
+        const float f = exp2f(M - use);
+        v.x *= f;
+        v.y *= f;
+        v.z *= f;
+        v.w *= f;
+        L = L * f + exp2f(s - use);
+        M = N;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing: zeros
+    const size_t row = (size_t)t * a.H + head;
+    *reinterpret_cast<uint2 *>(a.y + row * D + 4 * d4) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
+    if (a.lse && d4 == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+}
 template <int FMT, int D>
 __global__ void k_kv_write(KvWriteArgs a);
 template <int FMT, int D>
 __global__ void k_kv_read(KvReadArgs a);
 template <int FMT, int D>
 __global__ void k_kv_attn_rows(KvAttnArgs a);
+template <int FMT, int D, int NT>
+__global__ void k_kv_attn_few(const KvAttnArgs a, int *pre, float *part);
+template <int D, int NT>
+__global__ void k_kv_attn_join(const KvAttnArgs a, const int *pre, const float *part, int grid);
+template <int FMT, int D, int NT>
+size_t kv_few_smem();
 
 }  // namespace moeb

@@ -3,6 +3,9 @@
 #include <math.h>
 #include <stdio.h>
 
+#include <map>
+#include <mutex>
+
 #include "../../include/moelab_b200.h"
 #include "kv.cuh"
 
@@ -26,8 +29,8 @@ int launched(cudaError_t e, const char *what) {
 
 // Programmatic dependent launch, as every kernel of this library: the kernel waits (pdl_wait) before it reads or
 // writes anything.
-template <typename A>
-cudaError_t launch(void (*kern)(A), dim3 grid, int threads, size_t smem, cudaStream_t st, const A &args) {
+template <typename... K, typename... A>
+cudaError_t launch(void (*kern)(K...), dim3 grid, int threads, size_t smem, cudaStream_t st, const A &...args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -38,7 +41,39 @@ cudaError_t launch(void (*kern)(A), dim3 grid, int threads, size_t smem, cudaStr
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, args);
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+int sms() {
+    static std::mutex mu;
+    static std::map<int, int> cache;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 148;
+    }
+    std::lock_guard<std::mutex> lk(mu);
+    int &n = cache[dev];
+    if (!n && (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)) n = 148;
+    return n;
+}
+
+// Resident CTAs per SM of a kernel on the current device; its dynamic shared memory is allowed on the first call.
+int resident(const void *kern, int threads, size_t smem) {
+    static std::mutex mu;
+    static std::map<std::pair<const void *, int>, int> cache;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lk(mu);
+    int &n = cache[{kern, dev}];
+    if (!n) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n < 1)
+            n = 0;
+    }
+    return n;
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -85,6 +120,35 @@ int check_seqs(int T, const int *cu, const int *lens, bool need_lens, const int 
     ((c)->format == MOEB_KV_Q4 ? ((c)->head_dim == 64 ? kern<FMT_Q4, 64> : kern<FMT_Q4, 128>) \
                                : ((c)->head_dim == 64 ? kern<FMT_FP4, 64> : kern<FMT_FP4, 128>))
 
+// Workspace of the kernel for few rows: blocks before each sequence, then two partial results per CTA.
+struct FewLayout {
+    size_t part, total;
+};
+constexpr int FEW_RESIDENT = 4;  // CTAs per SM at most (the kernel's launch bound)
+FewLayout few_layout(int B, int nc, int D) {
+    FewLayout l;
+    l.part = up256(4 * ((size_t)B + 1));
+    l.total = l.part + (size_t)FEW_RESIDENT * sms() * 2 * nc * (D + 2) * 4;
+    return l;
+}
+
+template <int FMT, int D, int NT>
+int launch_few(const KvAttnArgs &a, void *ws, cudaStream_t st) {
+    const size_t smem = kv_few_smem<FMT, D, NT>();
+    const int per = resident((const void *)k_kv_attn_few<FMT, D, NT>, 128, smem);
+    if (!per) return launched(cudaErrorInvalidConfiguration, "kv_attention");
+    const FewLayout l = few_layout(a.s.B, 8 * NT, D);
+    int *pre = (int *)ws;
+    float *part = (float *)((char *)ws + l.part);
+    // at most one block of 64 keys per CTA: the page tables' width bounds the blocks (the first tokens' may be cut twice)
+    const long most = (long)a.s.B * a.c.Hkv * ((((long)a.s.P << a.c.pshift) >> 6) + 2);
+    const int grid = (int)(most < (long)per * sms() ? most : (long)per * sms());
+    cudaError_t e = launch(k_kv_attn_few<FMT, D, NT>, dim3(grid), 128, smem, st, a, pre, part);
+    if (e == cudaSuccess)
+        e = launch(k_kv_attn_join<D, NT>, dim3(a.s.B * a.c.Hkv, a.few), 256, 0, st, a, (const int *)pre, (const float *)part, grid);
+    return launched(e, "kv_attention");
+}
+
 bool rows_ok(const void *p, long row, long head) { return p && aligned16(p) && row % 8 == 0 && head % 8 == 0; }
 
 }  // namespace
@@ -127,8 +191,8 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
 }
 
 size_t moeb_kv_attention_workspace_bytes(int T, int B, int H, int kv_heads, int head_dim, int max_q) {
-    (void)T; (void)B; (void)H; (void)kv_heads; (void)head_dim; (void)max_q;
-    return 0;
+    if (T <= 0 || B <= 0 || H <= 0 || kv_heads <= 0 || head_dim <= 0 || max_q <= 0) return 0;
+    return few_layout(B, (long)max_q * (H / kv_heads) <= 8 ? 8 : 16, head_dim).total;
 }
 
 int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, long q_head, int T, int H, const int *cu,
@@ -150,7 +214,7 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
     if (!y || !aligned16(y)) return bad("y must be 16-byte aligned");
     if (ws_bytes < moeb_kv_attention_workspace_bytes(T, B, H, cache->kv_heads, cache->head_dim, max_q))
         return bad("the workspace is too small: see moeb_kv_attention_workspace_bytes");
-    (void)ws;
+    if (!ws || !aligned16(ws)) return bad("the workspace must be 16-byte aligned");
     a.q = (const uint16_t *)q;
     a.q_row = q_row;
     a.q_head = q_head;
@@ -162,6 +226,23 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
     a.sink_logits = sink_logits;
     a.y = (uint16_t *)y;
     a.lse = lse;
+    // Sequences whose (row, head) columns fit one or two tensor-core tiles go to the kernel for few rows. Without cu all
+    // sequences have T / B rows; with it, and more than one sequence, both kinds may be in the call.
+    const long cols = (long)max_q * a.Gq;
+    const bool only_few = cols <= 16, both = !only_few && cu && B > 1;
+    a.few = only_few || both ? 16 : 0;
+    if (a.few) {
+        const bool one = cols <= 8;
+        a.only = only_few;
+        a.few = one ? 8 : 16;
+        rc = cache->format == MOEB_KV_Q4
+                 ? (cache->head_dim == 64 ? (one ? launch_few<FMT_Q4, 64, 1>(a, ws, stream) : launch_few<FMT_Q4, 64, 2>(a, ws, stream))
+                                          : (one ? launch_few<FMT_Q4, 128, 1>(a, ws, stream) : launch_few<FMT_Q4, 128, 2>(a, ws, stream)))
+                 : (cache->head_dim == 64 ? (one ? launch_few<FMT_FP4, 64, 1>(a, ws, stream) : launch_few<FMT_FP4, 64, 2>(a, ws, stream))
+                                          : (one ? launch_few<FMT_FP4, 128, 1>(a, ws, stream) : launch_few<FMT_FP4, 128, 2>(a, ws, stream)));
+        if (rc) return rc;
+    }
+    if (only_few) return MOEB_OK;
     return launched(launch(KV_PICK(k_kv_attn_rows, cache), dim3(T, H), 128, 0, stream, a), "kv_attention");
 }
 

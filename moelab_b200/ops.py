@@ -375,7 +375,7 @@ class KVCache:
             _lib.KV_Q4 if fmt == "q4" else _lib.KV_MXFP4))
 
     def read_error(self):
-        """Sticky device error bits (DEVERR_PAGE); synchronises the current stream and clears them."""
+        """Sticky device error bits (DEVERR_PAGE, DEVERR_ROWS); synchronises the current stream and clears them."""
         out = ctypes.c_uint(0)
         with torch.cuda.device(self.device):
             _lib.call("moeb_kv_read_error", self._c, ctypes.byref(out), _stream())
