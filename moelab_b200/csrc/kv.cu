@@ -160,74 +160,9 @@ __global__ void __launch_bounds__(128) k_kv_read(KvReadArgs a) {
     *reinterpret_cast<uint4 *>((isv ? a.v : a.k) + ((size_t)t * a.c.Hkv + h) * D + 8 * w) = o;
 }
 
-// One CTA per (row, query head), a warp per key in turn: every case, nothing shared between rows.
-template <int FMT, int D>
-__global__ void __launch_bounds__(128) k_kv_attn_rows(KvAttnArgs a) {
-    constexpr int E = D / 32, W = D / 8, NW = 4;
-    __shared__ float sm[NW], sl[NW], so[NW][D];
-    pdl_wait();
-    const int t = blockIdx.x, h = blockIdx.y, hk = h / a.Gq, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int r0, r1;
-    const int b = kv_seq_of(a.s, t, r0, r1);
-    if (b < 0 || (r1 - r0) * a.Gq <= a.few) return;
-    const int p = a.s.lens[b] - (r1 - t);
-    float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        q[i] = bf2f(a.q[t * a.q_row + h * a.q_head + lane * E + i]);
-        o[i] = 0.f;
-    }
-    const int w = lane * E / 8, e0 = (lane * E) & 7;
-    for (int j = warp; j <= p; j += NW) {
-        if (a.window && j <= p - a.window && j >= a.sinks) continue;
-        const long page = kv_page(a.c, a.s, b, j);
-        if (page < 0) {
-            if (lane == 0) atomicOr(a.c.err, ERR_PAGE);
-            continue;
-        }
-        const size_t row = kv_row(a.c, page, hk, j);
-        float x[8], d = 0.f;
-        kv_word_values<FMT>(a.c.kq[row * W + kv_kpos<FMT, D>(w)], kv_par<FMT>(a.c.ks, row, w, D), x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i >= e0 && i < e0 + E) d += q[i - e0 < 0 ? 0 : (i - e0) % E] * x[i];
-        const float s = warp_sum(d) * a.scale, mn = fmaxf(m, s);
-        const float f = m == -INFINITY ? 0.f : exp2f(m - mn), pr = exp2f(s - mn);
-        kv_word_values<FMT>(kv_vword<FMT, D>(a.c.vq, row, w), kv_par<FMT>(a.c.vs, row, w, D), x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i >= e0 && i < e0 + E) o[(i - e0) % E] = o[(i - e0) % E] * f + pr * x[i];
-        l = l * f + pr;
-        m = mn;
-    }
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < E; ++i) so[warp][lane * E + i] = o[i];
-    __syncthreads();
-    const float snk = a.sink_logits ? a.sink_logits[h] * 1.4426950408889634f : -INFINITY;
-    float M = snk, L = 0.f, O = 0.f;
-    for (int i = 0; i < NW; ++i) M = fmaxf(M, sm[i]);
-    if (threadIdx.x < D) {
-        for (int i = 0; i < NW; ++i) {
-            if (sm[i] == -INFINITY && sl[i] == 0.f) continue;
-            const float f = exp2f(sm[i] - M);
-            L += sl[i] * f;
-            O += so[i][threadIdx.x] * f;
-        }
-        if (a.sink_logits) L += exp2f(snk - M);
-        a.y[((size_t)t * a.H + h) * D + threadIdx.x] = f2bf(L == 0.f ? 0.f : O / L);
-        if (a.lse && threadIdx.x == 0)
-            a.lse[(size_t)t * a.H + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-    }
-}
-
 #define KV_INST(F, D)                                \
     template __global__ void k_kv_write<F, D>(KvWriteArgs); \
-    template __global__ void k_kv_read<F, D>(KvReadArgs);   \
-    template __global__ void k_kv_attn_rows<F, D>(KvAttnArgs);
+    template __global__ void k_kv_read<F, D>(KvReadArgs);
 KV_INST(FMT_Q4, 64)
 KV_INST(FMT_Q4, 128)
 KV_INST(FMT_FP4, 64)

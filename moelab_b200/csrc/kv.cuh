@@ -169,13 +169,17 @@ template <int FMT, int D>
 __global__ void k_kv_write(KvWriteArgs a);
 template <int FMT, int D>
 __global__ void k_kv_read(KvReadArgs a);
-template <int FMT, int D>
-__global__ void k_kv_attn_rows(KvAttnArgs a);
 template <int FMT, int D, int NT>
 __global__ void k_kv_attn_few(const KvAttnArgs a, int *pre, float *part);
 template <int D, int NT>
 __global__ void k_kv_attn_join(const KvAttnArgs a, const int *pre, const float *part, int grid);
 template <int FMT, int D, int NT>
 size_t kv_few_smem();
+template <int FMT, int D>
+__global__ void k_kv_attn_prompt(const KvAttnArgs a, int tiles, float *part);
+template <int D>
+__global__ void k_kv_attn_join_splits(const KvAttnArgs a, const float *part, int ns);
+size_t kv_prompt_smem(int D);
+constexpr int KV_PROMPT_ROWS = 256, KV_PROMPT_THREADS = 512;
 
 }  // namespace moeb

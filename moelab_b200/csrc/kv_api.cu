@@ -3,6 +3,7 @@
 #include <math.h>
 #include <stdio.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 
@@ -149,6 +150,30 @@ int launch_few(const KvAttnArgs &a, void *ws, cudaStream_t st) {
     return launched(e, "kv_attention");
 }
 
+// Row tiles of the kernel for many rows, and into how many parts each tile's keys are cut: as many as give every SM a
+// CTA, where the rows alone do not.
+long prompt_tiles(int T, int B, int Gq, bool cu) {
+    return cu ? (long)T * Gq / KV_PROMPT_ROWS + B : (long)B * (((long)(T / B) * Gq + KV_PROMPT_ROWS - 1) / KV_PROMPT_ROWS);
+}
+long prompt_splits(long tiles, int Hkv) { return tiles * Hkv * 2 > sms() ? 1 : sms() / (tiles * Hkv); }
+
+template <int FMT, int D>
+int launch_prompt(const KvAttnArgs &a, void *ws, cudaStream_t st) {
+    const size_t smem = kv_prompt_smem(D);
+    if (!resident((const void *)k_kv_attn_prompt<FMT, D>, KV_PROMPT_THREADS, smem))
+        return launched(cudaErrorInvalidConfiguration, "kv_attention");
+    const long tiles = prompt_tiles(a.s.T, a.s.B, a.Gq, a.s.cu != nullptr);
+    const long keys = (((long)a.s.P << a.c.pshift) + 127) >> 7;  // key tiles at most
+    long ns = prompt_splits(tiles, a.c.Hkv);
+    if (ns > keys) ns = keys < 1 ? 1 : keys;
+    float *part = ns > 1 ? (float *)ws : nullptr;
+    cudaError_t e = launch(k_kv_attn_prompt<FMT, D>, dim3((unsigned)(tiles * a.c.Hkv), (unsigned)ns), KV_PROMPT_THREADS, smem, st, a,
+                           (int)tiles, part);
+    if (e == cudaSuccess && ns > 1)
+        e = launch(k_kv_attn_join_splits<D>, dim3((unsigned)(((size_t)a.s.T * a.H + 3) / 4)), 128, 0, st, a, (const float *)part, (int)ns);
+    return launched(e, "kv_attention");
+}
+
 bool rows_ok(const void *p, long row, long head) { return p && aligned16(p) && row % 8 == 0 && head % 8 == 0; }
 
 }  // namespace
@@ -192,7 +217,15 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
 
 size_t moeb_kv_attention_workspace_bytes(int T, int B, int H, int kv_heads, int head_dim, int max_q) {
     if (T <= 0 || B <= 0 || H <= 0 || kv_heads <= 0 || head_dim <= 0 || max_q <= 0) return 0;
-    return few_layout(B, (long)max_q * (H / kv_heads) <= 8 ? 8 : 16, head_dim).total;
+    const int Gq = H / kv_heads;
+    const long cols = (long)max_q * Gq;
+    size_t n = up256(few_layout(B, cols <= 8 ? 8 : 16, head_dim).total);
+    if (cols > 16) {
+        const long tiles = T % B ? prompt_tiles(T, B, Gq, true) : std::min(prompt_tiles(T, B, Gq, true), prompt_tiles(T, B, Gq, false));
+        const long ns = prompt_splits(tiles, kv_heads);
+        if (ns > 1) n += (size_t)ns * T * H * (head_dim + 2) * 4;
+    }
+    return n;
 }
 
 int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, long q_head, int T, int H, const int *cu,
@@ -243,7 +276,10 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
         if (rc) return rc;
     }
     if (only_few) return MOEB_OK;
-    return launched(launch(KV_PICK(k_kv_attn_rows, cache), dim3(T, H), 128, 0, stream, a), "kv_attention");
+    void *rest = (char *)ws + up256(few_layout(B, 16, cache->head_dim).total);
+    return cache->format == MOEB_KV_Q4
+               ? (cache->head_dim == 64 ? launch_prompt<FMT_Q4, 64>(a, rest, stream) : launch_prompt<FMT_Q4, 128>(a, rest, stream))
+               : (cache->head_dim == 64 ? launch_prompt<FMT_FP4, 64>(a, rest, stream) : launch_prompt<FMT_FP4, 128>(a, rest, stream));
 }
 
 int moeb_kv_read_error(const moeb_kv_cache *cache, unsigned *out, cudaStream_t stream) {
