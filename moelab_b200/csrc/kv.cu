@@ -113,14 +113,13 @@ __global__ void __launch_bounds__(128) k_kv_write(KvWriteArgs a) {
     const uint32_t word = FMT == FMT_Q4 ? kv_quant_q4(x, par) : kv_quant_fp4(x, par);
     if (page < 0) return;
     const size_t row = kv_row(a.c, page, h, p);
-    if (!isv) {
-        a.c.kq[row * W + kv_kpos<FMT, D>(w)] = word;
-    } else if (FMT == FMT_Q4) {
-        a.c.vq[row * W + kv_vpos_q4<D>(w)] = word;
+    uint32_t *codes = isv ? a.c.vq : a.c.kq;
+    if (FMT == FMT_Q4) {
+        codes[row * W + kv_pos_q4<D>(w)] = word;
     } else {
-        uint16_t *dst = reinterpret_cast<uint16_t *>(a.c.vq) + row * (D / 4);
-        dst[kv_vpos_fp4<D>(2 * w)] = (uint16_t)word;
-        dst[kv_vpos_fp4<D>(2 * w + 1)] = (uint16_t)(word >> 16);
+        uint16_t *dst = reinterpret_cast<uint16_t *>(codes) + row * (D / 4);
+        dst[kv_pos_fp4<D>(2 * w)] = (uint16_t)word;
+        dst[kv_pos_fp4<D>(2 * w + 1)] = (uint16_t)(word >> 16);
     }
     void *ps = isv ? a.c.vs : a.c.ks;
     if (FMT == FMT_Q4) {
@@ -150,7 +149,7 @@ __global__ void __launch_bounds__(128) k_kv_read(KvReadArgs a) {
     uint4 o = make_uint4(0, 0, 0, 0);
     if (page >= 0) {
         const size_t row = kv_row(a.c, page, h, (int)p);
-        const uint32_t word = isv ? kv_vword<FMT, D>(a.c.vq, row, w) : a.c.kq[row * W + kv_kpos<FMT, D>(w)];
+        const uint32_t word = kv_word<FMT, D>(isv ? a.c.vq : a.c.kq, row, w);
         float x[8];
         kv_word_values<FMT>(word, kv_par<FMT>(isv ? a.c.vs : a.c.ks, row, w, D), x);
         o = make_uint4(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7]));

@@ -7,12 +7,11 @@
 //   MXFP4 parameters  uint8  [pages][Hkv][page][D / 32]  (E8M0; value = E2M1(code) * 2^(byte - 127))
 // so a page's tokens of one head are one contiguous block, and 16 tokens (a tensor-core tile's rows) are D * 8 bytes in a
 // row. The order inside a row is the one the decode kernel's registers want (kv_attn.cu):
-//   int4 word: 8 values, element 2 p at nibble p, element 2 p + 1 at nibble p + 4 (as in the expert weights), w = 0 .. 7 in
-//     its group g of 64, G = D / 64;  K: at (w / 2) * 2 G + 2 g + w % 2,  V: at w * G + g
-//   MXFP4: groups of 32, H = D / 32;  K: words of 8 values, element i at nibble i, word w = 0 .. 3 of group g at w * H + g,
-//     V: half-words of 4 values, element i at nibble i, half-word u = 0 .. 7 of group g at half-word u * H + g
-// With it a lane's codes of one key (K: 1 / 4 of the row, V: 1 / 8) are one load of 4 to 16 bytes, and hold the same part of
-// every group.
+//   int4: words of 8 values, element 2 p at nibble p, element 2 p + 1 at nibble p + 4 (as in the expert weights); word w = 0 .. 7
+//     of group g (of G = D / 64) at w * G + g
+//   MXFP4: half-words of 4 values, element i at nibble i; half-word u = 0 .. 7 of group g (of H = D / 32) at half-word u * H + g
+// With it a lane's codes of one key (1 / 4 of the row for K, 1 / 8 for V) are one load of 4 to 16 bytes, and hold the same part
+// of every group.
 #pragma once
 #include "common.cuh"
 #include "kernels.h"
@@ -38,15 +37,11 @@ struct KvSeqs {
     int B, P, T, each;
 };
 
-// place in its row of K's word w (values 8 w ..), of V's word w (int4), of V's half-word u (values 4 u .., MXFP4)
-template <int FMT, int D>
-MOEB_DEV int kv_kpos(int w) {
-    return FMT == FMT_Q4 ? ((w & 7) >> 1) * (D / 32) + 2 * (w >> 3) + (w & 1) : (w & 3) * (D / 32) + (w >> 2);
-}
+// place in its row of word w (values 8 w ..; int4), of half-word u (values 4 u ..; MXFP4)
 template <int D>
-MOEB_DEV int kv_vpos_q4(int w) { return (w & 7) * (D / 64) + (w >> 3); }
+MOEB_DEV int kv_pos_q4(int w) { return (w & 7) * (D / 64) + (w >> 3); }
 template <int D>
-MOEB_DEV int kv_vpos_fp4(int u) { return (u & 7) * (D / 32) + (u >> 3); }
+MOEB_DEV int kv_pos_fp4(int u) { return (u & 7) * (D / 32) + (u >> 3); }
 
 MOEB_DEV int kv_clamp_row(int v, int T) { return v < 0 ? 0 : (v > T ? T : v); }
 // rows [r0, r1) of sequence b, inside [0, T)
@@ -113,12 +108,12 @@ MOEB_DEV uint32_t kv_par(const void *ps, size_t row, int w, int D) {
     return static_cast<const uint8_t *>(ps)[row * (D / 32) + (w >> 2)];
 }
 
-// V's word w of a row in natural order of its values
+// word w (values 8 w ..) of a row
 template <int FMT, int D>
-MOEB_DEV uint32_t kv_vword(const uint32_t *vq, size_t row, int w) {
-    if (FMT == FMT_Q4) return vq[row * (D / 8) + kv_vpos_q4<D>(w)];
-    const uint16_t *p = reinterpret_cast<const uint16_t *>(vq) + row * (D / 4);
-    return p[kv_vpos_fp4<D>(2 * w)] | (uint32_t)p[kv_vpos_fp4<D>(2 * w + 1)] << 16;
+MOEB_DEV uint32_t kv_word(const uint32_t *codes, size_t row, int w) {
+    if (FMT == FMT_Q4) return codes[row * (D / 8) + kv_pos_q4<D>(w)];
+    const uint16_t *p = reinterpret_cast<const uint16_t *>(codes) + row * (D / 4);
+    return p[kv_pos_fp4<D>(2 * w)] | (uint32_t)p[kv_pos_fp4<D>(2 * w + 1)] << 16;
 }
 
 struct KvWriteArgs {
@@ -180,6 +175,6 @@ __global__ void k_kv_attn_prompt(const KvAttnArgs a, int tiles, float *part);
 template <int D>
 __global__ void k_kv_attn_join_splits(const KvAttnArgs a, const float *part, int ns);
 size_t kv_prompt_smem(int D);
-constexpr int KV_PROMPT_ROWS = 256, KV_PROMPT_THREADS = 512;
+constexpr int KV_PROMPT_ROWS = 256, KV_PROMPT_THREADS = 640;
 
 }  // namespace moeb

@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
                         for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            const uint32_t ua = wa[2 * g + (x >> 1)], ub = wb[2 * g + (x >> 1)];
+                            const uint32_t ua = wa[(x >> 1) * NG + g], ub = wb[(x >> 1) * NG + g];
                             const int p = 2 * (x & 1);
                             const uint32_t A[4] = {q4pair(ua, p), q4pair(ub, p), q4pair(ua, p + 1), q4pair(ub, p + 1)};
 #pragma unroll
@@ -367,8 +367,16 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
                         float acc[NT][4];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-                        const uint32_t A0[4] = {e2m1_f16x2<0>(wa[g]), e2m1_f16x2<0>(wb[g]), e2m1_f16x2<1>(wa[g]), e2m1_f16x2<1>(wb[g])};
-                        const uint32_t A1[4] = {e2m1_f16x2<2>(wa[g]), e2m1_f16x2<2>(wb[g]), e2m1_f16x2<3>(wa[g]), e2m1_f16x2<3>(wb[g])};
+                        // half-words 2 c (product 0) and 2 c + 1 of the group
+                        const int x0 = g >> 1, x1 = NG / 2 + (g >> 1);
+                        uint32_t A0[4], A1[4];
+                        if (g & 1) {
+                            A0[0] = e2m1_f16x2<2>(wa[x0]); A0[1] = e2m1_f16x2<2>(wb[x0]); A0[2] = e2m1_f16x2<3>(wa[x0]); A0[3] = e2m1_f16x2<3>(wb[x0]);
+                            A1[0] = e2m1_f16x2<2>(wa[x1]); A1[1] = e2m1_f16x2<2>(wb[x1]); A1[2] = e2m1_f16x2<3>(wa[x1]); A1[3] = e2m1_f16x2<3>(wb[x1]);
+                        } else {
+                            A0[0] = e2m1_f16x2<0>(wa[x0]); A0[1] = e2m1_f16x2<0>(wb[x0]); A0[2] = e2m1_f16x2<1>(wa[x0]); A0[3] = e2m1_f16x2<1>(wb[x0]);
+                            A1[0] = e2m1_f16x2<0>(wa[x1]); A1[1] = e2m1_f16x2<0>(wb[x1]); A1[2] = e2m1_f16x2<1>(wa[x1]); A1[3] = e2m1_f16x2<1>(wb[x1]);
+                        }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             mma_f16(acc[nt], A0, qf[nt][2 * g][0], qf[nt][2 * g][1]);

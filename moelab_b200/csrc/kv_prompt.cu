@@ -2,16 +2,17 @@
 // 5th-generation tensor cores (layout of the cache: kv.cuh).
 //
 // A CTA takes 256 rows of one (sequence, KV head): the sequence's n tokens x Gq query heads in a row, as two tiles of 128
-// (the tensor core's M), and walks the keys that any of them sees in tiles of 128. Per key tile and row tile
-//   S [128 x 128] = Q . K^T (operands in shared memory), P = 2^(S - m) as fp16 into the TMEM columns S leaves,
+// (the tensor core's M), and walks the keys that any of them sees in tiles of 128, two halves of 64. Per half and row tile
+//   S [128 x 64] = Q . K^T (operands in shared memory), P = 2^(S - m) as fp16 into the TMEM columns S leaves,
 //   O [128 x D] += P . V (P from TMEM, V in shared memory, its D contiguous: the MN-major operand form).
-// TMEM: O of both tiles (2 D columns), S / P of both tiles (2 x 128). While one row tile is in its softmax the other one's
-// products run, so the tensor core and the exponentials work side by side.
+// TMEM: O of both tiles (2 D columns), S / P of both tiles and halves (4 x 64). A row tile's products for one half run while
+// its softmax is at the other half, and the two row tiles run side by side.
 //   warps 0 - 3, 4 - 7: softmax of row tile 0, 1: a thread per row, statistics in registers; they also rescale O, only when
 //     a row's maximum grew by more than 2^8 since it was last used (P <= 2^14 in fp16 until then)
-//   warps 8 - 11: fetch codes (a tile ahead, in registers), dequantize K and V into fp16 tiles, 128-byte swizzle
-//   warps 12, 13: one lane each issues the products of row tile 0, 1 (14, 15 fill the warpgroup)
-// Registers: 512 x 128 at launch; the softmax warpgroups go to 160, the others to 120 and 56 (63488 of 65536 in all).
+//   warps 8 - 11, 12 - 15: fetch the codes of K, of V (a tile ahead, in registers), dequantize them into fp16 tiles, 128-byte
+//     swizzle
+//   warps 16, 17: one lane each issues the products of row tile 0, 1 (18, 19 fill the warpgroup)
+// Registers: 640 x 96 at launch; the softmax warpgroups go to 128, the others to 88 and 40 (60416 of 61440 in all).
 // fp16 and not bf16 operands: both formats' values, and P, would lose 2^-9 to bf16, as much as the result's own rounding;
 // fp16 keeps 2^-12. Its range is kept by powers of two: one per query row, one per K tile (both go into the softmax's
 // scale), and a running one for V (a change rescales O; it leaves room for 2^6 of growth, so that it hardly happens).
@@ -28,7 +29,7 @@ namespace moeb {
 namespace {
 
 constexpr int PR = 256;               // rows per CTA
-constexpr int PT = 512;               // threads: four warpgroups
+constexpr int PT = 640;               // threads: five warpgroups
 constexpr float P_OFF = 6.f;          // P = 2^(score - m + 6)
 constexpr float P_LAZY = 8.f;
 
@@ -43,13 +44,14 @@ struct Pr {
 };
 
 struct PrShared {
-    uint64_t kfull[3], kempty[3], vfull[3], vempty[3], sfull[2], pfull[2], ofull[2];
+    uint64_t kfull[3], kempty[3], vfull[3], vempty[3], sfull[2][2], pfull[2][2], pv[2], ofull[2];  // [row tile][half]
     float kmul[4];             // by key tile % 4: 2^e of the K tile
     unsigned hole[4][4];       // by key tile % 4: keys without a page
     float vfix[3];             // by stage: what O is multiplied by before this V tile
     unsigned pz[3];            // by stage: byte per dequantizing warp, a NaN group among its rows
     uint8_t pm[3][128];        // by stage and key: its NaN groups
-    unsigned mx[2][4][2];      // exchange of the tile's largest magnitudes
+    unsigned mx[2][2][4];      // exchange of the tiles' largest magnitudes: K or V, tile % 2, warp
+    float qmul[PR];            // the rows' scale
     float vun;                 // 2^e of O at the end
     uint32_t tmem;
     int b, tile, fail;
@@ -63,6 +65,23 @@ MOEB_DEV float ex2p(float x) {
 MOEB_DEV uint32_t h2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// pairs of fp32 in one 64-bit register: one instruction for two sums or products
+MOEB_DEV uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+MOEB_DEV void unpair(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+MOEB_DEV uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+MOEB_DEV uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
     return r;
 }
 MOEB_DEV uint32_t hmul2u(uint32_t a, uint32_t b) {
@@ -82,27 +101,30 @@ MOEB_DEV bool pr_wait(uint64_t *bar, unsigned parity, const int *fail) {
         if ((i & 31u) == 0 && (*reinterpret_cast<const volatile int *>(fail) || globaltimer_ns() - t0 > 2000000000ull)) return false;
     }
 }
-// 128-byte swizzled operand descriptor: 8 rows of 128 bytes every 1024; lbo: bytes between 64-element chunks of an MN-major
-// operand (K-major ones do not use it)
-MOEB_DEV uint64_t sdesc(uint32_t saddr, uint32_t lbo) {
-    uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(lbo >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-MOEB_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// 128-byte swizzled operand descriptors: 8 rows of 128 bytes every 1024; LBO: bytes between 64-element chunks of an MN-major
+// operand (K-major ones do not use it). The upper word is constant, the lower one is address / 16 and LBO / 16.
+constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+template <uint32_t LBO>
+MOEB_DEV uint32_t desc_lo(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | (LBO >> 4) << 16; }
+MOEB_DEV void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a),
-        "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(DESC_HI)
         : "memory");
 }
-MOEB_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+MOEB_DEV void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a),
-        "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 db;\n mov.b64 db, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(DESC_HI)
         : "memory");
+}
+// one lane of a converged warp, the same one every time
+MOEB_DEV bool elect() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
 }
 MOEB_DEV void commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -121,12 +143,11 @@ MOEB_DEV void ld32(uint32_t addr, float *v) {
         : "r"(addr));
 }
 #define KV_W8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
-MOEB_DEV void st32(uint32_t addr, const uint32_t *v) {
+MOEB_DEV void ld16(uint32_t addr, float *v) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
-        "%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-        KV_W8(v, 0), KV_W8(v, 8), KV_W8(v, 16), KV_W8(v, 24)
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : KV_R8(v, 0), KV_R8(v, 8)
+        : "r"(addr));
 }
 MOEB_DEV void st16(uint32_t addr, const uint32_t *v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
@@ -148,10 +169,10 @@ MOEB_DEV PrKeys pr_keys(const KvAttnArgs &a, int pmin, int pmax) {
 }
 MOEB_DEV int pr_tok(const PrKeys &k, int i) { return (i < k.ns ? i : (k.lo >> 7) + i - k.ns) << 7; }
 
-// natural 8-value word of a row at physical word x of K (the order Q takes too)
+// first value of the 4 that physical half-word u of a row holds (K, and Q with it, and V's columns of O keep this order)
 template <int FMT, int D>
-MOEB_DEV int pr_kword(int x) {
-    return FMT == FMT_Q4 ? 8 * ((x >> 1) % (D / 64)) + 2 * (x / (D / 32)) + (x & 1) : 4 * (x % (D / 32)) + x / (D / 32);
+MOEB_DEV int pr_dim(int u) {
+    return FMT == FMT_Q4 ? 64 * ((u >> 1) % (D / 64)) + 8 * ((u >> 1) / (D / 64)) + 4 * (u & 1) : 32 * (u % (D / 32)) + 4 * (u / (D / 32));
 }
 
 // a code word of 8 values to fp16, in the word's order; q4: s2 / b2 scale and bias, MXFP4: s2 / b2 the scales of the word's
@@ -187,6 +208,9 @@ MOEB_DEV uint4 pr_word(uint32_t w, uint32_t s2, uint32_t b2) {
     return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
+// the n lowest of 64 bits
+MOEB_DEV unsigned long long pr_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
+
 // Largest magnitude (bits) that a row's parameters allow, NaN groups apart; nan: which groups are NaN.
 template <int FMT, int NG>
 MOEB_DEV uint32_t pr_top(const float (&s)[NG], const float (&b)[NG], unsigned &nan) {
@@ -202,13 +226,248 @@ MOEB_DEV uint32_t pr_top(const float (&s)[NG], const float (&b)[NG], unsigned &n
     return top;
 }
 
+// One warpgroup's work on K or V: every key tile's codes to fp16 in its stage. Warp w has keys 32 i + 8 w + r, r = lane / 4, in
+// four passes i, a lane a quarter of each row; lane (r, c) is the owner of key 32 c + 8 w + r: it looks up the page, reads the
+// parameters and prepares them for all, the passes take them by shuffles. Codes are on their way a tile ahead, parameters and
+// page ids two. One body for K and V: five kinds of warps share the instruction cache.
+template <int FMT, int D>
+MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, const PrKeys &keys, int b, int h, int k0, int nk, int pmax, int Lk,
+                      int w, int lane, bool V) {
+    using L = Pr<D>;
+    constexpr int NST = L::NST, W4 = D / 32, NG = FMT == FMT_Q4 ? D / 64 : D / 32, NP = FMT == FMT_Q4 ? NG : 1;
+    constexpr int PB = FMT == FMT_Q4 ? 4 * NG : NG;  // parameter bytes per row
+    const int r = lane >> 2, c = lane & 3, mine = 32 * c + 8 * w + r;
+    const unsigned char *codes = reinterpret_cast<const unsigned char *>(V ? a.c.vq : a.c.kq) + ((size_t)h << a.c.pshift) * (D / 2) + c * (D / 8);
+    const unsigned char *pars = static_cast<const unsigned char *>(V ? a.c.vs : a.c.ks) + ((size_t)h << a.c.pshift) * PB;
+    const size_t per_page = (size_t)a.c.Hkv << a.c.pshift;  // rows
+    const int *table = a.s.table + (size_t)b * a.s.trow;
+    const int pmask = (1 << a.c.pshift) - 1;
+    uint64_t *full = V ? sh.vfull : sh.kfull, *empty = V ? sh.vempty : sh.kempty;
+    unsigned char *dst0 = sm + (V ? L::OFF_V : L::OFF_K) + (8 * w + r) * 128;
+    uint32_t code[4][W4], par[NP];
+    // page id of this lane's key of tile k: -1 where no row sees the key, -2 where it has no page
+    auto page = [&](int k) {
+        const int j = pr_tok(keys, k0 + k) + mine;
+        if (k >= nk || j > pmax || j >= Lk || (j < keys.lo && j >= a.sinks)) return -1;
+        const int pi = j >> a.c.pshift, id = pi < a.s.P ? table[pi] : -1;
+        return id < 0 || id >= a.c.pages ? -2 : id;
+    };
+    auto fetch_par = [&](int k, int id) {
+#pragma unroll
+        for (int x = 0; x < NP; ++x) par[x] = 0u;
+        if (id < 0) return;
+        const unsigned char *p = pars + (id * per_page + (size_t)((pr_tok(keys, k0 + k) + mine) & pmask)) * PB;
+        if (PB == 8) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(p);
+            par[0] = x.x;
+            par[NP - 1] = x.y;
+        } else if (PB == 4) {
+            par[0] = *reinterpret_cast<const uint32_t *>(p);
+        } else {
+            par[0] = *reinterpret_cast<const uint16_t *>(p);
+        }
+    };
+    auto fetch_codes = [&](int k, int id) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int pid = __shfl_sync(0xffffffffu, id, (lane & 28) | i);
+#pragma unroll
+            for (int x = 0; x < W4; ++x) code[i][x] = 0u;
+            if (pid >= 0) {
+                const unsigned char *p = codes + (pid * per_page + (size_t)((pr_tok(keys, k0 + k) + 32 * i + 8 * w + r) & pmask)) * (D / 2);
+                if (D == 128) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(p);
+                    code[i][0] = x.x; code[i][1] = x.y; code[i][W4 - 2] = x.z; code[i][W4 - 1] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(p);
+                    code[i][0] = x.x; code[i][1] = x.y;
+                }
+            }
+        }
+    };
+    int id = page(0), id1 = page(1);
+    fetch_par(0, id);
+    fetch_codes(0, id);
+    uint32_t vlim = 0;  // V: bits of the largest value that the running power of two takes; that power, its inverse
+    float vmul = 1.f, vun = 1.f;
+    bool ok = true;
+    int st = 0;
+    unsigned ph = 1;
+#pragma unroll 1
+    for (int j = 0; j < nk; ++j) {  // a warp that gave up still comes to the barrier
+        // ---- this lane's key: the largest magnitude its parameters allow, its NaN groups
+        float s[NG], bb[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            s[g] = FMT == FMT_Q4 ? bf16lo(par[FMT == FMT_Q4 ? g : 0]) : kv_e8m0((par[0] >> (8 * g)) & 255u);
+            bb[g] = FMT == FMT_Q4 ? bf16hi(par[FMT == FMT_Q4 ? g : 0]) : 0.f;
+        }
+        unsigned nan;
+        uint32_t top = pr_top<FMT, NG>(s, bb, nan);
+        if (id < 0) top = 0;  // zeros (MXFP4: codes of zero)
+        const unsigned hole = __ballot_sync(0xffffffffu, id == -2);
+        id = id1;
+        fetch_par(j + 1, id);  // of the next tile; what this one needs is in s and bb
+        id1 = page(j + 2);
+        top = __reduce_max_sync(0xffffffffu, top);
+        unsigned *mx = sh.mx[V][j & 1];
+        if (lane == 0) mx[w] = top;
+        asm volatile("bar.sync %0, 128;" ::"r"(V ? 2 : 1) : "memory");
+        top = max(max(mx[0], mx[1]), max(mx[2], mx[3]));
+        if (ok && j >= NST && !__all_sync(0xffffffffu, pr_wait(empty + st, ph, &sh.fail))) ok = false;
+        if (ok) {
+            // ---- the tile's power of two
+            float mul, fix = 1.f;
+            if (!V || top > vlim) {
+                const uint32_t e = min(max(top >> 23, 9u), 248u);
+                const float nm = __uint_as_float((262u - e) << 23), nu = __uint_as_float((e - 8u) << 23);
+                fix = nm * vun;
+                vmul = nm;
+                vun = nu;
+                vlim = (e + 6u) << 23;
+            }
+            mul = vmul;
+            uint32_t s2[NG], b2[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                if (V && ((nan >> g) & 1u)) s[g] = bb[g] = 0.f;  // the rows that see the key are marked instead
+                s2[g] = h2(s[g] * mul, s[g] * mul);
+                b2[g] = h2(bb[g] * mul, bb[g] * mul);
+            }
+            unsigned char *dst = dst0 + st * L::TILE;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t ps[NG], pb[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    ps[g] = __shfl_sync(0xffffffffu, s2[g], (lane & 28) | i);
+                    pb[g] = FMT == FMT_Q4 ? __shfl_sync(0xffffffffu, b2[g], (lane & 28) | i) : 0u;
+                }
+#pragma unroll
+                for (int x = 0; x < W4; ++x) {
+                    const int u = c * W4 + x;
+                    const uint4 v = FMT == FMT_Q4 ? pr_word<FMT>(code[i][x], ps[x % NG], pb[x % NG])
+                                                  : pr_word<FMT>(code[i][x], ps[(2 * x) % NG], ps[(2 * x + 1) % NG]);
+                    *reinterpret_cast<uint4 *>(dst + (u >> 3) * 16384 + i * 4096 + (((u & 7) ^ r) << 4)) = v;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            // ---- what the softmax has to know of the tile
+            if (V) {
+                const bool any = __any_sync(0xffffffffu, nan != 0);
+                if (any) sh.pm[st][mine] = (uint8_t)nan;
+                if (lane == 0) {
+                    reinterpret_cast<uint8_t *>(&sh.pz[st])[w] = any;
+                    if (w == 0) {
+                        sh.vfix[st] = fix;
+                        sh.vun = vun;
+                    }
+                }
+            } else {
+                if (lane < 4) {  // byte w of word `lane`: keys 32 lane + 8 w .., their bits are 4 r + lane
+                    unsigned x = (hole >> lane) & 0x11111111u;
+                    x = (x | x >> 3) & 0x03030303u;
+                    x = (x | x >> 6) & 0x000F000Fu;
+                    x = (x | x >> 12) & 0xFFu;
+                    reinterpret_cast<uint8_t *>(sh.hole[j & 3])[4 * lane + w] = (uint8_t)x;
+                    if (x) atomicOr(a.c.err, ERR_PAGE);
+                }
+                if (w == 0 && lane == 0) sh.kmul[j & 3] = vun;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + st);
+        }
+        fetch_codes(j + 1, id);
+        if (++st == NST) {
+            st = 0;
+            ph ^= 1;
+        }
+    }
+    if (!ok && lane == 0) {
+        atomicOr(a.c.err, ERR_TIMEOUT);
+        *reinterpret_cast<volatile int *>(&sh.fail) = 1;
+    }
+}
+
+// The products of row tile T. The whole warp goes along and one lane issues: what the instructions take (addresses, counts)
+// is the warp's own, so that it sits in uniform registers; a lane on its own needs 150 cycles to issue a product.
+template <int D, int T>
+MOEB_DEV void pr_products(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, int nk_, uint32_t tmem_) {
+    using L = Pr<D>;
+    constexpr int NST = L::NST;
+    constexpr uint32_t id_s = (1u << 4) | (8u << 17) | (8u << 24);
+    constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+    const int nk = __shfl_sync(0xffffffffu, nk_, 0);
+    if (nk == 0) return;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_, 0), base = __shfl_sync(0xffffffffu, smem_u32(sm), 0);
+    const uint32_t ds = tmem + L::S0 + 128 * T, dout = tmem + D * T;
+    const uint32_t qa = desc_lo<16>(base + T * L::TILE), ka0 = desc_lo<16>(base + L::OFF_K), va0 = desc_lo<16384>(base + L::OFF_V);
+    bool ok = true;
+    // S of half i of key tile j (stage st, phase ph); the last product of K's stage frees it
+    auto scores = [&](int st, unsigned ph, int i) {
+        if (i == 0 && !__all_sync(0xffffffffu, pr_wait(sh.kfull + st, ph, &sh.fail))) return false;
+        fence_after();
+        const uint32_t ka = ka0 + (st * L::TILE + i * 8192) / 16;
+        if (elect()) {
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) {
+                const uint32_t off = ((s >> 2) * 16384 + (s & 3) * 32) / 16;
+                mma_ss(ds + 64 * i, qa + off, ka + off, id_s, s > 0);
+            }
+            commit(&sh.sfull[T][i]);
+            if (i) commit(sh.kempty + st);
+        }
+        __syncwarp();
+        return true;
+    };
+    ok = scores(0, 0, 0) && scores(0, 0, 1);
+    int st = 0, sn = NST > 1 ? 1 : 0;  // stage of this tile and of the next, with their phases
+    unsigned ph = 0, pn = 0;
+    for (int j = 0; j < nk && ok; ++j) {
+        const uint32_t va = va0 + st * (L::TILE / 16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (i == 0) ok = __all_sync(0xffffffffu, pr_wait(sh.vfull + st, ph, &sh.fail));
+            ok = ok && __all_sync(0xffffffffu, pr_wait(&sh.pfull[T][i], j & 1, &sh.fail));
+            if (!ok) break;
+            fence_after();
+            if (elect()) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    mma_ts(dout, ds + 64 * i + 8 * s, va + (i * 8192 + s * 2048) / 16, id_o, i > 0 || s > 0 ? 1u : (j > 0));
+                commit(sh.pv + T);
+                if (i) commit(sh.vempty + st);
+            }
+            __syncwarp();
+            if (j + 1 < nk) ok = scores(sn, pn, i);
+            if (!ok) break;
+        }
+        st = sn;
+        ph = pn;
+        if (++sn == NST) {
+            sn = 0;
+            pn ^= 1;
+        }
+    }
+    if (elect()) {
+        if (!ok) {
+            atomicOr(a.c.err, ERR_TIMEOUT);
+            *reinterpret_cast<volatile int *>(&sh.fail) = 1;
+        }
+        commit(sh.ofull + T);
+    }
+    __syncwarp();
+    const int none = 0;
+    pr_wait(sh.ofull + T, 0, &none);  // nothing is in flight when TMEM is released
+}
+
 }  // namespace
 
 // part: null, or the workspace of split calls: [splits][T][H][D] sums, then [splits][T][H] (max, sum)
 template <int FMT, int D>
 __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, int tiles, float *part) {
     using L = Pr<D>;
-    constexpr int NST = L::NST, W4 = D / 32, NG = FMT == FMT_Q4 ? D / 64 : D / 32;
+    constexpr int NST = L::NST, NG = FMT == FMT_Q4 ? D / 64 : D / 32;
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     __shared__ PrShared sh;
@@ -274,55 +533,58 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             mbar_init(sh.vempty + i, 2);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(sh.sfull + i, 1);
-            mbar_init(sh.pfull + i, 4);
+            for (int x = 0; x < 2; ++x) {
+                mbar_init(&sh.sfull[i][x], 1);
+                mbar_init(&sh.pfull[i][x], 4);
+            }
+            mbar_init(sh.pv + i, 1);
             mbar_init(sh.ofull + i, 1);
         }
         mbar_fence_init();
         sh.vun = 1.f;
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // ---- queries: fp16 after a power of two per row (the largest value near 2^8), K's order of words, swizzled
-    float qmul = 1.f;
-    int pos = -1, row_t = 0, row_h = 0;
+    // ---- queries: fp16 after a power of two per row (the largest value near 2^8), K's order of words, swizzled. D / 8
+    // lanes have a row (one word of 8 values each), so that the loads are whole lines.
     if (warp < 8) {
-        const int t = warp >> 2, row = (warp & 3) * 32 + lane, R = R0 + t * 128 + row;
-        uint4 w[D / 8];
-        uint32_t top = 0;
-        if (R < NR) {
-            const int i = R / a.Gq;
-            pos = p0 + i;
-            row_t = r0 + i;
-            row_h = h * a.Gq + R - i * a.Gq;
-            const uint16_t *src = a.q + row_t * a.q_row + row_h * a.q_head;
+        constexpr int LR = D / 8, RW = 32 / LR;  // lanes per row, rows per load
+        const int x = lane % LR;
+        uint4 w[32 / RW];
 #pragma unroll
-            for (int x = 0; x < D / 8; ++x) w[x] = *reinterpret_cast<const uint4 *>(src + 8 * pr_kword<FMT, D>(x));
-        } else {
-#pragma unroll
-            for (int x = 0; x < D / 8; ++x) w[x] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 32 / RW; ++i) {
+            const int R = R0 + warp * 32 + i * RW + lane / LR;
+            w[i] = make_uint4(0, 0, 0, 0);
+            if (R < NR) {
+                const int ri = R / a.Gq;
+                const uint16_t *src = a.q + (r0 + ri) * a.q_row + (h * a.Gq + R - ri * a.Gq) * a.q_head;
+                const uint2 lo = *reinterpret_cast<const uint2 *>(src + pr_dim<FMT, D>(2 * x));
+                const uint2 hi = *reinterpret_cast<const uint2 *>(src + pr_dim<FMT, D>(2 * x + 1));
+                w[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
         }
 #pragma unroll
-        for (int x = 0; x < D / 8; ++x) {
-            const uint32_t u[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+        for (int i = 0; i < 32 / RW; ++i) {
+            const int row = warp * 32 + i * RW + lane / LR;
+            const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            uint32_t top = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7fffu, (u[e] >> 16) & 0x7fffu));
-        }
-        const int e = min(max((int)(top >> 7), 9), 254);
-        float down = __uint_as_float((uint32_t)(262 - e) << 23);
-        qmul = fabsf(a.scale) * __uint_as_float((uint32_t)(e - 8) << 23);
-        if (a.scale < 0.f) down = -down;      // the softmax's scale stays positive: it takes the maximum before scaling
-        if (a.scale == 0.f) down = 0.f, qmul = 1.f;
-        unsigned char *dst = sm + t * L::TILE + row * 128;
 #pragma unroll
-        for (int x = 0; x < D / 8; ++x) {
-            const uint32_t u[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+            for (int e = 1; e < LR; e <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, e));
+            const int e = min(max((int)(top >> 7), 9), 254);
+            float down = __uint_as_float((uint32_t)(262 - e) << 23);
+            float qmul = fabsf(a.scale) * __uint_as_float((uint32_t)(e - 8) << 23);
+            if (a.scale < 0.f) down = -down;  // the softmax's scale stays positive: it takes the maximum before scaling
+            if (a.scale == 0.f) down = 0.f, qmul = 1.f;
             uint32_t o[4];
 #pragma unroll
             for (int e2 = 0; e2 < 4; ++e2) o[e2] = h2(bf16lo(u[e2]) * down, bf16hi(u[e2]) * down);
-            *reinterpret_cast<uint4 *>(dst + (x >> 3) * 16384 + (((x & 7) ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4 *>(sm + (row >> 7) * L::TILE + (x >> 3) * 16384 + (row & 127) * 128 + (((x & 7) ^ (row & 7)) << 4)) =
+                make_uint4(o[0], o[1], o[2], o[3]);
+            if (x == 0) sh.qmul[row] = qmul;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -331,296 +593,71 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
     fence_after();
     const uint32_t tmem = sh.tmem;
 
-    if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        // ------------------------------------------------------------ products of row tile t
-        if (warp < 14 && lane == 0 && nk > 0) {
-            const int t = warp - 12;
-            const uint32_t id_s = (1u << 4) | (16u << 17) | (8u << 24);
-            const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
-            const uint32_t ds = tmem + L::S0 + 128 * t, dp = ds + 64, dout = tmem + D * t;
-            const uint32_t qa = smem_u32(sm + t * L::TILE);
-            bool ok = true;
-            for (int j = 0; j < nk; ++j) {
-                const int st = j % NST;
-                const unsigned ph = (j / NST) & 1;
-                if (!pr_wait(sh.kfull + st, ph, &sh.fail)) { ok = false; break; }
-                fence_after();
-                const uint32_t ka = smem_u32(sm + L::OFF_K + st * L::TILE);
-#pragma unroll
-                for (int s = 0; s < D / 16; ++s) {
-                    const uint32_t off = (s >> 2) * 16384 + (s & 3) * 32;
-                    mma_ss(ds, sdesc(qa + off, 16), sdesc(ka + off, 16), id_s, s > 0);
-                }
-                commit(sh.kempty + st);
-                commit(sh.sfull + t);
-                if (!pr_wait(sh.vfull + st, ph, &sh.fail) || !pr_wait(sh.pfull + t, j & 1, &sh.fail)) { ok = false; break; }
-                fence_after();
-                const uint32_t va = smem_u32(sm + L::OFF_V + st * L::TILE);
-#pragma unroll
-                for (int s = 0; s < 8; ++s) mma_ts(dout, dp + 8 * s, sdesc(va + s * 2048, 16384), id_o, j > 0 || s > 0);
-                commit(sh.vempty + st);
-            }
-            if (!ok) {
-                atomicOr(a.c.err, ERR_TIMEOUT);
-                *reinterpret_cast<volatile int *>(&sh.fail) = 1;
-            }
-            commit(sh.ofull + t);
-            const int none = 0;
-            pr_wait(sh.ofull + t, 0, &none);  // nothing is in flight when TMEM is released
-        }
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        // ------------------------------------------------------------ products, a warp per row tile
+        if (warp == 16) pr_products<D, 0>(a, sh, sm, nk, tmem);
+        if (warp == 17) pr_products<D, 1>(a, sh, sm, nk, tmem);
     } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
-        // ------------------------------------------------------------ codes -> fp16 tiles
-        const int w = warp - 8, r = lane >> 2, c = lane & 3;
-        uint32_t kc[4][W4], vc[4][W4];
-        uint32_t kp[4][FMT == FMT_Q4 ? NG : 1], vp[4][FMT == FMT_Q4 ? NG : 1];
-        long pid[4];          // of the tile that is fetched next: page, -1: none where one should be, -2: no row sees the key
-        unsigned hole_next = 0, hole_now = 0;  // bit per pass: pid == -1
-        auto pages = [&](int k) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                pid[i] = -2;
-                if (k < k1) {
-                    const int j = pr_tok(keys, k) + 32 * i + 8 * w + r;
-                    if (j <= pmax && j < Lk && (j >= keys.lo || j < a.sinks)) pid[i] = kv_page(a.c, a.s, b, j);
-                }
-            }
-        };
-        auto fetch = [&](int k) {
-            hole_next = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (pid[i] == -1) hole_next |= 1u << i;
-#pragma unroll
-                for (int x = 0; x < W4; ++x) kc[i][x] = vc[i][x] = 0u;
-#pragma unroll
-                for (int x = 0; x < (FMT == FMT_Q4 ? NG : 1); ++x) kp[i][x] = vp[i][x] = 0u;
-                if (pid[i] < 0) continue;
-                const size_t row = kv_row(a.c, pid[i], h, pr_tok(keys, k) + 32 * i + 8 * w + r);
-                const uint32_t *ks = a.c.kq + row * (D / 8) + c * W4, *vs = a.c.vq + row * (D / 8) + c * W4;
-                if (D == 128) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(ks), y = *reinterpret_cast<const uint4 *>(vs);
-                    kc[i][0] = x.x; kc[i][1] = x.y; kc[i][W4 - 2] = x.z; kc[i][W4 - 1] = x.w;
-                    vc[i][0] = y.x; vc[i][1] = y.y; vc[i][W4 - 2] = y.z; vc[i][W4 - 1] = y.w;
-                } else {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(ks), y = *reinterpret_cast<const uint2 *>(vs);
-                    kc[i][0] = x.x; kc[i][1] = x.y;
-                    vc[i][0] = y.x; vc[i][1] = y.y;
-                }
-                if (FMT == FMT_Q4) {
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        kp[i][g] = static_cast<const uint32_t *>(a.c.ks)[row * NG + g];
-                        vp[i][g] = static_cast<const uint32_t *>(a.c.vs)[row * NG + g];
-                    }
-                } else if (D == 128) {
-                    kp[i][0] = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(a.c.ks) + row * NG);
-                    vp[i][0] = *reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(a.c.vs) + row * NG);
-                } else {
-                    kp[i][0] = *reinterpret_cast<const uint16_t *>(static_cast<const uint8_t *>(a.c.ks) + row * NG);
-                    vp[i][0] = *reinterpret_cast<const uint16_t *>(static_cast<const uint8_t *>(a.c.vs) + row * NG);
-                }
-            }
-        };
-        // parameters of one row as fp32 (MXFP4: byte 0 of an unseen key stands for 2^-127, times codes of zero)
-        auto params = [&](const uint32_t (&p)[FMT == FMT_Q4 ? NG : 1], float (&s)[NG], float (&bb)[NG]) {
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                if (FMT == FMT_Q4) {
-                    s[g] = bf16lo(p[g]);
-                    bb[g] = bf16hi(p[g]);
-                } else {
-                    s[g] = kv_e8m0((p[0] >> (8 * g)) & 255u);
-                    bb[g] = 0.f;
-                }
-            }
-        };
-        // the tile's rows, dequantized after multiplication by `mul`; NaN groups of V as zeros
-        auto dequant = [&](unsigned char *dst, const uint32_t (&code)[4][W4], const uint32_t (&par)[4][FMT == FMT_Q4 ? NG : 1], float mul,
-                           bool isv) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 32 * i + 8 * w + r;
-                float s[NG], bb[NG];
-                params(par[i], s, bb);
-                uint32_t s2[NG], b2[NG];
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    if (isv && !(fabsf(s[g]) <= 3.4028234e38f && fabsf(bb[g]) <= 3.4028234e38f)) s[g] = bb[g] = 0.f;
-                    s2[g] = h2(s[g] * mul, s[g] * mul);
-                    b2[g] = h2(bb[g] * mul, bb[g] * mul);
-                }
-#pragma unroll
-                for (int x = 0; x < W4; ++x) {
-                    // group of physical word c * W4 + x. int4: K (x / 2) of the lane's, V x; MXFP4: K x, V half-words 2 x, 2 x + 1
-                    uint4 v;
-                    if (FMT == FMT_Q4) {
-                        const int g = isv ? x % NG : (x >> 1) % NG;
-                        v = pr_word<FMT>(code[i][x], s2[g], b2[g]);
-                    } else {
-                        const int g = isv ? (2 * x) % NG : x % NG, g1 = isv ? (2 * x + 1) % NG : g;
-                        v = pr_word<FMT>(code[i][x], s2[g], s2[g1]);
-                    }
-                    const int u = c * W4 + x;
-                    *reinterpret_cast<uint4 *>(dst + (u >> 3) * 16384 + row * 128 + (((u & 7) ^ (row & 7)) << 4)) = v;
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-        };
-        pages(k0);
-        fetch(k0);
-        pages(k0 + 1);
-        uint32_t vlim = 0;
-        float vmul = 1.f, vun = 1.f;
-        bool ok = true;
-        for (int j = 0; j < nk; ++j) {  // a warp that gave up still comes to the barrier
-            const int st = j % NST;
-            const unsigned ph = (j / NST + 1) & 1;
-            hole_now = hole_next;
-            // the tile's largest magnitudes, NaN groups of V
-            uint32_t tk = 0, tv = 0;
-            unsigned nan[4], any = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float s[NG], bb[NG];
-                unsigned drop;
-                params(kp[i], s, bb);
-                tk = max(tk, pr_top<FMT, NG>(s, bb, drop));
-                params(vp[i], s, bb);
-                tv = max(tv, pr_top<FMT, NG>(s, bb, nan[i]));
-                any |= nan[i];
-            }
-            tk = __reduce_max_sync(0xffffffffu, tk);
-            tv = __reduce_max_sync(0xffffffffu, tv);
-            if (lane == 0) {
-                sh.mx[j & 1][w][0] = tk;
-                sh.mx[j & 1][w][1] = tv;
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                tk = max(tk, sh.mx[j & 1][i][0]);
-                tv = max(tv, sh.mx[j & 1][i][1]);
-            }
-            // ---- K
-            if (ok && j >= NST && !__all_sync(0xffffffffu, pr_wait(sh.kempty + st, ph, &sh.fail))) ok = false;
-            if (ok) {
-                const uint32_t e = min(max(tk >> 23, 9u), 254u);
-                dequant(sm + L::OFF_K + st * L::TILE, kc, kp, __uint_as_float((262u - e) << 23), false);
-                if (w == 0 && lane == 0) sh.kmul[j & 3] = __uint_as_float((e - 8u) << 23);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    unsigned x = __ballot_sync(0xffffffffu, (hole_now >> i) & 1u) & 0x11111111u;
-                    x = (x | x >> 3) & 0x03030303u;
-                    x = (x | x >> 6) & 0x000F000Fu;
-                    x = (x | x >> 12) & 0xFFu;
-                    if (lane == 0) reinterpret_cast<uint8_t *>(sh.hole[j & 3])[4 * i + w] = (uint8_t)x;
-                    if (lane == 0 && x) atomicOr(a.c.err, ERR_PAGE);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sh.kfull + st);
-                // ---- V
-                if (j >= NST && !__all_sync(0xffffffffu, pr_wait(sh.vempty + st, ph, &sh.fail))) ok = false;
-            }
-            if (ok) {
-                float fix = 1.f;
-                if (tv > vlim) {
-                    const uint32_t e = min(max(tv >> 23, 9u), 248u);
-                    const float nm = __uint_as_float((262u - e) << 23);
-                    fix = nm * vun;
-                    vmul = nm;
-                    vun = __uint_as_float((e - 8u) << 23);
-                    vlim = (e + 6u) << 23;
-                }
-                dequant(sm + L::OFF_V + st * L::TILE, vc, vp, vmul, true);
-                const bool anyw = __any_sync(0xffffffffu, any != 0);
-                if (anyw && c == 0) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sh.pm[st][32 * i + 8 * w + r] = (uint8_t)nan[i];
-                }
-                if (lane == 0) {
-                    reinterpret_cast<uint8_t *>(&sh.pz[st])[w] = anyw;
-                    if (w == 0) {
-                        sh.vfix[st] = fix;
-                        sh.vun = vun;
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sh.vfull + st);
-                if (j + 1 < nk) {
-                    fetch(k0 + j + 1);
-                    pages(k0 + j + 2);
-                }
-            }
-        }
-        if (!ok && lane == 0) {
-            atomicOr(a.c.err, ERR_TIMEOUT);
-            *reinterpret_cast<volatile int *>(&sh.fail) = 1;
-        }
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        // ------------------------------------------------------------ codes -> fp16 tiles, K or V
+        pr_feed<FMT, D>(a, sh, sm, keys, b, h, k0, nk, pmax, Lk, warp & 3, lane, warp >= 12);
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         // ------------------------------------------------------------ softmax of row tile t, a thread per row
-        const int t = warp >> 2;
+        const int t = warp >> 2, row = (warp & 3) * 32 + lane, R = R0 + t * 128 + row;
+        const bool have = R < NR;
+        const int ri = R / a.Gq, pos = have ? p0 + ri : -1, row_t = have ? r0 + ri : 0, row_h = h * a.Gq + R - ri * a.Gq;
+        const float qmul = sh.qmul[t * 128 + row];
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + L::S0 + 128 * t, to = tmem + lanes + D * t;
         const int q0 = R0 + t * 128;
         const int tmin = p0 + q0 / a.Gq, tmax = p0 + (min(q0 + 128, NR) - 1) / a.Gq;  // positions of the tile's rows
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f, sc = 0.f, vfix = 1.f;
         unsigned poison = 0;
         bool ok = true;
-        for (int j = 0; j < nk; ++j) {
-            const int st = j % NST, j0 = pr_tok(keys, k0 + j);
-            if (!__all_sync(0xffffffffu, pr_wait(sh.sfull + t, j & 1, &sh.fail))) { ok = false; break; }
+        for (int jh = 0; jh < 2 * nk; ++jh) {
+            const int j = jh >> 1, i2 = jh & 1, st = j % NST, j0 = pr_tok(keys, k0 + j) + 64 * i2;
+            if (!__all_sync(0xffffffffu, pr_wait(&sh.sfull[t][i2], j & 1, &sh.fail))) { ok = false; break; }
             fence_after();
-            const float sc = fmaxf(qmul * sh.kmul[j & 3], 1.2e-38f);  // above zero: a hidden score of -inf stays -inf
-            const unsigned h0 = sh.hole[j & 3][0], h1 = sh.hole[j & 3][1], h2m = sh.hole[j & 3][2], h3 = sh.hole[j & 3][3];
-            const bool full = j0 + 127 <= tmin && (!a.window || j0 > tmax - a.window || j0 + 127 < a.sinks) && !(h0 | h1 | h2m | h3);
-            const int ce = pos - j0, we = a.window ? pos - a.window + 1 - j0 : -1, se = a.sinks - j0;
-            auto mask = [&](float (&v)[64], int half) {
-#pragma unroll
-                for (int i = 0; i < 64; ++i) {
-                    const int e = half * 64 + i;
-                    const unsigned hw = half ? (i < 32 ? h2m : h3) : (i < 32 ? h0 : h1);
-                    const bool vis = e <= ce && (e >= we || e < se) && !((hw >> (i & 31)) & 1u);
-                    v[i] = vis ? v[i] : -INFINITY;
-                }
-            };
-            auto top = [&](const float (&v)[64]) {
-                float x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
-#pragma unroll
-                for (int i = 4; i < 64; i += 4) {
-                    x0 = fmaxf(x0, v[i]);
-                    x1 = fmaxf(x1, v[i + 1]);
-                    x2 = fmaxf(x2, v[i + 2]);
-                    x3 = fmaxf(x3, v[i + 3]);
-                }
-                return fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
-            };
-            // the row's maximum: keys 0 .. 63, then 64 .. 127, which stay in registers
             float v[64];
-            ld32(ts, v);
-            ld32(ts + 32, v + 32);
-            wait_ld();
-            if (!full) mask(v, 0);
-            float mt = top(v);
-            ld32(ts + 64, v);
-            ld32(ts + 96, v + 32);
-            wait_ld();
-            if (!full) mask(v, 1);
-            mt = fmaxf(mt, top(v)) * sc;
-            if (!(mt > -INFINITY)) mt = -INFINITY;  // every score a NaN: the weights and the row become NaN
-            // V's stage: its power of two, its NaN groups
-            if (!__all_sync(0xffffffffu, pr_wait(sh.vfull + st, (j / NST) & 1, &sh.fail))) { ok = false; break; }
-            const float vfix = sh.vfix[st];
-            if (const unsigned pz = sh.pz[st]) {
-                for (int e = 0; e < 128; ++e) {
-                    if (!((pz >> (8 * ((e >> 3) & 3))) & 1u)) continue;
-                    const unsigned g = sh.pm[st][e];
-                    if (g && e <= ce && (e >= we || e < se)) poison |= g;
+            ld32(ts + 64 * i2, v);
+            ld32(ts + 64 * i2 + 32, v + 32);
+            const int ce = pos - j0, we = a.window ? pos - a.window + 1 - j0 : -1, se = a.sinks - j0;
+            if (i2 == 0) {
+                sc = fmaxf(qmul * sh.kmul[j & 3], 1.2e-38f);  // above zero: a hidden score of -inf stays -inf
+                // V's stage: its power of two, its NaN groups
+                if (!__all_sync(0xffffffffu, pr_wait(sh.vfull + st, (j / NST) & 1, &sh.fail))) { ok = false; break; }
+                vfix = sh.vfix[st];
+                if (const unsigned pz = sh.pz[st]) {
+                    for (int e = 0; e < 128; ++e) {
+                        if (!((pz >> (8 * ((e >> 3) & 3))) & 1u)) continue;
+                        const unsigned g = sh.pm[st][e];
+                        if (g && e <= ce && (e >= we || e < se)) poison |= g;
+                    }
+                    __syncwarp();
                 }
             }
+            const unsigned h0 = sh.hole[j & 3][2 * i2], h1 = sh.hole[j & 3][2 * i2 + 1];
+            const bool full = j0 + 63 <= tmin && (!a.window || j0 > tmax - a.window || j0 + 63 < a.sinks) && !(h0 | h1);
+            wait_ld();
+            if (!full) {
+                // bit i: this row sees key i of the half
+                const unsigned long long see = pr_below(ce + 1) & (~pr_below(we) | pr_below(se)) & ~((unsigned long long)h1 << 32 | h0);
+                const unsigned s0 = (unsigned)see, s1 = (unsigned)(see >> 32);
+#pragma unroll
+                for (int i = 0; i < 64; ++i) v[i] = (i < 32 ? s0 >> i : s1 >> (i - 32)) & 1u ? v[i] : -INFINITY;
+            }
+            float x0 = fmaxf(v[0], v[1]), x1 = fmaxf(v[2], v[3]), x2 = fmaxf(v[4], v[5]), x3 = fmaxf(v[6], v[7]);
+#pragma unroll
+            for (int i = 8; i < 64; i += 8) {
+                x0 = fmaxf(x0, fmaxf(v[i], v[i + 1]));
+                x1 = fmaxf(x1, fmaxf(v[i + 2], v[i + 3]));
+                x2 = fmaxf(x2, fmaxf(v[i + 4], v[i + 5]));
+                x3 = fmaxf(x3, fmaxf(v[i + 6], v[i + 7]));
+            }
+            float mt = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * sc;
+            if (!(mt > -INFINITY)) mt = -INFINITY;  // every score a NaN: the weights and the row become NaN
             // rescale O when a maximum grew far, or V's power of two changed
             float f = 1.f;
             if (mt > m + P_LAZY || (m == -INFINITY && mt > m)) {
@@ -628,44 +665,46 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
                 m = mt;
                 l *= f;
             }
-            if (j > 0 && __any_sync(0xffffffffu, f != 1.f || vfix != 1.f)) {
+            if (jh > 0 && __any_sync(0xffffffffu, f != 1.f || vfix != 1.f)) {
+                if (!__all_sync(0xffffffffu, pr_wait(sh.pv + t, (jh - 1) & 1, &sh.fail))) { ok = false; break; }
+                fence_after();
                 const float ff = f * vfix;
-#pragma unroll
-                for (int x = 0; x < D; x += 32) {
-                    float o[32];
-                    ld32(to + x, o);
+#pragma unroll 1
+                for (int x = 0; x < D; x += 16) {
+                    float o[16];
+                    ld16(to + x, o);
                     wait_ld();
-                    uint32_t u[32];
+                    uint32_t u[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * ff);
-                    st32(to + x, u);
+                    for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * ff);
+                    st16(to + x, u);
                 }
             }
+            vfix = 1.f;
             const float off = m == -INFINITY ? 0.f : P_OFF - m;
-            // weights: keys 64 .. 127 to columns 96 .., then 0 .. 63 to columns 64 .. (S's upper half, both read by then)
-            float l0 = 0.f, l1 = 0.f;
-            auto weights = [&](const float (&s)[64], uint32_t col) {
-                uint32_t u[32];
+            const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+            uint64_t l2 = pair(l, 0.f);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float x = ex2p(fmaf(s[2 * i], sc, off)), y = ex2p(fmaf(s[2 * i + 1], sc, off));
-                    l0 += x;
-                    l1 += y;
+            for (int q = 0; q < 2; ++q) {
+                uint32_t u[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float x, y;
+                    unpair(fma2(pair(v[32 * q + 2 * i], v[32 * q + 2 * i + 1]), sc2, off2), x, y);
+                    x = ex2p(x);
+                    y = ex2p(y);
+                    l2 = add2(l2, pair(x, y));
                     u[i] = h2(x, y);
                 }
-                st32(ts + col, u);
-            };
-            weights(v, 96);
-            ld32(ts, v);
-            ld32(ts + 32, v + 32);
-            wait_ld();
-            if (!full) mask(v, 0);
-            weights(v, 64);
+                st16(ts + 64 * i2 + 16 * q, u);
+            }
+            float la, lb;
+            unpair(l2, la, lb);
+            l = la + lb;
             wait_st();
-            l += l0 + l1;
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(sh.pfull + t);
+            if (lane == 0) mbar_arrive(&sh.pfull[t][i2]);
         }
         if (nk > 0 && !__all_sync(0xffffffffu, pr_wait(sh.ofull + t, 0, &sh.fail))) ok = false;
         fence_after();
@@ -676,7 +715,6 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         // ---- the rows' results (m is off by P_OFF against the weights' sum: undone here)
         const float M = m == -INFINITY ? m : m - P_OFF;
         float mul = nk > 0 ? sh.vun : 0.f, Ls = l, sum_m = M;
-        const bool have = R0 + t * 128 + (warp & 3) * 32 + lane < NR;
         if (!part) {
             if (a.sink_logits && have) {
                 const float s = a.sink_logits[row_h] * 1.4426950408889634f, N = fmaxf(M, s), use = N == -INFINITY ? 0.f : N;
@@ -688,6 +726,8 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             mul = Ls == 0.f ? 0.f : mul / Ls;
         }
         const size_t orow = (size_t)row_t * a.H + row_h;
+        // bf16 rows go through the tile's place of Q (its products are over), so that the stores are whole lines.
+        unsigned char *stage = sm + t * L::TILE + (warp & 3) * (32 * D * 2);
         float *pd = part ? part + ((size_t)sp * a.s.T * a.H + orow) * D : nullptr;
 #pragma unroll
         for (int x = 0; x < D; x += 32) {
@@ -699,27 +739,33 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = 0.f;
             }
-            if (have) {
-            // int4: physical word u of V is word u / G of group u % G; MXFP4: half-word u of 4 values, u / H of group u % H
-            constexpr int ST = FMT == FMT_Q4 ? 8 : 4;
 #pragma unroll
-            for (int i = 0; i < 32; i += ST) {
-                const int u = (x + i) / ST, g = u % NG, dim = FMT == FMT_Q4 ? 64 * g + 8 * (u / NG) : 32 * g + 4 * (u / NG);
-                float y[ST];
+            for (int i = 0; i < 32; i += 4) {
+                const int d = pr_dim<FMT, D>((x + i) / 4), g = d / (FMT == FMT_Q4 ? 64 : 32);
+                float y[4];
                 const bool nanv = (poison >> g) & 1u;
 #pragma unroll
-                for (int e = 0; e < ST; ++e) y[e] = nanv ? __uint_as_float(0x7fffffffu) : mul == 0.f && l == 0.f ? 0.f : o[i + e] * mul;
-                if (part) {
-#pragma unroll
-                    for (int e = 0; e < ST; e += 4) *reinterpret_cast<float4 *>(pd + dim + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < ST; e += 4)
-                        *reinterpret_cast<uint2 *>(a.y + orow * D + dim + e) = make_uint2(pack_bf2(y[e], y[e + 1]), pack_bf2(y[e + 2], y[e + 3]));
+                for (int e = 0; e < 4; ++e) y[e] = nanv ? __uint_as_float(0x7fffffffu) : mul == 0.f && l == 0.f ? 0.f : o[i + e] * mul;
+                if (!part) {
+                    *reinterpret_cast<uint2 *>(stage + lane * (D * 2) + (((d >> 3) ^ (lane & 7)) << 4) + (d & 4) * 2) =
+                        make_uint2(pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]));
+                } else if (have) {
+                    *reinterpret_cast<float4 *>(pd + d) = make_float4(y[0], y[1], y[2], y[3]);
                 }
             }
-            }
             __syncwarp();
+        }
+        if (!part) {
+            constexpr int LR = D / 8, RW = 32 / LR;
+#pragma unroll 4
+            for (int i = 0; i < 32; i += RW) {
+                const int rr = i + lane / LR, x = lane % LR, Rr = R0 + t * 128 + (warp & 3) * 32 + rr;
+                if (Rr < NR) {
+                    const int ri2 = Rr / a.Gq;
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * (D * 2) + ((x ^ (rr & 7)) << 4));
+                    *reinterpret_cast<uint4 *>(a.y + ((size_t)(r0 + ri2) * a.H + h * a.Gq + Rr - ri2 * a.Gq) * D + 8 * x) = v;
+                }
+            }
         }
         if (have) {
             if (part) reinterpret_cast<float2 *>(part + (size_t)ns * a.s.T * a.H * D)[(size_t)sp * a.s.T * a.H + orow] = make_float2(M, l);
@@ -728,7 +774,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         fence_before();
     }
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         __syncwarp();
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");

@@ -369,7 +369,7 @@ class KVCache:
         self.kq, self.vq = (torch.zeros(*rows, head_dim // 8, dtype=torch.int32, device=device) for _ in range(2))
         self.ks, self.vs = (torch.zeros(*rows, par[0], dtype=par[1], device=device) for _ in range(2))
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
-        self.device = self.kq.device
+        self.device, self.index, self._ws_bytes = self.kq.device, self.kq.get_device(), {}
         self._c = ctypes.pointer(_lib.KvCacheStruct(
             *(t.data_ptr() for t in (self.kq, self.ks, self.vq, self.vs, self.err)), pages, page_size, kv_heads, head_dim,
             _lib.KV_Q4 if fmt == "q4" else _lib.KV_MXFP4))
@@ -382,61 +382,70 @@ class KVCache:
         return out.value
 
 
-def _kv_ints(t, name, cache, size=None):
+# The checks of these calls are written for the good case: a decode step makes them for every layer, so each tensor is asked
+# once for what it has, and the reason is looked for only when something is wrong.
+_BF16, _I32 = torch.bfloat16, torch.int32
+
+
+def _kv_ints(t, name, cache, size):
     if t is None:
         return None
-    _need(t, torch.int32, name)
-    if t.device != cache.device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    if t.dim() != 1 or (size is not None and t.shape[0] != size):
-        raise ValueError(f"{name} must be int32 [{size}], got {tuple(t.shape)}")
+    if t.dtype != _I32 or t.get_device() != cache.index or t.shape != (size,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 [{size}] tensor on {cache.device} (a CUDA device), got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _kv_table(table, cache):
-    if not table.is_cuda or table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be a CUDA int32 [sequences, pages] tensor with contiguous rows")
-    if table.device != cache.device:
-        raise ValueError(f"table is on {table.device}, the cache on {cache.device}")
+    if table.dtype != _I32 or table.get_device() != cache.index or table.dim() != 2:
+        raise ValueError(f"table must be an int32 [sequences, pages] tensor on {cache.device} (a CUDA device), got {table.dtype} "
+                         f"{tuple(table.shape)} on {table.device}")
     B, P = table.shape
-    if B > 1 and table.stride(0) < P:
-        raise ValueError("table rows overlap")
-    return table.data_ptr(), max(table.stride(0), P), B, P
+    row, one = table.stride()
+    if (P > 1 and one != 1) or (B > 1 and row < P):
+        raise ValueError("table must have contiguous rows that do not overlap")
+    return table.data_ptr(), max(row, P), B, P
 
 
 def _kv_rows(t, name, cache, heads=None):
-    if not t.is_cuda or t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != cache.head_dim:
-        raise ValueError(f"{name} must be a CUDA bfloat16 [rows, heads, {cache.head_dim}] tensor, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}")
-    if t.device != cache.device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    if heads is not None and t.shape[1] != heads:
-        raise ValueError(f"{name} has {t.shape[1]} heads, the cache {heads}")
-    r, h, one = t.stride()
-    if one != 1 or r % 8 or h % 8 or t.data_ptr() % 16:
+    if t.dtype != _BF16 or t.get_device() != cache.index or t.dim() != 3:
+        raise ValueError(f"{name} must be a bfloat16 [rows, heads, {cache.head_dim}] tensor on {cache.device} (a CUDA device), "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    T, H, D = t.shape
+    if D != cache.head_dim:
+        raise ValueError(f"{name} has rows of {D} values, the cache of {cache.head_dim}")
+    if heads is not None and H != heads:
+        raise ValueError(f"{name} has {H} heads, the cache {heads}")
+    row, head, one = t.stride()
+    ptr = t.data_ptr()
+    if one != 1 or row % 8 or head % 8 or ptr % 16:
         raise ValueError(f"{name} must have contiguous values, row and head strides that are multiples of 8, and a 16-byte "
                          f"aligned start")
-    return t.data_ptr(), r, h
+    return ptr, row, head, T, H
 
 
-def _kv_out(t, name, shape, dtype, device):
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous() or t.data_ptr() % 16:
-        raise ValueError(f"{name} must be a contiguous, 16-byte aligned {dtype} {tuple(shape)} tensor on {device}")
+def _kv_out(t, name, shape, cache):
+    if t.dtype != _BF16 or t.shape != shape or t.get_device() != cache.index or not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"{name} must be a contiguous, 16-byte aligned bfloat16 {tuple(shape)} tensor on {cache.device}")
     return t
 
 
 def _kv_call(cache, name, *args):
     """The call on the cache's device and that device's current stream."""
-    if cache.device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    i = cache.index
+    stream = torch._C._cuda_getCurrentRawStream(i)
+    if i == torch.cuda.current_device():
+        _lib.call(name, *args, stream)
     else:
-        with torch.cuda.device(cache.device):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(i):
+            _lib.call(name, *args, stream)
 
 
 def _kv_cu(cu, T, B, cache):
-    if cu is None and B and T % B:
-        raise ValueError(f"{T} rows for {B} sequences: give cu, or the same number of rows for each")
+    if cu is None:
+        if B and T % B:
+            raise ValueError(f"{T} rows for {B} sequences: give cu, or the same number of rows for each")
+        return None
     return _kv_ints(cu, "cu", cache, B + 1)
 
 
@@ -445,13 +454,13 @@ def kv_write(cache, k, v, table, lens, cu=None):
     into the cache. table int32 [B, P]: page ids of each sequence; lens int32 [B]: its tokens, these included; cu int32
     [B + 1]: sequence b has rows cu[b] .. cu[b + 1] - 1 (None: T / B rows each), its last ones. Rows behind the last
     sequence are passed over; a token without a valid page is dropped and sets DEVERR_PAGE (cache.read_error())."""
-    kp, vp = _kv_rows(k, "k", cache, cache.kv_heads), _kv_rows(v, "v", cache, cache.kv_heads)
-    T = k.shape[0]
-    if v.shape[0] != T:
-        raise ValueError(f"k has {T} rows, v {v.shape[0]}")
+    kp, krow, khead, T, _ = _kv_rows(k, "k", cache, cache.kv_heads)
+    vp, vrow, vhead, Tv, _ = _kv_rows(v, "v", cache, cache.kv_heads)
+    if Tv != T:
+        raise ValueError(f"k has {T} rows, v {Tv}")
     tp, trow, B, P = _kv_table(table, cache)
-    _kv_call(cache, "moeb_kv_write", cache._c, *kp, *vp, T, _kv_cu(cu, T, B, cache), _kv_ints(lens, "lens", cache, B), tp,
-             trow, B, P)
+    _kv_call(cache, "moeb_kv_write", cache._c, kp, krow, khead, vp, vrow, vhead, T, _kv_cu(cu, T, B, cache),
+             _kv_ints(lens, "lens", cache, B), tp, trow, B, P)
 
 
 def kv_read(cache, table, cu, rows, first=None, out=None):
@@ -465,7 +474,7 @@ def kv_read(cache, table, cu, rows, first=None, out=None):
         new = torch.empty if cu is None else torch.zeros
         k, v = (new(shape, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
     else:
-        k, v = (_kv_out(t, "out", shape, torch.bfloat16, cache.device) for t in out)
+        k, v = (_kv_out(t, "out", shape, cache) for t in out)
     _kv_call(cache, "moeb_kv_read", cache._c, rows, cp, fp, tp, trow, B, P, k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -479,8 +488,8 @@ def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=
     bound picks the better kernels). scale: of the scores (None: head_dim ** -0.5). out: y to fill, whose rows behind the
     last sequence are left as they were; without it those rows are zero. Returns y bf16 [T, H, head_dim] (and, with
     return_lse, the fp32 [T, H] logarithm of each softmax's sum). A row that sees nothing is zero (lse -inf)."""
-    qp = _kv_rows(q, "q", cache)
-    T, H, D = q.shape
+    qp, qrow, qhead, T, H = _kv_rows(q, "q", cache)
+    D = cache.head_dim
     tp, trow, B, P = _kv_table(table, cache)
     cp, lp = _kv_cu(cu, T, B, cache), _kv_ints(lens, "lens", cache, B)
     if H == 0 or H % cache.kv_heads:
@@ -495,12 +504,17 @@ def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=
     if T and max_q <= 0:
         raise ValueError("max_q must be positive")
     new = torch.empty if cu is None else torch.zeros
-    y = new((T, H, D), dtype=torch.bfloat16, device=cache.device) if out is None else \
-        _kv_out(out, "out", (T, H, D), torch.bfloat16, cache.device)
+    y = new((T, H, D), dtype=_BF16, device=cache.device) if out is None else _kv_out(out, "out", (T, H, D), cache)
     lse = torch.full((T, H), -float("inf"), device=cache.device) if return_lse else None
-    nbytes = _lib.load().moeb_kv_attention_workspace_bytes(T, B, H, cache.kv_heads, D, max_q)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
-    _kv_call(cache, "moeb_kv_attention", cache._c, *qp, T, H, cp, lp, tp, trow, B, P, max_q,
+    key = (T, B, H, max_q)
+    nbytes = cache._ws_bytes.get(key)
+    if nbytes is None:
+        if len(cache._ws_bytes) > 4096:
+            cache._ws_bytes.clear()
+        with torch.cuda.device(cache.index):
+            nbytes = cache._ws_bytes[key] = _lib.load().moeb_kv_attention_workspace_bytes(T, B, H, cache.kv_heads, D, max_q)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None  # of this call alone
+    _kv_call(cache, "moeb_kv_attention", cache._c, qp, qrow, qhead, T, H, cp, lp, tp, trow, B, P, max_q,
              D ** -0.5 if scale is None else float(scale), int(window), int(sinks),
              None if sink_logits is None else sink_logits.data_ptr(), y.data_ptr(), None if lse is None else lse.data_ptr(),
              None if ws is None else ws.data_ptr(), nbytes)

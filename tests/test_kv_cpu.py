@@ -93,7 +93,7 @@ def test_python_checks():
         ops.KVCache(4, 2, 64, device="cpu")
 
     class Fake:
-        device, kv_heads, head_dim = torch.device("cuda", 0), 2, 64
+        device, index, kv_heads, head_dim = torch.device("cuda", 0), 0, 2, 64
     cpu = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA"):
         ops.kv_write(Fake, cpu, cpu, torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32))
