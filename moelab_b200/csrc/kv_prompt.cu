@@ -46,9 +46,11 @@ struct Pr {
 struct PrShared {
     uint64_t kfull[3], kempty[3], vfull[3], vempty[3], sfull[2][2], pfull[2][2], pv[2], ofull[2];  // [row tile][half]
     float kmul[4];             // by key tile % 4: 2^e of the K tile
-    unsigned hole[4][4];       // by key tile % 4: keys without a page
-    float vfix[3];             // by stage: what O is multiplied by before this V tile
-    unsigned pz[3];            // by stage: byte per dequantizing warp, a NaN group among its rows
+    unsigned holes[4], hole[4][4];  // by key tile % 4: byte per feeding warp, keys without a page among its own; those keys
+    struct {
+        float fix;             // what O is multiplied by before this V tile
+        unsigned pz;           // byte per feeding warp, a NaN group among its rows
+    } v[3];                    // by stage
     uint8_t pm[3][128];        // by stage and key: its NaN groups
     unsigned mx[2][2][4];      // exchange of the tiles' largest magnitudes: K or V, tile % 2, warp
     float qmul[PR];            // the rows' scale
@@ -61,6 +63,11 @@ MOEB_DEV float ex2p(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+MOEB_DEV float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
 }
 MOEB_DEV uint32_t h2(float lo, float hi) {
     uint32_t r;
@@ -92,13 +99,15 @@ MOEB_DEV uint32_t hfma2u(uint32_t a, uint32_t b, uint32_t c) {
     const __half2 r = __hfma2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b), *reinterpret_cast<__half2 *>(&c));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-// Waits for a phase, at most 2 s of wall time or until another role has given up.
-MOEB_DEV bool pr_wait(uint64_t *bar, unsigned parity, const int *fail) {
-    if (mbar_try_wait(bar, parity)) return true;
+// Waits for a phase, at most 2 s of wall time. After that `fail` is set and every later wait returns at once: all roles go
+// through their loops to the end (every address stays in bounds), so that none is left behind and TMEM is released.
+MOEB_DEV void pr_wait(uint64_t *bar, unsigned parity, int *fail) {
+    if (mbar_try_wait(bar, parity)) return;
     const uint64_t t0 = globaltimer_ns();
-    for (unsigned i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 31u) == 0 && (*reinterpret_cast<const volatile int *>(fail) || globaltimer_ns() - t0 > 2000000000ull)) return false;
+    for (unsigned i = 1; !mbar_try_wait(bar, parity); ++i) {
+        if (i & 31u) continue;
+        if (*reinterpret_cast<volatile int *>(fail)) return;
+        if (globaltimer_ns() - t0 > 2000000000ull) *reinterpret_cast<volatile int *>(fail) = 1;
     }
 }
 // 128-byte swizzled operand descriptors: 8 rows of 128 bytes every 1024; LBO: bytes between 64-element chunks of an MN-major
@@ -290,11 +299,10 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
     fetch_codes(0, id);
     uint32_t vlim = 0;  // V: bits of the largest value that the running power of two takes; that power, its inverse
     float vmul = 1.f, vun = 1.f;
-    bool ok = true;
     int st = 0;
     unsigned ph = 1;
 #pragma unroll 1
-    for (int j = 0; j < nk; ++j) {  // a warp that gave up still comes to the barrier
+    for (int j = 0; j < nk; ++j) {
         // ---- this lane's key: the largest magnitude its parameters allow, its NaN groups
         float s[NG], bb[NG];
 #pragma unroll
@@ -314,8 +322,8 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
         if (lane == 0) mx[w] = top;
         asm volatile("bar.sync %0, 128;" ::"r"(V ? 2 : 1) : "memory");
         top = max(max(mx[0], mx[1]), max(mx[2], mx[3]));
-        if (ok && j >= NST && !__all_sync(0xffffffffu, pr_wait(empty + st, ph, &sh.fail))) ok = false;
-        if (ok) {
+        if (j >= NST) pr_wait(empty + st, ph, &sh.fail);
+        {
             // ---- the tile's power of two
             float mul, fix = 1.f;
             if (!V || top > vlim) {
@@ -357,9 +365,9 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
                 const bool any = __any_sync(0xffffffffu, nan != 0);
                 if (any) sh.pm[st][mine] = (uint8_t)nan;
                 if (lane == 0) {
-                    reinterpret_cast<uint8_t *>(&sh.pz[st])[w] = any;
+                    reinterpret_cast<uint8_t *>(&sh.v[st].pz)[w] = any;
                     if (w == 0) {
-                        sh.vfix[st] = fix;
+                        sh.v[st].fix = fix;
                         sh.vun = vun;
                     }
                 }
@@ -372,7 +380,10 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
                     reinterpret_cast<uint8_t *>(sh.hole[j & 3])[4 * lane + w] = (uint8_t)x;
                     if (x) atomicOr(a.c.err, ERR_PAGE);
                 }
-                if (w == 0 && lane == 0) sh.kmul[j & 3] = vun;
+                if (lane == 0) {
+                    reinterpret_cast<uint8_t *>(&sh.holes[j & 3])[w] = hole != 0;
+                    if (w == 0) sh.kmul[j & 3] = vun;
+                }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(full + st);
@@ -382,10 +393,6 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
             st = 0;
             ph ^= 1;
         }
-    }
-    if (!ok && lane == 0) {
-        atomicOr(a.c.err, ERR_TIMEOUT);
-        *reinterpret_cast<volatile int *>(&sh.fail) = 1;
     }
 }
 
@@ -402,10 +409,9 @@ MOEB_DEV void pr_products(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, 
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_, 0), base = __shfl_sync(0xffffffffu, smem_u32(sm), 0);
     const uint32_t ds = tmem + L::S0 + 128 * T, dout = tmem + D * T;
     const uint32_t qa = desc_lo<16>(base + T * L::TILE), ka0 = desc_lo<16>(base + L::OFF_K), va0 = desc_lo<16384>(base + L::OFF_V);
-    bool ok = true;
     // S of half i of key tile j (stage st, phase ph); the last product of K's stage frees it
     auto scores = [&](int st, unsigned ph, int i) {
-        if (i == 0 && !__all_sync(0xffffffffu, pr_wait(sh.kfull + st, ph, &sh.fail))) return false;
+        if (i == 0) pr_wait(sh.kfull + st, ph, &sh.fail);
         fence_after();
         const uint32_t ka = ka0 + (st * L::TILE + i * 8192) / 16;
         if (elect()) {
@@ -418,18 +424,18 @@ MOEB_DEV void pr_products(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, 
             if (i) commit(sh.kempty + st);
         }
         __syncwarp();
-        return true;
     };
-    ok = scores(0, 0, 0) && scores(0, 0, 1);
+    scores(0, 0, 0);
+    scores(0, 0, 1);
     int st = 0, sn = NST > 1 ? 1 : 0;  // stage of this tile and of the next, with their phases
     unsigned ph = 0, pn = 0;
-    for (int j = 0; j < nk && ok; ++j) {
+#pragma unroll 1
+    for (int j = 0; j < nk; ++j) {
         const uint32_t va = va0 + st * (L::TILE / 16);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (i == 0) ok = __all_sync(0xffffffffu, pr_wait(sh.vfull + st, ph, &sh.fail));
-            ok = ok && __all_sync(0xffffffffu, pr_wait(&sh.pfull[T][i], j & 1, &sh.fail));
-            if (!ok) break;
+            if (i == 0) pr_wait(sh.vfull + st, ph, &sh.fail);
+            pr_wait(&sh.pfull[T][i], j & 1, &sh.fail);
             fence_after();
             if (elect()) {
 #pragma unroll
@@ -439,8 +445,7 @@ MOEB_DEV void pr_products(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, 
                 if (i) commit(sh.vempty + st);
             }
             __syncwarp();
-            if (j + 1 < nk) ok = scores(sn, pn, i);
-            if (!ok) break;
+            if (j + 1 < nk) scores(sn, pn, i);
         }
         st = sn;
         ph = pn;
@@ -449,16 +454,10 @@ MOEB_DEV void pr_products(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, 
             pn ^= 1;
         }
     }
-    if (elect()) {
-        if (!ok) {
-            atomicOr(a.c.err, ERR_TIMEOUT);
-            *reinterpret_cast<volatile int *>(&sh.fail) = 1;
-        }
-        commit(sh.ofull + T);
-    }
+    if (elect()) commit(sh.ofull + T);
     __syncwarp();
-    const int none = 0;
-    pr_wait(sh.ofull + T, 0, &none);  // nothing is in flight when TMEM is released
+    int own = 0;
+    pr_wait(sh.ofull + T, 0, &own);  // nothing is in flight when TMEM is released, after a failure either
 }
 
 }  // namespace
@@ -613,74 +612,88 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         const uint32_t ts = tmem + lanes + L::S0 + 128 * t, to = tmem + lanes + D * t;
         const int q0 = R0 + t * 128;
         const int tmin = p0 + q0 / a.Gq, tmax = p0 + (min(q0 + 128, NR) - 1) / a.Gq;  // positions of the tile's rows
-        float m = -INFINITY, l = 0.f, sc = 0.f, vfix = 1.f;
+        float m = -INFINITY, l = 0.f, sc = 0.f;
         unsigned poison = 0;
-        bool ok = true;
+        int st = 0, j0 = pr_tok(keys, k0);
+        unsigned vph = 0;
+#pragma unroll 1
         for (int jh = 0; jh < 2 * nk; ++jh) {
-            const int j = jh >> 1, i2 = jh & 1, st = j % NST, j0 = pr_tok(keys, k0 + j) + 64 * i2;
-            if (!__all_sync(0xffffffffu, pr_wait(&sh.sfull[t][i2], j & 1, &sh.fail))) { ok = false; break; }
+            const int j = jh >> 1, i2 = jh & 1;
+            pr_wait(&sh.sfull[t][i2], j & 1, &sh.fail);
             fence_after();
             float v[64];
             ld32(ts + 64 * i2, v);
             ld32(ts + 64 * i2 + 32, v + 32);
-            const int ce = pos - j0, we = a.window ? pos - a.window + 1 - j0 : -1, se = a.sinks - j0;
+            float vfix = 1.f;
+            const unsigned holes = sh.holes[j & 3];
             if (i2 == 0) {
                 sc = fmaxf(qmul * sh.kmul[j & 3], 1.2e-38f);  // above zero: a hidden score of -inf stays -inf
                 // V's stage: its power of two, its NaN groups
-                if (!__all_sync(0xffffffffu, pr_wait(sh.vfull + st, (j / NST) & 1, &sh.fail))) { ok = false; break; }
-                vfix = sh.vfix[st];
-                if (const unsigned pz = sh.pz[st]) {
+                pr_wait(sh.vfull + st, vph, &sh.fail);
+                vfix = sh.v[st].fix;
+                if (const unsigned pz = sh.v[st].pz) {
                     for (int e = 0; e < 128; ++e) {
                         if (!((pz >> (8 * ((e >> 3) & 3))) & 1u)) continue;
                         const unsigned g = sh.pm[st][e];
-                        if (g && e <= ce && (e >= we || e < se)) poison |= g;
+                        if (g && e <= pos - j0 && (!a.window || e > pos - a.window - j0 || e < a.sinks - j0)) poison |= g;
                     }
                     __syncwarp();
                 }
             }
-            const unsigned h0 = sh.hole[j & 3][2 * i2], h1 = sh.hole[j & 3][2 * i2 + 1];
-            const bool full = j0 + 63 <= tmin && (!a.window || j0 > tmax - a.window || j0 + 63 < a.sinks) && !(h0 | h1);
+            const bool full = j0 + 63 <= tmin && (!a.window || j0 > tmax - a.window || j0 + 63 < a.sinks) && !holes;
             wait_ld();
             if (!full) {
                 // bit i: this row sees key i of the half
-                const unsigned long long see = pr_below(ce + 1) & (~pr_below(we) | pr_below(se)) & ~((unsigned long long)h1 << 32 | h0);
+                const unsigned long long hole = (unsigned long long)sh.hole[j & 3][2 * i2 + 1] << 32 | sh.hole[j & 3][2 * i2];
+                const unsigned long long old = a.window ? pr_below(pos - a.window + 1 - j0) & ~pr_below(a.sinks - j0) : 0ull;
+                const unsigned long long see = pr_below(pos - j0 + 1) & ~old & ~hole;
                 const unsigned s0 = (unsigned)see, s1 = (unsigned)(see >> 32);
 #pragma unroll
                 for (int i = 0; i < 64; ++i) v[i] = (i < 32 ? s0 >> i : s1 >> (i - 32)) & 1u ? v[i] : -INFINITY;
             }
-            float x0 = fmaxf(v[0], v[1]), x1 = fmaxf(v[2], v[3]), x2 = fmaxf(v[4], v[5]), x3 = fmaxf(v[6], v[7]);
-#pragma unroll
-            for (int i = 8; i < 64; i += 8) {
-                x0 = fmaxf(x0, fmaxf(v[i], v[i + 1]));
-                x1 = fmaxf(x1, fmaxf(v[i + 2], v[i + 3]));
-                x2 = fmaxf(x2, fmaxf(v[i + 4], v[i + 5]));
-                x3 = fmaxf(x3, fmaxf(v[i + 6], v[i + 7]));
+            // the next half's first key, V's stage
+            j0 += 64;
+            if (i2 && ++st == NST) {
+                st = 0;
+                vph ^= 1;
             }
-            float mt = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * sc;
+            if (i2 && k0 + j + 1 == keys.ns) j0 = pr_tok(keys, keys.ns);
+            float x0 = max3(v[0], v[1], v[2]), x1 = max3(v[3], v[4], v[5]), x2 = max3(v[6], v[7], v[8]), x3 = max3(v[9], v[10], v[11]);
+#pragma unroll
+            for (int i = 12; i < 60; i += 8) {
+                x0 = max3(x0, v[i], v[i + 1]);
+                x1 = max3(x1, v[i + 2], v[i + 3]);
+                x2 = max3(x2, v[i + 4], v[i + 5]);
+                x3 = max3(x3, v[i + 6], v[i + 7]);
+            }
+            float mt = max3(max3(x0, v[60], v[61]), max3(x1, v[62], v[63]), fmaxf(x2, x3)) * sc;
             if (!(mt > -INFINITY)) mt = -INFINITY;  // every score a NaN: the weights and the row become NaN
             // rescale O when a maximum grew far, or V's power of two changed
-            float f = 1.f;
-            if (mt > m + P_LAZY || (m == -INFINITY && mt > m)) {
-                f = m == -INFINITY ? 0.f : ex2p(m - mt);
-                m = mt;
-                l *= f;
-            }
-            if (jh > 0 && __any_sync(0xffffffffu, f != 1.f || vfix != 1.f)) {
-                if (!__all_sync(0xffffffffu, pr_wait(sh.pv + t, (jh - 1) & 1, &sh.fail))) { ok = false; break; }
-                fence_after();
-                const float ff = f * vfix;
+            const bool grew = mt > m + P_LAZY;
+            if (__any_sync(0xffffffffu, grew || vfix != 1.f)) {
+                float ff = vfix;
+                if (grew) {
+                    const float f = ex2p(m - mt);
+                    m = mt;
+                    l *= f;
+                    ff *= f;
+                }
+                if (jh > 0) {
+                    pr_wait(sh.pv + t, (jh - 1) & 1, &sh.fail);
+                    fence_after();
 #pragma unroll 1
-                for (int x = 0; x < D; x += 16) {
-                    float o[16];
-                    ld16(to + x, o);
-                    wait_ld();
-                    uint32_t u[16];
+                    for (int x = 0; x < D; x += 16) {
+                        float o[16];
+                        __syncwarp();
+                        ld16(to + x, o);
+                        wait_ld();
+                        uint32_t u[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * ff);
-                    st16(to + x, u);
+                        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * ff);
+                        st16(to + x, u);
+                    }
                 }
             }
-            vfix = 1.f;
             const float off = m == -INFINITY ? 0.f : P_OFF - m;
             const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
             uint64_t l2 = pair(l, 0.f);
@@ -706,12 +719,9 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.pfull[t][i2]);
         }
-        if (nk > 0 && !__all_sync(0xffffffffu, pr_wait(sh.ofull + t, 0, &sh.fail))) ok = false;
+        if (nk > 0) pr_wait(sh.ofull + t, 0, &sh.fail);
         fence_after();
-        if (!ok && lane == 0) {
-            atomicOr(a.c.err, ERR_TIMEOUT);
-            *reinterpret_cast<volatile int *>(&sh.fail) = 1;
-        }
+        __syncwarp();
         // ---- the rows' results (m is off by P_OFF against the weights' sum: undone here)
         const float M = m == -INFINITY ? m : m - P_OFF;
         float mul = nk > 0 ? sh.vun : 0.f, Ls = l, sum_m = M;
@@ -774,6 +784,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         fence_before();
     }
     __syncthreads();
+    if (threadIdx.x == 0 && sh.fail) atomicOr(a.c.err, ERR_TIMEOUT);
     if (warp == 16) {
         __syncwarp();
         fence_after();
