@@ -1,9 +1,34 @@
-// Writing K and V rows into the 4-bit cache, and reading them back (layout: kv.cuh). Both are one pass over memory:
-// one thread per code word (8 values: a 16-byte load or store of bf16), the lanes of a group (8 for int4's 64 values, 4
-// for MXFP4's 32) reduce its extremes by shuffles.
+// Writing K and V rows into the 4-bit cache, and reading them back (layout: kv.cuh). Both are one pass over memory. A thread
+// has what one lane of the cache's readers has: the same word of every group of a row (int4: 1 / 8 of the row, MXFP4: 1 / 4),
+// so that its codes are one load or store and the page arithmetic is done once for all of them; and KV_U tokens of one head,
+// so that as many loads are in flight. The lanes of a group reduce its extremes by shuffles.
 #include "kv.cuh"
 
 namespace moeb {
+
+constexpr int KV_U = 4;
+template <int FMT, int D>
+struct Wd {
+    static constexpr int LR = FMT == FMT_Q4 ? 8 : 4;  // lanes per row, = words of 8 values in a group
+    static constexpr int NG = D / (8 * LR);           // groups in a row, = words per lane
+    static constexpr int R = 128 / LR;                // rows per CTA and pass
+};
+template <int N>
+struct Vec { using T = uint32_t; };
+template <>
+struct Vec<2> { using T = uint2; };
+template <>
+struct Vec<4> { using T = uint4; };
+// physical codes of a lane <-> its words (values 8 (LR g + w) .. of group g): int4 as they are; MXFP4 two half-words apart
+template <int FMT, int N>
+MOEB_DEV void lane_words(const uint32_t (&in)[N], uint32_t (&out)[N], bool to_words) {
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+        if (FMT == FMT_Q4) out[g] = in[g];
+        else if (to_words) out[g] = __byte_perm(in[g / 2], in[N / 2 + g / 2], g & 1 ? 0x7632 : 0x5410);
+        else out[g] = g < N / 2 ? __byte_perm(in[2 * g], in[2 * g + 1], 0x5410) : __byte_perm(in[2 * g - N], in[2 * g + 1 - N], 0x7632);
+    }
+}
 
 // Quantizes 8 values of a group spread over LANES neighbouring lanes, operation for operation as the weight quantizers
 // (quant.cu), so a cache row equals mx.quantize of it. A group that holds an infinity or a NaN, or whose span passes
@@ -36,12 +61,27 @@ MOEB_DEV uint32_t kv_quant_q4(const float (&v)[8], uint32_t &par) {
         scale = __fdiv_rn(edge, q0);
         bias = edge;
     }
+    // code = rint(d / scale), d = v - bias, the quotient rounded to fp32. r = d * (1 / scale) is within 3 * 2^-24 of it
+    // relatively, so within 2^-18 where it counts (quotients to 16): the two round to the same whole number unless r is
+    // that near to a half, and only then the division is made.
+    const float inv = __frcp_rn(scale);
+    float r[8];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        r[i] = __fmul_rn(__fsub_rn(v[i], bias), inv);
+        near |= !(fabsf(r[i] - rintf(r[i])) <= 0.5f - 7.62939453125e-6f);  // 2^-17; a NaN is near too
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = __fdiv_rn(__fsub_rn(v[i], bias), scale);
+    }
     uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        float q = rintf(__fdiv_rn(__fsub_rn(v[i], bias), scale));
-        q = fminf(fmaxf(q, 0.0f), 15.0f);
-        word |= (uint32_t)q << (4 * ((i >> 1) + 4 * (i & 1)));
+        // the low bits of 2^23 + whole number: rounded to even as rintf does
+        const float q = __fadd_rn(fminf(fmaxf(r[i], 0.0f), 15.0f), 8388608.f);
+        word |= (__float_as_uint(q) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
     }
     // q0 = 0: the largest magnitude is below half the smallest scale, every code is 0 and the values are zeros. The weight
     // quantizer keeps that scale; here it is 0, so that attention, which takes codes less 8, meets nothing to cancel.
@@ -62,106 +102,134 @@ MOEB_DEV uint32_t kv_quant_fp4(const float (&v)[8], uint32_t &par) {
     const int e = max((int)(top >> 23) - 127 - 2, -127);
     par = (uint32_t)(e + 127);
     const float inv = __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e, e <= 125
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(__fmul_rn(v[i], inv));
-        uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-        c |= (__float_as_uint(v[i]) >> 28) & 8u;
-        word |= c << (4 * i);
-    }
+    // to the nearest E2M1 value, halves to the even code, 6 at most, the sign kept
+    uint32_t word;
+    asm("{\n .reg .b8 b0, b1, b2, b3;\n cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n mov.b32 %0, {b0, b1, b2, b3};\n}"
+        : "=r"(word)
+        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
     return word;
 }
 
+// CTA: R * KV_U tokens of K or V of one head (blockIdx.y = 2 * head + is V)
 template <int FMT, int D>
-__global__ void __launch_bounds__(128) k_kv_write(KvWriteArgs a) {
-    constexpr int W = D / 8;
+__global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
+    using X = Wd<FMT, D>;
+    constexpr int NG = X::NG;
+    const int w = threadIdx.x % X::LR, h = blockIdx.y >> 1;
+    const bool isv = blockIdx.y & 1;
+    const uint16_t *src = (isv ? a.v + h * a.v_head : a.k + h * a.k_head) + 8 * w;
+    const long stride = isv ? a.v_row : a.k_row;
+    uint32_t *codes = (isv ? a.c.vq : a.c.kq) + w * NG;
+    unsigned char *ps = static_cast<unsigned char *>(isv ? a.c.vs : a.c.ks);
+    const int t0 = (int)blockIdx.x * (X::R * KV_U) + (int)threadIdx.x / X::LR;
     pdl_wait();
-    const long gid = (long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int w = (int)(gid % W);
-    long r = gid / W;  // (t, K or V, h), h fastest
-    const int h = (int)(r % a.c.Hkv);
-    r /= a.c.Hkv;
-    const bool isv = (r & 1) != 0;
-    const long t = r >> 1;
-    long page = -1;
-    int p = -1;
-    if (t < a.s.T) {
-        int r0, r1;
-        const int b = kv_seq_of(a.s, (int)t, r0, r1);
-        if (b >= 0) p = a.s.lens[b] - (r1 - (int)t);
-        if (p >= 0) {
-            page = kv_page(a.c, a.s, b, p);
-            if (page < 0 && w == 0) atomicOr(a.c.err, ERR_PAGE);
-        }
-    }
-    float x[8];
+    uint4 u[KV_U][NG];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (page >= 0) {
-        const uint16_t *src = isv ? a.v + t * a.v_row + h * a.v_head : a.k + t * a.k_row + h * a.k_head;
-        const uint4 u = *reinterpret_cast<const uint4 *>(src + 8 * w);
-        const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+    for (int i = 0; i < KV_U; ++i) {
+        const int t = t0 + i * X::R;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = bf16lo(uu[i]);
-            x[2 * i + 1] = bf16hi(uu[i]);
+        for (int g = 0; g < NG; ++g)
+            u[i][g] = t < a.s.T ? *reinterpret_cast<const uint4 *>(src + t * stride + g * (8 * X::LR)) : make_uint4(0, 0, 0, 0);
+    }
+    int r0 = 0, r1 = 0, b = -1;
+#pragma unroll
+    for (int i = 0; i < KV_U; ++i) {
+        const int t = t0 + i * X::R;
+        long page = -1;
+        int p = -1;
+        if (t < a.s.T) {
+            if (t >= r1 || t < r0) b = kv_seq_of(a.s, t, r0, r1);
+            if (b >= 0) p = a.s.lens[b] - (r1 - t);
+            if (p >= 0) {
+                page = kv_page(a.c, a.s, b, p);
+                if (page < 0 && w == 0) atomicOr(a.c.err, ERR_PAGE);
+            }
         }
-    }
-    // every lane takes part in the shuffles; a group's lanes are all inside one row
-    uint32_t par;
-    const uint32_t word = FMT == FMT_Q4 ? kv_quant_q4(x, par) : kv_quant_fp4(x, par);
-    if (page < 0) return;
-    const size_t row = kv_row(a.c, page, h, p);
-    uint32_t *codes = isv ? a.c.vq : a.c.kq;
-    if (FMT == FMT_Q4) {
-        codes[row * W + kv_pos_q4<D>(w)] = word;
-    } else {
-        uint16_t *dst = reinterpret_cast<uint16_t *>(codes) + row * (D / 4);
-        dst[kv_pos_fp4<D>(2 * w)] = (uint16_t)word;
-        dst[kv_pos_fp4<D>(2 * w + 1)] = (uint16_t)(word >> 16);
-    }
-    void *ps = isv ? a.c.vs : a.c.ks;
-    if (FMT == FMT_Q4) {
-        if ((w & 7) == 0) static_cast<uint32_t *>(ps)[row * (D / 64) + (w >> 3)] = par;
-    } else if ((w & 3) == 0) {
-        static_cast<uint8_t *>(ps)[row * (D / 32) + (w >> 2)] = (uint8_t)par;
+        // every lane takes part in the shuffles; a group's lanes are all inside one row
+        __syncwarp();
+        uint32_t word[NG], out[NG], par[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const uint32_t uu[4] = {u[i][g].x, u[i][g].y, u[i][g].z, u[i][g].w};
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[2 * e] = bf16lo(uu[e]);
+                x[2 * e + 1] = bf16hi(uu[e]);
+            }
+            word[g] = FMT == FMT_Q4 ? kv_quant_q4(x, par[g]) : kv_quant_fp4(x, par[g]);
+        }
+        if (page < 0) continue;
+        const size_t row = kv_row(a.c, page, h, p);
+        lane_words<FMT>(word, out, false);
+        using T = typename Vec<NG>::T;
+        *reinterpret_cast<T *>(codes + row * (D / 8)) = *reinterpret_cast<const T *>(out);
+        if (w == 0) {
+            if (FMT == FMT_Q4) {
+                *reinterpret_cast<T *>(ps + row * (4 * NG)) = *reinterpret_cast<const T *>(par);
+            } else if (NG == 4) {
+                *reinterpret_cast<uint32_t *>(ps + row * NG) = par[0] | par[1] << 8 | par[NG - 2] << 16 | par[NG - 1] << 24;
+            } else {
+                *reinterpret_cast<uint16_t *>(ps + row * NG) = (uint16_t)(par[0] | par[1 % NG] << 8);
+            }
+        }
     }
 }
 
 template <int FMT, int D>
-__global__ void __launch_bounds__(128) k_kv_read(KvReadArgs a) {
-    constexpr int W = D / 8;
+__global__ void __launch_bounds__(128) k_kv_read(const KvReadArgs a) {
+    using X = Wd<FMT, D>;
+    constexpr int NG = X::NG;
+    using T = typename Vec<NG>::T;
+    const int w = threadIdx.x % X::LR, h = blockIdx.y >> 1;
+    const bool isv = blockIdx.y & 1;
+    const int t0 = (int)blockIdx.x * (X::R * KV_U) + (int)threadIdx.x / X::LR;
+    const uint32_t *codes = (isv ? a.c.vq : a.c.kq) + w * NG;
+    const unsigned char *ps = static_cast<const unsigned char *>(isv ? a.c.vs : a.c.ks);
     pdl_wait();
-    const long gid = (long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int w = (int)(gid % W);
-    long r = gid / W;
-    const int h = (int)(r % a.c.Hkv);
-    r /= a.c.Hkv;
-    const bool isv = (r & 1) != 0;
-    const long t = r >> 1;
-    if (t >= a.s.T) return;
-    int r0, r1;
-    const int b = kv_seq_of(a.s, (int)t, r0, r1);
-    if (b < 0) return;
-    const long p = (long)(a.first ? a.first[b] : 0) + (t - r0);
-    const long page = p >= 0 && p <= 0x7fffffffL ? kv_page(a.c, a.s, b, (int)p) : -1;
-    uint4 o = make_uint4(0, 0, 0, 0);
-    if (page >= 0) {
+    uint32_t code[KV_U][NG], par[KV_U][FMT == FMT_Q4 ? NG : 1];
+    int has = 0, got = 0;  // bit i: row i is some sequence's, its page is valid
+    int r0 = 0, r1 = 0, b = -1;
+#pragma unroll
+    for (int i = 0; i < KV_U; ++i) {
+        const int t = t0 + i * X::R;
+        if (t >= a.s.T) continue;
+        if (t >= r1 || t < r0) b = kv_seq_of(a.s, t, r0, r1);
+        if (b < 0) continue;
+        has |= 1 << i;
+        const long p = (long)(a.first ? a.first[b] : 0) + (t - r0);
+        const long page = p >= 0 && p <= 0x7fffffffL ? kv_page(a.c, a.s, b, (int)p) : -1;
+        if (page < 0) {
+            if (w == 0) atomicOr(a.c.err, ERR_PAGE);
+            continue;
+        }
+        got |= 1 << i;
         const size_t row = kv_row(a.c, page, h, (int)p);
-        const uint32_t word = kv_word<FMT, D>(isv ? a.c.vq : a.c.kq, row, w);
-        float x[8];
-        kv_word_values<FMT>(word, kv_par<FMT>(isv ? a.c.vs : a.c.ks, row, w, D), x);
-        o = make_uint4(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7]));
-    } else if (w == 0) {
-        atomicOr(a.c.err, ERR_PAGE);
+        *reinterpret_cast<T *>(code[i]) = *reinterpret_cast<const T *>(codes + row * (D / 8));
+        if (FMT == FMT_Q4) *reinterpret_cast<T *>(par[i]) = *reinterpret_cast<const T *>(ps + row * (4 * NG));
+        else par[i][0] = NG == 4 ? *reinterpret_cast<const uint32_t *>(ps + row * NG) : *reinterpret_cast<const uint16_t *>(ps + row * NG);
     }
-    *reinterpret_cast<uint4 *>((isv ? a.v : a.k) + ((size_t)t * a.c.Hkv + h) * D + 8 * w) = o;
+    uint16_t *dst = (isv ? a.v : a.k) + (size_t)h * D + 8 * w;
+#pragma unroll
+    for (int i = 0; i < KV_U; ++i) {
+        if (!((has >> i) & 1)) continue;
+        uint32_t word[NG];
+        lane_words<FMT>(code[i], word, true);
+        uint16_t *to = dst + (size_t)(t0 + i * X::R) * a.c.Hkv * D;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            float x[8];
+            kv_word_values<FMT>(word[g], FMT == FMT_Q4 ? par[i][FMT == FMT_Q4 ? g : 0] : (par[i][0] >> (8 * g)) & 255u, x);
+            const uint4 o = make_uint4(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7]));
+            *reinterpret_cast<uint4 *>(to + g * (8 * X::LR)) = (got >> i) & 1 ? o : make_uint4(0, 0, 0, 0);
+        }
+    }
 }
 
 #define KV_INST(F, D)                                \
-    template __global__ void k_kv_write<F, D>(KvWriteArgs); \
-    template __global__ void k_kv_read<F, D>(KvReadArgs);
+    template __global__ void k_kv_write<F, D>(const KvWriteArgs); \
+    template __global__ void k_kv_read<F, D>(const KvReadArgs);
 KV_INST(FMT_Q4, 64)
 KV_INST(FMT_Q4, 128)
 KV_INST(FMT_FP4, 64)

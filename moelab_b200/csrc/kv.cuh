@@ -13,6 +13,8 @@
 // With it a lane's codes of one key (1 / 4 of the row for K, 1 / 8 for V) are one load of 4 to 16 bytes, and hold the same part
 // of every group.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -36,12 +38,6 @@ struct KvSeqs {
     long trow;
     int B, P, T, each;
 };
-
-// place in its row of word w (values 8 w ..; int4), of half-word u (values 4 u ..; MXFP4)
-template <int D>
-MOEB_DEV int kv_pos_q4(int w) { return (w & 7) * (D / 64) + (w >> 3); }
-template <int D>
-MOEB_DEV int kv_pos_fp4(int u) { return (u & 7) * (D / 32) + (u >> 3); }
 
 MOEB_DEV int kv_clamp_row(int v, int T) { return v < 0 ? 0 : (v > T ? T : v); }
 // rows [r0, r1) of sequence b, inside [0, T)
@@ -81,41 +77,36 @@ MOEB_DEV size_t kv_row(const KvCache &c, long page, int h, int p) {
     return (((size_t)page * c.Hkv + h) << c.pshift) + (size_t)(p & ((1 << c.pshift) - 1));
 }
 
-// value of one code
-MOEB_DEV float kv_q4_value(uint32_t code, uint32_t sb) { return __fmaf_rn(bf16lo(sb), (float)code, bf16hi(sb)); }
-MOEB_DEV float kv_fp4_value(uint32_t code) {
-    const uint32_t m = code & 7u, e = m >> 1;
-    const float v = 0.5f * (float)(e ? (2u + (m & 1u)) << (e - 1) : m);
-    return (code & 8u) ? -v : v;
-}
 // 2^(byte - 127), NaN for 255
 MOEB_DEV float kv_e8m0(uint32_t byte) {
     return byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte ? byte << 23 : 0x00400000u);
 }
-// the 8 values of code word `word` (natural element order)
+// the 8 values of code word `word` in their natural order. int4: the code into the low bits of 2^23, one exact subtraction and
+// one fused product; MXFP4: E2M1 to fp16 (exact) to fp32, times the power of two
 template <int FMT>
 MOEB_DEV void kv_word_values(uint32_t word, uint32_t par, float (&o)[8]) {
+    if (FMT == FMT_Q4) {
+        const float s = bf16lo(par), b = bf16hi(par);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (FMT == FMT_Q4) o[i] = kv_q4_value((word >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u, par);
-        else o[i] = kv_fp4_value((word >> (4 * i)) & 15u) * kv_e8m0(par);
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t c = (word >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u;
+            o[i] = __fmaf_rn(s, __uint_as_float(0x4B000000u | c) - 8388608.f, b);
+        }
+    } else {
+        const float s = kv_e8m0(par);
+        uint32_t h[4];
+        asm("{\n .reg .b8 b0, b1, b2, b3;\n mov.b32 {b0, b1, b2, b3}, %4;\n cvt.rn.f16x2.e2m1x2 %0, b0;\n cvt.rn.f16x2.e2m1x2 %1, b1;\n"
+            " cvt.rn.f16x2.e2m1x2 %2, b2;\n cvt.rn.f16x2.e2m1x2 %3, b3;\n}"
+            : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+            : "r"(word));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+            o[2 * i] = f.x * s;
+            o[2 * i + 1] = f.y * s;
+        }
     }
 }
-// parameters of word w of row `row` (int4: scale|bias; MXFP4: the E8M0 byte)
-template <int FMT>
-MOEB_DEV uint32_t kv_par(const void *ps, size_t row, int w, int D) {
-    if (FMT == FMT_Q4) return static_cast<const uint32_t *>(ps)[row * (D / 64) + (w >> 3)];
-    return static_cast<const uint8_t *>(ps)[row * (D / 32) + (w >> 2)];
-}
-
-// word w (values 8 w ..) of a row
-template <int FMT, int D>
-MOEB_DEV uint32_t kv_word(const uint32_t *codes, size_t row, int w) {
-    if (FMT == FMT_Q4) return codes[row * (D / 8) + kv_pos_q4<D>(w)];
-    const uint16_t *p = reinterpret_cast<const uint16_t *>(codes) + row * (D / 4);
-    return p[kv_pos_fp4<D>(2 * w)] | (uint32_t)p[kv_pos_fp4<D>(2 * w + 1)] << 16;
-}
-
 struct KvWriteArgs {
     KvCache c;
     KvSeqs s;
@@ -161,9 +152,9 @@ MOEB_DEV void kv_finish(const KvAttnArgs &a, int t, int head, int d4, float4 v, 
     if (a.lse && d4 == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 template <int FMT, int D>
-__global__ void k_kv_write(KvWriteArgs a);
+__global__ void k_kv_write(const KvWriteArgs a);
 template <int FMT, int D>
-__global__ void k_kv_read(KvReadArgs a);
+__global__ void k_kv_read(const KvReadArgs a);
 template <int FMT, int D, int NT>
 __global__ void k_kv_attn_few(const KvAttnArgs a, int *pre, float *part);
 template <int D, int NT>

@@ -121,6 +121,12 @@ int check_seqs(int T, const int *cu, const int *lens, bool need_lens, const int 
     ((c)->format == MOEB_KV_Q4 ? ((c)->head_dim == 64 ? kern<FMT_Q4, 64> : kern<FMT_Q4, 128>) \
                                : ((c)->head_dim == 64 ? kern<FMT_FP4, 64> : kern<FMT_FP4, 128>))
 
+// Grid of the kernels that write and read rows: per CTA 4 x 16 (int4) or 4 x 32 (MXFP4) tokens of one head's K or V.
+dim3 word_grid(const moeb_kv_cache *c, int T) {
+    const int tokens = c->format == MOEB_KV_Q4 ? 64 : 128;
+    return dim3((unsigned)((T + tokens - 1) / tokens), 2u * c->kv_heads);
+}
+
 // Workspace of the kernel for few rows: blocks before each sequence, then two partial results per CTA.
 struct FewLayout {
     size_t part, total;
@@ -196,8 +202,7 @@ int moeb_kv_write(const moeb_kv_cache *cache, const void *k, long k_row, long k_
     a.k_head = k_head;
     a.v_row = v_row;
     a.v_head = v_head;
-    const long n = (long)T * 2 * cache->kv_heads * (cache->head_dim / 8);
-    return launched(launch(KV_PICK(k_kv_write, cache), dim3((unsigned)((n + 127) / 128)), 128, 0, stream, a), "kv_write");
+    return launched(launch(KV_PICK(k_kv_write, cache), word_grid(cache, T), 128, 0, stream, a), "kv_write");
 }
 
 int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *first, const int *table, long table_row,
@@ -211,8 +216,7 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
     a.first = first;
     a.k = (uint16_t *)k;
     a.v = (uint16_t *)v;
-    const long n = (long)T * 2 * cache->kv_heads * (cache->head_dim / 8);
-    return launched(launch(KV_PICK(k_kv_read, cache), dim3((unsigned)((n + 127) / 128)), 128, 0, stream, a), "kv_read");
+    return launched(launch(KV_PICK(k_kv_read, cache), word_grid(cache, T), 128, 0, stream, a), "kv_read");
 }
 
 size_t moeb_kv_attention_workspace_bytes(int T, int B, int H, int kv_heads, int head_dim, int max_q) {

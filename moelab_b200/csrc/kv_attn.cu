@@ -21,8 +21,6 @@
 // Softmax statistics and sums are fp32; a column's maximum is shared by the warp's lanes (three shuffles), warps join at
 // the end of a run of blocks. MMA row r is key r / 2 + 4 (r % 2) of its eight, which makes the four keys of a lane's V
 // operand consecutive rows of shared memory (no bank conflicts) and costs K nothing.
-#include <cuda_fp16.h>
-
 #include "kv.cuh"
 
 namespace moeb {

@@ -20,8 +20,6 @@
 // product: such a group enters as zeros, and the rows that see its key are marked and written as NaN.
 //
 // Every wait is bounded: after its limit the kernel records MOEB_DEVERR_TIMEOUT, its roles stop, TMEM is released.
-#include <cuda_fp16.h>
-
 #include "kv.cuh"
 
 namespace moeb {
