@@ -30,65 +30,89 @@ MOEB_DEV void lane_words(const uint32_t (&in)[N], uint32_t (&out)[N], bool to_wo
     }
 }
 
-// Quantizes 8 values of a group spread over LANES neighbouring lanes, operation for operation as the weight quantizers
-// (quant.cu), so a cache row equals mx.quantize of it. A group that holds an infinity or a NaN, or whose span passes
-// fp32, is stored with NaN parameters: it reads back as NaN everywhere, and nothing else is touched by it.
-MOEB_DEV uint32_t kv_quant_q4(const float (&v)[8], uint32_t &par) {
-    float hi = v[0], lo = v[0];
-    bool bad = !(fabsf(v[0]) <= 3.4028234e38f);
+// int4: a group's 64 values lie in 8 neighbouring lanes, 8 in each. The operations are those of the weight quantizer
+// (quant.cu), so a cache row equals mx.quantize of it. A group that holds an infinity or a NaN, or whose span passes fp32, is
+// stored with NaN parameters: it reads back as NaN everywhere, and nothing else is touched by it. Bound by its instructions, not
+// by memory: pairs of values go through packed operations, and where a lane has two groups, four of the eight lanes work
+// out the parameters of one, four those of the other.
+struct Q4Group {
+    float scale, bias, inv;
+    uint32_t par;  // as stored; 0: all zeros
+};
+// (largest, -smallest) of the group; a NaN stays
+MOEB_DEV __nv_bfloat162 kv_q4_range(const uint4 u) {
+    const __nv_bfloat162 x0 = *reinterpret_cast<const __nv_bfloat162 *>(&u.x), x1 = *reinterpret_cast<const __nv_bfloat162 *>(&u.y),
+                         x2 = *reinterpret_cast<const __nv_bfloat162 *>(&u.z), x3 = *reinterpret_cast<const __nv_bfloat162 *>(&u.w);
+    const __nv_bfloat162 mx = __hmax2_nan(__hmax2_nan(x0, x1), __hmax2_nan(x2, x3)), mn = __hmin2_nan(__hmin2_nan(x0, x1), __hmin2_nan(x2, x3));
+    __nv_bfloat162 m = __halves2bfloat162(__hmax_nan(__low2bfloat16(mx), __high2bfloat16(mx)), __hneg(__hmin_nan(__low2bfloat16(mn), __high2bfloat16(mn))));
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        hi = fmaxf(hi, v[i]);
-        lo = fminf(lo, v[i]);
-        bad |= !(fabsf(v[i]) <= 3.4028234e38f);
-    }
-#pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) {
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    }
-    const unsigned group = 0xffu << (threadIdx.x & 24);
-    bad = (__ballot_sync(0xffffffffu, bad) & group) != 0;
+    for (int o = 4; o >= 1; o >>= 1) m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+MOEB_DEV Q4Group kv_q4_group(const __nv_bfloat162 m) {
+    Q4Group g;
+    const float hi = __low2float(m), lo = -__high2float(m);
     const bool mask = fabsf(lo) > fabsf(hi);
     float scale = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
-    bad |= !(scale <= 3.4028234e38f);
+    const bool bad = !(scale <= 3.4028234e38f);  // NaN, infinity, or a span that is none
     scale = scale > 1e-7f ? scale : 1e-7f;
     scale = mask ? scale : -scale;
     const float edge = mask ? lo : hi;
     const float q0 = rintf(__fdiv_rn(edge, scale));
-    float bias = 0.0f;
+    g.bias = 0.0f;
     if (q0 != 0.0f) {
         scale = __fdiv_rn(edge, q0);
-        bias = edge;
+        g.bias = edge;
     }
-    // code = rint(d / scale), d = v - bias, the quotient rounded to fp32. r = d * (1 / scale) is within 3 * 2^-24 of it
-    // relatively, so within 2^-18 where it counts (quotients to 16): the two round to the same whole number unless r is
-    // that near to a half, and only then the division is made.
-    const float inv = __frcp_rn(scale);
-    float r[8];
-    bool near = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        r[i] = __fmul_rn(__fsub_rn(v[i], bias), inv);
-        near |= !(fabsf(r[i] - rintf(r[i])) <= 0.5f - 7.62939453125e-6f);  // 2^-17; a NaN is near too
-    }
-    if (near) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = __fdiv_rn(__fsub_rn(v[i], bias), scale);
-    }
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        // the low bits of 2^23 + whole number: rounded to even as rintf does
-        const float q = __fadd_rn(fminf(fmaxf(r[i], 0.0f), 15.0f), 8388608.f);
-        word |= (__float_as_uint(q) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
-    }
+    g.scale = scale;
+    g.inv = __frcp_rn(scale);
     // q0 = 0: the largest magnitude is below half the smallest scale, every code is 0 and the values are zeros. The weight
     // quantizer keeps that scale; here it is 0, so that attention, which takes codes less 8, meets nothing to cancel.
-    par = bad ? 0x7fff7fffu : q0 == 0.0f ? 0u : (uint32_t)f2bf(scale) | ((uint32_t)f2bf(bias) << 16);
-    return bad ? 0u : word;
+    g.par = bad ? 0x7fff7fffu : q0 == 0.0f ? 0u : (uint32_t)f2bf(scale) | ((uint32_t)f2bf(g.bias) << 16);
+    return g;
 }
-MOEB_DEV uint32_t kv_quant_fp4(const float (&v)[8], uint32_t &par) {
+MOEB_DEV uint32_t kv_quant_q4(const uint4 u, const Q4Group &g) {
+    const float scale = g.scale, bias = g.bias, inv = g.inv;
+    // code = rint(d / scale), d = v - bias, the quotient rounded to fp32; it is not negative, as the bias is the end of the
+    // range that the scale's sign points away from. r = d * (1 / scale) is within 3 * 2^-24 of the quotient relatively, so
+    // within 2^-18 where it counts (to 16): the two round to the same whole number unless r is that near to a half, and only
+    // then the division is made. Adding 1.5 * 2^23 rounds to a whole number, to even as rintf does.
+    const float big = 12582912.f;
+    const uint64_t b2 = pair(-bias, -bias), i2 = pair(inv, inv), up = pair(big, big), down = pair(-big, -big), neg = pair(-1.f, -1.f);
+    const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+    uint64_t d[4], q[4];
+    float far = 0.f;  // from the whole numbers
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        d[i] = add2(pair(bf16lo(uu[i]), bf16hi(uu[i])), b2);
+        const uint64_t r = mul2(d[i], i2);
+        q[i] = add2(add2(r, up), down);
+        float f0, f1;
+        unpair(fma2(q[i], neg, r), f0, f1);
+        far = fmaxf(far, fmaxf(fabsf(f0), fabsf(f1)));
+    }
+    if (far > 0.5f - 7.62939453125e-6f) {  // 2^-17
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float d0, d1;
+            unpair(d[i], d0, d1);
+            q[i] = pair(rintf(__fdiv_rn(d0, scale)), rintf(__fdiv_rn(d1, scale)));
+        }
+    }
+    // four codes of 16 bits each side: sums of code * 16^p below 2^16 are exact, the low bits of 2^23 + sum are the half-words
+    uint64_t acc = pair(8388608.f, 8388608.f);
+#pragma unroll
+    for (int p = 3; p >= 0; --p) {
+        float c0, c1;
+        unpair(q[p], c0, c1);
+        const float w = (float)(1 << (4 * p));
+        acc = fma2(pair(fminf(c0, 15.f), fminf(c1, 15.f)), pair(w, w), acc);
+    }
+    const uint32_t word = __byte_perm((uint32_t)acc, (uint32_t)(acc >> 32), 0x5410);
+    return g.par == 0u || g.par == 0x7fff7fffu ? 0u : word;
+}
+MOEB_DEV uint32_t kv_quant_fp4(const uint4 u, uint32_t &par) {
+    const float v[8] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y), bf16lo(u.z), bf16hi(u.z), bf16lo(u.w), bf16hi(u.w)};
     uint32_t top = 0;  // the largest magnitude's bits: they order as the values do, with NaN on top
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -124,18 +148,21 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
     unsigned char *ps = static_cast<unsigned char *>(isv ? a.c.vs : a.c.ks);
     const int t0 = (int)blockIdx.x * (X::R * KV_U) + (int)threadIdx.x / X::LR;
     pdl_wait();
-    uint4 u[KV_U][NG];
-#pragma unroll
-    for (int i = 0; i < KV_U; ++i) {
-        const int t = t0 + i * X::R;
+    uint4 next[NG];
+    auto fetch = [&](int t) {
 #pragma unroll
         for (int g = 0; g < NG; ++g)
-            u[i][g] = t < a.s.T ? *reinterpret_cast<const uint4 *>(src + t * stride + g * (8 * X::LR)) : make_uint4(0, 0, 0, 0);
-    }
+            next[g] = t < a.s.T ? *reinterpret_cast<const uint4 *>(src + t * stride + g * (8 * X::LR)) : make_uint4(0, 0, 0, 0);
+    };
+    fetch(t0);
     int r0 = 0, r1 = 0, b = -1;
-#pragma unroll
+#pragma unroll 1  // once in the instruction cache
     for (int i = 0; i < KV_U; ++i) {
         const int t = t0 + i * X::R;
+        uint4 u[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) u[g] = next[g];
+        if (i + 1 < KV_U) fetch(t + X::R);
         long page = -1;
         int p = -1;
         if (t < a.s.T) {
@@ -149,16 +176,29 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
         // every lane takes part in the shuffles; a group's lanes are all inside one row
         __syncwarp();
         uint32_t word[NG], out[NG], par[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const uint32_t uu[4] = {u[i][g].x, u[i][g].y, u[i][g].z, u[i][g].w};
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[2 * e] = bf16lo(uu[e]);
-                x[2 * e + 1] = bf16hi(uu[e]);
+        if (FMT == FMT_Q4) {
+            __nv_bfloat162 m = kv_q4_range(u[0]);
+            if (NG == 2) {
+                const __nv_bfloat162 m1 = kv_q4_range(u[NG - 1]);
+                if (w & 4) m = m1;
             }
-            word[g] = FMT == FMT_Q4 ? kv_quant_q4(x, par[g]) : kv_quant_fp4(x, par[g]);
+            const Q4Group mine = kv_q4_group(m);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                Q4Group q = mine;
+                if (NG == 2) {
+                    const int from = ((int)threadIdx.x & 24) | 4 * g;
+                    q.scale = __shfl_sync(0xffffffffu, mine.scale, from);
+                    q.bias = __shfl_sync(0xffffffffu, mine.bias, from);
+                    q.inv = __shfl_sync(0xffffffffu, mine.inv, from);
+                    q.par = __shfl_sync(0xffffffffu, mine.par, from);
+                }
+                par[g] = q.par;
+                word[g] = kv_quant_q4(u[g], q);
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) word[g] = kv_quant_fp4(u[g], par[g]);
         }
         if (page < 0) continue;
         const size_t row = kv_row(a.c, page, h, p);

@@ -39,6 +39,29 @@ struct KvSeqs {
     int B, P, T, each;
 };
 
+// pairs of fp32 in one 64-bit register: one instruction for two sums or products
+MOEB_DEV uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+MOEB_DEV void unpair(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+MOEB_DEV uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+MOEB_DEV uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+MOEB_DEV uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
 MOEB_DEV int kv_clamp_row(int v, int T) { return v < 0 ? 0 : (v > T ? T : v); }
 // rows [r0, r1) of sequence b, inside [0, T)
 MOEB_DEV void kv_rows(const KvSeqs &s, int b, int &r0, int &r1) {
