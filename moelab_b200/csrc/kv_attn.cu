@@ -4,23 +4,26 @@
 // one tensor-core tile, so the cache is read once for all of them. The kernel is bound by the cache's bytes when the
 // caches are long, and by the chain lengths -> page table -> codes -> sums when they are short.
 //
-// Work split: the visible keys of every (sequence, KV head) are cut into blocks of 64; all blocks of the call in a row are
+// Work split: the visible keys of every (sequence, KV head) are cut into blocks of 128; all blocks of the call in a row are
 // dealt to the CTAs in equal runs, so uneven lengths cost nothing and the host needs to know none of them (a captured
 // graph replays with other lengths). A CTA that holds all blocks of a (sequence, head) writes y; otherwise it leaves its
 // unnormalised sum, maximum and sum of weights, and k_kv_attn_join joins them.
 //
-// A warp takes 16 keys of each block, straight from a cp.async ring of its own (no block-wide barrier in the loop), and
+// A warp takes 32 keys of each block, straight from a cp.async ring of its own (no block-wide barrier in the loop; the next
+// run's first copies are on their way while a run's warps join; bulk copies from single lanes cost twice the instructions), and
 // feeds the codes to mma.sync m16n8k16 without dequantizing them:
 //   scores^T [16 keys x NC] = K codes . q. int4: 128 + code is one bf16 operation away (code | 0x4300), so with group g's
 //     scale s and bias b, score = sum_g s (acc_g - 128 qsum_g) + b qsum_g in fp32. MXFP4: E2M1 codes convert to fp16, q is
 //     taken to fp16 with a power of two per row (8 bits of significand fit 11), score = sum_g 2^e acc_g.
-//   y^T [D x NC] += V^T codes . P, P = fp16(p * scale of the key's group) after one running power of two per warp, which
-//     keeps p * scale in fp16's range whatever the values' size; codes - 8 (int4) or E2M1 in fp16, exact. fp16 and not
+//   y^T [D x NC] += V^T codes . P, P = fp16(p * scale of the key's group). A running power of two per warp, taken into p's
+//     exponent, keeps the product in fp16's range whatever the values' size; codes - 8 (int4) or E2M1 in fp16, exact. fp16 and not
 //     bf16: P is the only rounding here, 2^-11 keeps it below the result's own 2^-8. int4's bias term is summed in fp32
 //     (b + 8 s, so that neither sum is a small difference of large ones).
 // Softmax statistics and sums are fp32; a column's maximum is shared by the warp's lanes (three shuffles), warps join at
 // the end of a run of blocks. MMA row r is key r / 2 + 4 (r % 2) of its eight, which makes the four keys of a lane's V
 // operand consecutive rows of shared memory (no bank conflicts) and costs K nothing.
+#include <type_traits>
+
 #include "kv.cuh"
 
 namespace moeb {
@@ -28,13 +31,14 @@ namespace moeb {
 namespace {
 
 constexpr int FW = 4, FT = 32 * FW;  // warps per CTA, threads
-constexpr int FS = 4;                // ring stages
+constexpr int FS = 2;                // ring stages
+constexpr int FB = 32 * FW;          // keys per block
 
 template <int FMT, int D>
 struct Few {
     static constexpr int W = D / 8, G = D / 64, NG = FMT == FMT_Q4 ? D / 64 : D / 32;
-    static constexpr int CODE = 16 * D / 2, PAR = FMT == FMT_Q4 ? 16 * G * 4 : 16 * NG;  // bytes of 16 rows
-    static constexpr int STAGE = 2 * CODE + 2 * PAR;
+    static constexpr int ROW = D / 2, PROW = FMT == FMT_Q4 ? G * 4 : NG;  // bytes of a row's codes, of its parameters
+    static constexpr int O_V = 32 * ROW, O_KP = 2 * O_V, O_VP = O_KP + 32 * PROW, STAGE = O_VP + 32 * PROW;  // 32 rows
 };
 
 MOEB_DEV float ex2(float x) {
@@ -75,6 +79,32 @@ MOEB_DEV uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+// A key's parameters in fp32. int4: scale, and bias + c scale; MXFP4: the powers of two.
+template <int FMT, int NG>
+MOEB_DEV void few_params(const unsigned char *p, float c, float (&s)[NG], float (&b)[NG]) {
+    if (FMT == FMT_Q4) {
+        uint32_t w[2];
+        if (NG == 2) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(p);
+            w[0] = x.x;
+            w[1] = x.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t *>(p);
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            s[g] = bf16lo(w[g]);
+            b[g] = fmaf(c, s[g], bf16hi(w[g]));
+        }
+    } else {
+        const uint32_t w = NG == 4 ? *reinterpret_cast<const uint32_t *>(p) : *reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+        for (int g = 0; g < NG; g += 2) {
+            e8m0_2(w >> (8 * g), s[g], s[g + 1]);
+            b[g] = b[g + 1] = 0.f;
+        }
+    }
+}
 // codes - 8 of nibble P of both halves of t, as f16x2: 1024 + q or 1024 + 16 q by one lop3, then one exact operation
 template <int P>
 MOEB_DEV uint32_t q4_f16x2(uint32_t t) {
@@ -91,11 +121,11 @@ MOEB_DEV uint32_t q4_f16x2(uint32_t t) {
     return *reinterpret_cast<uint32_t *>(&v);
 }
 
-// One sequence as the kernels see it: its rows, and the blocks of 64 keys that any of them sees.
+// One sequence as the kernels see it: its rows, and the blocks of FB keys that any of them sees.
 struct FewSeq {
     int r0, n, L, lo, ns, nb;
 };
-// blocks [0, ns): the first tokens; then from lo / 64 on. A sequence with rows has at least one block (its rows are
+// blocks [0, ns): the first tokens; then from lo / FB on. A sequence with rows has at least one block (its rows are
 // written), one with more rows than fit has none.
 template <int NC>
 MOEB_DEV FewSeq few_seq(const KvAttnArgs &a, int b) {
@@ -106,10 +136,11 @@ MOEB_DEV FewSeq few_seq(const KvAttnArgs &a, int b) {
     q.L = max(a.s.lens[b], 0);
     const int p0 = max(q.L - q.n, 0);
     q.lo = a.window ? max(p0 - a.window + 1, 0) : 0;
-    q.ns = min((min(a.sinks, q.lo) + 63) >> 6, q.lo >> 6);
-    q.nb = q.n > 0 && q.n * a.Gq <= NC ? max(q.ns + ((q.L + 63) >> 6) - (q.lo >> 6), 1) : 0;
+    q.ns = min((min(a.sinks, q.lo) + FB - 1) / FB, q.lo / FB);
+    q.nb = q.n > 0 && (long)q.n * a.Gq <= NC ? max(q.ns + (int)(((long)q.L + FB - 1) / FB) - q.lo / FB, 1) : 0;
     return q;
 }
+MOEB_DEV int few_tok(const FewSeq &q, int k) { return (k < q.ns ? k : q.lo / FB + k - q.ns) * FB; }
 MOEB_DEV long few_start(long W, long c, long n) { return W * c / n; }
 
 }  // namespace
@@ -119,12 +150,12 @@ template <int FMT, int D, int NT>
 __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAttnArgs a, int *pre, float *part) {
     using F = Few<FMT, D>;
     constexpr int NC = 8 * NT, NG = F::NG;
-    extern __shared__ __align__(16) unsigned char sm[];
-    unsigned char *ring = sm + (threadIdx.x >> 5) * (FS * F::STAGE);
+    extern __shared__ __align__(128) unsigned char sm[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+    unsigned char *ring = sm + warp * (FS * F::STAGE);
     float *so = reinterpret_cast<float *>(sm + FW * FS * F::STAGE);  // [FW][NC][D]
     __shared__ float s_m[FW][NC], s_l[FW][NC];
     __shared__ int s_sum[FW], s_b, s_pre;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
     pdl_wait();
 
     // every sequence's blocks: prefix sums over the CTA's threads, and the sequence of this CTA's first block
@@ -178,46 +209,54 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
         h = off / q.nb;
         k0 = off - h * q.nb;
     }
-    const int ta = (r >> 1) + 4 * (r & 1);  // this lane's keys of a step: ta and ta + 8
+    const int ta = (r >> 1) + 4 * (r & 1);  // this lane's keys of 16: ta and ta + 8
 
-    while (u < ue) {
-        // ---- one run of blocks [k0, k1) of (b, h)
-        const int k1 = (int)min((long)q.nb, k0 + (ue - u));
-        const int p0 = q.L - q.n, plast = q.L - 1;  // positions of the first and the last row
-        unsigned ok = 0;
-        auto issue = [&](int k) {
-            if (k < k1) {
-                const int tok = ((k < q.ns ? k : (q.lo >> 6) + k - q.ns) << 6) + 16 * warp;
-                const unsigned bit = 1u << (k % FS);
-                ok &= ~bit;
-                if (tok <= plast && (tok + 15 >= q.lo || tok < a.sinks)) {
-                    const long page = kv_page(a.c, a.s, b, tok);
-                    if (page < 0) {
-                        if (lane == 0) atomicOr(a.c.err, ERR_PAGE);
-                    } else {
-                        ok |= bit;
-                        const size_t row = kv_row(a.c, page, h, tok);
-                        unsigned char *st = ring + (k % FS) * F::STAGE;
-                        const unsigned char *kq = reinterpret_cast<const unsigned char *>(a.c.kq) + row * (D / 2);
-                        const unsigned char *vq = reinterpret_cast<const unsigned char *>(a.c.vq) + row * (D / 2);
+    // Copies of this warp's 32 keys of block k of (b, h), in two halves of 16 (a page at least). ok: bit 2 s + x says that half x
+    // of stage s is seen by some row and has a page.
+    unsigned ok = 0;
+    int slot_in = 0, slot = 0;  // stage of the next copy, of the next use
+    auto issue = [&](const FewSeq &q, int b, int h, int k, int k1) {
+        if (k < k1) {
+            const int tok0 = few_tok(q, k) + 32 * warp, plast = q.L - 1;
+            unsigned has = 0;
 #pragma unroll
-                        for (int i = 0; i < F::CODE / 512; ++i) {
-                            cp_async16(st + (i * 32 + lane) * 16, kq + (i * 32 + lane) * 16);
-                            cp_async16(st + F::CODE + (i * 32 + lane) * 16, vq + (i * 32 + lane) * 16);
-                        }
-                        constexpr int NP = F::PAR / 16;
-                        if (lane < 2 * NP) {
-                            const unsigned char *ps = static_cast<const unsigned char *>(lane < NP ? a.c.ks : a.c.vs) + row * (F::PAR / 16);
-                            cp_async16(st + 2 * F::CODE + lane * 16, ps + (lane % NP) * 16);
-                        }
-                    }
+            for (int x = 0; x < 2; ++x) {
+                const int tok = tok0 + 16 * x;
+                if (tok > plast || (tok + 15 < q.lo && tok >= a.sinks)) continue;
+                const long page = kv_page(a.c, a.s, b, tok);
+                if (page < 0) {
+                    if (lane == 0) atomicOr(a.c.err, ERR_PAGE);
+                    continue;
+                }
+                has |= 1u << x;
+                const size_t row = kv_row(a.c, page, h, tok);
+                unsigned char *st = ring + slot_in * F::STAGE + x * (16 * F::ROW) + lane * 16;
+                const unsigned char *kq = reinterpret_cast<const unsigned char *>(a.c.kq) + row * F::ROW + lane * 16;
+                const unsigned char *vq = reinterpret_cast<const unsigned char *>(a.c.vq) + row * F::ROW + lane * 16;
+#pragma unroll
+                for (int i = 0; i < F::ROW / 32; ++i) {
+                    cp_async16(st + i * 512, kq + i * 512);
+                    cp_async16(st + F::O_V + i * 512, vq + i * 512);
+                }
+                if (lane < 2 * F::PROW) {  // lanes 0 .. PROW - 1: K's parameters, the next as many V's
+                    const bool v = lane >= F::PROW;
+                    const int i = v ? lane - F::PROW : lane;
+                    cp_async16(ring + slot_in * F::STAGE + (v ? F::O_VP : F::O_KP) + x * (16 * F::PROW) + i * 16,
+                               static_cast<const unsigned char *>(v ? a.c.vs : a.c.ks) + row * F::PROW + i * 16);
                 }
             }
-            cp_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < FS - 1; ++i) issue(k0 + i);
+            ok = (ok & ~(3u << (2 * slot_in))) | has << (2 * slot_in);
+            if (++slot_in == FS) slot_in = 0;
+        }
+        cp_commit();
+    };
+    int k1 = (int)min((long)q.nb, k0 + (ue - u));
+#pragma unroll 1
+    for (int i = 0; i < FS; ++i) issue(q, b, h, k0 + i, k1);
 
+    while (true) {
+        // ---- one run of blocks [k0, k1) of (b, h), whose first copies are on their way
+        const int p0 = q.L - q.n, plast = q.L - 1;  // positions of the first and the last row
         // ---- queries: column nt * 8 + r is row (column / Gq) of the sequence, head h * Gq + column % Gq
         uint32_t qf[NT][D / 16][2];
         float qs[NT][FMT == FMT_Q4 ? NG : 1][2], cs[NT][2];
@@ -234,7 +273,12 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
                 const int word = FMT == FMT_Q4 ? 8 * (j >> 1) + 2 * c + (j & 1) : 4 * j + c;
                 w[j] = have ? *reinterpret_cast<const uint4 *>(src + 8 * word) : make_uint4(0, 0, 0, 0);
             }
-            float mul = a.scale;
+            // the scale's sign goes into q, so that the maximum can be taken before scaling; a scale of zero makes q zero
+            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+            float mul = a.scale == 0.f ? 1.f : fabsf(a.scale);
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j)
+                w[j] = a.scale == 0.f ? make_uint4(0, 0, 0, 0) : make_uint4(w[j].x ^ flip, w[j].y ^ flip, w[j].z ^ flip, w[j].w ^ flip);
             if (FMT == FMT_FP4) {  // to fp16 by the row's power of two: its largest value near 2^8
                 uint32_t t16 = 0;
 #pragma unroll
@@ -247,7 +291,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
                 t16 = max(t16, __shfl_xor_sync(0xffffffffu, t16, 2));
                 const int e = min(max((int)(t16 >> 7), 9), 254);           // biased exponent of the largest value
                 const float down = __uint_as_float((uint32_t)(262 - e) << 23);  // 2^(8 - (e - 127))
-                mul = a.scale * __uint_as_float((uint32_t)(e - 8) << 23);
+                mul *= __uint_as_float((uint32_t)(e - 8) << 23);
 #pragma unroll
                 for (int j = 0; j < D / 32; ++j) {
                     uint32_t ww[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
@@ -281,7 +325,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                cs[nt][e] = __shfl_sync(0xffffffffu, mul, 8 * c + 4 * e);
+                cs[nt][e] = fmaxf(__shfl_sync(0xffffffffu, mul, 8 * c + 4 * e), 1.2e-38f);  // above zero: a hidden -inf stays -inf
                 const int ce = nt * 8 + 2 * c + e, ie = ce / a.Gq;
                 pos[nt][e] = ie < q.n ? p0 + ie : -1;  // a column without a row sees nothing
             }
@@ -300,171 +344,148 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
                 for (int g = 0; g < (FMT == FMT_Q4 ? NG : 1); ++g) bs[nt][g][e] = 0.f;
             }
         }
-        uint32_t vlim = 0;           // bits of the largest value scale that the running power of two takes
-        float vmul = 1.f, vun = 1.f;  // that power and its inverse
+        uint32_t vlim = 0;  // bits of the largest value scale that the running power of two takes
+        float vexp = 0.f;   // its exponent: weights are 2^(score - m + vexp), and o, l and bs are sums of them
 
+#pragma unroll 1
         for (int k = k0; k < k1; ++k) {
-            cp_wait<FS - 2>();
+            cp_wait<FS - 1>();
             __syncwarp();
-            if (ok >> (k % FS) & 1) {
-                const unsigned char *st = ring + (k % FS) * F::STAGE;
-                const int tok = ((k < q.ns ? k : (q.lo >> 6) + k - q.ns) << 6) + 16 * warp;
-                // ---- scores of keys ta, ta + 8 for columns 2 c, 2 c + 1
-                float s[NT][4];
+            const unsigned has = (ok >> (2 * slot)) & 3u;
+            const unsigned char *st = ring + slot * F::STAGE;
+            const int tok = few_tok(q, k) + 32 * warp;
+            const bool all = has == 3u && tok + 31 <= p0 && (!a.window || tok > plast - a.window || tok + 31 < a.sinks);
+            // full: every row sees all 32 keys
+            auto step = [&](auto full_) {
+                constexpr bool full32 = decltype(full_)::value;
+                // ---- scores of keys 16 x + ta, 16 x + ta + 8 for columns 2 c, 2 c + 1
+                float s[2][NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-                uint32_t wa[D / 32], wb[D / 32];
-                {
-                    const unsigned char *ra = st + ta * (D / 2) + c * (D / 8);
+                for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) s[x][nt][0] = s[x][nt][1] = s[x][nt][2] = s[x][nt][3] = 0.f;
+                    uint32_t wa[D / 32], wb[D / 32];
+                    const unsigned char *ra = st + (16 * x + ta) * F::ROW + c * (D / 8);
                     if (D == 128) {
-                        const uint4 x = *reinterpret_cast<const uint4 *>(ra), y = *reinterpret_cast<const uint4 *>(ra + 4 * D);
-                        wa[0] = x.x; wa[1] = x.y; wa[D / 32 - 2] = x.z; wa[D / 32 - 1] = x.w;
-                        wb[0] = y.x; wb[1] = y.y; wb[D / 32 - 2] = y.z; wb[D / 32 - 1] = y.w;
+                        const uint4 y = *reinterpret_cast<const uint4 *>(ra), z = *reinterpret_cast<const uint4 *>(ra + 8 * F::ROW);
+                        wa[0] = y.x; wa[1] = y.y; wa[D / 32 - 2] = y.z; wa[D / 32 - 1] = y.w;
+                        wb[0] = z.x; wb[1] = z.y; wb[D / 32 - 2] = z.z; wb[D / 32 - 1] = z.w;
                     } else {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(ra), y = *reinterpret_cast<const uint2 *>(ra + 4 * D);
-                        wa[0] = x.x; wa[1] = x.y;
-                        wb[0] = y.x; wb[1] = y.y;
+                        const uint2 y = *reinterpret_cast<const uint2 *>(ra), z = *reinterpret_cast<const uint2 *>(ra + 8 * F::ROW);
+                        wa[0] = y.x; wa[1] = y.y;
+                        wb[0] = z.x; wb[1] = z.y;
                     }
-                }
-                const unsigned char *pk = st + 2 * F::CODE, *pv = pk + F::PAR;
-                if (FMT == FMT_Q4) {
+                    float xa[NG], ya[NG], xb[NG], yb[NG];
+                    few_params<FMT, NG>(st + F::O_KP + (16 * x + ta) * F::PROW, -128.f, xa, ya);
+                    few_params<FMT, NG>(st + F::O_KP + (16 * x + ta + 8) * F::PROW, -128.f, xb, yb);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         float acc[NT][4];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t ua = wa[(x >> 1) * NG + g], ub = wb[(x >> 1) * NG + g];
-                            const int p = 2 * (x & 1);
-                            const uint32_t A[4] = {q4pair(ua, p), q4pair(ub, p), q4pair(ua, p + 1), q4pair(ub, p + 1)};
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt], A, qf[nt][4 * g + x][0], qf[nt][4 * g + x][1]);
-                        }
-                        const uint32_t sa = *reinterpret_cast<const uint32_t *>(pk + (ta * NG + g) * 4);
-                        const uint32_t sb = *reinterpret_cast<const uint32_t *>(pk + ((ta + 8) * NG + g) * 4);
-                        const float xa = bf16lo(sa), ya = fmaf(-128.f, xa, bf16hi(sa)), xb = bf16lo(sb), yb = fmaf(-128.f, xb, bf16hi(sb));
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                s[nt][e] += fmaf(xa, acc[nt][e], ya * qs[nt][g][e]);
-                                s[nt][2 + e] += fmaf(xb, acc[nt][2 + e], yb * qs[nt][g][e]);
-                            }
-                        }
-                    }
-                } else {
-                    float xa[NG], xb[NG];
-#pragma unroll
-                    for (int g = 0; g < NG; g += 2) {
-                        e8m0_2(*reinterpret_cast<const uint16_t *>(pk + ta * NG + g), xa[g], xa[g + 1]);
-                        e8m0_2(*reinterpret_cast<const uint16_t *>(pk + (ta + 8) * NG + g), xb[g], xb[g + 1]);
-                    }
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        float acc[NT][4];
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-                        // half-words 2 c (product 0) and 2 c + 1 of the group
-                        const int x0 = g >> 1, x1 = NG / 2 + (g >> 1);
-                        uint32_t A0[4], A1[4];
-                        if (g & 1) {
-                            A0[0] = e2m1_f16x2<2>(wa[x0]); A0[1] = e2m1_f16x2<2>(wb[x0]); A0[2] = e2m1_f16x2<3>(wa[x0]); A0[3] = e2m1_f16x2<3>(wb[x0]);
-                            A1[0] = e2m1_f16x2<2>(wa[x1]); A1[1] = e2m1_f16x2<2>(wb[x1]); A1[2] = e2m1_f16x2<3>(wa[x1]); A1[3] = e2m1_f16x2<3>(wb[x1]);
-                        } else {
-                            A0[0] = e2m1_f16x2<0>(wa[x0]); A0[1] = e2m1_f16x2<0>(wb[x0]); A0[2] = e2m1_f16x2<1>(wa[x0]); A0[3] = e2m1_f16x2<1>(wb[x0]);
-                            A1[0] = e2m1_f16x2<0>(wa[x1]); A1[1] = e2m1_f16x2<0>(wb[x1]); A1[2] = e2m1_f16x2<1>(wa[x1]); A1[3] = e2m1_f16x2<1>(wb[x1]);
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma_f16(acc[nt], A0, qf[nt][2 * g][0], qf[nt][2 * g][1]);
-                            mma_f16(acc[nt], A1, qf[nt][2 * g + 1][0], qf[nt][2 * g + 1][1]);
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                s[nt][e] = fmaf(xa[g], acc[nt][e], s[nt][e]);
-                                s[nt][2 + e] = fmaf(xb[g], acc[nt][2 + e], s[nt][2 + e]);
-                            }
-                        }
-                    }
-                }
-                // ---- the value scales of keys ta, ta + 8 (zero where no row sees the key: what lies there is not looked at)
-                float va[NG], vb[NG], ba[NG], bb[NG];
-                const int ja = tok + ta, jb = ja + 8;
-                const bool full = tok + 15 <= p0 && (!a.window || tok > plast - a.window || tok + 15 < a.sinks);
-                if (FMT == FMT_Q4) {
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const uint32_t sa = *reinterpret_cast<const uint32_t *>(pv + (ta * NG + g) * 4);
-                        const uint32_t sb = *reinterpret_cast<const uint32_t *>(pv + ((ta + 8) * NG + g) * 4);
-                        va[g] = bf16lo(sa);
-                        ba[g] = fmaf(8.f, va[g], bf16hi(sa));
-                        vb[g] = bf16lo(sb);
-                        bb[g] = fmaf(8.f, vb[g], bf16hi(sb));
-                    }
-                } else {
-#pragma unroll
-                    for (int g = 0; g < NG; g += 2) {
-                        e8m0_2(*reinterpret_cast<const uint16_t *>(pv + ta * NG + g), va[g], va[g + 1]);
-                        e8m0_2(*reinterpret_cast<const uint16_t *>(pv + (ta + 8) * NG + g), vb[g], vb[g + 1]);
-                    }
-                }
-                if (!full) {
-                    const bool sa = ja <= plast && (ja >= q.lo || ja < a.sinks), sb = jb <= plast && (jb >= q.lo || jb < a.sinks);
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        va[g] = sa ? va[g] : 0.f;
-                        vb[g] = sb ? vb[g] : 0.f;
                         if (FMT == FMT_Q4) {
-                            ba[g] = sa ? ba[g] : 0.f;
-                            bb[g] = sb ? bb[g] : 0.f;
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {
+                                const uint32_t ua = wa[(y >> 1) * NG + g], ub = wb[(y >> 1) * NG + g];
+                                const int p = 2 * (y & 1);
+                                const uint32_t A[4] = {q4pair(ua, p), q4pair(ub, p), q4pair(ua, p + 1), q4pair(ub, p + 1)};
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt], A, qf[nt][4 * g + y][0], qf[nt][4 * g + y][1]);
+                            }
+                        } else {
+                            // half-words 2 c (product 0) and 2 c + 1 of the group
+                            const int x0 = g >> 1, x1 = NG / 2 + (g >> 1);
+                            uint32_t A0[4], A1[4];
+                            if (g & 1) {
+                                A0[0] = e2m1_f16x2<2>(wa[x0]); A0[1] = e2m1_f16x2<2>(wb[x0]); A0[2] = e2m1_f16x2<3>(wa[x0]); A0[3] = e2m1_f16x2<3>(wb[x0]);
+                                A1[0] = e2m1_f16x2<2>(wa[x1]); A1[1] = e2m1_f16x2<2>(wb[x1]); A1[2] = e2m1_f16x2<3>(wa[x1]); A1[3] = e2m1_f16x2<3>(wb[x1]);
+                            } else {
+                                A0[0] = e2m1_f16x2<0>(wa[x0]); A0[1] = e2m1_f16x2<0>(wb[x0]); A0[2] = e2m1_f16x2<1>(wa[x0]); A0[3] = e2m1_f16x2<1>(wb[x0]);
+                                A1[0] = e2m1_f16x2<0>(wa[x1]); A1[1] = e2m1_f16x2<0>(wb[x1]); A1[2] = e2m1_f16x2<1>(wa[x1]); A1[3] = e2m1_f16x2<1>(wb[x1]);
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma_f16(acc[nt], A0, qf[nt][2 * g][0], qf[nt][2 * g][1]);
+                                mma_f16(acc[nt], A1, qf[nt][2 * g + 1][0], qf[nt][2 * g + 1][1]);
+                            }
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                if (FMT == FMT_Q4) {
+                                    s[x][nt][e] = fmaf(ya[g], qs[nt][FMT == FMT_Q4 ? g : 0][e], s[x][nt][e]);
+                                    s[x][nt][2 + e] = fmaf(yb[g], qs[nt][FMT == FMT_Q4 ? g : 0][e], s[x][nt][2 + e]);
+                                }
+                                s[x][nt][e] = fmaf(xa[g], acc[nt][e], s[x][nt][e]);
+                                s[x][nt][2 + e] = fmaf(xb[g], acc[nt][2 + e], s[x][nt][2 + e]);
+                            }
                         }
                     }
                 }
-                uint32_t top = 0;
+                // ---- the value parameters of the same keys (zero where no row sees the key: what lies there is not looked at)
+                float va[2][NG], vb[2][NG], ba[2][NG], bb[2][NG];
+                unsigned vis[NT];  // bit 4 x + 2 i + e: column 2 c + e sees key 16 x + ta + 8 i
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const uint32_t x = __float_as_uint(va[g]) & 0x7fffffffu, y = __float_as_uint(vb[g]) & 0x7fffffffu;
-                    top = max(top, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u));
+                for (int x = 0; x < 2; ++x) {
+                    few_params<FMT, NG>(st + F::O_VP + (16 * x + ta) * F::PROW, 8.f, va[x], ba[x]);
+                    few_params<FMT, NG>(st + F::O_VP + (16 * x + ta + 8) * F::PROW, 8.f, vb[x], bb[x]);
                 }
-                top = __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) vis[nt] = 0xffu;
+                if (!full32) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int ja = tok + 16 * x + ta, jb = ja + 8;
+                        const bool half = (has >> x) & 1u;
+                        const bool sa = half && ja <= plast && (ja >= q.lo || ja < a.sinks), sb = half && jb <= plast && (jb >= q.lo || jb < a.sinks);
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            va[x][g] = sa ? va[x][g] : 0.f;
+                            vb[x][g] = sb ? vb[x][g] : 0.f;
+                            ba[x][g] = sa ? ba[x][g] : 0.f;
+                            bb[x][g] = sb ? bb[x][g] : 0.f;
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int p = pos[nt][e];
+                                const bool wa_ = half && ja <= p && (!a.window || ja > p - a.window || ja < a.sinks);
+                                const bool wb_ = half && jb <= p && (!a.window || jb > p - a.window || jb < a.sinks);
+                                if (!wa_) { s[x][nt][e] = -INFINITY; vis[nt] &= ~(1u << (4 * x + e)); }
+                                if (!wb_) { s[x][nt][2 + e] = -INFINITY; vis[nt] &= ~(1u << (4 * x + 2 + e)); }
+                            }
+                        }
+                    }
+                }
+                float big = 0.f;  // the largest scale; fmaxf passes NaN over
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) big = fmaxf(big, fmaxf(fabsf(va[x][g]), fabsf(vb[x][g])));
+                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
                 float fix = 1.f;
                 if (top > vlim) {  // larger than the power of two takes: scale to 2^8, with room to 2^14
-                    const uint32_t e = min(max(top >> 23, 9u), 248u);
-                    const float nm = __uint_as_float((262u - e) << 23);
-                    fix = nm * vun;
-                    vmul = nm;
-                    vun = __uint_as_float((e - 8u) << 23);
+                    const uint32_t e = min(max(top >> 23, 35u), 248u);
+                    const float ne = (float)(135 - (int)e);
+                    fix = ex2(ne - vexp);
+                    vexp = ne;
                     vlim = (e + 6u) << 23;
                 }
-                // ---- mask, running maximum, weights
+                // ---- running maximum, weights
                 bool grew = fix != 1.f;
-                float f[NT][2];
-                bool vis[NT][4];
+                float mn[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        s[nt][e] *= cs[nt][e];
-                        s[nt][2 + e] *= cs[nt][e];
-                        vis[nt][e] = vis[nt][2 + e] = true;
-                        if (!full) {
-                            const int p = pos[nt][e];
-                            vis[nt][e] = ja <= p && (!a.window || ja > p - a.window || ja < a.sinks);
-                            vis[nt][2 + e] = jb <= p && (!a.window || jb > p - a.window || jb < a.sinks);
-                            if (!vis[nt][e]) s[nt][e] = -INFINITY;
-                            if (!vis[nt][2 + e]) s[nt][2 + e] = -INFINITY;
-                        }
-                        float t = fmaxf(s[nt][e], s[nt][2 + e]);
+                        float t = fmaxf(fmaxf(s[0][nt][e], s[0][nt][2 + e]), fmaxf(s[1][nt][e], s[1][nt][2 + e]));
                         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
                         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
                         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-                        const float mn = fmaxf(m[nt][e], t);
-                        grew |= mn > m[nt][e];
-                        const float use = mn == -INFINITY ? 0.f : mn;
-                        f[nt][e] = ex2(m[nt][e] - use);
-                        m[nt][e] = mn;
-                        s[nt][e] = ex2(s[nt][e] - use);
-                        s[nt][2 + e] = ex2(s[nt][2 + e] - use);
+                        mn[nt][e] = fmaxf(m[nt][e], t * cs[nt][e]);
+                        grew |= mn[nt][e] > m[nt][e];
                     }
                 }
                 if (__any_sync(0xffffffffu, grew)) {
@@ -472,100 +493,135 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
                     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            l[nt][e] *= f[nt][e];
+                            const float f = ex2(m[nt][e] - (mn[nt][e] == -INFINITY ? 0.f : mn[nt][e])) * fix;
+                            m[nt][e] = mn[nt][e];
+                            l[nt][e] *= f;
                             if (FMT == FMT_Q4) {
 #pragma unroll
-                                for (int g = 0; g < NG; ++g) bs[nt][g][e] *= f[nt][e];
+                                for (int g = 0; g < NG; ++g) bs[nt][FMT == FMT_Q4 ? g : 0][e] *= f;
                             }
-                            const float ff = f[nt][e] * fix;
 #pragma unroll
                             for (int i = 0; i < D / 16; ++i) {
-                                o[nt][i][e] *= ff;
-                                o[nt][i][2 + e] *= ff;
+                                o[nt][i][e] *= f;
+                                o[nt][i][2 + e] *= f;
                             }
                         }
                     }
                 }
-                uint32_t pf[NT][NG][2];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t pf[NT][NG][2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) l[nt][e] += s[nt][e] + s[nt][2 + e];
+                    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const float xa = va[g] * vmul, xb = vb[g] * vmul;
-                        float w[4] = {s[nt][0] * xa, s[nt][1] * xa, s[nt][2] * xb, s[nt][3] * xb};
-                        if (!full) {  // a key that one row sees and another does not may hold a NaN
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = vis[nt][e] ? w[e] : 0.f;
+                        for (int e = 0; e < 2; ++e) {
+                            const float off = m[nt][e] == -INFINITY ? 0.f : vexp - m[nt][e];
+                            s[x][nt][e] = ex2(fmaf(s[x][nt][e], cs[nt][e], off));
+                            s[x][nt][2 + e] = ex2(fmaf(s[x][nt][2 + e], cs[nt][e], off));
+                            l[nt][e] += s[x][nt][e] + s[x][nt][2 + e];
                         }
-                        pf[nt][g][0] = transpose8(pack_h2(w[0], w[1]));
-                        pf[nt][g][1] = transpose8(pack_h2(w[2], w[3]));
+                        const float(&w)[4] = s[x][nt];
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            const float xa = va[x][g], xb = vb[x][g];
+                            float y[4] = {w[0] * xa, w[1] * xa, w[2] * xb, w[3] * xb};
+                            if (!full32) {  // a key that one row sees and another does not may hold a NaN
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) y[e] = (vis[nt] >> (4 * x + e)) & 1u ? y[e] : 0.f;
+                            }
+                            pf[nt][g][0] = transpose8(pack_h2(y[0], y[1]));
+                            pf[nt][g][1] = transpose8(pack_h2(y[2], y[3]));
+                            if (FMT == FMT_Q4) {
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    float &t = bs[nt][FMT == FMT_Q4 ? g : 0][e];
+                                    if (full32) {
+                                        t = fmaf(w[2 + e], bb[x][g], fmaf(w[e], ba[x][g], t));
+                                    } else {
+                                        t += (vis[nt] >> (4 * x + e)) & 1u ? w[e] * ba[x][g] : 0.f;
+                                        t += (vis[nt] >> (4 * x + 2 + e)) & 1u ? w[2 + e] * bb[x][g] : 0.f;
+                                    }
+                                }
+                            }
+                        }
+                    }
+                    // ---- values: keys 16 x + c, + 4, + 8, + 12
+                    const unsigned char *rv = st + F::O_V + (16 * x + c) * F::ROW + r * (D / 16);
+                    uint32_t vw[4][D / 64];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        if (D == 128) {
+                            const uint2 y = *reinterpret_cast<const uint2 *>(rv + t * 4 * F::ROW);
+                            vw[t][0] = y.x;
+                            vw[t][D / 64 - 1] = y.y;
+                        } else {
+                            vw[t][0] = *reinterpret_cast<const uint32_t *>(rv + t * 4 * F::ROW);
+                        }
+                    }
+#pragma unroll
+                    for (int g = 0; g < D / 64; ++g) {
                         if (FMT == FMT_Q4) {
+                            const uint32_t l0 = __byte_perm(vw[0][g], vw[1][g], 0x5410), h0 = __byte_perm(vw[0][g], vw[1][g], 0x7632);
+                            const uint32_t l1 = __byte_perm(vw[2][g], vw[3][g], 0x5410), h1 = __byte_perm(vw[2][g], vw[3][g], 0x7632);
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float x = s[nt][e] * ba[g], y = s[nt][2 + e] * bb[g];
-                                bs[nt][g][e] += (vis[nt][e] ? x : 0.f) + (vis[nt][2 + e] ? y : 0.f);
+                            for (int p = 0; p < 4; ++p) {
+                                uint32_t A[4];
+                                if (p == 0) { A[0] = q4_f16x2<0>(l0); A[1] = q4_f16x2<0>(h0); A[2] = q4_f16x2<0>(l1); A[3] = q4_f16x2<0>(h1); }
+                                if (p == 1) { A[0] = q4_f16x2<1>(l0); A[1] = q4_f16x2<1>(h0); A[2] = q4_f16x2<1>(l1); A[3] = q4_f16x2<1>(h1); }
+                                if (p == 2) { A[0] = q4_f16x2<2>(l0); A[1] = q4_f16x2<2>(h0); A[2] = q4_f16x2<2>(l1); A[3] = q4_f16x2<2>(h1); }
+                                if (p == 3) { A[0] = q4_f16x2<3>(l0); A[1] = q4_f16x2<3>(h0); A[2] = q4_f16x2<3>(l1); A[3] = q4_f16x2<3>(h1); }
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * g + p], A, pf[nt][g][0], pf[nt][g][1]);
+                            }
+                        } else {
+                            const uint32_t mk = 0x0F0F0F0Fu;
+                            const uint32_t e0 = (vw[0][g] & mk) | ((vw[1][g] << 4) & ~mk), d0 = ((vw[0][g] >> 4) & mk) | (vw[1][g] & ~mk);
+                            const uint32_t e1 = (vw[2][g] & mk) | ((vw[3][g] << 4) & ~mk), d1 = ((vw[2][g] >> 4) & mk) | (vw[3][g] & ~mk);
+                            const uint32_t A0[4] = {e2m1_f16x2<0>(e0), e2m1_f16x2<0>(d0), e2m1_f16x2<0>(e1), e2m1_f16x2<0>(d1)};
+                            const uint32_t A1[4] = {e2m1_f16x2<1>(e0), e2m1_f16x2<1>(d0), e2m1_f16x2<1>(e1), e2m1_f16x2<1>(d1)};
+                            const uint32_t A2[4] = {e2m1_f16x2<2>(e0), e2m1_f16x2<2>(d0), e2m1_f16x2<2>(e1), e2m1_f16x2<2>(d1)};
+                            const uint32_t A3[4] = {e2m1_f16x2<3>(e0), e2m1_f16x2<3>(d0), e2m1_f16x2<3>(e1), e2m1_f16x2<3>(d1)};
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma_f16(o[nt][4 * g + 0], A0, pf[nt][2 * g][0], pf[nt][2 * g][1]);
+                                mma_f16(o[nt][4 * g + 1], A1, pf[nt][2 * g][0], pf[nt][2 * g][1]);
+                                mma_f16(o[nt][4 * g + 2], A2, pf[nt][2 * g + 1][0], pf[nt][2 * g + 1][1]);
+                                mma_f16(o[nt][4 * g + 3], A3, pf[nt][2 * g + 1][0], pf[nt][2 * g + 1][1]);
                             }
                         }
                     }
                 }
-                // ---- values: keys c, c + 4, c + 8, c + 12
-                const unsigned char *rv = st + F::CODE + c * (D / 2) + r * (D / 16);
-                uint32_t vw[4][D / 64];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if (D == 128) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(rv + t * 2 * D);
-                        vw[t][0] = x.x;
-                        vw[t][D / 64 - 1] = x.y;
-                    } else {
-                        vw[t][0] = *reinterpret_cast<const uint32_t *>(rv + t * 2 * D);
-                    }
-                }
-#pragma unroll
-                for (int g = 0; g < D / 64; ++g) {
-                    if (FMT == FMT_Q4) {
-                        const uint32_t l0 = __byte_perm(vw[0][g], vw[1][g], 0x5410), h0 = __byte_perm(vw[0][g], vw[1][g], 0x7632);
-                        const uint32_t l1 = __byte_perm(vw[2][g], vw[3][g], 0x5410), h1 = __byte_perm(vw[2][g], vw[3][g], 0x7632);
-#pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            uint32_t A[4];
-                            if (p == 0) { A[0] = q4_f16x2<0>(l0); A[1] = q4_f16x2<0>(h0); A[2] = q4_f16x2<0>(l1); A[3] = q4_f16x2<0>(h1); }
-                            if (p == 1) { A[0] = q4_f16x2<1>(l0); A[1] = q4_f16x2<1>(h0); A[2] = q4_f16x2<1>(l1); A[3] = q4_f16x2<1>(h1); }
-                            if (p == 2) { A[0] = q4_f16x2<2>(l0); A[1] = q4_f16x2<2>(h0); A[2] = q4_f16x2<2>(l1); A[3] = q4_f16x2<2>(h1); }
-                            if (p == 3) { A[0] = q4_f16x2<3>(l0); A[1] = q4_f16x2<3>(h0); A[2] = q4_f16x2<3>(l1); A[3] = q4_f16x2<3>(h1); }
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * g + p], A, pf[nt][g][0], pf[nt][g][1]);
-                        }
-                    } else {
-                        const uint32_t mk = 0x0F0F0F0Fu;
-                        const uint32_t e0 = (vw[0][g] & mk) | ((vw[1][g] << 4) & ~mk), d0 = ((vw[0][g] >> 4) & mk) | (vw[1][g] & ~mk);
-                        const uint32_t e1 = (vw[2][g] & mk) | ((vw[3][g] << 4) & ~mk), d1 = ((vw[2][g] >> 4) & mk) | (vw[3][g] & ~mk);
-                        const uint32_t A0[4] = {e2m1_f16x2<0>(e0), e2m1_f16x2<0>(d0), e2m1_f16x2<0>(e1), e2m1_f16x2<0>(d1)};
-                        const uint32_t A1[4] = {e2m1_f16x2<1>(e0), e2m1_f16x2<1>(d0), e2m1_f16x2<1>(e1), e2m1_f16x2<1>(d1)};
-                        const uint32_t A2[4] = {e2m1_f16x2<2>(e0), e2m1_f16x2<2>(d0), e2m1_f16x2<2>(e1), e2m1_f16x2<2>(d1)};
-                        const uint32_t A3[4] = {e2m1_f16x2<3>(e0), e2m1_f16x2<3>(d0), e2m1_f16x2<3>(e1), e2m1_f16x2<3>(d1)};
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma_f16(o[nt][4 * g + 0], A0, pf[nt][2 * g][0], pf[nt][2 * g][1]);
-                            mma_f16(o[nt][4 * g + 1], A1, pf[nt][2 * g][0], pf[nt][2 * g][1]);
-                            mma_f16(o[nt][4 * g + 2], A2, pf[nt][2 * g + 1][0], pf[nt][2 * g + 1][1]);
-                            mma_f16(o[nt][4 * g + 3], A3, pf[nt][2 * g + 1][0], pf[nt][2 * g + 1][1]);
-                        }
-                    }
-                }
-            }
+            };
+            if (all) step(std::true_type{});
+            else if (has) step(std::false_type{});
             __syncwarp();
-            issue(k + FS - 1);
+            issue(q, b, h, k + FS, k1);
+            if (++slot == FS) slot = 0;
         }
-        cp_wait<0>();
+        // ---- the next run: its first copies go out before this one's warps join
+        const int h_ = h, k0_ = k0, k1_ = k1;
+        const bool first_run = u == us;
+        u += k1 - k0;
+        const bool more = u < ue;
+        FewSeq qn = q;
+        if (more) {
+            k0 = 0;
+            if (++h == a.c.Hkv) {
+                h = 0;
+                do qn = few_seq<NC>(a, ++b);
+                while (qn.nb == 0);
+            }
+            k1 = (int)min((long)qn.nb, ue - u);
+#pragma unroll 1
+            for (int i = 0; i < FS; ++i) issue(qn, b, h, i, k1);
+        }
 
-        // ---- the warps' sums join in shared memory
+        // ---- the warps' sums join in shared memory; m becomes what the weights are relative to
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                m[nt][e] -= vexp;
 #pragma unroll
                 for (int x = 4; x <= 16; x <<= 1) {
                     l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
@@ -598,15 +654,15 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
                     const int dim = FMT == FMT_Q4 ? 64 * (i >> 2) + 8 * r + 2 * (i & 3) : 32 * (i >> 1) + 4 * r + 2 * (i & 1);
                     const float add = FMT == FMT_Q4 ? bs[nt][i >> 2 < NG ? i >> 2 : 0][e] : 0.f;
                     float2 v;
-                    v.x = fmaf(o[nt][i][e], vun, add) * fm;
-                    v.y = fmaf(o[nt][i][2 + e], vun, add) * fm;
+                    v.x = (o[nt][i][e] + add) * fm;
+                    v.y = (o[nt][i][2 + e] + add) * fm;
                     *reinterpret_cast<float2 *>(dst + dim) = v;
                 }
             }
         }
         __syncthreads();
-        const bool whole = k0 == 0 && k1 == q.nb;
-        float *pt = part + ((size_t)blockIdx.x * 2 + (u == us ? 0 : 1)) * (NC * (D + 2));
+        const bool whole = k0_ == 0 && k1_ == q.nb;
+        float *pt = part + ((size_t)blockIdx.x * 2 + (first_run ? 0 : 1)) * (NC * (D + 2));
         for (int i = threadIdx.x; i < q.n * a.Gq * (D / 4); i += FT) {
             const int col = i / (D / 4), d4 = i % (D / 4);
             float M = s_m[0][col], L = 0.f;
@@ -624,23 +680,16 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
                 L += s_l[x][col] * ex2(s_m[x][col] - use);
             }
             if (whole) {
-                const int ri = col / a.Gq, head = h * a.Gq + col - ri * a.Gq;
+                const int ri = col / a.Gq, head = h_ * a.Gq + col - ri * a.Gq;
                 kv_finish<D>(a, q.r0 + ri, head, d4, v, M, L);
             } else {
                 *reinterpret_cast<float4 *>(pt + col * D + 4 * d4) = v;
                 if (d4 == 0) *reinterpret_cast<float2 *>(pt + NC * D + 2 * col) = make_float2(M, L);
             }
         }
+        if (!more) break;
+        q = qn;
         __syncthreads();
-
-        // ---- the next run
-        u += k1 - k0;
-        k0 = 0;
-        if (u < ue && ++h == a.c.Hkv) {
-            h = 0;
-            do q = few_seq<NC>(a, ++b);
-            while (q.nb == 0);
-        }
     }
 }
 
