@@ -148,6 +148,7 @@ struct KvAttnArgs {
     const uint16_t *q;
     long q_row, q_head;
     int H, Gq;         // query heads, query heads per KV head
+    unsigned Gdiv;     // ceil(2^32 / Gq), 0 for 1: see kv_div
     float scale;       // of the scores, times log2(e)
     int window, sinks;
     int few;           // sequences of at most this many (row, head) columns are another kernel's
@@ -156,6 +157,8 @@ struct KvAttnArgs {
     uint16_t *y;       // [T][H][D]
     float *lse;        // [T][H] or null
 };
+// n / Gq for n < 2^16 (columns and rows of a tile): the product of n and 2^32 / Gq, rounded up, is less than 1 / Gq too large
+MOEB_DEV int kv_div(int n, unsigned div) { return div ? (int)__umulhi((unsigned)n, div) : n; }
 // Four values of one row's result: v is the sum of weights 2^(score - M) times values, L the sum of the weights.
 template <int D>
 MOEB_DEV void kv_finish(const KvAttnArgs &a, int t, int head, int d4, float4 v, float M, float L) {

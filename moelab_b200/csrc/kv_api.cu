@@ -131,7 +131,7 @@ dim3 word_grid(const moeb_kv_cache *c, int T) {
 struct FewLayout {
     size_t part, total;
 };
-constexpr int FEW_RESIDENT = 4;  // CTAs per SM at most (the kernel's launch bound)
+constexpr int FEW_RESIDENT = 3;  // CTAs per SM at most (the kernel's launch bound)
 FewLayout few_layout(int B, int nc, int D) {
     FewLayout l;
     l.part = up256(4 * ((size_t)B + 1));
@@ -257,6 +257,7 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
     a.q_head = q_head;
     a.H = H;
     a.Gq = H / cache->kv_heads;
+    a.Gdiv = a.Gq == 1 ? 0u : (unsigned)((0x100000000ull + a.Gq - 1) / a.Gq);
     a.scale = scale * 1.4426950408889634f;
     a.window = window;
     a.sinks = sinks;

@@ -31,7 +31,7 @@ namespace moeb {
 namespace {
 
 constexpr int FW = 4, FT = 32 * FW;  // warps per CTA, threads
-constexpr int FS = 2;                // ring stages
+constexpr int FS = 3;                // ring stages
 constexpr int FB = 32 * FW;          // keys per block
 
 template <int FMT, int D>
@@ -147,7 +147,7 @@ MOEB_DEV long few_start(long W, long c, long n) { return W * c / n; }
 
 // ws: prefix[B + 1] int32 (blocks before each sequence), then 2 partials per CTA: NC rows of D sums, NC (max, sum).
 template <int FMT, int D, int NT>
-__global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAttnArgs a, int *pre, float *part) {
+__global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAttnArgs a, int *pre, float *part) {
     using F = Few<FMT, D>;
     constexpr int NC = 8 * NT, NG = F::NG;
     extern __shared__ __align__(128) unsigned char sm[];
@@ -211,25 +211,30 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
     }
     const int ta = (r >> 1) + 4 * (r & 1);  // this lane's keys of 16: ta and ta + 8
 
-    // Copies of this warp's 32 keys of block k of (b, h), in two halves of 16 (a page at least). ok: bit 2 s + x says that half x
-    // of stage s is seen by some row and has a page.
+    // Page ids of 16 blocks from kb on: lane 2 i + x has half x (16 keys, a page at least) of this warp's keys of block kb + i.
+    // -1: no row sees the half; -2: it has no page.
+    auto pages = [&](const FewSeq &q, int b, int kb, int k1) {
+        const int k = kb + (lane >> 1), tok = few_tok(q, k) + 32 * warp + 16 * (lane & 1);
+        if (k >= k1 || tok >= q.L || (tok + 15 < q.lo && tok >= a.sinks)) return -1;
+        const long page = kv_page(a.c, a.s, b, tok);
+        return page < 0 ? -2 : (int)page;
+    };
+    // Copies of this warp's 32 keys of block k of head h. ok: bit 2 s + x says that half x of stage s has come.
     unsigned ok = 0;
     int slot_in = 0, slot = 0;  // stage of the next copy, of the next use
-    auto issue = [&](const FewSeq &q, int b, int h, int k, int k1) {
+    auto issue = [&](const FewSeq &q, int h, int k, int k1, int ids, int kb) {
         if (k < k1) {
-            const int tok0 = few_tok(q, k) + 32 * warp, plast = q.L - 1;
+            const int off = few_tok(q, k) + 32 * warp;
             unsigned has = 0;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const int tok = tok0 + 16 * x;
-                if (tok > plast || (tok + 15 < q.lo && tok >= a.sinks)) continue;
-                const long page = kv_page(a.c, a.s, b, tok);
+                const int page = __shfl_sync(0xffffffffu, ids, 2 * (k - kb) + x);
                 if (page < 0) {
-                    if (lane == 0) atomicOr(a.c.err, ERR_PAGE);
+                    if (page == -2 && lane == 0) atomicOr(a.c.err, ERR_PAGE);
                     continue;
                 }
                 has |= 1u << x;
-                const size_t row = kv_row(a.c, page, h, tok);
+                const size_t row = kv_row(a.c, page, h, off + 16 * x);
                 unsigned char *st = ring + slot_in * F::STAGE + x * (16 * F::ROW) + lane * 16;
                 const unsigned char *kq = reinterpret_cast<const unsigned char *>(a.c.kq) + row * F::ROW + lane * 16;
                 const unsigned char *vq = reinterpret_cast<const unsigned char *>(a.c.vq) + row * F::ROW + lane * 16;
@@ -250,20 +255,36 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
         }
         cp_commit();
     };
-    int k1 = (int)min((long)q.nb, k0 + (ue - u));
+    int k1 = (int)min((long)q.nb, k0 + (ue - u)), kb = k0;
+    int ids = pages(q, b, kb, k1);
 #pragma unroll 1
-    for (int i = 0; i < FS; ++i) issue(q, b, h, k0 + i, k1);
+    for (int i = 0; i < FS; ++i) issue(q, h, k0 + i, k1, ids, kb);
 
     while (true) {
         // ---- one run of blocks [k0, k1) of (b, h), whose first copies are on their way
         const int p0 = q.L - q.n, plast = q.L - 1;  // positions of the first and the last row
+        // the next run: where it is and its first page ids, in time for its copies
+        const bool first_run = u == us;
+        u += k1 - k0;
+        const bool more = u < ue;
+        FewSeq qn = q;
+        int bn = b, hn = h + 1, kn = 0, idn = -1;
+        if (more) {
+            if (hn == a.c.Hkv) {
+                hn = 0;
+                do qn = few_seq<NC>(a, ++bn);
+                while (qn.nb == 0);
+            }
+            kn = (int)min((long)qn.nb, ue - u);
+            idn = pages(qn, bn, 0, kn);
+        }
         // ---- queries: column nt * 8 + r is row (column / Gq) of the sequence, head h * Gq + column % Gq
         uint32_t qf[NT][D / 16][2];
         float qs[NT][FMT == FMT_Q4 ? NG : 1][2], cs[NT][2];
         int pos[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int col = nt * 8 + r, i = col / a.Gq;
+            const int col = nt * 8 + r, i = kv_div(col, a.Gdiv);
             const bool have = i < q.n;
             const uint16_t *src = a.q + (have ? (q.r0 + i) * a.q_row + (h * a.Gq + col - i * a.Gq) * a.q_head : 0);
             uint4 w[D / 32];
@@ -326,7 +347,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 cs[nt][e] = fmaxf(__shfl_sync(0xffffffffu, mul, 8 * c + 4 * e), 1.2e-38f);  // above zero: a hidden -inf stays -inf
-                const int ce = nt * 8 + 2 * c + e, ie = ce / a.Gq;
+                const int ce = nt * 8 + 2 * c + e, ie = kv_div(ce, a.Gdiv);
                 pos[nt][e] = ie < q.n ? p0 + ie : -1;  // a column without a row sees nothing
             }
         }
@@ -595,25 +616,17 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
             if (all) step(std::true_type{});
             else if (has) step(std::false_type{});
             __syncwarp();
-            issue(q, b, h, k + FS, k1);
+            if (k + FS == kb + 16) {
+                kb = k + FS;
+                ids = pages(q, b, kb, k1);
+            }
+            issue(q, h, k + FS, k1, ids, kb);
             if (++slot == FS) slot = 0;
         }
-        // ---- the next run: its first copies go out before this one's warps join
-        const int h_ = h, k0_ = k0, k1_ = k1;
-        const bool first_run = u == us;
-        u += k1 - k0;
-        const bool more = u < ue;
-        FewSeq qn = q;
+        // ---- the next run's first copies go out before this one's warps join
         if (more) {
-            k0 = 0;
-            if (++h == a.c.Hkv) {
-                h = 0;
-                do qn = few_seq<NC>(a, ++b);
-                while (qn.nb == 0);
-            }
-            k1 = (int)min((long)qn.nb, ue - u);
 #pragma unroll 1
-            for (int i = 0; i < FS; ++i) issue(qn, b, h, i, k1);
+            for (int i = 0; i < FS; ++i) issue(qn, hn, i, kn, idn, 0);
         }
 
         // ---- the warps' sums join in shared memory; m becomes what the weights are relative to
@@ -661,7 +674,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
             }
         }
         __syncthreads();
-        const bool whole = k0_ == 0 && k1_ == q.nb;
+        const bool whole = k0 == 0 && k1 == q.nb;
         float *pt = part + ((size_t)blockIdx.x * 2 + (first_run ? 0 : 1)) * (NC * (D + 2));
         for (int i = threadIdx.x; i < q.n * a.Gq * (D / 4); i += FT) {
             const int col = i / (D / 4), d4 = i % (D / 4);
@@ -680,7 +693,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
                 L += s_l[x][col] * ex2(s_m[x][col] - use);
             }
             if (whole) {
-                const int ri = col / a.Gq, head = h_ * a.Gq + col - ri * a.Gq;
+                const int ri = kv_div(col, a.Gdiv), head = h * a.Gq + col - ri * a.Gq;
                 kv_finish<D>(a, q.r0 + ri, head, d4, v, M, L);
             } else {
                 *reinterpret_cast<float4 *>(pt + col * D + 4 * d4) = v;
@@ -689,6 +702,11 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 4 : 3) k_kv_attn_few(const KvAtt
         }
         if (!more) break;
         q = qn;
+        b = bn;
+        h = hn;
+        k0 = kb = 0;
+        k1 = kn;
+        ids = idn;
         __syncthreads();
     }
 }
@@ -749,7 +767,7 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a, const 
         v.w += w.w * f;
         L += s_l[i] * f;
     }
-    const int ri = col / a.Gq;
+    const int ri = kv_div(col, a.Gdiv);
     kv_finish<D>(a, q.r0 + ri, h * a.Gq + col - ri * a.Gq, threadIdx.x, v, M, L);
 }
 
