@@ -12,13 +12,12 @@
 // A warp takes 32 keys of each block, straight from a cp.async ring of its own (no block-wide barrier in the loop; the next
 // run's first copies are on their way while a run's warps join; bulk copies from single lanes cost twice the instructions), and
 // feeds the codes to mma.sync m16n8k16 without dequantizing them:
-//   scores^T [16 keys x NC] = K codes . q. int4: 128 + code is one bf16 operation away (code | 0x4300), so with group g's
-//     scale s and bias b, score = sum_g s (acc_g - 128 qsum_g) + b qsum_g in fp32. MXFP4: E2M1 codes convert to fp16, q is
-//     taken to fp16 with a power of two per row (8 bits of significand fit 11), score = sum_g 2^e acc_g.
+//   scores^T [16 keys x NC] = K codes . q, q in fp16 after a power of two per row (8 bits of significand fit 11). int4: a
+//     masked code is an fp16 subnormal, code * 2^-24, so that an operand costs one instruction; with group g's scale s and bias
+//     b, score = sum_g s acc_g + b qsum_g in fp32. MXFP4: E2M1 codes convert to fp16, score = sum_g 2^e acc_g.
 //   y^T [D x NC] += V^T codes . P, P = fp16(p * scale of the key's group). A running power of two per warp, taken into p's
-//     exponent, keeps the product in fp16's range whatever the values' size; codes - 8 (int4) or E2M1 in fp16, exact. fp16 and not
-//     bf16: P is the only rounding here, 2^-11 keeps it below the result's own 2^-8. int4's bias term is summed in fp32
-//     (b + 8 s, so that neither sum is a small difference of large ones).
+//     exponent, keeps the product in fp16's range whatever the values' size; codes as subnormals (int4) or E2M1 in fp16, exact. fp16 and not
+//     bf16: P is the only rounding here, 2^-11 keeps it below the result's own 2^-8. int4's bias term is summed in fp32.
 // Softmax statistics and sums are fp32; a column's maximum is shared by the warp's lanes (three shuffles), warps join at
 // the end of a run of blocks. MMA row r is key r / 2 + 4 (r % 2) of its eight, which makes the four keys of a lane's V
 // operand consecutive rows of shared memory (no bank conflicts) and costs K nothing.
@@ -75,13 +74,21 @@ MOEB_DEV void e8m0_2(uint32_t two, float &lo, float &hi) {
     lo = bf16lo(r);
     hi = bf16hi(r);
 }
+MOEB_DEV float h2_sum(uint32_t v) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+    return f.x + f.y;
+}
+MOEB_DEV uint32_t h2_mul(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
 MOEB_DEV uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// A key's parameters in fp32. int4: scale, and bias + c scale; MXFP4: the powers of two.
+// A key's parameters in fp32. int4: scale and bias; MXFP4: the powers of two.
 template <int FMT, int NG>
-MOEB_DEV void few_params(const unsigned char *p, float c, float (&s)[NG], float (&b)[NG]) {
+MOEB_DEV void few_params(const unsigned char *p, float (&s)[NG], float (&b)[NG]) {
     if (FMT == FMT_Q4) {
         uint32_t w[2];
         if (NG == 2) {
@@ -94,7 +101,7 @@ MOEB_DEV void few_params(const unsigned char *p, float c, float (&s)[NG], float 
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             s[g] = bf16lo(w[g]);
-            b[g] = fmaf(c, s[g], bf16hi(w[g]));
+            b[g] = bf16hi(w[g]);
         }
     } else {
         const uint32_t w = NG == 4 ? *reinterpret_cast<const uint32_t *>(p) : *reinterpret_cast<const uint16_t *>(p);
@@ -105,20 +112,14 @@ MOEB_DEV void few_params(const unsigned char *p, float c, float (&s)[NG], float 
         }
     }
 }
-// codes - 8 of nibble P of both halves of t, as f16x2: 1024 + q or 1024 + 16 q by one lop3, then one exact operation
+MOEB_DEV void few_copy(unsigned smem, const unsigned char *gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
+// int4 codes of nibble P of both halves of t as f16x2 subnormals: code * 2^-24 (P even) or code * 2^-20 (P odd), exact and
+// without an operation on them but the mask
 template <int P>
-MOEB_DEV uint32_t q4_f16x2(uint32_t t) {
-    const uint32_t s = P & 2 ? t >> 8 : t;
-    uint32_t r;
-    __half2 v;
-    if (P & 1) {
-        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(s), "r"(0x00F000F0u), "r"(0x64006400u));
-        v = __hfma2(*reinterpret_cast<__half2 *>(&r), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
-    } else {
-        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(s), "r"(0x000F000Fu), "r"(0x64006400u));
-        v = __hadd2(*reinterpret_cast<__half2 *>(&r), __float2half2_rn(-1032.f));
-    }
-    return *reinterpret_cast<uint32_t *>(&v);
+MOEB_DEV uint32_t q4_sub(uint32_t t) {
+    return (P & 2 ? t >> 8 : t) & (P & 1 ? 0x00F000F0u : 0x000F000Fu);
 }
 
 // One sequence as the kernels see it: its rows, and the blocks of FB keys that any of them sees.
@@ -219,12 +220,20 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
         const long page = kv_page(a.c, a.s, b, tok);
         return page < 0 ? -2 : (int)page;
     };
-    // Copies of this warp's 32 keys of block k of head h. ok: bit 2 s + x says that half x of stage s has come.
+    // Copies of this warp's 32 keys of block k of head h. ok: bit 2 s + x says that half x of stage s has come. Addresses are
+    // the lane's place in the arrays' first page, and one 64-bit product for codes and one for parameters per half.
     unsigned ok = 0;
     int slot_in = 0, slot = 0;  // stage of the next copy, of the next use
+    const unsigned per_page = (unsigned)a.c.Hkv << a.c.pshift, pmask = (1u << a.c.pshift) - 1u;  // rows
+    const unsigned char *kq = reinterpret_cast<const unsigned char *>(a.c.kq) + lane * 16, *vq = reinterpret_cast<const unsigned char *>(a.c.vq) + lane * 16;
+    // lanes 0 .. PROW - 1: K's parameters, the next as many V's
+    const bool parv = lane >= F::PROW;
+    const unsigned char *pq = static_cast<const unsigned char *>(parv ? a.c.vs : a.c.ks) + (parv ? lane - F::PROW : lane) * 16;
+    const unsigned st0 = smem_u32(ring) + lane * 16, sp0 = smem_u32(ring) + (parv ? F::O_VP + (lane - F::PROW) * 16 : F::O_KP + lane * 16);
     auto issue = [&](const FewSeq &q, int h, int k, int k1, int ids, int kb) {
         if (k < k1) {
-            const int off = few_tok(q, k) + 32 * warp;
+            const unsigned row0 = ((unsigned)h << a.c.pshift) + ((unsigned)(few_tok(q, k) + 32 * warp) & pmask);
+            const unsigned stage = slot_in * F::STAGE;
             unsigned has = 0;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
@@ -234,21 +243,17 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                     continue;
                 }
                 has |= 1u << x;
-                const size_t row = kv_row(a.c, page, h, off + 16 * x);
-                unsigned char *st = ring + slot_in * F::STAGE + x * (16 * F::ROW) + lane * 16;
-                const unsigned char *kq = reinterpret_cast<const unsigned char *>(a.c.kq) + row * F::ROW + lane * 16;
-                const unsigned char *vq = reinterpret_cast<const unsigned char *>(a.c.vq) + row * F::ROW + lane * 16;
+                // a page of 16 keys: the second half starts at its page's first row
+                const unsigned row = x == 0 ? row0 : ((unsigned)h << a.c.pshift) + ((unsigned)(few_tok(q, k) + 32 * warp + 16) & pmask);
+                const size_t at = (size_t)(unsigned)page * per_page + row;
+                const unsigned char *ks = kq + at * F::ROW, *vs = vq + at * F::ROW;
+                const unsigned st = st0 + stage + x * (16 * F::ROW);
 #pragma unroll
                 for (int i = 0; i < F::ROW / 32; ++i) {
-                    cp_async16(st + i * 512, kq + i * 512);
-                    cp_async16(st + F::O_V + i * 512, vq + i * 512);
+                    few_copy(st + i * 512, ks + i * 512);
+                    few_copy(st + F::O_V + i * 512, vs + i * 512);
                 }
-                if (lane < 2 * F::PROW) {  // lanes 0 .. PROW - 1: K's parameters, the next as many V's
-                    const bool v = lane >= F::PROW;
-                    const int i = v ? lane - F::PROW : lane;
-                    cp_async16(ring + slot_in * F::STAGE + (v ? F::O_VP : F::O_KP) + x * (16 * F::PROW) + i * 16,
-                               static_cast<const unsigned char *>(v ? a.c.vs : a.c.ks) + row * F::PROW + i * 16);
-                }
+                if (lane < 2 * F::PROW) few_copy(sp0 + stage + x * (16 * F::PROW), pq + at * F::PROW);
             }
             ok = (ok & ~(3u << (2 * slot_in))) | has << (2 * slot_in);
             if (++slot_in == FS) slot_in = 0;
@@ -294,13 +299,17 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                 const int word = FMT == FMT_Q4 ? 8 * (j >> 1) + 2 * c + (j & 1) : 4 * j + c;
                 w[j] = have ? *reinterpret_cast<const uint4 *>(src + 8 * word) : make_uint4(0, 0, 0, 0);
             }
+            float qsum[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) qsum[g] = 0.f;
             // the scale's sign goes into q, so that the maximum can be taken before scaling; a scale of zero makes q zero
             const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
             float mul = a.scale == 0.f ? 1.f : fabsf(a.scale);
 #pragma unroll
             for (int j = 0; j < D / 32; ++j)
                 w[j] = a.scale == 0.f ? make_uint4(0, 0, 0, 0) : make_uint4(w[j].x ^ flip, w[j].y ^ flip, w[j].z ^ flip, w[j].w ^ flip);
-            if (FMT == FMT_FP4) {  // to fp16 by the row's power of two: its largest value near 2^8
+            {  // to fp16 by the row's power of two: its largest value near 2^14 (int4), 2^8 (MXFP4)
+                constexpr int UP = FMT == FMT_Q4 ? 14 : 8;
                 uint32_t t16 = 0;
 #pragma unroll
                 for (int j = 0; j < D / 32; ++j) {
@@ -310,14 +319,21 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                 }
                 t16 = max(t16, __shfl_xor_sync(0xffffffffu, t16, 1));
                 t16 = max(t16, __shfl_xor_sync(0xffffffffu, t16, 2));
-                const int e = min(max((int)(t16 >> 7), 9), 254);           // biased exponent of the largest value
-                const float down = __uint_as_float((uint32_t)(262 - e) << 23);  // 2^(8 - (e - 127))
-                mul *= __uint_as_float((uint32_t)(e - 8) << 23);
+                const int e = min(max((int)(t16 >> 7), UP + 1), 254);  // biased exponent of the largest value
+                const float down = __uint_as_float((uint32_t)(254 + UP - e) << 23);  // 2^(UP - (e - 127))
+                // what undoes it; int4: and 2^24 for the codes, taken out of qsum below
+                mul *= __uint_as_float((uint32_t)(e - UP) << 23) * (FMT == FMT_Q4 ? 16777216.f : 1.f);
 #pragma unroll
                 for (int j = 0; j < D / 32; ++j) {
                     uint32_t ww[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) ww[x] = pack_h2(bf16lo(ww[x]) * down, bf16hi(ww[x]) * down);
+                    if (FMT == FMT_Q4) {
+                        qsum[j / 2 < NG ? j / 2 : 0] += h2_sum(ww[0]) + h2_sum(ww[1]) + h2_sum(ww[2]) + h2_sum(ww[3]);
+                        // the odd pairs meet codes * 2^-20: words 1 and 3 hold values 2, 3 and 6, 7 of eight
+                        ww[1] = h2_mul(ww[1], 0x2C002C00u);
+                        ww[3] = h2_mul(ww[3], 0x2C002C00u);
+                    }
                     w[j] = make_uint4(ww[0], ww[1], ww[2], ww[3]);
                 }
             }
@@ -331,13 +347,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
             if (FMT == FMT_Q4) {
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    float t = 0.f;
-#pragma unroll
-                    for (int j = 2 * g; j < 2 * g + 2; ++j) {
-                        const uint32_t ww[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) t += bf16lo(ww[e]) + bf16hi(ww[e]);
-                    }
+                    float t = qsum[g] * 5.9604644775390625e-8f;  // 2^-24
                     t += __shfl_xor_sync(0xffffffffu, t, 1);
                     t += __shfl_xor_sync(0xffffffffu, t, 2);
                     qs[nt][g][0] = __shfl_sync(0xffffffffu, t, 8 * c);
@@ -397,8 +407,8 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                         wb[0] = z.x; wb[1] = z.y;
                     }
                     float xa[NG], ya[NG], xb[NG], yb[NG];
-                    few_params<FMT, NG>(st + F::O_KP + (16 * x + ta) * F::PROW, -128.f, xa, ya);
-                    few_params<FMT, NG>(st + F::O_KP + (16 * x + ta + 8) * F::PROW, -128.f, xb, yb);
+                    few_params<FMT, NG>(st + F::O_KP + (16 * x + ta) * F::PROW, xa, ya);
+                    few_params<FMT, NG>(st + F::O_KP + (16 * x + ta + 8) * F::PROW, xb, yb);
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         float acc[NT][4];
@@ -408,10 +418,11 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
 #pragma unroll
                             for (int y = 0; y < 4; ++y) {
                                 const uint32_t ua = wa[(y >> 1) * NG + g], ub = wb[(y >> 1) * NG + g];
-                                const int p = 2 * (y & 1);
-                                const uint32_t A[4] = {q4pair(ua, p), q4pair(ub, p), q4pair(ua, p + 1), q4pair(ub, p + 1)};
+                                uint32_t A[4];
+                                if (y & 1) { A[0] = q4_sub<2>(ua); A[1] = q4_sub<2>(ub); A[2] = q4_sub<3>(ua); A[3] = q4_sub<3>(ub); }
+                                else { A[0] = q4_sub<0>(ua); A[1] = q4_sub<0>(ub); A[2] = q4_sub<1>(ua); A[3] = q4_sub<1>(ub); }
 #pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt], A, qf[nt][4 * g + y][0], qf[nt][4 * g + y][1]);
+                                for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt], A, qf[nt][4 * g + y][0], qf[nt][4 * g + y][1]);
                             }
                         } else {
                             // half-words 2 c (product 0) and 2 c + 1 of the group
@@ -449,8 +460,8 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                 unsigned vis[NT];  // bit 4 x + 2 i + e: column 2 c + e sees key 16 x + ta + 8 i
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    few_params<FMT, NG>(st + F::O_VP + (16 * x + ta) * F::PROW, 8.f, va[x], ba[x]);
-                    few_params<FMT, NG>(st + F::O_VP + (16 * x + ta + 8) * F::PROW, 8.f, vb[x], bb[x]);
+                    few_params<FMT, NG>(st + F::O_VP + (16 * x + ta) * F::PROW, va[x], ba[x]);
+                    few_params<FMT, NG>(st + F::O_VP + (16 * x + ta + 8) * F::PROW, vb[x], bb[x]);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) vis[nt] = 0xffu;
@@ -587,10 +598,10 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
 #pragma unroll
                             for (int p = 0; p < 4; ++p) {
                                 uint32_t A[4];
-                                if (p == 0) { A[0] = q4_f16x2<0>(l0); A[1] = q4_f16x2<0>(h0); A[2] = q4_f16x2<0>(l1); A[3] = q4_f16x2<0>(h1); }
-                                if (p == 1) { A[0] = q4_f16x2<1>(l0); A[1] = q4_f16x2<1>(h0); A[2] = q4_f16x2<1>(l1); A[3] = q4_f16x2<1>(h1); }
-                                if (p == 2) { A[0] = q4_f16x2<2>(l0); A[1] = q4_f16x2<2>(h0); A[2] = q4_f16x2<2>(l1); A[3] = q4_f16x2<2>(h1); }
-                                if (p == 3) { A[0] = q4_f16x2<3>(l0); A[1] = q4_f16x2<3>(h0); A[2] = q4_f16x2<3>(l1); A[3] = q4_f16x2<3>(h1); }
+                                if (p == 0) { A[0] = q4_sub<0>(l0); A[1] = q4_sub<0>(h0); A[2] = q4_sub<0>(l1); A[3] = q4_sub<0>(h1); }
+                                if (p == 1) { A[0] = q4_sub<1>(l0); A[1] = q4_sub<1>(h0); A[2] = q4_sub<1>(l1); A[3] = q4_sub<1>(h1); }
+                                if (p == 2) { A[0] = q4_sub<2>(l0); A[1] = q4_sub<2>(h0); A[2] = q4_sub<2>(l1); A[3] = q4_sub<2>(h1); }
+                                if (p == 3) { A[0] = q4_sub<3>(l0); A[1] = q4_sub<3>(h0); A[2] = q4_sub<3>(l1); A[3] = q4_sub<3>(h1); }
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * g + p], A, pf[nt][g][0], pf[nt][g][1]);
                             }
@@ -667,8 +678,9 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                     const int dim = FMT == FMT_Q4 ? 64 * (i >> 2) + 8 * r + 2 * (i & 3) : 32 * (i >> 1) + 4 * r + 2 * (i & 1);
                     const float add = FMT == FMT_Q4 ? bs[nt][i >> 2 < NG ? i >> 2 : 0][e] : 0.f;
                     float2 v;
-                    v.x = (o[nt][i][e] + add) * fm;
-                    v.y = (o[nt][i][2 + e] + add) * fm;
+                    const float up = FMT == FMT_FP4 ? 1.f : i & 1 ? 1048576.f : 16777216.f;  // codes were * 2^-20, 2^-24
+                    v.x = fmaf(o[nt][i][e], up, add) * fm;
+                    v.y = fmaf(o[nt][i][2 + e], up, add) * fm;
                     *reinterpret_cast<float2 *>(dst + dim) = v;
                 }
             }

@@ -72,10 +72,10 @@ class Batch:
         step of int4, at most 2/15 of the largest |k|, so below 2^-11 scale |q|_1 max|k| / 7). A score moved by e moves the
         weighted mean by at most 2 e A.
 
-        The probabilities' rounding, for int4: a value is s (code - 8) + (b + 8 s), the second part is summed in fp32, so what
-        a rounded p scales is s (code - 8), not the value: at most 8 s, and s <= (max - min) / 15 <= 2 / 15 of the group's
-        largest |v|. So that term is 2^-11 sum_j p_j 16 / 15 max_group |v_j|, which is more than 2^-11 A where a value lies
-        near zero in a group that does not (the step s of the stored value itself is 2^8 times that)."""
+        The probabilities' rounding, for int4: a value is s code + b, the second part is summed in fp32, so what a rounded p
+        scales is s code, not the value: at most 15 s, and s <= (max - min) / 15 <= 2 / 15 of the group's largest |v|. So that
+        term is 2^-11 sum_j p_j 2 max_group |v_j|, which is more than 2^-11 A where a value lies near zero in a group that does
+        not (the step s of the stored value itself is 2^7 times that)."""
         scale = self.D ** -0.5 if scale is None else scale
         G = self.H // self.Hkv
         y = torch.zeros(self.T, self.H, self.D, dtype=torch.float64)
@@ -109,7 +109,7 @@ class Batch:
                 Ap = A
                 if self.fmt == "q4":
                     top = vv.abs().nan_to_num().unflatten(-1, (-1, 64)).amax(-1, keepdim=True)
-                    Ap = p @ top.expand(-1, -1, 64).flatten(1) * (16 / 15)
+                    Ap = p @ top.expand(-1, -1, 64).flatten(1) * 2
                 e = (qq.abs() @ kk.abs().T * scale).masked_fill(~see, 0.0).amax(-1, keepdim=True) if L else 0.0
                 e = U_FP16 * e + U_FP16 / 7 * scale * qq.abs().sum(-1, keepdim=True) * (kk.abs().max() if L else 0.0)
                 bound[at:at + n, h] = (U_BF16 * out.abs() + ((2 * e + U_FP16 + 2.0 ** -15) * A + U_FP16 * Ap) * (1 + U_BF16)).cpu() + 1e-30
