@@ -147,8 +147,8 @@ int launch_few(const KvAttnArgs &a, void *ws, cudaStream_t st) {
     const FewLayout l = few_layout(a.s.B, 8 * NT, D);
     int *pre = (int *)ws;
     float *part = (float *)((char *)ws + l.part);
-    // at most one block of 128 keys per CTA: the page tables' width bounds the blocks (the first tokens' may be cut twice)
-    const long most = (long)a.s.B * a.c.Hkv * ((((long)a.s.P << a.c.pshift) >> 7) + 2);
+    // at most one block of 128 keys per CTA: the page tables' width bounds the blocks, each (sequence, head) has 2 more in the count
+    const long most = (long)a.s.B * a.c.Hkv * ((((long)a.s.P << a.c.pshift) >> 7) + 4);
     const int grid = (int)(most < (long)per * sms() ? most : (long)per * sms());
     cudaError_t e = launch(k_kv_attn_few<FMT, D, NT>, dim3(grid), 128, smem, st, a, pre, part);
     if (e == cudaSuccess)

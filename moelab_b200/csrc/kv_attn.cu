@@ -6,7 +6,8 @@
 //
 // Work split: the visible keys of every (sequence, KV head) are cut into blocks of 128; all blocks of the call in a row are
 // dealt to the CTAs in equal runs, so uneven lengths cost nothing and the host needs to know none of them (a captured
-// graph replays with other lengths). A CTA that holds all blocks of a (sequence, head) writes y; otherwise it leaves its
+// graph replays with other lengths). A run's start and end cost about as much as FR blocks, which each (sequence, head) has in
+// the count before its first one (without them CTAs with many short sequences end last). A CTA that holds all blocks of a (sequence, head) writes y; otherwise it leaves its
 // unnormalised sum, maximum and sum of weights, and k_kv_attn_join joins them.
 //
 // A warp takes 32 keys of each block, straight from a cp.async ring of its own (no block-wide barrier in the loop; the next
@@ -32,6 +33,7 @@ namespace {
 constexpr int FW = 4, FT = 32 * FW;  // warps per CTA, threads
 constexpr int FS = 3;                // ring stages
 constexpr int FB = 32 * FW;          // keys per block
+constexpr int FR = 2;                // blocks that a run costs besides its own
 
 template <int FMT, int D>
 struct Few {
@@ -141,6 +143,7 @@ MOEB_DEV FewSeq few_seq(const KvAttnArgs &a, int b) {
     q.nb = q.n > 0 && (long)q.n * a.Gq <= NC ? max(q.ns + (int)(((long)q.L + FB - 1) / FB) - q.lo / FB, 1) : 0;
     return q;
 }
+MOEB_DEV int few_units(const FewSeq &q) { return q.nb ? q.nb + FR : 0; }  // of each of its heads
 MOEB_DEV int few_tok(const FewSeq &q, int k) { return (k < q.ns ? k : q.lo / FB + k - q.ns) * FB; }
 MOEB_DEV long few_start(long W, long c, long n) { return W * c / n; }
 
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
     // every sequence's blocks: prefix sums over the CTA's threads, and the sequence of this CTA's first block
     const int per = (a.s.B + FT - 1) / FT, bb0 = min((int)threadIdx.x * per, a.s.B), bb1 = min(bb0 + per, a.s.B);
     int mine = 0;
-    for (int b = bb0; b < bb1; ++b) mine += few_seq<NC>(a, b).nb;
+    for (int b = bb0; b < bb1; ++b) mine += few_units(few_seq<NC>(a, b));
     int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -183,18 +186,17 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
         for (int b = bb0; b < bb1; ++b) {
             const FewSeq s = few_seq<NC>(a, b);
             pre[b] = at;
-            at += s.nb;
+            at += few_units(s);
             if (a.only && s.n * a.Gq > NC) atomicOr(a.c.err, ERR_ROWS);
         }
         if (threadIdx.x == 0) pre[a.s.B] = total;
     }
     if ((long)blockIdx.x >= nct) return;
-    long u = few_start(units, blockIdx.x, nct);
-    const long ue = few_start(units, blockIdx.x + 1, nct), us = u;
+    const long us = few_start(units, blockIdx.x, nct), ue = few_start(units, blockIdx.x + 1, nct), u = us;
     if (u >= (long)base * a.c.Hkv && u < (long)(base + mine) * a.c.Hkv) {
         int at = base, b = bb0;
         for (;; ++b) {
-            const int nb = few_seq<NC>(a, b).nb;
+            const int nb = few_units(few_seq<NC>(a, b));
             if (u < (long)(at + nb) * a.c.Hkv) break;
             at += nb;
         }
@@ -205,11 +207,28 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
     int b = s_b, h;
     FewSeq q = few_seq<NC>(a, b);
     int k0;
-    {
-        const int off = (int)(u - (long)s_pre * a.c.Hkv);
-        h = off / q.nb;
-        k0 = off - h * q.nb;
-    }
+    // blocks [k0, k1) of the first run; a CTA whose share of a (sequence, head) is in its FR has none of its blocks
+    long seg = (long)s_pre * a.c.Hkv;  // first unit of the run's (sequence, head)
+    int k1;
+    auto locate = [&](bool next) {
+        for (;; next = true) {
+            if (next) {
+                seg += q.nb + FR;
+                if (++h == a.c.Hkv) {
+                    h = 0;
+                    do q = few_seq<NC>(a, ++b);
+                    while (q.nb == 0);
+                }
+            }
+            k0 = (int)max(us - seg - FR, 0L);
+            k1 = (int)min(ue - seg - FR, (long)q.nb);
+            if (k1 > k0 || ue <= seg + q.nb + FR) return;
+        }
+    };
+    h = (int)((us - seg) / (q.nb + FR));
+    seg += (long)h * (q.nb + FR);
+    locate(false);
+    if (k1 <= k0) return;
     const int ta = (r >> 1) + 4 * (r & 1);  // this lane's keys of 16: ta and ta + 8
 
     // Page ids of 16 blocks from kb on: lane 2 i + x has half x (16 keys, a page at least) of this warp's keys of block kb + i.
@@ -260,7 +279,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
         }
         cp_commit();
     };
-    int k1 = (int)min((long)q.nb, k0 + (ue - u)), kb = k0;
+    int kb = k0;
     int ids = pages(q, b, kb, k1);
 #pragma unroll 1
     for (int i = 0; i < FS; ++i) issue(q, h, k0 + i, k1, ids, kb);
@@ -269,19 +288,16 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
         // ---- one run of blocks [k0, k1) of (b, h), whose first copies are on their way
         const int p0 = q.L - q.n, plast = q.L - 1;  // positions of the first and the last row
         // the next run: where it is and its first page ids, in time for its copies
-        const bool first_run = u == us;
-        u += k1 - k0;
-        const bool more = u < ue;
-        FewSeq qn = q;
-        int bn = b, hn = h + 1, kn = 0, idn = -1;
+        const FewSeq qr = q;
+        const int hr = h, kr0 = k0, kr1 = k1;
+        const long segr = seg;
+        const int br = b;
+        bool more = ue > seg + q.nb + FR;
+        int idn = -1;
         if (more) {
-            if (hn == a.c.Hkv) {
-                hn = 0;
-                do qn = few_seq<NC>(a, ++bn);
-                while (qn.nb == 0);
-            }
-            kn = (int)min((long)qn.nb, ue - u);
-            idn = pages(qn, bn, 0, kn);
+            locate(true);
+            more = k1 > k0;
+            if (more) idn = pages(q, b, k0, k1);
         }
         // ---- queries: column nt * 8 + r is row (column / Gq) of the sequence, head h * Gq + column % Gq
         uint32_t qf[NT][D / 16][2];
@@ -290,8 +306,8 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int col = nt * 8 + r, i = kv_div(col, a.Gdiv);
-            const bool have = i < q.n;
-            const uint16_t *src = a.q + (have ? (q.r0 + i) * a.q_row + (h * a.Gq + col - i * a.Gq) * a.q_head : 0);
+            const bool have = i < qr.n;
+            const uint16_t *src = a.q + (have ? (qr.r0 + i) * a.q_row + (hr * a.Gq + col - i * a.Gq) * a.q_head : 0);
             uint4 w[D / 32];
             // words of this lane: int4 2 c, 2 c + 1 of every group of 64; MXFP4 c of every group of 32
 #pragma unroll
@@ -358,7 +374,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
             for (int e = 0; e < 2; ++e) {
                 cs[nt][e] = fmaxf(__shfl_sync(0xffffffffu, mul, 8 * c + 4 * e), 1.2e-38f);  // above zero: a hidden -inf stays -inf
                 const int ce = nt * 8 + 2 * c + e, ie = kv_div(ce, a.Gdiv);
-                pos[nt][e] = ie < q.n ? p0 + ie : -1;  // a column without a row sees nothing
+                pos[nt][e] = ie < qr.n ? p0 + ie : -1;  // a column without a row sees nothing
             }
         }
 
@@ -379,12 +395,12 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
         float vexp = 0.f;   // its exponent: weights are 2^(score - m + vexp), and o, l and bs are sums of them
 
 #pragma unroll 1
-        for (int k = k0; k < k1; ++k) {
+        for (int k = kr0; k < kr1; ++k) {
             cp_wait<FS - 1>();
             __syncwarp();
             const unsigned has = (ok >> (2 * slot)) & 3u;
             const unsigned char *st = ring + slot * F::STAGE;
-            const int tok = few_tok(q, k) + 32 * warp;
+            const int tok = few_tok(qr, k) + 32 * warp;
             const bool all = has == 3u && tok + 31 <= p0 && (!a.window || tok > plast - a.window || tok + 31 < a.sinks);
             // full: every row sees all 32 keys
             auto step = [&](auto full_) {
@@ -470,7 +486,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                     for (int x = 0; x < 2; ++x) {
                         const int ja = tok + 16 * x + ta, jb = ja + 8;
                         const bool half = (has >> x) & 1u;
-                        const bool sa = half && ja <= plast && (ja >= q.lo || ja < a.sinks), sb = half && jb <= plast && (jb >= q.lo || jb < a.sinks);
+                        const bool sa = half && ja <= plast && (ja >= qr.lo || ja < a.sinks), sb = half && jb <= plast && (jb >= qr.lo || jb < a.sinks);
 #pragma unroll
                         for (int g = 0; g < NG; ++g) {
                             va[x][g] = sa ? va[x][g] : 0.f;
@@ -629,15 +645,15 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
             __syncwarp();
             if (k + FS == kb + 16) {
                 kb = k + FS;
-                ids = pages(q, b, kb, k1);
+                ids = pages(qr, br, kb, kr1);
             }
-            issue(q, h, k + FS, k1, ids, kb);
+            issue(qr, hr, k + FS, kr1, ids, kb);
             if (++slot == FS) slot = 0;
         }
         // ---- the next run's first copies go out before this one's warps join
         if (more) {
 #pragma unroll 1
-            for (int i = 0; i < FS; ++i) issue(qn, hn, i, kn, idn, 0);
+            for (int i = 0; i < FS; ++i) issue(q, h, k0 + i, k1, idn, k0);
         }
 
         // ---- the warps' sums join in shared memory; m becomes what the weights are relative to
@@ -686,9 +702,9 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
             }
         }
         __syncthreads();
-        const bool whole = k0 == 0 && k1 == q.nb;
-        float *pt = part + ((size_t)blockIdx.x * 2 + (first_run ? 0 : 1)) * (NC * (D + 2));
-        for (int i = threadIdx.x; i < q.n * a.Gq * (D / 4); i += FT) {
+        const bool whole = kr0 == 0 && kr1 == qr.nb;
+        float *pt = part + ((size_t)blockIdx.x * 2 + (us >= segr ? 0 : 1)) * (NC * (D + 2));
+        for (int i = threadIdx.x; i < qr.n * a.Gq * (D / 4); i += FT) {
             const int col = i / (D / 4), d4 = i % (D / 4);
             float M = s_m[0][col], L = 0.f;
 #pragma unroll
@@ -705,19 +721,15 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                 L += s_l[x][col] * ex2(s_m[x][col] - use);
             }
             if (whole) {
-                const int ri = kv_div(col, a.Gdiv), head = h * a.Gq + col - ri * a.Gq;
-                kv_finish<D>(a, q.r0 + ri, head, d4, v, M, L);
+                const int ri = kv_div(col, a.Gdiv), head = hr * a.Gq + col - ri * a.Gq;
+                kv_finish<D>(a, qr.r0 + ri, head, d4, v, M, L);
             } else {
                 *reinterpret_cast<float4 *>(pt + col * D + 4 * d4) = v;
                 if (d4 == 0) *reinterpret_cast<float2 *>(pt + NC * D + 2 * col) = make_float2(M, L);
             }
         }
         if (!more) break;
-        q = qn;
-        b = bn;
-        h = hn;
-        k0 = kb = 0;
-        k1 = kn;
+        kb = k0;
         ids = idn;
         __syncthreads();
     }
@@ -732,12 +744,12 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a, const 
     __shared__ float so[8][D];
     pdl_wait();
     const int col = blockIdx.y, h = blockIdx.x % a.c.Hkv, b = blockIdx.x / a.c.Hkv;
-    const int at = pre[b], nb = pre[b + 1] - at;
+    const int at = pre[b], nu = pre[b + 1] - at, nb = nu - FR;
     if (nb < 2) return;  // none, or one block: one CTA had it
     const FewSeq q = few_seq<NC>(a, b);
     if (col >= q.n * a.Gq) return;
     const long units = (long)pre[a.s.B] * a.c.Hkv, n = min((long)grid, units);
-    const long u0 = (long)at * a.c.Hkv + (long)h * nb, u1 = u0 + nb;
+    const long seg = (long)at * a.c.Hkv + (long)h * nu, u0 = seg + FR, u1 = seg + nu;
     const int c0 = (int)(((u0 + 1) * n - 1) / units), c1 = (int)((u1 * n - 1) / units);  // CTAs of the first and last block
     if (c0 == c1) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -746,7 +758,7 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a, const 
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = 0.f;
     for (int x = c0 + warp; x <= c1; x += 8) {
-        const float *pt = part + ((size_t)x * 2 + (few_start(units, x, n) >= u0 ? 0 : 1)) * (NC * (D + 2));
+        const float *pt = part + ((size_t)x * 2 + (few_start(units, x, n) >= seg ? 0 : 1)) * (NC * (D + 2));
         const float2 ml = *reinterpret_cast<const float2 *>(pt + NC * D + 2 * col);
         const float mn = fmaxf(m, ml.x), use = mn == -INFINITY ? 0.f : mn;
         const float f = ex2(m - use), g = ex2(ml.x - use);
