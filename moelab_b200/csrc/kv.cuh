@@ -151,8 +151,9 @@ struct KvAttnArgs {
     unsigned Gdiv;     // ceil(2^32 / Gq), 0 for 1: see kv_div
     float scale;       // of the scores, times log2(e)
     int window, sinks;
-    int few;           // sequences of at most this many (row, head) columns are another kernel's
-    int only;          // the kernel for few rows has the call to itself (longer sequences are an error)
+    int few;           // sequences of at most this many (row, head) columns are the kernel for few rows', the others not
+    int only;          // that kernel has the call to itself (longer sequences are an error)
+    int whole;         // it does not cut a (sequence, head) into parts
     const float *sink_logits;  // [H] or null
     uint16_t *y;       // [T][H][D]
     float *lse;        // [T][H] or null

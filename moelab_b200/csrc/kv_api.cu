@@ -151,7 +151,7 @@ int launch_few(const KvAttnArgs &a, void *ws, cudaStream_t st) {
     const long most = (long)a.s.B * a.c.Hkv * ((((long)a.s.P << a.c.pshift) >> 7) + 4);
     const int grid = (int)(most < (long)per * sms() ? most : (long)per * sms());
     cudaError_t e = launch(k_kv_attn_few<FMT, D, NT>, dim3(grid), 128, smem, st, a, pre, part);
-    if (e == cudaSuccess)
+    if (e == cudaSuccess && !a.whole)
         e = launch(k_kv_attn_join<D, NT>, dim3(a.s.B * a.c.Hkv, a.few), 256, 0, st, a, (const int *)pre, (const float *)part, grid);
     return launched(e, "kv_attention");
 }
@@ -268,10 +268,18 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
     // sequences have T / B rows; with it, and more than one sequence, both kinds may be in the call.
     const long cols = (long)max_q * a.Gq;
     const bool only_few = cols <= 16, both = !only_few && cu && B > 1;
-    a.few = only_few || both ? 16 : 0;
+    a.few = only_few ? (int)cols : both ? 16 : 0;
     if (a.few) {
         const bool one = cols <= 8;
         a.only = only_few;
+        // Up to 4 blocks of 128 keys one after the other cost as much as a second launch to join parts of them. The bound is
+        // known here from the page tables' width, or from the window (its keys may start and end inside a block).
+        long keys = (long)P << a.c.pshift;
+        if (window) {
+            const long seen = (long)window + std::min<long>(max_q, 16) + std::min<long>(sinks, keys);
+            keys = std::min(keys, seen + 128 + (sinks ? 128 : 0));
+        }
+        a.whole = keys <= 512;
         a.few = one ? 8 : 16;
         rc = cache->format == MOEB_KV_Q4
                  ? (cache->head_dim == 64 ? (one ? launch_few<FMT_Q4, 64, 1>(a, ws, stream) : launch_few<FMT_Q4, 64, 2>(a, ws, stream))

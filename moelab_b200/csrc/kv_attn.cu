@@ -140,12 +140,17 @@ MOEB_DEV FewSeq few_seq(const KvAttnArgs &a, int b) {
     const int p0 = max(q.L - q.n, 0);
     q.lo = a.window ? max(p0 - a.window + 1, 0) : 0;
     q.ns = min((min(a.sinks, q.lo) + FB - 1) / FB, q.lo / FB);
-    q.nb = q.n > 0 && (long)q.n * a.Gq <= NC ? max(q.ns + (int)(((long)q.L + FB - 1) / FB) - q.lo / FB, 1) : 0;
+    q.nb = q.n > 0 && (long)q.n * a.Gq <= a.few ? max(q.ns + (int)(((long)q.L + FB - 1) / FB) - q.lo / FB, 1) : 0;
     return q;
 }
 MOEB_DEV int few_units(const FewSeq &q) { return q.nb ? q.nb + FR : 0; }  // of each of its heads
 MOEB_DEV int few_tok(const FewSeq &q, int k) { return (k < q.ns ? k : q.lo / FB + k - q.ns) * FB; }
-MOEB_DEV long few_start(long W, long c, long n) { return W * c / n; }
+// first unit of CTA c when W units are dealt to n CTAs: floor(W c / n), with divisions of 32 bits for all but huge calls
+MOEB_DEV long few_start(long W, unsigned c, unsigned n) {
+    if (W >> 32) return W * c / n;
+    const unsigned w = (unsigned)W, q = w / n, r = w - q * n;
+    return (long)q * c + r * c / n;
+}
 
 }  // namespace
 
@@ -180,18 +185,19 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
         if (i < warp) base += s_sum[i];
         total += s_sum[i];
     }
-    const long units = (long)total * a.c.Hkv, nct = min((long)gridDim.x, units);
+    const long units = (long)total * a.c.Hkv;
+    const unsigned nct = (unsigned)min((long)gridDim.x, units);
     if (blockIdx.x == 0) {
         int at = base;
         for (int b = bb0; b < bb1; ++b) {
             const FewSeq s = few_seq<NC>(a, b);
             pre[b] = at;
             at += few_units(s);
-            if (a.only && s.n * a.Gq > NC) atomicOr(a.c.err, ERR_ROWS);
+            if (a.only && (long)s.n * a.Gq > a.few) atomicOr(a.c.err, ERR_ROWS);
         }
         if (threadIdx.x == 0) pre[a.s.B] = total;
     }
-    if ((long)blockIdx.x >= nct) return;
+    if (blockIdx.x >= nct) return;
     const long us = few_start(units, blockIdx.x, nct), ue = few_start(units, blockIdx.x + 1, nct), u = us;
     if (u >= (long)base * a.c.Hkv && u < (long)(base + mine) * a.c.Hkv) {
         int at = base, b = bb0;
@@ -220,12 +226,17 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                     while (q.nb == 0);
                 }
             }
-            k0 = (int)max(us - seg - FR, 0L);
-            k1 = (int)min(ue - seg - FR, (long)q.nb);
+            if (a.whole) {  // a CTA has the (sequence, head)s that start in its share
+                k0 = 0;
+                k1 = seg >= us && seg < ue ? q.nb : 0;
+            } else {
+                k0 = (int)max(us - seg - FR, 0L);
+                k1 = (int)min(ue - seg - FR, (long)q.nb);
+            }
             if (k1 > k0 || ue <= seg + q.nb + FR) return;
         }
     };
-    h = (int)((us - seg) / (q.nb + FR));
+    h = us - seg < 0x7fffffffL ? (int)((unsigned)(us - seg) / (unsigned)(q.nb + FR)) : (int)((us - seg) / (q.nb + FR));
     seg += (long)h * (q.nb + FR);
     locate(false);
     if (k1 <= k0) return;
@@ -748,7 +759,8 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a, const 
     if (nb < 2) return;  // none, or one block: one CTA had it
     const FewSeq q = few_seq<NC>(a, b);
     if (col >= q.n * a.Gq) return;
-    const long units = (long)pre[a.s.B] * a.c.Hkv, n = min((long)grid, units);
+    const long units = (long)pre[a.s.B] * a.c.Hkv;
+    const unsigned n = (unsigned)min((long)grid, units);
     const long seg = (long)at * a.c.Hkv + (long)h * nu, u0 = seg + FR, u1 = seg + nu;
     const int c0 = (int)(((u0 + 1) * n - 1) / units), c1 = (int)((u1 * n - 1) / units);  // CTAs of the first and last block
     if (c0 == c1) return;
