@@ -1,7 +1,8 @@
 // Writing K and V rows into the 4-bit cache, and reading them back (layout: kv.cuh). Both are one pass over memory. A thread
 // has what one lane of the cache's readers has: the same word of every group of a row (int4: 1 / 8 of the row, MXFP4: 1 / 4),
 // so that its codes are one load or store and the page arithmetic is done once for all of them; and KV_U tokens of one head,
-// so that as many loads are in flight. The lanes of a group reduce its extremes by shuffles.
+// so that as many loads are in flight (one token in calls too small to fill the GPU). The lanes of a group reduce its extremes
+// by shuffles.
 #include "kv.cuh"
 
 namespace moeb {
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
     const long stride = isv ? a.v_row : a.k_row;
     uint32_t *codes = (isv ? a.c.vq : a.c.kq) + w * NG;
     unsigned char *ps = static_cast<unsigned char *>(isv ? a.c.vs : a.c.ks);
-    const int t0 = (int)blockIdx.x * (X::R * KV_U) + (int)threadIdx.x / X::LR;
+    const int t0 = (int)blockIdx.x * (X::R * a.passes) + (int)threadIdx.x / X::LR;
     pdl_wait();
     uint4 next[NG];
     auto fetch = [&](int t) {
@@ -157,12 +158,12 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
     fetch(t0);
     int r0 = 0, r1 = 0, b = -1;
 #pragma unroll 1  // once in the instruction cache
-    for (int i = 0; i < KV_U; ++i) {
+    for (int i = 0; i < a.passes; ++i) {
         const int t = t0 + i * X::R;
         uint4 u[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) u[g] = next[g];
-        if (i + 1 < KV_U) fetch(t + X::R);
+        if (i + 1 < a.passes) fetch(t + X::R);
         long page = -1;
         int p = -1;
         if (t < a.s.T) {
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(128) k_kv_read(const KvReadArgs a) {
     using T = typename Vec<NG>::T;
     const int w = threadIdx.x % X::LR, h = blockIdx.y >> 1;
     const bool isv = blockIdx.y & 1;
-    const int t0 = (int)blockIdx.x * (X::R * KV_U) + (int)threadIdx.x / X::LR;
+    const int t0 = (int)blockIdx.x * (X::R * a.passes) + (int)threadIdx.x / X::LR;
     const uint32_t *codes = (isv ? a.c.vq : a.c.kq) + w * NG;
     const unsigned char *ps = static_cast<const unsigned char *>(isv ? a.c.vs : a.c.ks);
     pdl_wait();
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(128) k_kv_read(const KvReadArgs a) {
 #pragma unroll
     for (int i = 0; i < KV_U; ++i) {
         const int t = t0 + i * X::R;
-        if (t >= a.s.T) continue;
+        if (t >= a.s.T || i >= a.passes) continue;
         if (t >= r1 || t < r0) b = kv_seq_of(a.s, t, r0, r1);
         if (b < 0) continue;
         has |= 1 << i;

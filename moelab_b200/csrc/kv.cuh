@@ -81,7 +81,14 @@ MOEB_DEV int kv_seq_of(const KvSeqs &s, int t, int &r0, int &r1) {
         kv_rows(s, b, r0, r1);
         return b;
     }
-    int lo = 0, hi = s.B;  // the last b with cu[b] <= t
+    // the last b with cu[b] <= t; first where it is when all sequences have as many rows
+    const int guess = (int)((long)t * s.B / s.T);
+    if (s.cu[guess] <= t && t < s.cu[guess + 1] && s.cu[guess + 1] <= s.T && s.cu[guess] >= 0) {
+        r0 = s.cu[guess];
+        r1 = s.cu[guess + 1];
+        return guess;
+    }
+    int lo = 0, hi = s.B;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (s.cu[mid] <= t) lo = mid; else hi = mid;
@@ -135,12 +142,14 @@ struct KvWriteArgs {
     KvSeqs s;
     const uint16_t *k, *v;
     long k_row, k_head, v_row, v_head;  // strides in elements
+    int passes;                         // of a CTA's rows
 };
 struct KvReadArgs {
     KvCache c;
     KvSeqs s;          // s.lens = null: rows start at first[b] (null: 0)
     const int *first;
     uint16_t *k, *v;   // [T][Hkv][D]
+    int passes;
 };
 struct KvAttnArgs {
     KvCache c;
@@ -153,7 +162,7 @@ struct KvAttnArgs {
     int window, sinks;
     int few;           // sequences of at most this many (row, head) columns are the kernel for few rows', the others not
     int only;          // that kernel has the call to itself (longer sequences are an error)
-    int whole;         // it does not cut a (sequence, head) into parts
+    int direct;        // CTAs that share a (sequence, head) in its own cluster; 0: all blocks are dealt to all CTAs
     const float *sink_logits;  // [H] or null
     uint16_t *y;       // [T][H][D]
     float *lse;        // [T][H] or null

@@ -31,18 +31,25 @@ int launched(cudaError_t e, const char *what) {
 // Programmatic dependent launch, as every kernel of this library: the kernel waits (pdl_wait) before it reads or
 // writes anything.
 template <typename... K, typename... A>
-cudaError_t launch(void (*kern)(K...), dim3 grid, int threads, size_t smem, cudaStream_t st, const A &...args) {
+cudaError_t launch_cluster(void (*kern)(K...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, const A &...args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+template <typename... K, typename... A>
+cudaError_t launch(void (*kern)(K...), dim3 grid, int threads, size_t smem, cudaStream_t st, const A &...args) {
+    return launch_cluster(kern, grid, threads, smem, 1, st, args...);
 }
 
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -121,9 +128,14 @@ int check_seqs(int T, const int *cu, const int *lens, bool need_lens, const int 
     ((c)->format == MOEB_KV_Q4 ? ((c)->head_dim == 64 ? kern<FMT_Q4, 64> : kern<FMT_Q4, 128>) \
                                : ((c)->head_dim == 64 ? kern<FMT_FP4, 64> : kern<FMT_FP4, 128>))
 
-// Grid of the kernels that write and read rows: per CTA 4 x 16 (int4) or 4 x 32 (MXFP4) tokens of one head's K or V.
-dim3 word_grid(const moeb_kv_cache *c, int T) {
-    const int tokens = c->format == MOEB_KV_Q4 ? 64 : 128;
+// The kernels that write and read rows: a CTA takes 16 (int4) or 32 (MXFP4) tokens of one head's K or V at a time, 4 times
+// where that still gives every SM eight CTAs.
+int word_passes(const moeb_kv_cache *c, int T) {
+    const long ctas = (((long)T + (c->format == MOEB_KV_Q4 ? 15 : 31)) / (c->format == MOEB_KV_Q4 ? 16 : 32)) * 2 * c->kv_heads;
+    return ctas >= 32L * sms() ? 4 : 1;
+}
+dim3 word_grid(const moeb_kv_cache *c, int T, int passes) {
+    const int tokens = (c->format == MOEB_KV_Q4 ? 16 : 32) * passes;
     return dim3((unsigned)((T + tokens - 1) / tokens), 2u * c->kv_heads);
 }
 
@@ -150,8 +162,11 @@ int launch_few(const KvAttnArgs &a, void *ws, cudaStream_t st) {
     // at most one block of 128 keys per CTA: the page tables' width bounds the blocks, each (sequence, head) has 2 more in the count
     const long most = (long)a.s.B * a.c.Hkv * ((((long)a.s.P << a.c.pshift) >> 7) + 4);
     const int grid = (int)(most < (long)per * sms() ? most : (long)per * sms());
+    if (a.direct)
+        return launched(launch_cluster(k_kv_attn_few<FMT, D, NT>, dim3(a.s.B * a.c.Hkv * a.direct), 128, smem, a.direct, st, a, pre, part),
+                        "kv_attention");
     cudaError_t e = launch(k_kv_attn_few<FMT, D, NT>, dim3(grid), 128, smem, st, a, pre, part);
-    if (e == cudaSuccess && !a.whole)
+    if (e == cudaSuccess)
         e = launch(k_kv_attn_join<D, NT>, dim3(a.s.B * a.c.Hkv, a.few), 256, 0, st, a, (const int *)pre, (const float *)part, grid);
     return launched(e, "kv_attention");
 }
@@ -202,7 +217,8 @@ int moeb_kv_write(const moeb_kv_cache *cache, const void *k, long k_row, long k_
     a.k_head = k_head;
     a.v_row = v_row;
     a.v_head = v_head;
-    return launched(launch(KV_PICK(k_kv_write, cache), word_grid(cache, T), 128, 0, stream, a), "kv_write");
+    a.passes = word_passes(cache, T);
+    return launched(launch(KV_PICK(k_kv_write, cache), word_grid(cache, T, a.passes), 128, 0, stream, a), "kv_write");
 }
 
 int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *first, const int *table, long table_row,
@@ -216,7 +232,8 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
     a.first = first;
     a.k = (uint16_t *)k;
     a.v = (uint16_t *)v;
-    return launched(launch(KV_PICK(k_kv_read, cache), word_grid(cache, T), 128, 0, stream, a), "kv_read");
+    a.passes = word_passes(cache, T);
+    return launched(launch(KV_PICK(k_kv_read, cache), word_grid(cache, T, a.passes), 128, 0, stream, a), "kv_read");
 }
 
 size_t moeb_kv_attention_workspace_bytes(int T, int B, int H, int kv_heads, int head_dim, int max_q) {
@@ -272,15 +289,16 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
     if (a.few) {
         const bool one = cols <= 8;
         a.only = only_few;
-        // Up to 4 blocks of 128 keys one after the other cost as much as a second launch to join parts of them. The bound is
-        // known here from the page tables' width, or from the window (its keys may start and end inside a block).
+        // Up to 4 blocks of 128 keys one after the other cost as much as a second launch to join parts of them: one CTA has
+        // them, or, where that many CTAs fit the GPU at once, one of a cluster of 8 has (keys to 4096). The bound is known here from
+        // the page tables' width, or from the window (its keys may start and end inside a block).
         long keys = (long)P << a.c.pshift;
         if (window) {
             const long seen = (long)window + std::min<long>(max_q, 16) + std::min<long>(sinks, keys);
             keys = std::min(keys, seen + 128 + (sinks ? 128 : 0));
         }
-        a.whole = keys <= 512;
-        a.few = one ? 8 : 16;
+        const long heads = (long)B * a.c.Hkv;
+        a.direct = keys > 128 && keys <= 4096 && heads * 8 <= 2L * sms() ? 8 : keys <= 512 ? 1 : 0;
         rc = cache->format == MOEB_KV_Q4
                  ? (cache->head_dim == 64 ? (one ? launch_few<FMT_Q4, 64, 1>(a, ws, stream) : launch_few<FMT_Q4, 64, 2>(a, ws, stream))
                                           : (one ? launch_few<FMT_Q4, 128, 1>(a, ws, stream) : launch_few<FMT_Q4, 128, 2>(a, ws, stream)))

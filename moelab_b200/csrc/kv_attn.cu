@@ -8,7 +8,9 @@
 // dealt to the CTAs in equal runs, so uneven lengths cost nothing and the host needs to know none of them (a captured
 // graph replays with other lengths). A run's start and end cost about as much as FR blocks, which each (sequence, head) has in
 // the count before its first one (without them CTAs with many short sequences end last). A CTA that holds all blocks of a (sequence, head) writes y; otherwise it leaves its
-// unnormalised sum, maximum and sum of weights, and k_kv_attn_join joins them.
+// unnormalised sum, maximum and sum of weights, and k_kv_attn_join joins them. Where the page tables' width or the window bounds
+// the keys to a few blocks there is no second launch: a CTA (a.direct = 1) or a cluster of 8 CTAs, which join through their
+// shared memories, has a (sequence, head).
 //
 // A warp takes 32 keys of each block, straight from a cp.async ring of its own (no block-wide barrier in the loop; the next
 // run's first copies are on their way while a run's warps join; bulk copies from single lanes cost twice the instructions), and
@@ -114,6 +116,26 @@ MOEB_DEV void few_params(const unsigned char *p, float (&s)[NG], float (&b)[NG])
         }
     }
 }
+MOEB_DEV void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// from CTA `rank` of the cluster, at this CTA's shared address
+MOEB_DEV float4 cluster_ld4(unsigned addr, unsigned rank) {
+    float4 v;
+    asm volatile("{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %4, %5;\n ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [r];\n}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr), "r"(rank)
+                 : "memory");
+    return v;
+}
+MOEB_DEV float2 cluster_ld2(unsigned addr, unsigned rank) {
+    float2 v;
+    asm volatile("{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %2, %3;\n ld.shared::cluster.v2.f32 {%0, %1}, [r];\n}"
+                 : "=f"(v.x), "=f"(v.y)
+                 : "r"(addr), "r"(rank)
+                 : "memory");
+    return v;
+}
 MOEB_DEV void few_copy(unsigned smem, const unsigned char *gmem) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
@@ -167,55 +189,10 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
     __shared__ int s_sum[FW], s_b, s_pre;
     pdl_wait();
 
-    // every sequence's blocks: prefix sums over the CTA's threads, and the sequence of this CTA's first block
-    const int per = (a.s.B + FT - 1) / FT, bb0 = min((int)threadIdx.x * per, a.s.B), bb1 = min(bb0 + per, a.s.B);
-    int mine = 0;
-    for (int b = bb0; b < bb1; ++b) mine += few_units(few_seq<NC>(a, b));
-    int inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-    }
-    if (lane == 31) s_sum[warp] = inc;
-    __syncthreads();
-    int base = inc - mine, total = 0;
-#pragma unroll
-    for (int i = 0; i < FW; ++i) {
-        if (i < warp) base += s_sum[i];
-        total += s_sum[i];
-    }
-    const long units = (long)total * a.c.Hkv;
-    const unsigned nct = (unsigned)min((long)gridDim.x, units);
-    if (blockIdx.x == 0) {
-        int at = base;
-        for (int b = bb0; b < bb1; ++b) {
-            const FewSeq s = few_seq<NC>(a, b);
-            pre[b] = at;
-            at += few_units(s);
-            if (a.only && (long)s.n * a.Gq > a.few) atomicOr(a.c.err, ERR_ROWS);
-        }
-        if (threadIdx.x == 0) pre[a.s.B] = total;
-    }
-    if (blockIdx.x >= nct) return;
-    const long us = few_start(units, blockIdx.x, nct), ue = few_start(units, blockIdx.x + 1, nct), u = us;
-    if (u >= (long)base * a.c.Hkv && u < (long)(base + mine) * a.c.Hkv) {
-        int at = base, b = bb0;
-        for (;; ++b) {
-            const int nb = few_units(few_seq<NC>(a, b));
-            if (u < (long)(at + nb) * a.c.Hkv) break;
-            at += nb;
-        }
-        s_b = b;
-        s_pre = at;
-    }
-    __syncthreads();
-    int b = s_b, h;
-    FewSeq q = few_seq<NC>(a, b);
-    int k0;
-    // blocks [k0, k1) of the first run; a CTA whose share of a (sequence, head) is in its FR has none of its blocks
-    long seg = (long)s_pre * a.c.Hkv;  // first unit of the run's (sequence, head)
-    int k1;
+    int b, h, k0, k1;
+    FewSeq q;
+    long us = 0, ue = 0, seg = 0;  // this CTA's units; the first unit of its run's (sequence, head)
+    // blocks [k0, k1) of the next run; a CTA whose share of a (sequence, head) is in its FR has none of its blocks
     auto locate = [&](bool next) {
         for (;; next = true) {
             if (next) {
@@ -226,20 +203,75 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                     while (q.nb == 0);
                 }
             }
-            if (a.whole) {  // a CTA has the (sequence, head)s that start in its share
-                k0 = 0;
-                k1 = seg >= us && seg < ue ? q.nb : 0;
-            } else {
-                k0 = (int)max(us - seg - FR, 0L);
-                k1 = (int)min(ue - seg - FR, (long)q.nb);
-            }
+            k0 = (int)max(us - seg - FR, 0L);
+            k1 = (int)min(ue - seg - FR, (long)q.nb);
             if (k1 > k0 || ue <= seg + q.nb + FR) return;
         }
     };
-    h = us - seg < 0x7fffffffL ? (int)((unsigned)(us - seg) / (unsigned)(q.nb + FR)) : (int)((us - seg) / (q.nb + FR));
-    seg += (long)h * (q.nb + FR);
-    locate(false);
-    if (k1 <= k0) return;
+    const unsigned rank = a.direct ? blockIdx.x % a.direct : 0;
+    if (a.direct) {
+        const unsigned i = blockIdx.x / a.direct;
+        b = i / a.c.Hkv;
+        h = i - b * a.c.Hkv;
+        q = few_seq<NC>(a, b);
+        if (rank == 0 && h == 0 && threadIdx.x == 0 && a.only && (long)q.n * a.Gq > a.few) atomicOr(a.c.err, ERR_ROWS);
+        if (q.nb == 0) return;  // the whole cluster
+        k0 = (int)((unsigned)q.nb * rank / a.direct);
+        k1 = (int)((unsigned)q.nb * (rank + 1) / a.direct);
+    } else {
+        // every sequence's blocks: prefix sums over the CTA's threads, and the sequence of this CTA's first block
+        const int per = (a.s.B + FT - 1) / FT, bb0 = min((int)threadIdx.x * per, a.s.B), bb1 = min(bb0 + per, a.s.B);
+        int mine = 0;
+        for (int b = bb0; b < bb1; ++b) mine += few_units(few_seq<NC>(a, b));
+        int inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) s_sum[warp] = inc;
+        __syncthreads();
+        int base = inc - mine, total = 0;
+#pragma unroll
+        for (int i = 0; i < FW; ++i) {
+            if (i < warp) base += s_sum[i];
+            total += s_sum[i];
+        }
+        const long units = (long)total * a.c.Hkv;
+        const unsigned nct = (unsigned)min((long)gridDim.x, units);
+        if (blockIdx.x == 0) {
+            int at = base;
+            for (int b = bb0; b < bb1; ++b) {
+                const FewSeq s = few_seq<NC>(a, b);
+                pre[b] = at;
+                at += few_units(s);
+                if (a.only && (long)s.n * a.Gq > a.few) atomicOr(a.c.err, ERR_ROWS);
+            }
+            if (threadIdx.x == 0) pre[a.s.B] = total;
+        }
+        if (blockIdx.x >= nct) return;
+        us = few_start(units, blockIdx.x, nct);
+        ue = few_start(units, blockIdx.x + 1, nct);
+        const long u = us;
+        if (u >= (long)base * a.c.Hkv && u < (long)(base + mine) * a.c.Hkv) {
+            int at = base, x = bb0;
+            for (;; ++x) {
+                const int nb = few_units(few_seq<NC>(a, x));
+                if (u < (long)(at + nb) * a.c.Hkv) break;
+                at += nb;
+            }
+            s_b = x;
+            s_pre = at;
+        }
+        __syncthreads();
+        b = s_b;
+        q = few_seq<NC>(a, b);
+        seg = (long)s_pre * a.c.Hkv;
+        h = us - seg < 0x7fffffffL ? (int)((unsigned)(us - seg) / (unsigned)(q.nb + FR)) : (int)((us - seg) / (q.nb + FR));
+        seg += (long)h * (q.nb + FR);
+        locate(false);
+        if (k1 <= k0) return;
+    }
     const int ta = (r >> 1) + 4 * (r & 1);  // this lane's keys of 16: ta and ta + 8
 
     // Page ids of 16 blocks from kb on: lane 2 i + x has half x (16 keys, a page at least) of this warp's keys of block kb + i.
@@ -303,7 +335,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
         const int hr = h, kr0 = k0, kr1 = k1;
         const long segr = seg;
         const int br = b;
-        bool more = ue > seg + q.nb + FR;
+        bool more = !a.direct && ue > seg + q.nb + FR;
         int idn = -1;
         if (more) {
             locate(true);
@@ -731,13 +763,43 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                 v.w += w.w;
                 L += s_l[x][col] * ex2(s_m[x][col] - use);
             }
-            if (whole) {
+            if (a.direct > 1) {  // to the front of the rings, which are empty now
+                float *mine = reinterpret_cast<float *>(sm);
+                *reinterpret_cast<float4 *>(mine + col * D + 4 * d4) = v;
+                if (d4 == 0) *reinterpret_cast<float2 *>(mine + NC * D + 2 * col) = make_float2(M, L);
+            } else if (whole) {
                 const int ri = kv_div(col, a.Gdiv), head = hr * a.Gq + col - ri * a.Gq;
                 kv_finish<D>(a, qr.r0 + ri, head, d4, v, M, L);
             } else {
                 *reinterpret_cast<float4 *>(pt + col * D + 4 * d4) = v;
                 if (d4 == 0) *reinterpret_cast<float2 *>(pt + NC * D + 2 * col) = make_float2(M, L);
             }
+        }
+        if (a.direct > 1) {
+            // column i is CTA i % direct's: it adds up what all of them have
+            cluster_sync();
+            const unsigned at = smem_u32(sm);
+            const int nc = qr.n * a.Gq, mine = ((int)(nc - rank) + a.direct - 1) / a.direct;  // columns of this CTA
+            for (int i = threadIdx.x; i < mine * (D / 4); i += FT) {
+                const int col = (int)rank + i / (D / 4) * a.direct, d4 = i % (D / 4);
+                float M = -INFINITY, L = 0.f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int x = 0; x < a.direct; ++x) M = fmaxf(M, cluster_ld2(at + (NC * D + 2 * col) * 4, x).x);
+                const float use = M == -INFINITY ? 0.f : M;
+                for (int x = 0; x < a.direct; ++x) {
+                    const float2 ml = cluster_ld2(at + (NC * D + 2 * col) * 4, x);
+                    const float4 w = cluster_ld4(at + (col * D + 4 * d4) * 4, x);
+                    const float f = ex2(ml.x - use);
+                    v.x += w.x * f;
+                    v.y += w.y * f;
+                    v.z += w.z * f;
+                    v.w += w.w * f;
+                    L += ml.y * f;
+                }
+                const int ri = kv_div(col, a.Gdiv);
+                kv_finish<D>(a, qr.r0 + ri, hr * a.Gq + col - ri * a.Gq, d4, v, M, L);
+            }
+            cluster_sync();  // nobody leaves while its sums are read
         }
         if (!more) break;
         kb = k0;
