@@ -72,7 +72,7 @@ SIGNATURES = {
     "moeb_ep_p2p_read_error": (_I, [_P, _I, _I, _I, ctypes.POINTER(ctypes.c_uint), _P]),
     "moeb_kv_write": (_I, [_C, _P, _L, _L, _P, _L, _L, _I, _P, _P, _P, _L, _I, _I, _P]),
     "moeb_kv_read": (_I, [_C, _I, _P, _P, _P, _L, _I, _I, _P, _P, _P]),
-    "moeb_kv_attention_workspace_bytes": (_S, [_I] * 6),
+    "moeb_kv_attention_workspace_bytes": (_S, [_I] * 11),
     "moeb_kv_attention": (_I, [_C, _P, _L, _L, _I, _I, _P, _P, _P, _L, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P, _S, _P]),
     "moeb_kv_read_error": (_I, [_C, ctypes.POINTER(ctypes.c_uint), _P]),
     "moeb_probe_tc_issue": (_I, [_I] * 7 + [ctypes.POINTER(ctypes.c_double)] * 3),

@@ -82,7 +82,7 @@ MOEB_DEV int kv_seq_of(const KvSeqs &s, int t, int &r0, int &r1) {
         return b;
     }
     // the last b with cu[b] <= t; first where it is when all sequences have as many rows
-    const int guess = (int)((long)t * s.B / s.T);
+    const int guess = min((int)__fdividef((float)t * (float)s.B, (float)s.T), s.B - 1);
     if (s.cu[guess] <= t && t < s.cu[guess + 1] && s.cu[guess + 1] <= s.T && s.cu[guess] >= 0) {
         r0 = s.cu[guess];
         r1 = s.cu[guess + 1];

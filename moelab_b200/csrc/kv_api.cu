@@ -139,26 +139,69 @@ dim3 word_grid(const moeb_kv_cache *c, int T, int passes) {
     return dim3((unsigned)((T + tokens - 1) / tokens), 2u * c->kv_heads);
 }
 
-// Workspace of the kernel for few rows: blocks before each sequence, then two partial results per CTA.
-struct FewLayout {
-    size_t part, total;
+// What a call of moeb_kv_attention launches, from what the host knows: the rows, the page tables' width and the window.
+struct Plan {
+    long keys;          // keys that one row tile or one sequence's few rows can see, at most
+    int few, only;      // sequences of at most `few` (row, head) columns go to the kernel for few rows; all of them do
+    int nc, direct;     // its columns per tile; CTAs that share a (sequence, head) (0: all blocks are dealt to all CTAs)
+    size_t part, few_bytes;
+    long tiles, splits; // row tiles of the kernel for many rows; parts that each one's keys are cut into
+    size_t split_bytes;
 };
 constexpr int FEW_RESIDENT = 3;  // CTAs per SM at most (the kernel's launch bound)
-FewLayout few_layout(int B, int nc, int D) {
-    FewLayout l;
-    l.part = up256(4 * ((size_t)B + 1));
-    l.total = l.part + (size_t)FEW_RESIDENT * sms() * 2 * nc * (D + 2) * 4;
-    return l;
+
+Plan plan_of(int T, int B, int P, int page_size, int H, int Hkv, int D, int max_q, int window, int sinks, bool cu) {
+    Plan p = {};
+    const int Gq = H / Hkv;
+    const long cols = (long)max_q * Gq, all = (long)P * page_size;
+    // The window's keys may start and end inside a block of 128; so may the first tokens'.
+    auto seen = [&](long rows) { return window ? std::min(all, (long)window + rows + std::min<long>(sinks, all) + 128 + (sinks ? 128 : 0)) : all; };
+    // Sequences whose (row, head) columns fit one or two tensor-core tiles go to the kernel for few rows. Without cu all
+    // sequences have T / B rows; with it, and more than one sequence, both kinds may be in the call.
+    p.only = cols <= 16;
+    p.few = p.only ? (int)cols : cu && B > 1 ? 16 : 0;
+    if (p.few) {
+        p.nc = cols <= 8 ? 8 : 16;
+        // Up to 4 blocks of 128 keys one after the other cost as much as a second launch to join parts of them: one CTA has
+        // them, or, where that many CTAs fit the GPU at once, one of a cluster of 8 has (keys to 4096).
+        const long keys = seen(std::min(max_q, 16));
+        p.direct = keys > 128 && keys <= 4096 && (long)B * Hkv * 8 <= 2L * sms() ? 8 : keys <= 512 ? 1 : 0;
+        if (!p.direct) {  // blocks before each sequence, then two partial results per CTA
+            p.part = up256(4 * ((size_t)B + 1));
+            p.few_bytes = up256(p.part + (size_t)FEW_RESIDENT * sms() * 2 * p.nc * (D + 2) * 4);
+        }
+    }
+    if (!p.only) {
+        // Row tiles: with cu each sequence may have one that is not full.
+        p.tiles = cu ? (long)T * Gq / KV_PROMPT_ROWS + B : (long)B * (((long)(T / B) * Gq + KV_PROMPT_ROWS - 1) / KV_PROMPT_ROWS);
+        const long ctas = p.tiles * Hkv, key_tiles = (seen(KV_PROMPT_ROWS) + 127) / 128;
+        // One CTA per SM: where the row tiles alone are less than three waves, their keys are cut into as many parts (8 key tiles
+        // or more each) as make the last wave fullest. A key tile takes about 2 us; a part's sums are written and read once more.
+        p.splits = 1;
+        if (ctas < 3L * sms()) {
+            double best = 0;
+            const long most = std::max(1L, std::min(key_tiles / 8, ctas * 2 <= sms() ? sms() / std::max(ctas, 1L) : 8L));
+            for (long n = 1; n <= most; ++n) {
+                const double waves = (double)((ctas * n + sms() - 1) / sms());
+                const double us = waves * ((double)key_tiles / n * 2.0 + 6.0) + (n > 1 ? 3.0 + (double)n * T * H * D * 8 / 5e6 : 0.0);
+                if (n == 1 || us < best * 0.97) {
+                    best = us;
+                    p.splits = n;
+                }
+            }
+        }
+        if (p.splits > 1) p.split_bytes = (size_t)p.splits * T * H * (D + 2) * 4;
+    }
+    return p;
 }
 
 template <int FMT, int D, int NT>
-int launch_few(const KvAttnArgs &a, void *ws, cudaStream_t st) {
+int launch_few(const KvAttnArgs &a, const Plan &p, void *ws, cudaStream_t st) {
     const size_t smem = kv_few_smem<FMT, D, NT>();
     const int per = resident((const void *)k_kv_attn_few<FMT, D, NT>, 128, smem);
     if (!per) return launched(cudaErrorInvalidConfiguration, "kv_attention");
-    const FewLayout l = few_layout(a.s.B, 8 * NT, D);
     int *pre = (int *)ws;
-    float *part = (float *)((char *)ws + l.part);
+    float *part = (float *)((char *)ws + p.part);
     // at most one block of 128 keys per CTA: the page tables' width bounds the blocks, each (sequence, head) has 2 more in the count
     const long most = (long)a.s.B * a.c.Hkv * ((((long)a.s.P << a.c.pshift) >> 7) + 4);
     const int grid = (int)(most < (long)per * sms() ? most : (long)per * sms());
@@ -171,27 +214,16 @@ int launch_few(const KvAttnArgs &a, void *ws, cudaStream_t st) {
     return launched(e, "kv_attention");
 }
 
-// Row tiles of the kernel for many rows, and into how many parts each tile's keys are cut: as many as give every SM a
-// CTA, where the rows alone do not.
-long prompt_tiles(int T, int B, int Gq, bool cu) {
-    return cu ? (long)T * Gq / KV_PROMPT_ROWS + B : (long)B * (((long)(T / B) * Gq + KV_PROMPT_ROWS - 1) / KV_PROMPT_ROWS);
-}
-long prompt_splits(long tiles, int Hkv) { return tiles * Hkv * 2 > sms() ? 1 : sms() / (tiles * Hkv); }
-
 template <int FMT, int D>
-int launch_prompt(const KvAttnArgs &a, void *ws, cudaStream_t st) {
+int launch_prompt(const KvAttnArgs &a, const Plan &p, void *ws, cudaStream_t st) {
     const size_t smem = kv_prompt_smem(D);
     if (!resident((const void *)k_kv_attn_prompt<FMT, D>, KV_PROMPT_THREADS, smem))
         return launched(cudaErrorInvalidConfiguration, "kv_attention");
-    const long tiles = prompt_tiles(a.s.T, a.s.B, a.Gq, a.s.cu != nullptr);
-    const long keys = (((long)a.s.P << a.c.pshift) + 127) >> 7;  // key tiles at most
-    long ns = prompt_splits(tiles, a.c.Hkv);
-    if (ns > keys) ns = keys < 1 ? 1 : keys;
-    float *part = ns > 1 ? (float *)ws : nullptr;
-    cudaError_t e = launch(k_kv_attn_prompt<FMT, D>, dim3((unsigned)(tiles * a.c.Hkv), (unsigned)ns), KV_PROMPT_THREADS, smem, st, a,
-                           (int)tiles, part);
-    if (e == cudaSuccess && ns > 1)
-        e = launch(k_kv_attn_join_splits<D>, dim3((unsigned)(((size_t)a.s.T * a.H + 3) / 4)), 128, 0, st, a, (const float *)part, (int)ns);
+    float *part = p.splits > 1 ? (float *)ws : nullptr;
+    cudaError_t e = launch(k_kv_attn_prompt<FMT, D>, dim3((unsigned)(p.tiles * a.c.Hkv), (unsigned)p.splits), KV_PROMPT_THREADS, smem, st, a,
+                           (int)p.tiles, part);
+    if (e == cudaSuccess && part)
+        e = launch(k_kv_attn_join_splits<D>, dim3((unsigned)(((size_t)a.s.T * a.H + 3) / 4)), 128, 0, st, a, (const float *)part, (int)p.splits);
     return launched(e, "kv_attention");
 }
 
@@ -236,17 +268,11 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
     return launched(launch(KV_PICK(k_kv_read, cache), word_grid(cache, T, a.passes), 128, 0, stream, a), "kv_read");
 }
 
-size_t moeb_kv_attention_workspace_bytes(int T, int B, int H, int kv_heads, int head_dim, int max_q) {
-    if (T <= 0 || B <= 0 || H <= 0 || kv_heads <= 0 || head_dim <= 0 || max_q <= 0) return 0;
-    const int Gq = H / kv_heads;
-    const long cols = (long)max_q * Gq;
-    size_t n = up256(few_layout(B, cols <= 8 ? 8 : 16, head_dim).total);
-    if (cols > 16) {
-        const long tiles = T % B ? prompt_tiles(T, B, Gq, true) : std::min(prompt_tiles(T, B, Gq, true), prompt_tiles(T, B, Gq, false));
-        const long ns = prompt_splits(tiles, kv_heads);
-        if (ns > 1) n += (size_t)ns * T * H * (head_dim + 2) * 4;
-    }
-    return n;
+size_t moeb_kv_attention_workspace_bytes(int T, int B, int P, int page_size, int H, int kv_heads, int head_dim, int max_q,
+                                         int window, int sinks, int with_cu) {
+    if (T <= 0 || B <= 0 || P < 0 || page_size <= 0 || kv_heads <= 0 || H < kv_heads || head_dim <= 0 || max_q <= 0) return 0;
+    const Plan p = plan_of(T, B, P, page_size, H, kv_heads, head_dim, max_q, window, sinks, with_cu != 0);
+    return p.few_bytes + p.split_bytes;
 }
 
 int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, long q_head, int T, int H, const int *cu,
@@ -266,9 +292,10 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
     if (!rows_ok(q, q_row, q_head))
         return bad("q must be 16-byte aligned, with row and head strides that are multiples of 8 elements");
     if (!y || !aligned16(y)) return bad("y must be 16-byte aligned");
-    if (ws_bytes < moeb_kv_attention_workspace_bytes(T, B, H, cache->kv_heads, cache->head_dim, max_q))
+    const Plan p = plan_of(T, B, P, cache->page_size, H, cache->kv_heads, cache->head_dim, max_q, window, sinks, cu != nullptr);
+    if (p.few_bytes + p.split_bytes > 0 && (!ws || !aligned16(ws))) return bad("the workspace must be 16-byte aligned");
+    if (ws_bytes < p.few_bytes + p.split_bytes)
         return bad("the workspace is too small: see moeb_kv_attention_workspace_bytes");
-    if (!ws || !aligned16(ws)) return bad("the workspace must be 16-byte aligned");
     a.q = (const uint16_t *)q;
     a.q_row = q_row;
     a.q_head = q_head;
@@ -281,36 +308,22 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
     a.sink_logits = sink_logits;
     a.y = (uint16_t *)y;
     a.lse = lse;
-    // Sequences whose (row, head) columns fit one or two tensor-core tiles go to the kernel for few rows. Without cu all
-    // sequences have T / B rows; with it, and more than one sequence, both kinds may be in the call.
-    const long cols = (long)max_q * a.Gq;
-    const bool only_few = cols <= 16, both = !only_few && cu && B > 1;
-    a.few = only_few ? (int)cols : both ? 16 : 0;
-    if (a.few) {
-        const bool one = cols <= 8;
-        a.only = only_few;
-        // Up to 4 blocks of 128 keys one after the other cost as much as a second launch to join parts of them: one CTA has
-        // them, or, where that many CTAs fit the GPU at once, one of a cluster of 8 has (keys to 4096). The bound is known here from
-        // the page tables' width, or from the window (its keys may start and end inside a block).
-        long keys = (long)P << a.c.pshift;
-        if (window) {
-            const long seen = (long)window + std::min<long>(max_q, 16) + std::min<long>(sinks, keys);
-            keys = std::min(keys, seen + 128 + (sinks ? 128 : 0));
-        }
-        const long heads = (long)B * a.c.Hkv;
-        a.direct = keys > 128 && keys <= 4096 && heads * 8 <= 2L * sms() ? 8 : keys <= 512 ? 1 : 0;
-        rc = cache->format == MOEB_KV_Q4
-                 ? (cache->head_dim == 64 ? (one ? launch_few<FMT_Q4, 64, 1>(a, ws, stream) : launch_few<FMT_Q4, 64, 2>(a, ws, stream))
-                                          : (one ? launch_few<FMT_Q4, 128, 1>(a, ws, stream) : launch_few<FMT_Q4, 128, 2>(a, ws, stream)))
-                 : (cache->head_dim == 64 ? (one ? launch_few<FMT_FP4, 64, 1>(a, ws, stream) : launch_few<FMT_FP4, 64, 2>(a, ws, stream))
-                                          : (one ? launch_few<FMT_FP4, 128, 1>(a, ws, stream) : launch_few<FMT_FP4, 128, 2>(a, ws, stream)));
-        if (rc) return rc;
+    a.few = p.few;
+    a.only = p.only;
+    a.direct = p.direct;
+    const bool q4 = cache->format == MOEB_KV_Q4, d64 = cache->head_dim == 64;
+    if (p.few) {
+        if (p.nc == 8)
+            rc = q4 ? (d64 ? launch_few<FMT_Q4, 64, 1>(a, p, ws, stream) : launch_few<FMT_Q4, 128, 1>(a, p, ws, stream))
+                    : (d64 ? launch_few<FMT_FP4, 64, 1>(a, p, ws, stream) : launch_few<FMT_FP4, 128, 1>(a, p, ws, stream));
+        else
+            rc = q4 ? (d64 ? launch_few<FMT_Q4, 64, 2>(a, p, ws, stream) : launch_few<FMT_Q4, 128, 2>(a, p, ws, stream))
+                    : (d64 ? launch_few<FMT_FP4, 64, 2>(a, p, ws, stream) : launch_few<FMT_FP4, 128, 2>(a, p, ws, stream));
+        if (rc || p.only) return rc;
     }
-    if (only_few) return MOEB_OK;
-    void *rest = (char *)ws + up256(few_layout(B, 16, cache->head_dim).total);
-    return cache->format == MOEB_KV_Q4
-               ? (cache->head_dim == 64 ? launch_prompt<FMT_Q4, 64>(a, rest, stream) : launch_prompt<FMT_Q4, 128>(a, rest, stream))
-               : (cache->head_dim == 64 ? launch_prompt<FMT_FP4, 64>(a, rest, stream) : launch_prompt<FMT_FP4, 128>(a, rest, stream));
+    void *rest = (char *)ws + p.few_bytes;
+    return q4 ? (d64 ? launch_prompt<FMT_Q4, 64>(a, p, rest, stream) : launch_prompt<FMT_Q4, 128>(a, p, rest, stream))
+              : (d64 ? launch_prompt<FMT_FP4, 64>(a, p, rest, stream) : launch_prompt<FMT_FP4, 128>(a, p, rest, stream));
 }
 
 int moeb_kv_read_error(const moeb_kv_cache *cache, unsigned *out, cudaStream_t stream) {

@@ -17,7 +17,8 @@
 // fp16 keeps 2^-12. Its range is kept by powers of two: one per query row, one per K tile (both go into the softmax's
 // scale), and a running one for V (a change rescales O; it leaves room for 2^6 of growth, so that it hardly happens).
 // A value that is NaN (a group that held one) must not reach rows that do not see its key, and 0 x NaN is NaN in a
-// product: such a group enters as zeros, and the rows that see its key are marked and written as NaN.
+// product: such a group enters as zeros, and the rows that see its key are marked and written as NaN. Likewise keys and
+// queries, so that no score is NaN.
 //
 // Every wait is bounded: after its limit the kernel records MOEB_DEVERR_TIMEOUT, its roles stop, TMEM is released.
 #include "kv.cuh"
@@ -30,6 +31,7 @@ constexpr int PR = 256;               // rows per CTA
 constexpr int PT = 640;               // threads: five warpgroups
 constexpr float P_OFF = 6.f;          // P = 2^(score - m + 6)
 constexpr float P_LAZY = 8.f;
+constexpr int P_POLY = 1;                // of 4 pairs of weights, those by ex2_poly
 
 template <int D>
 struct Pr {
@@ -44,7 +46,8 @@ struct Pr {
 struct PrShared {
     uint64_t kfull[3], kempty[3], vfull[3], vempty[3], sfull[2][2], pfull[2][2], pv[2], ofull[2];  // [row tile][half]
     float kmul[4];             // by key tile % 4: 2^e of the K tile
-    unsigned holes[4], hole[4][4];  // by key tile % 4: byte per feeding warp, keys without a page among its own; those keys
+    // by key tile % 4: byte per feeding warp, a key without a page or with a NaN among its own; those keys
+    unsigned odd[4], hole[4][4], knan[4][4];
     struct {
         float fix;             // what O is multiplied by before this V tile
         unsigned pz;           // byte per feeding warp, a NaN group among its rows
@@ -61,6 +64,21 @@ MOEB_DEV float ex2p(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// 2^x of two values by the FMA units, for some of the weights: the unit that does ex2 gives 16 a clock per SM and would set the
+// pace alone. x = n + r, n whole (added to 1.5 * 2^23, whose low bits are then n), |r| <= 1/2; 2^r by the polynomial of degree
+// 3 with the least relative error there (7.5e-5, a Remez exchange; the weights' rounding to fp16 is 2.4e-4), n into the exponent.
+MOEB_DEV void ex2_poly(uint64_t xy, float &x, float &y) {
+    float a, b;
+    unpair(xy, a, b);
+    xy = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const uint64_t t = add2(xy, pair(12582912.f, 12582912.f));
+    const uint64_t r = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), xy);
+    uint64_t p = fma2(r, pair(0.05517166852951050f, 0.05517166852951050f), pair(0.2426111251115799f, 0.2426111251115799f));
+    p = fma2(p, r, pair(0.6932609677314758f, 0.6932609677314758f));
+    p = fma2(p, r, pair(0.9999280571937561f, 0.9999280571937561f));
+    x = __uint_as_float((uint32_t)p + ((uint32_t)t << 23));
+    y = __uint_as_float((uint32_t)(p >> 32) + ((uint32_t)(t >> 32) << 23));
 }
 MOEB_DEV float max3(float x, float y, float z) {
     float r;
@@ -201,6 +219,14 @@ MOEB_DEV uint4 pr_word(uint32_t w, uint32_t s2, uint32_t b2) {
 // the n lowest of 64 bits
 MOEB_DEV unsigned long long pr_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
+// bits 0, 4, 8 .. 28 as a byte
+MOEB_DEV unsigned pr_byte(unsigned x) {
+    x &= 0x11111111u;
+    x = (x | x >> 3) & 0x03030303u;
+    x = (x | x >> 6) & 0x000F000Fu;
+    return (x | x >> 12) & 0xFFu;
+}
+
 // Largest magnitude (bits) that a row's parameters allow, NaN groups apart; nan: which groups are NaN.
 template <int FMT, int NG>
 MOEB_DEV uint32_t pr_top(const float (&s)[NG], const float (&b)[NG], unsigned &nan) {
@@ -319,7 +345,7 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
             uint32_t s2[NG], b2[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                if (V && ((nan >> g) & 1u)) s[g] = bb[g] = 0.f;  // the rows that see the key are marked instead
+                if ((nan >> g) & 1u) s[g] = bb[g] = 0.f;  // the rows that see the key are marked instead
                 s2[g] = h2(s[g] * mul, s[g] * mul);
                 b2[g] = h2(bb[g] * mul, bb[g] * mul);
             }
@@ -353,16 +379,15 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
                     }
                 }
             } else {
+                const unsigned bad = __ballot_sync(0xffffffffu, nan != 0);
                 if (lane < 4) {  // byte w of word `lane`: keys 32 lane + 8 w .., their bits are 4 r + lane
-                    unsigned x = (hole >> lane) & 0x11111111u;
-                    x = (x | x >> 3) & 0x03030303u;
-                    x = (x | x >> 6) & 0x000F000Fu;
-                    x = (x | x >> 12) & 0xFFu;
+                    const unsigned x = pr_byte(hole >> lane);
                     reinterpret_cast<uint8_t *>(sh.hole[j & 3])[4 * lane + w] = (uint8_t)x;
+                    reinterpret_cast<uint8_t *>(sh.knan[j & 3])[4 * lane + w] = (uint8_t)pr_byte(bad >> lane);
                     if (x) atomicOr(a.c.err, ERR_PAGE);
                 }
                 if (lane == 0) {
-                    reinterpret_cast<uint8_t *>(&sh.holes[j & 3])[w] = hole != 0;
+                    reinterpret_cast<uint8_t *>(&sh.odd[j & 3])[w] = (hole | bad) != 0;
                     if (w == 0) sh.kmul[j & 3] = vun;
                 }
             }
@@ -559,9 +584,11 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             float qmul = fabsf(a.scale) * __uint_as_float((uint32_t)(e - 8) << 23);
             if (a.scale < 0.f) down = -down;  // the softmax's scale stays positive: it takes the maximum before scaling
             if (a.scale == 0.f) down = 0.f, qmul = 1.f;
+            const bool fine = top < 0x7f80u;
             uint32_t o[4];
 #pragma unroll
-            for (int e2 = 0; e2 < 4; ++e2) o[e2] = h2(bf16lo(u[e2]) * down, bf16hi(u[e2]) * down);
+            for (int e2 = 0; e2 < 4; ++e2) o[e2] = fine ? h2(bf16lo(u[e2]) * down, bf16hi(u[e2]) * down) : 0u;
+            if (!fine) qmul = -1.f;  // an infinity or a NaN in the row: its result is NaN
             *reinterpret_cast<uint4 *>(sm + (row >> 7) * L::TILE + (x >> 3) * 16384 + (row & 127) * 128 + (((x & 7) ^ (row & 7)) << 4)) =
                 make_uint4(o[0], o[1], o[2], o[3]);
             if (x == 0) sh.qmul[row] = qmul;
@@ -589,12 +616,12 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         const bool have = R < NR;
         const int ri = R / a.Gq, pos = have ? p0 + ri : -1, row_t = have ? r0 + ri : 0, row_h = h * a.Gq + R - ri * a.Gq;
         const float qmul = sh.qmul[t * 128 + row];
+        unsigned poison = qmul < 0.f ? 1u << 31 : 0u;  // bit g: group g of the row is NaN; bit 31: all of it
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + L::S0 + 128 * t, to = tmem + lanes + D * t;
         const int q0 = R0 + t * 128;
         const int tmin = p0 + q0 / a.Gq, tmax = p0 + (min(q0 + 128, NR) - 1) / a.Gq;  // positions of the tile's rows
         float m = -INFINITY, l = 0.f, sc = 0.f;
-        unsigned poison = 0;
         int st = 0, j0 = pr_tok(keys, k0);
         unsigned vph = 0;
 #pragma unroll 1
@@ -606,9 +633,9 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             ld32(ts + 64 * i2, v);
             ld32(ts + 64 * i2 + 32, v + 32);
             float vfix = 1.f;
-            const unsigned holes = sh.holes[j & 3];
+            const unsigned odd = sh.odd[j & 3];
             if (i2 == 0) {
-                sc = fmaxf(qmul * sh.kmul[j & 3], 1.2e-38f);  // above zero: a hidden score of -inf stays -inf
+                sc = fmaxf(fabsf(qmul) * sh.kmul[j & 3], 1.2e-38f);  // above zero: a hidden score of -inf stays -inf
                 // V's stage: its power of two, its NaN groups
                 pr_wait(sh.vfull + st, vph, &sh.fail);
                 vfix = sh.v[st].fix;
@@ -621,7 +648,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
                     __syncwarp();
                 }
             }
-            const bool full = j0 + 63 <= tmin && (!a.window || j0 > tmax - a.window || j0 + 63 < a.sinks) && !holes;
+            const bool full = j0 + 63 <= tmin && (!a.window || j0 > tmax - a.window || j0 + 63 < a.sinks) && !odd;
             wait_ld();
             if (!full) {
                 // bit i: this row sees key i of the half
@@ -629,6 +656,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
                 const unsigned long long old = a.window ? pr_below(pos - a.window + 1 - j0) & ~pr_below(a.sinks - j0) : 0ull;
                 const unsigned long long see = pr_below(pos - j0 + 1) & ~old & ~hole;
                 const unsigned s0 = (unsigned)see, s1 = (unsigned)(see >> 32);
+                if (odd && ((s0 & sh.knan[j & 3][2 * i2]) | (s1 & sh.knan[j & 3][2 * i2 + 1]))) poison |= 1u << 31;
 #pragma unroll
                 for (int i = 0; i < 64; ++i) v[i] = (i < 32 ? s0 >> i : s1 >> (i - 32)) & 1u ? v[i] : -INFINITY;
             }
@@ -648,7 +676,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
                 x3 = max3(x3, v[i + 6], v[i + 7]);
             }
             float mt = max3(max3(x0, v[60], v[61]), max3(x1, v[62], v[63]), fmaxf(x2, x3)) * sc;
-            if (!(mt > -INFINITY)) mt = -INFINITY;  // every score a NaN: the weights and the row become NaN
+            if (mt == INFINITY) poison |= 1u << 31;  // a score past fp32: inf - inf
             // rescale O when a maximum grew far, or V's power of two changed
             const bool grew = mt > m + P_LAZY;
             if (__any_sync(0xffffffffu, grew || vfix != 1.f)) {
@@ -684,9 +712,14 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     float x, y;
-                    unpair(fma2(pair(v[32 * q + 2 * i], v[32 * q + 2 * i + 1]), sc2, off2), x, y);
-                    x = ex2p(x);
-                    y = ex2p(y);
+                    const uint64_t xy = fma2(pair(v[32 * q + 2 * i], v[32 * q + 2 * i + 1]), sc2, off2);
+                    if (i % 4 < P_POLY) {
+                        ex2_poly(xy, x, y);
+                    } else {
+                        unpair(xy, x, y);
+                        x = ex2p(x);
+                        y = ex2p(y);
+                    }
                     l2 = add2(l2, pair(x, y));
                     u[i] = h2(x, y);
                 }
@@ -703,6 +736,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         if (nk > 0) pr_wait(sh.ofull + t, 0, &sh.fail);
         fence_after();
         __syncwarp();
+        if (poison >> 31) l = __uint_as_float(0x7fffffffu);
         // ---- the rows' results (m is off by P_OFF against the weights' sum: undone here)
         const float M = m == -INFINITY ? m : m - P_OFF;
         float mul = nk > 0 ? sh.vun : 0.f, Ls = l, sum_m = M;

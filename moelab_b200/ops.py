@@ -434,7 +434,7 @@ def _kv_call(cache, name, *args):
     """The call on the cache's device and that device's current stream."""
     i = cache.index
     stream = torch._C._cuda_getCurrentRawStream(i)
-    if i == torch.cuda.current_device():
+    if i == torch._C._cuda_getDevice():
         _lib.call(name, *args, stream)
     else:
         with torch.cuda.device(i):
@@ -506,13 +506,14 @@ def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=
     new = torch.empty if cu is None else torch.zeros
     y = new((T, H, D), dtype=_BF16, device=cache.device) if out is None else _kv_out(out, "out", (T, H, D), cache)
     lse = torch.full((T, H), -float("inf"), device=cache.device) if return_lse else None
-    key = (T, B, H, max_q)
+    key = (T, B, P, H, max_q, window, sinks, cp is None)
     nbytes = cache._ws_bytes.get(key)
     if nbytes is None:
         if len(cache._ws_bytes) > 4096:
             cache._ws_bytes.clear()
         with torch.cuda.device(cache.index):
-            nbytes = cache._ws_bytes[key] = _lib.load().moeb_kv_attention_workspace_bytes(T, B, H, cache.kv_heads, D, max_q)
+            nbytes = cache._ws_bytes[key] = _lib.load().moeb_kv_attention_workspace_bytes(
+                T, B, P, cache.page_size, H, cache.kv_heads, D, max_q, window, sinks, cp is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None  # of this call alone
     _kv_call(cache, "moeb_kv_attention", cache._c, qp, qrow, qhead, T, H, cp, lp, tp, trow, B, P, max_q,
              D ** -0.5 if scale is None else float(scale), int(window), int(sinks),
