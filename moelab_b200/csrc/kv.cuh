@@ -202,6 +202,6 @@ __global__ void k_kv_attn_prompt(const KvAttnArgs a, int tiles, float *part);
 template <int D>
 __global__ void k_kv_attn_join_splits(const KvAttnArgs a, const float *part, int ns);
 size_t kv_prompt_smem(int D);
-constexpr int KV_PROMPT_ROWS = 256, KV_PROMPT_THREADS = 640;
+constexpr int KV_PROMPT_ROWS = 256, KV_PROMPT_THREADS = 896;
 
 }  // namespace moeb

@@ -7,12 +7,14 @@
 //   O [128 x D] += P . V (P from TMEM, V in shared memory, its D contiguous: the MN-major operand form).
 // TMEM: O of both tiles (2 D columns), S / P of both tiles and halves (4 x 64). A row tile's products for one half run while
 // its softmax is at the other half, and the two row tiles run side by side.
-//   warps 0 - 3, 4 - 7: softmax of row tile 0, 1: a thread per row, statistics in registers; they also rescale O, only when
-//     a row's maximum grew by more than 2^8 since it was last used (P <= 2^14 in fp16 until then)
-//   warps 8 - 11, 12 - 15: fetch the codes of K, of V (a tile ahead, in registers), dequantize them into fp16 tiles, 128-byte
+//   warps 0 - 15: softmax, two warpgroups per row tile: a thread has a row and 32 of a half's 64 keys, statistics in registers;
+//     the two threads of a row exchange their maxima in shared memory. (One thread per row leaves two such warps per scheduler,
+//     too few to cover the waits between its steps: 4096-token prompt 200 us.) They also rescale O, only when a row's
+//     maximum grew by more than 2^8 since it was last used (P <= 2^14 in fp16 until then)
+//   warps 16 - 19, 20 - 23: fetch the codes of K, of V (a tile ahead, in registers), dequantize them into fp16 tiles, 128-byte
 //     swizzle
-//   warps 16, 17: one lane each issues the products of row tile 0, 1 (18, 19 fill the warpgroup)
-// Registers: 640 x 96 at launch; the softmax warpgroups go to 128, the others to 88 and 40 (60416 of 61440 in all).
+//   warps 24, 25: issue the products of row tile 0, 1 (26, 27 fill the warpgroup)
+// Registers: 896 x 72 at launch; the softmax warpgroups go to 80, the others to 64 and 32 (61440 of 64512 in all).
 // fp16 and not bf16 operands: both formats' values, and P, would lose 2^-9 to bf16, as much as the result's own rounding;
 // fp16 keeps 2^-12. Its range is kept by powers of two: one per query row, one per K tile (both go into the softmax's
 // scale), and a running one for V (a change rescales O; it leaves room for 2^6 of growth, so that it hardly happens).
@@ -28,7 +30,7 @@ namespace moeb {
 namespace {
 
 constexpr int PR = 256;               // rows per CTA
-constexpr int PT = 640;               // threads: five warpgroups
+constexpr int PT = 896;               // threads: seven warpgroups
 constexpr float P_OFF = 6.f;          // P = 2^(score - m + 6)
 constexpr float P_LAZY = 8.f;
 constexpr int P_POLY = 1;                // of 4 pairs of weights, those by ex2_poly
@@ -45,16 +47,19 @@ struct Pr {
 
 struct PrShared {
     uint64_t kfull[3], kempty[3], vfull[3], vempty[3], sfull[2][2], pfull[2][2], pv[2], ofull[2];  // [row tile][half]
-    float kmul[4];             // by key tile % 4: 2^e of the K tile
-    // by key tile % 4: byte per feeding warp, a key without a page or with a NaN among its own; those keys
-    unsigned odd[4], hole[4][4], knan[4][4];
-    struct {
+    struct __align__(8) {
+        float mul;             // 2^e of the K tile
+        unsigned odd;          // byte per feeding warp: a key without a page or with a NaN among its own
+    } k[4];                    // by key tile % 4
+    unsigned hole[4][4], knan[4][4];  // those keys
+    struct __align__(8) {
         float fix;             // what O is multiplied by before this V tile
-        unsigned pz;           // byte per feeding warp, a NaN group among its rows
+        unsigned pz;           // byte per feeding warp: a NaN group among its rows
     } v[3];                    // by stage
     uint8_t pm[3][128];        // by stage and key: its NaN groups
     unsigned mx[2][2][4];      // exchange of the tiles' largest magnitudes: K or V, tile % 2, warp
     float qmul[PR];            // the rows' scale
+    float rowx[2][2][PR];      // exchange between the two threads of a row: by half % 2 (and the sums at the end), thread, row
     float vun;                 // 2^e of O at the end
     uint32_t tmem;
     int b, tile, fail;
@@ -98,23 +103,33 @@ MOEB_DEV uint32_t hfma2u(uint32_t a, uint32_t b, uint32_t c) {
     const __half2 r = __hfma2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b), *reinterpret_cast<__half2 *>(&c));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-// Waits for a phase, at most 2 s of wall time. After that `fail` is set and every later wait returns at once: all roles go
-// through their loops to the end (every address stays in bounds), so that none is left behind and TMEM is released.
-// SLEEP: nanoseconds between tries of a role that runs ahead of the others; its polling took a tenth of the issue slots.
+// Waits for a phase, 2^22 tries at most. After that `fail` is set and every later wait returns soon: all roles go through their
+// loops to the end (every address stays in bounds), so that none is left behind and TMEM is released. SLEEP: nanoseconds
+// between the tries of a role that runs ahead of the others; its polling took a tenth of the issue slots.
 template <int SLEEP = 0>
-MOEB_DEV void pr_wait(uint64_t *bar, unsigned parity, int *fail) {
-    if (mbar_try_wait(bar, parity)) return;
-    const uint64_t t0 = globaltimer_ns();
-    while (true) {
+MOEB_DEV void pr_wait(uint32_t bar, unsigned parity, int *fail) {
+    auto done = [&]() {
+        unsigned ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok)
+                     : "r"(bar), "r"(parity)
+                     : "memory");
+        return ok != 0;
+    };
+    if (done()) return;
 #pragma unroll 1
-        for (int i = 0; i < 256; ++i) {
-            if (mbar_try_wait(bar, parity)) return;
+    for (int n = 0; n < (SLEEP ? 1 << 14 : 1 << 12); ++n) {
+#pragma unroll 1
+        for (int i = 0; i < (SLEEP ? 256 : 1024); ++i) {
+            if (done()) return;
             if (SLEEP) __nanosleep(SLEEP);
         }
         if (*reinterpret_cast<volatile int *>(fail)) return;
-        if (globaltimer_ns() - t0 > 2000000000ull) *reinterpret_cast<volatile int *>(fail) = 1;
     }
+    *reinterpret_cast<volatile int *>(fail) = 1;
 }
+template <int SLEEP = 0>
+MOEB_DEV void pr_wait(uint64_t *bar, unsigned parity, int *fail) { pr_wait<SLEEP>(smem_u32(bar), parity, fail); }
 // 128-byte swizzled operand descriptors: 8 rows of 128 bytes every 1024; LBO: bytes between 64-element chunks of an MN-major
 // operand (K-major ones do not use it). The upper word is constant, the lower one is address / 16 and LBO / 16.
 constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
@@ -393,8 +408,8 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
                     if (x) atomicOr(a.c.err, ERR_PAGE);
                 }
                 if (lane == 0) {
-                    reinterpret_cast<uint8_t *>(&sh.odd[j & 3])[w] = (hole | bad) != 0;
-                    if (w == 0) sh.kmul[j & 3] = vun;
+                    reinterpret_cast<uint8_t *>(&sh.k[j & 3].odd)[w] = (hole | bad) != 0;
+                    if (w == 0) sh.k[j & 3].mul = vun;
                 }
             }
             __syncwarp();
@@ -546,7 +561,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         for (int i = 0; i < 2; ++i) {
             for (int x = 0; x < 2; ++x) {
                 mbar_init(&sh.sfull[i][x], 1);
-                mbar_init(&sh.pfull[i][x], 4);
+                mbar_init(&sh.pfull[i][x], 8);
             }
             mbar_init(sh.pv + i, 1);
             mbar_init(sh.ofull + i, 1);
@@ -554,19 +569,19 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         mbar_fence_init();
         sh.vun = 1.f;
     }
-    if (warp == 16) {
+    if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // ---- queries: fp16 after a power of two per row (the largest value near 2^8), K's order of words, swizzled. D / 8
     // lanes have a row (one word of 8 values each), so that the loads are whole lines.
-    if (warp < 8) {
+    if (warp < 16) {
         constexpr int LR = D / 8, RW = 32 / LR;  // lanes per row, rows per load
         const int x = lane % LR;
-        uint4 w[32 / RW];
+        uint4 w[16 / RW];
 #pragma unroll
-        for (int i = 0; i < 32 / RW; ++i) {
-            const int R = R0 + warp * 32 + i * RW + lane / LR;
+        for (int i = 0; i < 16 / RW; ++i) {
+            const int R = R0 + warp * 16 + i * RW + lane / LR;
             w[i] = make_uint4(0, 0, 0, 0);
             if (R < NR) {
                 const int ri = R / a.Gq;
@@ -577,8 +592,8 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             }
         }
 #pragma unroll
-        for (int i = 0; i < 32 / RW; ++i) {
-            const int row = warp * 32 + i * RW + lane / LR;
+        for (int i = 0; i < 16 / RW; ++i) {
+            const int row = warp * 16 + i * RW + lane / LR;
             const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
             uint32_t top = 0;
 #pragma unroll
@@ -606,119 +621,125 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
     fence_after();
     const uint32_t tmem = sh.tmem;
 
-    if (warp >= 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp >= 24) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
         // ------------------------------------------------------------ products, a warp per row tile
-        if (warp == 16) pr_products<D, 0>(a, sh, sm, nk, tmem);
-        if (warp == 17) pr_products<D, 1>(a, sh, sm, nk, tmem);
-    } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 24) pr_products<D, 0>(a, sh, sm, nk, tmem);
+        if (warp == 25) pr_products<D, 1>(a, sh, sm, nk, tmem);
+    } else if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         // ------------------------------------------------------------ codes -> fp16 tiles, K or V
-        pr_feed<FMT, D>(a, sh, sm, keys, b, h, k0, nk, pmax, Lk, warp & 3, lane, warp >= 12);
+        pr_feed<FMT, D>(a, sh, sm, keys, b, h, k0, nk, pmax, Lk, warp & 3, lane, warp >= 20);
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
-        // ------------------------------------------------------------ softmax of row tile t, a thread per row
-        const int t = warp >> 2, row = (warp & 3) * 32 + lane, R = R0 + t * 128 + row;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
+        // ------------------------------------------------------------ softmax of row tile t: two threads per row (sub)
+        const int t = warp >> 3, sub = (warp >> 2) & 1, row = (warp & 3) * 32 + lane, R = R0 + t * 128 + row;
         const bool have = R < NR;
         const int ri = R / a.Gq, pos = have ? p0 + ri : -1, row_t = have ? r0 + ri : 0, row_h = h * a.Gq + R - ri * a.Gq;
         const float qmul = sh.qmul[t * 128 + row];
         unsigned poison = qmul < 0.f ? 1u << 31 : 0u;  // bit g: group g of the row is NaN; bit 31: all of it
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + L::S0 + 128 * t, to = tmem + lanes + D * t;
+        const uint32_t ts = tmem + lanes + L::S0 + 128 * t, to = tmem + lanes + D * t + sub * (D / 2);
+        const int meet = 3 + 4 * t + (warp & 3);  // barrier of the two warps that have the same rows
+        auto other = [&](float mine, int buf) {  // the row's other thread's value
+            sh.rowx[buf][sub][t * 128 + row] = mine;
+            asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
+            return sh.rowx[buf][sub ^ 1][t * 128 + row];
+        };
         const int q0 = R0 + t * 128;
         const int tmin = p0 + q0 / a.Gq, tmax = p0 + (min(q0 + 128, NR) - 1) / a.Gq;  // positions of the tile's rows
-        float m = -INFINITY, l = 0.f, sc = 0.f;
+        // m: what the weights are relative to; a row that has seen no key yet has the lowest number and no weight
+        constexpr float LOW = -3e38f;
+        float m = LOW, l = 0.f, sc = 0.f;
         int st = 0, j0 = pr_tok(keys, k0);
-        unsigned vph = 0;
+        unsigned vph = 0, par = 0;
+        // every row sees all of a half from j0 on: j0 <= jf, and j0 > jw or j0 <= js
+        const int jf = tmin - 63, jw = a.window ? tmax - a.window : -1, js = a.window ? a.sinks - 64 : -1;
+        const uint32_t sf = smem_u32(&sh.sfull[t][0]), pf = smem_u32(&sh.pfull[t][0]), vf = smem_u32(sh.vfull);
 #pragma unroll 1
-        for (int jh = 0; jh < 2 * nk; ++jh) {
-            const int j = jh >> 1, i2 = jh & 1;
-            pr_wait(&sh.sfull[t][i2], j & 1, &sh.fail);
-            fence_after();
-            float v[64];
-            ld32(ts + 64 * i2, v);
-            ld32(ts + 64 * i2 + 32, v + 32);
-            float vfix = 1.f;
-            const unsigned odd = sh.odd[j & 3];
-            if (i2 == 0) {
-                sc = fmaxf(fabsf(qmul) * sh.kmul[j & 3], 1.2e-38f);  // above zero: a hidden score of -inf stays -inf
-                // V's stage: its power of two, its NaN groups
-                pr_wait(sh.vfull + st, vph, &sh.fail);
-                vfix = sh.v[st].fix;
-                if (const unsigned pz = sh.v[st].pz) {
-                    for (int e = 0; e < 128; ++e) {
-                        if (!((pz >> (8 * ((e >> 3) & 3))) & 1u)) continue;
-                        const unsigned g = sh.pm[st][e];
-                        if (g && e <= pos - j0 && (!a.window || e > pos - a.window - j0 || e < a.sinks - j0)) poison |= g;
-                    }
-                    __syncwarp();
-                }
-            }
-            const bool full = j0 + 63 <= tmin && (!a.window || j0 > tmax - a.window || j0 + 63 < a.sinks) && !odd;
-            wait_ld();
-            if (!full) {
-                // bit i: this row sees key i of the half
-                const unsigned long long hole = (unsigned long long)sh.hole[j & 3][2 * i2 + 1] << 32 | sh.hole[j & 3][2 * i2];
-                const unsigned long long old = a.window ? pr_below(pos - a.window + 1 - j0) & ~pr_below(a.sinks - j0) : 0ull;
-                const unsigned long long see = pr_below(pos - j0 + 1) & ~old & ~hole;
-                const unsigned s0 = (unsigned)see, s1 = (unsigned)(see >> 32);
-                if (odd && ((s0 & sh.knan[j & 3][2 * i2]) | (s1 & sh.knan[j & 3][2 * i2 + 1]))) poison |= 1u << 31;
+        for (int j = 0; j < nk; ++j) {
+            unsigned odd = 0;
 #pragma unroll
-                for (int i = 0; i < 64; ++i) v[i] = (i < 32 ? s0 >> i : s1 >> (i - 32)) & 1u ? v[i] : -INFINITY;
-            }
-            // the next half's first key, V's stage
-            j0 += 64;
-            if (i2 && ++st == NST) {
-                st = 0;
-                vph ^= 1;
-            }
-            if (i2 && k0 + j + 1 == keys.ns) j0 = pr_tok(keys, keys.ns);
-            float x0 = max3(v[0], v[1], v[2]), x1 = max3(v[3], v[4], v[5]), x2 = max3(v[6], v[7], v[8]), x3 = max3(v[9], v[10], v[11]);
-#pragma unroll
-            for (int i = 12; i < 60; i += 8) {
-                x0 = max3(x0, v[i], v[i + 1]);
-                x1 = max3(x1, v[i + 2], v[i + 3]);
-                x2 = max3(x2, v[i + 4], v[i + 5]);
-                x3 = max3(x3, v[i + 6], v[i + 7]);
-            }
-            float mt = max3(max3(x0, v[60], v[61]), max3(x1, v[62], v[63]), fmaxf(x2, x3)) * sc;
-            if (mt == INFINITY) poison |= 1u << 31;  // a score past fp32: inf - inf
-            // rescale O when a maximum grew far, or V's power of two changed
-            const bool grew = mt > m + P_LAZY;
-            if (__any_sync(0xffffffffu, grew || vfix != 1.f)) {
-                float ff = vfix;
-                if (grew) {
-                    const float f = ex2p(m - mt);
-                    m = mt;
-                    l *= f;
-                    ff *= f;
-                }
-                if (jh > 0) {
-                    pr_wait(sh.pv + t, (jh - 1) & 1, &sh.fail);
-                    fence_after();
+            for (int i2 = 0; i2 < 2; ++i2) {
+                pr_wait(sf + 8 * i2, par, &sh.fail);
+                fence_after();
+                float v[32];
+                ld32(ts + 64 * i2 + 32 * sub, v);
+                float vfix = 1.f;
+                if (i2 == 0) {
+                    sc = fmaxf(fabsf(qmul) * sh.k[j & 3].mul, 1.2e-38f);  // above zero: a hidden score of -inf stays -inf
+                    odd = sh.k[j & 3].odd;
+                    // V's stage: its power of two, its NaN groups
+                    pr_wait(vf + 8 * st, vph, &sh.fail);
+                    vfix = sh.v[st].fix;
+                    if (const unsigned pz = sh.v[st].pz) {
 #pragma unroll 1
-                    for (int x = 0; x < D; x += 16) {
-                        float o[16];
+                        for (int e = 0; e < 128; ++e) {
+                            if (!((pz >> (8 * ((e >> 3) & 3))) & 1u)) continue;
+                            const unsigned g = sh.pm[st][e];
+                            if (g && e <= pos - j0 && (!a.window || e > pos - a.window - j0 || e < a.sinks - j0)) poison |= g;
+                        }
                         __syncwarp();
-                        ld16(to + x, o);
-                        wait_ld();
-                        uint32_t u[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * ff);
-                        st16(to + x, u);
                     }
                 }
-            }
-            const float off = m == -INFINITY ? 0.f : P_OFF - m;
-            const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
-            uint64_t l2 = pair(l, 0.f);
+                wait_ld();
+                if (!(j0 <= jf && (j0 > jw || j0 <= js)) || odd) {
+                    // bit i: this row sees key i of the half
+                    const unsigned long long hole = (unsigned long long)sh.hole[j & 3][2 * i2 + 1] << 32 | sh.hole[j & 3][2 * i2];
+                    const unsigned long long old = a.window ? pr_below(pos - a.window + 1 - j0) & ~pr_below(a.sinks - j0) : 0ull;
+                    const unsigned long long see = pr_below(pos - j0 + 1) & ~old & ~hole;
+                    const unsigned s0 = (unsigned)see, s1 = (unsigned)(see >> 32), mine = sub ? s1 : s0;
+                    if (odd && ((s0 & sh.knan[j & 3][2 * i2]) | (s1 & sh.knan[j & 3][2 * i2 + 1]))) poison |= 1u << 31;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
+                    for (int i = 0; i < 32; ++i) v[i] = (mine >> i) & 1u ? v[i] : -INFINITY;
+                }
+                j0 += 64;
+                float x0 = max3(v[0], v[1], v[2]), x1 = max3(v[3], v[4], v[5]), x2 = max3(v[6], v[7], v[8]), x3 = max3(v[9], v[10], v[11]);
+#pragma unroll
+                for (int i = 12; i < 28; i += 8) {
+                    x0 = max3(x0, v[i], v[i + 1]);
+                    x1 = max3(x1, v[i + 2], v[i + 3]);
+                    x2 = max3(x2, v[i + 4], v[i + 5]);
+                    x3 = max3(x3, v[i + 6], v[i + 7]);
+                }
+                const float top = max3(max3(x0, v[28], v[29]), max3(x1, v[30], v[31]), fmaxf(x2, x3));
+                // both have read their scores when they meet: P may take their columns
+                const float mt = fmaxf(top, other(top, i2)) * sc;
+                // rescale O when a maximum grew far, or V's power of two changed
+                const bool grew = mt > m + P_LAZY;
+                if (__any_sync(0xffffffffu, grew || (i2 == 0 && vfix != 1.f))) {
+                    float ff = vfix;
+                    if (grew) {
+                        if (mt == INFINITY) poison |= 1u << 31;  // a score past fp32: inf - inf
+                        const float f = ex2p(m - mt);
+                        m = mt;
+                        l *= f;
+                        ff *= f;
+                    }
+                    if (j > 0 || i2 > 0) {
+                        pr_wait(sh.pv + t, i2 ^ 1, &sh.fail);  // the half before: phase 2 j + i2 - 1
+                        fence_after();
+#pragma unroll 1
+                        for (int x = 0; x < D / 2; x += 16) {
+                            float o[16];
+                            __syncwarp();
+                            ld16(to + x, o);
+                            wait_ld();
+                            uint32_t u[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * ff);
+                            st16(to + x, u);
+                        }
+                    }
+                }
+                const float off = P_OFF - m;
+                const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+                uint64_t l2 = pair(l, 0.f);
                 uint32_t u[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     float x, y;
-                    const uint64_t xy = fma2(pair(v[32 * q + 2 * i], v[32 * q + 2 * i + 1]), sc2, off2);
+                    const uint64_t xy = fma2(pair(v[2 * i], v[2 * i + 1]), sc2, off2);
                     if (i % 4 < P_POLY) {
                         ex2_poly(xy, x, y);
                     } else {
@@ -729,22 +750,34 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
                     l2 = add2(l2, pair(x, y));
                     u[i] = h2(x, y);
                 }
-                st16(ts + 64 * i2 + 16 * q, u);
+                st16(ts + 64 * i2 + 16 * sub, u);
+                float la, lb;
+                unpair(l2, la, lb);
+                l = la + lb;
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(pf + 8 * i2) : "memory");
             }
-            float la, lb;
-            unpair(l2, la, lb);
-            l = la + lb;
-            wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.pfull[t][i2]);
+            par ^= 1;
+            if (++st == NST) {
+                st = 0;
+                vph ^= 1;
+            }
+            if (k0 + j + 1 == keys.ns) j0 = pr_tok(keys, keys.ns);
         }
         if (nk > 0) pr_wait(sh.ofull + t, 0, &sh.fail);
         fence_after();
         __syncwarp();
+        {  // the row's sum: both threads add in the same order
+            const float o = other(l, 0);
+            l = sub ? o + l : l + o;
+        }
+        // The largest weight of a row that has seen a key is 2^6 or more; hidden keys may have left 2^-126 each.
+        if (l < 1.f) l = 0.f;
         if (poison >> 31) l = __uint_as_float(0x7fffffffu);
         // ---- the rows' results (m is off by P_OFF against the weights' sum: undone here)
-        const float M = m == -INFINITY ? m : m - P_OFF;
+        const float M = l == 0.f ? -INFINITY : m - P_OFF;
         float mul = nk > 0 ? sh.vun : 0.f, Ls = l, sum_m = M;
         if (!part) {
             if (a.sink_logits && have) {
@@ -761,7 +794,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         unsigned char *stage = sm + t * L::TILE + (warp & 3) * (32 * D * 2);
         float *pd = part ? part + ((size_t)sp * a.s.T * a.H + orow) * D : nullptr;
 #pragma unroll
-        for (int x = 0; x < D; x += 32) {
+        for (int x = 0; x < D / 2; x += 32) {
             float o[32];
             if (nk > 0) {
                 ld32(to + x, o);
@@ -772,7 +805,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             }
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-                const int d = pr_dim<FMT, D>((x + i) / 4), g = d / (FMT == FMT_Q4 ? 64 : 32);
+                const int d = sub ? pr_dim<FMT, D>((D / 2 + x + i) / 4) : pr_dim<FMT, D>((x + i) / 4), g = d / (FMT == FMT_Q4 ? 64 : 32);
                 float y[4];
                 const bool nanv = (poison >> g) & 1u;
 #pragma unroll
@@ -788,8 +821,9 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         }
         if (!part) {
             constexpr int LR = D / 8, RW = 32 / LR;
+            asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
 #pragma unroll 4
-            for (int i = 0; i < 32; i += RW) {
+            for (int i = 16 * sub; i < 16 * sub + 16; i += RW) {
                 const int rr = i + lane / LR, x = lane % LR, Rr = R0 + t * 128 + (warp & 3) * 32 + rr;
                 if (Rr < NR) {
                     const int ri2 = Rr / a.Gq;
@@ -798,7 +832,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
                 }
             }
         }
-        if (have) {
+        if (have && sub == 0) {
             if (part) reinterpret_cast<float2 *>(part + (size_t)ns * a.s.T * a.H * D)[(size_t)sp * a.s.T * a.H + orow] = make_float2(M, l);
             else if (a.lse) a.lse[orow] = Ls == 0.f ? -INFINITY : (sum_m + log2f(Ls)) * 0.6931471805599453f;
         }
@@ -806,7 +840,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
     }
     __syncthreads();
     if (threadIdx.x == 0 && sh.fail) atomicOr(a.c.err, ERR_TIMEOUT);
-    if (warp == 16) {
+    if (warp == 24) {
         __syncwarp();
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
