@@ -14,7 +14,7 @@
 //   warps 16 - 19, 20 - 23: fetch the codes of K, of V (a tile ahead, in registers), dequantize them into fp16 tiles, 128-byte
 //     swizzle
 //   warps 24, 25: issue the products of row tile 0, 1 (26, 27 fill the warpgroup)
-// Registers: 896 x 72 at launch; the softmax warpgroups go to 80, the others to 64 and 32 (61440 of 64512 in all).
+// Registers: 896 x 72 at launch; the softmax warpgroups go to 80, those of the products to 24 (62464 of 64512 in all).
 // fp16 and not bf16 operands: both formats' values, and P, would lose 2^-9 to bf16, as much as the result's own rounding;
 // fp16 keeps 2^-12. Its range is kept by powers of two: one per query row, one per K tile (both go into the softmax's
 // scale), and a running one for V (a change rescales O; it leaves room for 2^6 of growth, so that it hardly happens).
@@ -33,7 +33,6 @@ constexpr int PR = 256;               // rows per CTA
 constexpr int PT = 896;               // threads: seven warpgroups
 constexpr float P_OFF = 6.f;          // P = 2^(score - m + 6)
 constexpr float P_LAZY = 8.f;
-constexpr int P_POLY = 1;                // of 4 pairs of weights, those by ex2_poly
 
 template <int D>
 struct Pr {
@@ -69,21 +68,6 @@ MOEB_DEV float ex2p(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-// 2^x of two values by the FMA units, for some of the weights: the unit that does ex2 gives 16 a clock per SM and would set the
-// pace alone. x = n + r, n whole (added to 1.5 * 2^23, whose low bits are then n), |r| <= 1/2; 2^r by the polynomial of degree
-// 3 with the least relative error there (7.5e-5, a Remez exchange; the weights' rounding to fp16 is 2.4e-4), n into the exponent.
-MOEB_DEV void ex2_poly(uint64_t xy, float &x, float &y) {
-    float a, b;
-    unpair(xy, a, b);
-    xy = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
-    const uint64_t t = add2(xy, pair(12582912.f, 12582912.f));
-    const uint64_t r = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), xy);
-    uint64_t p = fma2(r, pair(0.05517166852951050f, 0.05517166852951050f), pair(0.2426111251115799f, 0.2426111251115799f));
-    p = fma2(p, r, pair(0.6932609677314758f, 0.6932609677314758f));
-    p = fma2(p, r, pair(0.9999280571937561f, 0.9999280571937561f));
-    x = __uint_as_float((uint32_t)p + ((uint32_t)t << 23));
-    y = __uint_as_float((uint32_t)(p >> 32) + ((uint32_t)(t >> 32) << 23));
 }
 MOEB_DEV float max3(float x, float y, float z) {
     float r;
@@ -622,12 +606,11 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
     const uint32_t tmem = sh.tmem;
 
     if (warp >= 24) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
         // ------------------------------------------------------------ products, a warp per row tile
         if (warp == 24) pr_products<D, 0>(a, sh, sm, nk, tmem);
         if (warp == 25) pr_products<D, 1>(a, sh, sm, nk, tmem);
     } else if (warp >= 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         // ------------------------------------------------------------ codes -> fp16 tiles, K or V
         pr_feed<FMT, D>(a, sh, sm, keys, b, h, k0, nk, pmax, Lk, warp & 3, lane, warp >= 20);
     } else {
@@ -739,14 +722,9 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     float x, y;
-                    const uint64_t xy = fma2(pair(v[2 * i], v[2 * i + 1]), sc2, off2);
-                    if (i % 4 < P_POLY) {
-                        ex2_poly(xy, x, y);
-                    } else {
-                        unpair(xy, x, y);
-                        x = ex2p(x);
-                        y = ex2p(y);
-                    }
+                    unpair(fma2(pair(v[2 * i], v[2 * i + 1]), sc2, off2), x, y);
+                    x = ex2p(x);
+                    y = ex2p(y);
                     l2 = add2(l2, pair(x, y));
                     u[i] = h2(x, y);
                 }
@@ -773,8 +751,6 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             const float o = other(l, 0);
             l = sub ? o + l : l + o;
         }
-        // The largest weight of a row that has seen a key is 2^6 or more; hidden keys may have left 2^-126 each.
-        if (l < 1.f) l = 0.f;
         if (poison >> 31) l = __uint_as_float(0x7fffffffu);
         // ---- the rows' results (m is off by P_OFF against the weights' sum: undone here)
         const float M = l == 0.f ? -INFINITY : m - P_OFF;
