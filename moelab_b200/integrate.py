@@ -19,6 +19,10 @@ one `layer` call for up to `max_tokens` tokens. Supported blocks:
   softmax over all experts, top-k without renormalisation, times `routed_scaling_factor` (e2e.py:136-140).
   int4.
 
+The attention of the same models (heads of 64 or 128 values; not DeepSeek's latent attention) can run over the 4-bit KV cache:
+`patch_hf_attention` routes it through the library for calls that carry a `QuantizedKVCache`, which takes the place of the
+model's cache in `model(...)` and `model.generate(...)`. gpt-oss's sliding windows and sink logits are arguments of the kernel.
+
 The library computes router logits in fp32 from bf16 inputs. Where a stock block computes them in the model
 dtype, near-ties can pick a different expert. `dequantize_into_stock` writes the variant's dequantized weights
 back into the stock parameters, so a stock model runs on exactly the weights the kernels see; the tests compare
@@ -175,3 +179,142 @@ def policy_for(T, block):
     """The expert kernel family the library picks for a T-token call of this block (for reports)."""
     st = block._moeb["state"]
     return ops.policy(T, st["E"], block._moeb["kw"]["k"])
+
+
+# ------------------------------------------------------------------ attention over the 4-bit KV cache
+ATTENTION = "moelab_b200_kv4"
+
+
+def _kv_cache_class():
+    """The cache class, made on first use (transformers is optional)."""
+    global QuantizedKVCache
+    if QuantizedKVCache is None:
+        from transformers import DynamicCache
+
+        class _QuantizedKVCache(DynamicCache):
+            """Keys and values of every layer in 4 bits (ops.KVCache), `batch` sequences of equal length, up to `max_len`
+            tokens each. Pass as past_key_values to a model patched with patch_hf_attention. Sequences advance together, so
+            padded batches are refused (by the mask function, when a prompt comes)."""
+
+            def __init__(self, config, batch, max_len, fmt="q4", page_size=64, device="cuda"):
+                super().__init__(config=config)
+                cfg = config.get_text_config()
+                dim = _head_dim(cfg)
+                heads = getattr(cfg, "num_key_value_heads", None) or cfg.num_attention_heads
+                per = -(-max_len // page_size)
+                self.moeb_max, self.moeb_batch = int(max_len), int(batch)
+                self.moeb_layers = [ops.KVCache(batch * per, heads, dim, page_size=page_size, fmt=fmt, device=device)
+                                    for _ in range(cfg.num_hidden_layers)]
+                dev = self.moeb_layers[0].device
+                self.moeb_table = torch.arange(batch * per, dtype=torch.int32, device=dev).view(batch, per)
+                self.moeb_lens = torch.zeros(batch, dtype=torch.int32, device=dev)
+                self.moeb_seen = [0] * cfg.num_hidden_layers
+
+            def get_seq_length(self, layer_idx=0):
+                return self.moeb_seen[layer_idx or 0]
+
+            def get_mask_sizes(self, new, layer_idx=0):
+                n = new if isinstance(new, int) else new.shape[0]
+                return self.get_seq_length(layer_idx) + n, 0
+
+            def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
+                B, H, n, D = key_states.shape
+                if B != self.moeb_batch:
+                    raise ValueError(f"a batch of {B} sequences, the cache is for {self.moeb_batch}")
+                seen = self.moeb_seen[layer_idx] + n
+                if seen > self.moeb_max:
+                    raise ValueError(f"{seen} tokens, the cache holds {self.moeb_max}")
+                if max(self.moeb_seen) < seen:  # the first layer of this step
+                    self.moeb_lens.fill_(seen)
+                self.moeb_seen[layer_idx] = seen
+                ops.kv_write(self.moeb_layers[layer_idx], _rows(key_states), _rows(value_states), self.moeb_table,
+                             self.moeb_lens)
+                key = key_states.view_as(key_states)  # a tensor of its own to mark
+                key._moeb_kv = (self, layer_idx)
+                return key, value_states
+
+            def to_stock(self):
+                """A DynamicCache with the stored values in bf16, to continue on the stock attention."""
+                out = DynamicCache()
+                for i, c in enumerate(self.moeb_layers):
+                    n = self.moeb_seen[i]
+                    kv = ops.kv_read(c, self.moeb_table, None, self.moeb_batch * n)
+                    out.update(*(t.view(self.moeb_batch, n, c.kv_heads, c.head_dim).transpose(1, 2) for t in kv), i)
+                return out
+
+        QuantizedKVCache = _QuantizedKVCache
+    return QuantizedKVCache
+
+
+QuantizedKVCache = None
+
+
+def quantized_kv_cache(model, batch, max_len, fmt="q4", page_size=64):
+    """A 4-bit cache for `model` (its layers' heads and widths): `batch` sequences of up to `max_len` tokens."""
+    return _kv_cache_class()(model.config, batch, max_len, fmt, page_size, next(model.parameters()).device)
+
+
+def _head_dim(cfg):
+    if getattr(cfg, "kv_lora_rank", None):
+        raise ValueError("latent attention (DeepSeek) has no per-head cache: not supported")
+    dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+    if dim not in (64, 128):
+        raise ValueError(f"heads of 64 or 128 values are supported, this model has {dim}")
+    return dim
+
+
+def _rows(t):
+    """[B, H, n, D] -> bf16 [B * n, H, D] (a view where the strides allow one)."""
+    B, H, n, D = t.shape
+    return t.detach().to(torch.bfloat16).transpose(1, 2).reshape(B * n, H, D)
+
+
+def _attention(module, query, key, value, attention_mask=None, scaling=None, sliding_window=None, s_aux=None, **_):
+    B, H, n, D = query.shape
+    window = int(sliding_window or 0)
+    tag = getattr(key, "_moeb_kv", None)
+    if tag is not None and not module.training:
+        cache, layer = tag
+        y = ops.kv_attention(_rows(query), cache.moeb_layers[layer], cache.moeb_table, cache.moeb_lens, scale=scaling,
+                             window=window, sink_logits=None if s_aux is None else s_aux.detach().float())
+        return y.view(B, n, H, D).to(query.dtype), None
+    # no 4-bit cache in this call: the definition, in plain torch
+    L, G = key.shape[2], H // key.shape[1]
+    k, v = (t.repeat_interleave(G, dim=1).float() for t in (key, value))
+    s = torch.matmul(query.float(), k.transpose(2, 3)) * (D ** -0.5 if scaling is None else scaling)
+    i, j = torch.arange(L - n, L, device=s.device)[:, None], torch.arange(L, device=s.device)
+    see = j <= i if not window else (j <= i) & (j > i - window)
+    s = s.masked_fill(~see, float("-inf"))
+    if s_aux is not None:
+        s = torch.cat([s, s_aux.float().view(1, H, 1, 1).expand(B, H, n, 1)], dim=-1)
+    p = torch.softmax(s, dim=-1)[..., :L]
+    return torch.matmul(p, v).transpose(1, 2).to(query.dtype).contiguous(), None
+
+
+def _attention_mask(*_, attention_mask=None, q_length=None, **__):
+    """No mask tensor: causality and the window are the kernel's. A prompt of a padded batch is refused here."""
+    if attention_mask is not None and (q_length is None or q_length > 1) and not bool(attention_mask.bool().all()):
+        raise ValueError("padded batches are not supported by the 4-bit KV cache attention")
+    return None
+
+
+def patch_hf_attention(model):
+    """Route the model's attention through the library for calls with a quantized_kv_cache (others run the same attention in
+    plain torch). Returns the name of the implementation that unpatch_hf_attention restores."""
+    from transformers import AttentionInterface, AttentionMaskInterface
+    _head_dim(model.config.get_text_config())
+    AttentionInterface.register(ATTENTION, _attention)
+    AttentionMaskInterface.register(ATTENTION, _attention_mask)
+    stock = model.config._attn_implementation
+    if stock != ATTENTION:
+        model._moeb_attention_stock = stock
+        model.set_attn_implementation(ATTENTION)
+    return model._moeb_attention_stock
+
+
+def unpatch_hf_attention(model):
+    """Restore the stock attention. Returns whether the model was patched."""
+    stock = model.__dict__.pop("_moeb_attention_stock", None)
+    if stock is not None:
+        model.set_attn_implementation(stock)
+    return stock is not None
