@@ -107,10 +107,15 @@ int check_cache(const moeb_kv_cache *c, KvCache *o) {
     return MOEB_OK;
 }
 
-int check_seqs(int T, const int *cu, const int *lens, bool need_lens, const int *table, long table_row, int B, int P, KvSeqs *o) {
+int check_seqs(const KvCache &c, int T, const int *cu, const int *lens, bool need_lens, const int *table, long table_row, int B, int P,
+               KvSeqs *o) {
+    const int o_pshift = c.pshift, kv_heads = c.Hkv;
     if (T < 0 || B < 0 || P < 0) return bad("negative number of rows, sequences or table entries");
     if (T > (1 << 26)) return bad("at most 2^26 rows a call");
-    if (T > 0 && B > 0 && (!table || (need_lens && !lens))) return bad("table or lens is null");
+    if (T > 0 && B > 0 && ((P > 0 && !table) || (need_lens && !lens))) return bad("table or lens is null");
+    if ((long)P << o_pshift > 1L << 30) return bad("at most 2^30 tokens a sequence");
+    if ((long)B * kv_heads > 1L << 24) return bad("at most 2^24 pairs of a sequence and a KV head a call");
+    if ((((long)P << o_pshift) / 128 + 4) * B > 0x7fffffffL) return bad("the page tables name more than 2^38 tokens");
     if (B > 1 && table_row < P) return bad("table rows overlap");
     if (!cu && B > 0 && T % B) return bad("without cu every sequence has the same number of rows: T must be a multiple of B");
     o->cu = cu;
@@ -157,9 +162,10 @@ Plan plan_of(int T, int B, int P, int page_size, int H, int Hkv, int D, int max_
     // The window's keys may start and end inside a block of 128; so may the first tokens'.
     auto seen = [&](long rows) { return window ? std::min(all, (long)window + rows + std::min<long>(sinks, all) + 128 + (sinks ? 128 : 0)) : all; };
     // Sequences whose (row, head) columns fit one or two tensor-core tiles go to the kernel for few rows. Without cu all
-    // sequences have T / B rows; with it, and more than one sequence, both kinds may be in the call.
+    // sequences have T / B rows; with it, and more than one sequence, both kinds may be in the call: over up to 1024 keys
+    // the kernel for many rows takes them all (8 key tiles, 16 us at most, against two more launches).
     p.only = cols <= 16;
-    p.few = p.only ? (int)cols : cu && B > 1 ? 16 : 0;
+    p.few = p.only ? (int)cols : cu && B > 1 && seen(max_q) > 1024 ? 16 : 0;
     if (p.few) {
         p.nc = cols <= 8 ? 8 : 16;
         // Up to 4 blocks of 128 keys one after the other cost as much as a second launch to join parts of them: one CTA has
@@ -239,7 +245,7 @@ int moeb_kv_write(const moeb_kv_cache *cache, const void *k, long k_row, long k_
     KvWriteArgs a;
     int rc = check_cache(cache, &a.c);
     if (rc) return rc;
-    if ((rc = check_seqs(T, cu, lens, true, table, table_row, B, P, &a.s))) return rc;
+    if ((rc = check_seqs(a.c, T, cu, lens, true, table, table_row, B, P, &a.s))) return rc;
     if (T == 0 || B == 0) return MOEB_OK;
     if (!rows_ok(k, k_row, k_head) || !rows_ok(v, v_row, v_head))
         return bad("k and v must be 16-byte aligned, with row and head strides that are multiples of 8 elements");
@@ -258,7 +264,7 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
     KvReadArgs a;
     int rc = check_cache(cache, &a.c);
     if (rc) return rc;
-    if ((rc = check_seqs(T, cu, nullptr, false, table, table_row, B, P, &a.s))) return rc;
+    if ((rc = check_seqs(a.c, T, cu, nullptr, false, table, table_row, B, P, &a.s))) return rc;
     if (T == 0 || B == 0) return MOEB_OK;
     if (!k || !v || !aligned16(k) || !aligned16(v)) return bad("k and v must be 16-byte aligned");
     a.first = first;
@@ -282,11 +288,16 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
     KvAttnArgs a;
     int rc = check_cache(cache, &a.c);
     if (rc) return rc;
-    if ((rc = check_seqs(T, cu, lens, true, table, table_row, B, P, &a.s))) return rc;
+    if ((rc = check_seqs(a.c, T, cu, lens, true, table, table_row, B, P, &a.s))) return rc;
     if (H <= 0 || H % cache->kv_heads) return bad("the query heads must be a positive multiple of the cache's kv_heads");
     if (H > 4096) return bad("at most 4096 query heads");
+    if ((long)T * H > 0x7fffffffL) return bad("at most 2^31 - 1 rows times query heads a call");
     if (window < 0 || sinks < 0) return bad("window and sinks must not be negative");
     if (!isfinite(scale)) return bad("scale must be finite");
+    // what the page tables cannot hold is beyond any window and any first tokens
+    const int all = P << a.c.pshift;
+    if (window > all) window = 0;
+    if (sinks > all) sinks = all;
     if (T == 0 || B == 0) return MOEB_OK;
     if (max_q <= 0) return bad("max_q must be positive");
     if (!rows_ok(q, q_row, q_head))

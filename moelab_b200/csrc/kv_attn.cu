@@ -150,6 +150,9 @@ MOEB_DEV uint32_t q4_sub(uint32_t t) {
 struct FewSeq {
     int r0, n, L, lo, ns, nb;
 };
+// End of the keys that a sequence of L tokens can have: its page table's, where that is shorter. It is a multiple of 16 then, so
+// that no half of 16 keys is cut by it, and the kernel need not look at it per key.
+MOEB_DEV int few_end(const KvAttnArgs &a, int L) { return min(L, a.s.P << a.c.pshift); }
 // blocks [0, ns): the first tokens; then from lo / FB on. A sequence with rows has at least one block (its rows are
 // written), one with more rows than fit has none.
 template <int NC>
@@ -162,7 +165,7 @@ MOEB_DEV FewSeq few_seq(const KvAttnArgs &a, int b) {
     const int p0 = max(q.L - q.n, 0);
     q.lo = a.window ? max(p0 - a.window + 1, 0) : 0;
     q.ns = min((min(a.sinks, q.lo) + FB - 1) / FB, q.lo / FB);
-    q.nb = q.n > 0 && (long)q.n * a.Gq <= a.few ? max(q.ns + (int)(((long)q.L + FB - 1) / FB) - q.lo / FB, 1) : 0;
+    q.nb = q.n > 0 && (long)q.n * a.Gq <= a.few ? max(q.ns + max((few_end(a, q.L) + FB - 1) / FB - q.lo / FB, 0), 1) : 0;
     return q;
 }
 MOEB_DEV int few_units(const FewSeq &q) { return q.nb ? q.nb + FR : 0; }  // of each of its heads
@@ -178,13 +181,17 @@ MOEB_DEV long few_start(long W, unsigned c, unsigned n) {
 
 // ws: prefix[B + 1] int32 (blocks before each sequence), then 2 partials per CTA: NC rows of D sums, NC (max, sum).
 template <int FMT, int D, int NT>
-__global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAttnArgs a, int *pre, float *part) {
+__global__ void __launch_bounds__(FT, NT == 1 || D == 64 ? 3 : 2) k_kv_attn_few(const KvAttnArgs a, int *pre, float *part) {
     using F = Few<FMT, D>;
     constexpr int NC = 8 * NT, NG = F::NG;
+    // The queries' operands stay in shared memory where that leaves registers for a third CTA per SM (two tiles of columns of
+    // 128 values need two CTAs' share all the same: in 168 registers they spill, 200001 tokens 77 against 52 us).
+    constexpr bool QS = NT == 2 && D == 64;
     extern __shared__ __align__(128) unsigned char sm[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
     unsigned char *ring = sm + warp * (FS * F::STAGE);
     float *so = reinterpret_cast<float *>(sm + FW * FS * F::STAGE);  // [FW][NC][D]
+    uint4 *sq = reinterpret_cast<uint4 *>(so + FW * NC * D);
     __shared__ float s_m[FW][NC], s_l[FW][NC];
     __shared__ int s_sum[FW], s_b, s_pre;
     pdl_wait();
@@ -215,6 +222,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
         h = i - b * a.c.Hkv;
         q = few_seq<NC>(a, b);
         if (rank == 0 && h == 0 && threadIdx.x == 0 && a.only && (long)q.n * a.Gq > a.few) atomicOr(a.c.err, ERR_ROWS);
+        if (rank == 0 && h == 0 && threadIdx.x == 0 && q.nb && few_end(a, q.L) < q.L) atomicOr(a.c.err, ERR_PAGE);
         if (q.nb == 0) return;  // the whole cluster
         k0 = (int)((unsigned)q.nb * rank / a.direct);
         k1 = (int)((unsigned)q.nb * (rank + 1) / a.direct);
@@ -245,6 +253,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                 const FewSeq s = few_seq<NC>(a, b);
                 pre[b] = at;
                 at += few_units(s);
+                if (s.nb && few_end(a, s.L) < s.L) atomicOr(a.c.err, ERR_PAGE);  // tokens that the table has no place for
                 if (a.only && (long)s.n * a.Gq > a.few) atomicOr(a.c.err, ERR_ROWS);
             }
             if (threadIdx.x == 0) pre[a.s.B] = total;
@@ -278,7 +287,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
     // -1: no row sees the half; -2: it has no page.
     auto pages = [&](const FewSeq &q, int b, int kb, int k1) {
         const int k = kb + (lane >> 1), tok = few_tok(q, k) + 32 * warp + 16 * (lane & 1);
-        if (k >= k1 || tok >= q.L || (tok + 15 < q.lo && tok >= a.sinks)) return -1;
+        if (k >= k1 || tok >= few_end(a, q.L) || (tok + 15 < q.lo && tok >= a.sinks)) return -1;
         const long page = kv_page(a.c, a.s, b, tok);
         return page < 0 ? -2 : (int)page;
     };
@@ -421,6 +430,28 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
             }
         }
 
+        if (QS) {  // the same for all warps
+            if (warp == 0) {
+#pragma unroll
+                for (int x = 0; x < D / 16; ++x) sq[x * 32 + lane] = make_uint4(qf[0][x][0], qf[0][x][1], qf[NT - 1][x][0], qf[NT - 1][x][1]);
+            }
+            __syncthreads();
+        }
+        auto query = [&](int x, uint32_t (&f)[NT][2]) {  // operands of product x
+            if (QS) {
+                const uint4 v = sq[x * 32 + lane];
+                f[0][0] = v.x;
+                f[0][1] = v.y;
+                f[NT - 1][0] = v.z;
+                f[NT - 1][1] = v.w;
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    f[nt][0] = qf[nt][x][0];
+                    f[nt][1] = qf[nt][x][1];
+                }
+            }
+        };
         float o[NT][D / 16][4], m[NT][2], l[NT][2], bs[NT][FMT == FMT_Q4 ? NG : 1][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -480,8 +511,10 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                                 uint32_t A[4];
                                 if (y & 1) { A[0] = q4_sub<2>(ua); A[1] = q4_sub<2>(ub); A[2] = q4_sub<3>(ua); A[3] = q4_sub<3>(ub); }
                                 else { A[0] = q4_sub<0>(ua); A[1] = q4_sub<0>(ub); A[2] = q4_sub<1>(ua); A[3] = q4_sub<1>(ub); }
+                                uint32_t f[NT][2];
+                                query(4 * g + y, f);
 #pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt], A, qf[nt][4 * g + y][0], qf[nt][4 * g + y][1]);
+                                for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt], A, f[nt][0], f[nt][1]);
                             }
                         } else {
                             // half-words 2 c (product 0) and 2 c + 1 of the group
@@ -494,10 +527,13 @@ __global__ void __launch_bounds__(FT, NT == 1 ? 3 : 2) k_kv_attn_few(const KvAtt
                                 A0[0] = e2m1_f16x2<0>(wa[x0]); A0[1] = e2m1_f16x2<0>(wb[x0]); A0[2] = e2m1_f16x2<1>(wa[x0]); A0[3] = e2m1_f16x2<1>(wb[x0]);
                                 A1[0] = e2m1_f16x2<0>(wa[x1]); A1[1] = e2m1_f16x2<0>(wb[x1]); A1[2] = e2m1_f16x2<1>(wa[x1]); A1[3] = e2m1_f16x2<1>(wb[x1]);
                             }
+                            uint32_t f0[NT][2], f1[NT][2];
+                            query(2 * g, f0);
+                            query(2 * g + 1, f1);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
-                                mma_f16(acc[nt], A0, qf[nt][2 * g][0], qf[nt][2 * g][1]);
-                                mma_f16(acc[nt], A1, qf[nt][2 * g + 1][0], qf[nt][2 * g + 1][1]);
+                                mma_f16(acc[nt], A0, f0[nt][0], f0[nt][1]);
+                                mma_f16(acc[nt], A1, f1[nt][0], f1[nt][1]);
                             }
                         }
 #pragma unroll
@@ -827,43 +863,47 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a, const 
     const int c0 = (int)(((u0 + 1) * n - 1) / units), c1 = (int)((u1 * n - 1) / units);  // CTAs of the first and last block
     if (c0 == c1) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int E = D / 32;
-    float m = -INFINITY, l = 0.f, o[E];
+    constexpr int E = D / 32, SIZE = NC * (D + 2);
+    // CTA x's partial: its first place when its share starts in this (sequence, head)
+    auto partial = [&](int x) { return part + ((size_t)x * 2 + (few_start(units, x, n) >= seg ? 0 : 1)) * SIZE; };
+    // the column's maximum first, so that the sums below do not wait for one another
+    float M = -INFINITY;
+    for (int x = c0 + (int)threadIdx.x; x <= c1; x += 256) M = fmaxf(M, partial(x)[NC * D + 2 * col]);
+#pragma unroll
+    for (int i = 16; i; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
+    if (lane == 0) s_m[warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) M = fmaxf(M, s_m[i]);
+    const float use = M == -INFINITY ? 0.f : M;
+    float l = 0.f, o[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = 0.f;
+#pragma unroll 4
     for (int x = c0 + warp; x <= c1; x += 8) {
-        const float *pt = part + ((size_t)x * 2 + (few_start(units, x, n) >= seg ? 0 : 1)) * (NC * (D + 2));
+        const float *pt = partial(x);
         const float2 ml = *reinterpret_cast<const float2 *>(pt + NC * D + 2 * col);
-        const float mn = fmaxf(m, ml.x), use = mn == -INFINITY ? 0.f : mn;
-        const float f = ex2(m - use), g = ex2(ml.x - use);
-        m = mn;
-        l = l * f + ml.y * g;
+        const float f = ex2(ml.x - use);
+        l += ml.y * f;
         const float *src = pt + col * D + lane * E;
 #pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = o[i] * f + src[i] * g;
+        for (int i = 0; i < E; ++i) o[i] += src[i] * f;
     }
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
+    if (lane == 0) s_l[warp] = l;
 #pragma unroll
     for (int i = 0; i < E; ++i) so[warp][lane * E + i] = o[i];
     __syncthreads();
     if (threadIdx.x >= D / 4) return;
-    float M = s_m[0], L = 0.f;
-#pragma unroll
-    for (int i = 1; i < 8; ++i) M = fmaxf(M, s_m[i]);
-    const float use = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float f = ex2(s_m[i] - use);
         const float4 w = *reinterpret_cast<const float4 *>(&so[i][4 * threadIdx.x]);
-        v.x += w.x * f;
-        v.y += w.y * f;
-        v.z += w.z * f;
-        v.w += w.w * f;
-        L += s_l[i] * f;
+        v.x += w.x;
+        v.y += w.y;
+        v.z += w.z;
+        v.w += w.w;
+        L += s_l[i];
     }
     const int ri = kv_div(col, a.Gdiv);
     kv_finish<D>(a, q.r0 + ri, h * a.Gq + col - ri * a.Gq, threadIdx.x, v, M, L);
@@ -871,7 +911,7 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a, const 
 
 template <int FMT, int D, int NT>
 size_t kv_few_smem() {
-    return (size_t)FW * FS * Few<FMT, D>::STAGE + (size_t)FW * 8 * NT * D * 4;
+    return (size_t)FW * FS * Few<FMT, D>::STAGE + (size_t)FW * 8 * NT * D * 4 + (NT == 2 && D == 64 ? D / 16 * 512 : 0);
 }
 
 #define KV_INST(F, D, NT)                                                          \

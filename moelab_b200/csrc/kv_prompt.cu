@@ -176,7 +176,8 @@ MOEB_DEV PrKeys pr_keys(const KvAttnArgs &a, int pmin, int pmax) {
     PrKeys k;
     k.lo = a.window ? max(max(pmin, 0) - a.window + 1, 0) : 0;
     k.ns = min((min(a.sinks, k.lo) + 127) >> 7, k.lo >> 7);
-    k.nt = k.ns + max(((pmax + 128) >> 7) - (k.lo >> 7), 0);
+    const int end = min(pmax + 1, a.s.P << a.c.pshift);  // of the keys: the last row's own, or the end of the page table
+    k.nt = k.ns + max(((end + 127) >> 7) - (k.lo >> 7), 0);
     if (pmax < 0) k.ns = k.nt = 0;
     return k;
 }
@@ -532,6 +533,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
     const int p0 = Lk - n;  // position of row 0
     const int pmin = p0 + R0 / a.Gq, pmax = p0 + (min(R0 + PR, NR) - 1) / a.Gq;
     const PrKeys keys = pr_keys(a, pmin, pmax);
+    if (threadIdx.x == 0 && pmax >= a.s.P << a.c.pshift) atomicOr(a.c.err, ERR_PAGE);  // tokens that the table has no place for
     const int ns = gridDim.y, sp = blockIdx.y;
     const int k0 = (int)((long)keys.nt * sp / ns), k1 = (int)((long)keys.nt * (sp + 1) / ns), nk = k1 - k0;
 

@@ -272,6 +272,51 @@ def test_pages_out_of_sight_are_not_read_and_bad_pages_are_passed_over(n):
     check(y, ref, bound)
 
 
+@pytest.mark.parametrize("n", (1, 3, 140))
+def test_lengths_beyond_the_table(n):
+    """lens that name more tokens than the page table holds: those keys are not there, and the error bit says so; the rows'
+    positions, and with them the others' window, are as lens has it. Lengths of garbage size end too."""
+    b = Batch([256 + n], [n], 4, 2, 64, "q4", page=64, seed=40)
+    c = b.cache(ops)
+    assert c.read_error() == 0
+    short = b.table[:, :4].contiguous()  # 256 tokens: the last n have no page
+    for kw in (dict(), dict(window=n + 40, sinks=3)):
+        y = ops.kv_attention(b.q, c, short, b.lens_t, **kw)
+        assert c.read_error() == _lib.DEVERR_PAGE
+        ref, bound, _ = b.reference(**kw, hole=(0, 256, 256 + n))
+        check(y, ref, bound)
+    far = torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    y = ops.kv_attention(b.q, c, short, far)
+    assert torch.isfinite(y).all() and c.read_error() == _lib.DEVERR_PAGE
+    assert not ops.kv_attention(b.q, c, short, far, window=100).any() and c.read_error() == _lib.DEVERR_PAGE
+    assert not ops.kv_attention(b.q, c, short[:, :0], b.lens_t).any() and c.read_error() == _lib.DEVERR_PAGE
+    ops.kv_write(c, b.new(b.k), b.new(b.v), short, far)
+    assert c.read_error() == _lib.DEVERR_PAGE
+
+
+@pytest.mark.parametrize("n", (1, 200))
+def test_windows_and_first_tokens_of_any_size(n):
+    """Bounds past the sequence are no bounds, up to the largest integers."""
+    b = Batch([n + 300], [n], 4, 2, 64, "mxfp4", page=64, seed=41)
+    c = b.cache(ops)
+    y = attend(b, c)
+    for w, s in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (n + 300, 0), (5, 2 ** 31 - 1), (5, n + 300)):
+        assert torch.equal(attend(b, c, window=w, sinks=s), y) or torch.allclose(
+            attend(b, c, window=w, sinks=s).float(), y.float(), rtol=2 ** -7, atol=1e-3), (w, s)
+
+
+def test_more_rows_than_max_q_says():
+    """A bound that is too small: the rows are left and the error word says so."""
+    b = Batch([60, 70], [1, 3], 8, 1, 64, "q4", page=16, seed=42)
+    c = b.cache(ops)
+    out = torch.full((4, 8, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    ops.kv_attention(b.q, c, b.table, b.lens_t, cu=b.cu, max_q=1, out=out)
+    assert c.read_error() == _lib.DEVERR_ROWS
+    ref, bound, _ = b.reference()
+    check(out[:1], ref[:1], bound[:1])
+    assert (out[1:] == 5).all()
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("ksc,vsc,qsc", [(1e-20, 1e-20, 1e20), (1e4, 1e5, 1e-4), (1e20, 1e30, 1e-20), (1.0, 1e-30, 1.0)])
 @pytest.mark.parametrize("n", (1, 150))

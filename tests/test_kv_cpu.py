@@ -21,8 +21,9 @@ def _read(cache, T=2, table=4096, B=2, k=4096):
     _lib.call("moeb_kv_read", cache, T, None, None, table, 4, B, 4, k, 4096, None)
 
 
-def _attend(cache, q=4096, q_row=256, T=2, H=4, B=2, max_q=1, scale=0.125, window=0, sinks=0, y=4096, ws=4096, ws_bytes=1 << 40):
-    _lib.call("moeb_kv_attention", cache, q, q_row, 64, T, H, None, 4096, 4096, 4, B, 4, max_q, scale, window, sinks, None, y,
+def _attend(cache, q=4096, q_row=256, T=2, H=4, B=2, P=4, max_q=1, scale=0.125, window=0, sinks=0, y=4096, ws=4096,
+            ws_bytes=1 << 40):
+    _lib.call("moeb_kv_attention", cache, q, q_row, 64, T, H, None, 4096, 4096, P, B, P, max_q, scale, window, sinks, None, y,
               None, ws, ws_bytes, None)
 
 
@@ -45,7 +46,9 @@ def test_null_cache_is_refused():
 @pytest.mark.parametrize("kw,match", [
     (dict(T=-1), "negative"), (dict(B=-1), "negative"), (dict(P=-1), "negative"), (dict(T=3), "multiple of B"),
     (dict(lens=None), "null"), (dict(table=None), "null"), (dict(trow=3), "overlap"), (dict(k=None), "16-byte"),
-    (dict(k=4100), "16-byte"), (dict(k_row=4), "16-byte"), (dict(k_head=63), "16-byte"), (dict(T=1 << 27), "2\\^26")])
+    (dict(k=4100), "16-byte"), (dict(k_row=4), "16-byte"), (dict(k_head=63), "16-byte"), (dict(T=1 << 27), "2\\^26"),
+    (dict(P=1 << 27, trow=1 << 27), "2\\^30"), (dict(B=1 << 24, T=1 << 24), "2\\^24"),
+    (dict(B=1 << 22, T=1 << 22, P=1 << 16, trow=1 << 16), "2\\^38")])
 def test_bad_write_is_refused(kw, match):
     with pytest.raises(_lib.MoebError, match=match):
         _write(_cache(), **kw)
@@ -55,7 +58,8 @@ def test_bad_write_is_refused(kw, match):
     (dict(H=3), "multiple"), (dict(H=0), "multiple"), (dict(H=8192), "4096"), (dict(window=-1), "negative"),
     (dict(sinks=-1), "negative"), (dict(scale=float("inf")), "finite"), (dict(scale=float("nan")), "finite"),
     (dict(max_q=0), "max_q"), (dict(q=4104), "16-byte"), (dict(q_row=4), "16-byte"), (dict(y=None), "aligned"),
-    (dict(y=8), "aligned"), (dict(T=-2), "negative")])
+    (dict(y=8), "aligned"), (dict(T=-2), "negative"), (dict(T=1 << 22, H=2048), "2\\^31"), (dict(ws_bytes=16, P=512), "small"),
+    (dict(ws=None, P=512), "workspace"), (dict(ws=4104, P=512), "workspace")])
 def test_bad_attention_is_refused(kw, match):
     with pytest.raises(_lib.MoebError, match=match):
         _attend(_cache(), **kw)
