@@ -14,7 +14,7 @@
 //   warps 16 - 19, 20 - 23: fetch the codes of K, of V (a tile ahead, in registers), dequantize them into fp16 tiles, 128-byte
 //     swizzle
 //   warps 24, 25: issue the products of row tile 0, 1 (26, 27 fill the warpgroup)
-// Registers: 896 x 72 at launch; the softmax warpgroups go to 80, those of the products to 24 (62464 of 64512 in all).
+// Registers: 896 x 72 at launch; the softmax warpgroups go to 80, those of the products to 40 (64512 in all).
 // fp16 and not bf16 operands: both formats' values, and P, would lose 2^-9 to bf16, as much as the result's own rounding;
 // fp16 keeps 2^-12. Its range is kept by powers of two: one per query row, one per K tile (both go into the softmax's
 // scale), and a running one for V (a change rescales O; it leaves room for 2^6 of growth, so that it hardly happens).
@@ -253,7 +253,7 @@ MOEB_DEV uint32_t pr_top(const float (&s)[NG], const float (&b)[NG], unsigned &n
 // parameters and prepares them for all, the passes take them by shuffles. Codes are on their way a tile ahead, parameters and
 // page ids two. One body for K and V: five kinds of warps share the instruction cache.
 template <int FMT, int D>
-MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, const PrKeys &keys, int b, int h, int k0, int nk, int pmax, int Lk,
+MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, const PrKeys &keys, int b, int h, int k0, int nk, int pmax,
                       int w, int lane, bool V) {
     using L = Pr<D>;
     constexpr int NST = L::NST, W4 = D / 32, NG = FMT == FMT_Q4 ? D / 64 : D / 32, NP = FMT == FMT_Q4 ? NG : 1;
@@ -270,7 +270,7 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
     // page id of this lane's key of tile k: -1 where no row sees the key, -2 where it has no page
     auto page = [&](int k) {
         const int j = pr_tok(keys, k0 + k) + mine;
-        if (k >= nk || j > pmax || j >= Lk || (j < keys.lo && j >= a.sinks)) return -1;
+        if (k >= nk || j > pmax || (j < keys.lo && j >= a.sinks)) return -1;
         const int pi = j >> a.c.pshift, id = pi < a.s.P ? table[pi] : -1;
         return id < 0 || id >= a.c.pages ? -2 : id;
     };
@@ -608,13 +608,13 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
     const uint32_t tmem = sh.tmem;
 
     if (warp >= 24) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         // ------------------------------------------------------------ products, a warp per row tile
         if (warp == 24) pr_products<D, 0>(a, sh, sm, nk, tmem);
         if (warp == 25) pr_products<D, 1>(a, sh, sm, nk, tmem);
     } else if (warp >= 16) {
         // ------------------------------------------------------------ codes -> fp16 tiles, K or V
-        pr_feed<FMT, D>(a, sh, sm, keys, b, h, k0, nk, pmax, Lk, warp & 3, lane, warp >= 20);
+        pr_feed<FMT, D>(a, sh, sm, keys, b, h, k0, nk, pmax, warp & 3, lane, warp >= 20);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
         // ------------------------------------------------------------ softmax of row tile t: two threads per row (sub)
