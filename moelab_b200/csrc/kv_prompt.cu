@@ -8,9 +8,10 @@
 // TMEM: O of both tiles (2 D columns), S / P of both tiles and halves (4 x 64). A row tile's products for one half run while
 // its softmax is at the other half, and the two row tiles run side by side.
 //   warps 0 - 15: softmax, two warpgroups per row tile: a thread has a row and 32 of a half's 64 keys, statistics in registers;
-//     the two threads of a row exchange their maxima in shared memory. (One thread per row leaves two such warps per scheduler,
-//     too few to cover the waits between its steps: 4096-token prompt 200 us.) They also rescale O, only when a row's
-//     maximum grew by more than 2^8 since it was last used (P <= 2^14 in fp16 until then)
+//     the two warps of 32 rows meet once per half, ask whether a row's maximum grew by more than 2^8 since it was last used
+//     (P <= 2^14 in fp16 until then), and only then exchange the maxima and rescale O. (One thread per row leaves two such
+//     warps per scheduler, too few to cover the waits between its steps: 4096-token prompt 200 us against 185. A thread with
+//     all 64 keys of one half reads its scores twice and has to wait for the other half: 238 us.)
 //   warps 16 - 19, 20 - 23: fetch the codes of K, of V (a tile ahead, in registers), dequantize them into fp16 tiles, 128-byte
 //     swizzle
 //   warps 24, 25: issue the products of row tile 0, 1 (26, 27 fill the warpgroup)
@@ -58,7 +59,7 @@ struct PrShared {
     uint8_t pm[3][128];        // by stage and key: its NaN groups
     unsigned mx[2][2][4];      // exchange of the tiles' largest magnitudes: K or V, tile % 2, warp
     float qmul[PR];            // the rows' scale
-    float rowx[2][2][PR];      // exchange between the two threads of a row: by half % 2 (and the sums at the end), thread, row
+    float rowx[2][PR];         // exchange between the two threads of a row
     float vun;                 // 2^e of O at the end
     uint32_t tmem;
     int b, tile, fail;
@@ -626,16 +627,23 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + L::S0 + 128 * t, to = tmem + lanes + D * t + sub * (D / 2);
         const int meet = 3 + 4 * t + (warp & 3);  // barrier of the two warps that have the same rows
-        auto other = [&](float mine, int buf) {  // the row's other thread's value
-            sh.rowx[buf][sub][t * 128 + row] = mine;
+        auto meet_any = [&](bool mine) {  // true for one of the two warps' threads
+            unsigned r;
+            asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, %2, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+                         : "=r"(r) : "r"((unsigned)mine), "r"(meet) : "memory");
+            return r != 0;
+        };
+        auto other = [&](float mine) {  // the row's other thread's value; the threads meet again before the next exchange
+            sh.rowx[sub][t * 128 + row] = mine;
             asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
-            return sh.rowx[buf][sub ^ 1][t * 128 + row];
+            return sh.rowx[sub ^ 1][t * 128 + row];
         };
         const int q0 = R0 + t * 128;
         const int tmin = p0 + q0 / a.Gq, tmax = p0 + (min(q0 + 128, NR) - 1) / a.Gq;  // positions of the tile's rows
         // m: what the weights are relative to; a row that has seen no key yet has the lowest number and no weight
         constexpr float LOW = -3e38f;
-        float m = LOW, l = 0.f, sc = 0.f;
+        float m = LOW, sc = 0.f;
+        uint64_t l2 = 0;  // two partial sums of the weights
         int st = 0, j0 = pr_tok(keys, k0);
         unsigned vph = 0, par = 0;
         // every row sees all of a half from j0 on: j0 <= jf, and j0 > jw or j0 <= js
@@ -688,17 +696,16 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
                     x3 = max3(x3, v[i + 6], v[i + 7]);
                 }
                 const float top = max3(max3(x0, v[28], v[29]), max3(x1, v[30], v[31]), fmaxf(x2, x3));
-                // both have read their scores when they meet: P may take their columns
-                const float mt = fmaxf(top, other(top, i2)) * sc;
-                // rescale O when a maximum grew far, or V's power of two changed
-                const bool grew = mt > m + P_LAZY;
-                if (__any_sync(0xffffffffu, grew || (i2 == 0 && vfix != 1.f))) {
+                // rescale O when a maximum of the two warps' rows grew far, or V's power of two changed. Both have read their
+                // scores when they meet: P may take their columns
+                if (meet_any(top * sc > m + P_LAZY || (i2 == 0 && vfix != 1.f))) {
+                    const float mt = fmaxf(top, other(top)) * sc;
                     float ff = vfix;
-                    if (grew) {
+                    if (mt > m + P_LAZY) {
                         if (mt == INFINITY) poison |= 1u << 31;  // a score past fp32: inf - inf
                         const float f = ex2p(m - mt);
                         m = mt;
-                        l *= f;
+                        l2 = mul2(l2, pair(f, f));
                         ff *= f;
                     }
                     if (j > 0 || i2 > 0) {
@@ -719,7 +726,6 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
                 }
                 const float off = P_OFF - m;
                 const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
-                uint64_t l2 = pair(l, 0.f);
                 uint32_t u[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -731,9 +737,6 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
                     u[i] = h2(x, y);
                 }
                 st16(ts + 64 * i2 + 16 * sub, u);
-                float la, lb;
-                unpair(l2, la, lb);
-                l = la + lb;
                 wait_st();
                 fence_before();
                 __syncwarp();
@@ -749,9 +752,12 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         if (nk > 0) pr_wait(sh.ofull + t, 0, &sh.fail);
         fence_after();
         __syncwarp();
+        float l;
         {  // the row's sum: both threads add in the same order
-            const float o = other(l, 0);
-            l = sub ? o + l : l + o;
+            float la, lb;
+            unpair(l2, la, lb);
+            const float mine = la + lb, o = other(mine);
+            l = sub ? o + mine : mine + o;
         }
         if (poison >> 31) l = __uint_as_float(0x7fffffffu);
         // ---- the rows' results (m is off by P_OFF against the weights' sum: undone here)
