@@ -75,30 +75,19 @@ MOEB_DEV Q4Group kv_q4_group(const __nv_bfloat162 m) {
 MOEB_DEV uint32_t kv_quant_q4(const uint4 u, const Q4Group &g) {
     const float scale = g.scale, bias = g.bias, inv = g.inv;
     // code = rint(d / scale), d = v - bias, the quotient rounded to fp32; it is not negative, as the bias is the end of the
-    // range that the scale's sign points away from. r = d * (1 / scale) is within 3 * 2^-24 of the quotient relatively, so
-    // within 2^-18 where it counts (to 16): the two round to the same whole number unless r is that near to a half, and only
-    // then the division is made. Adding 1.5 * 2^23 rounds to a whole number, to even as rintf does.
+    // range that the scale's sign points away from. Quotient: q = d * (1 / scale), then q + (d - q * scale) * (1 / scale) with the
+    // difference exact in a fused product, which is the quotient's rounding when 1 / scale is rounded to nearest (P. Markstein,
+    // Computation of elementary functions on the IBM RISC System/6000, 1990). No branch: bf16 values fall on halves so often
+    // that half of the warps took one that divided only there.
+    // Adding 1.5 * 2^23 rounds to a whole number, to even as rintf does.
     const float big = 12582912.f;
-    const uint64_t b2 = pair(-bias, -bias), i2 = pair(inv, inv), up = pair(big, big), down = pair(-big, -big), neg = pair(-1.f, -1.f);
+    const uint64_t b2 = pair(-bias, -bias), i2 = pair(inv, inv), s2 = pair(-scale, -scale), up = pair(big, big), down = pair(-big, -big);
     const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
-    uint64_t d[4], q[4];
-    float far = 0.f;  // from the whole numbers
+    uint64_t q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        d[i] = add2(pair(bf16lo(uu[i]), bf16hi(uu[i])), b2);
-        const uint64_t r = mul2(d[i], i2);
-        q[i] = add2(add2(r, up), down);
-        float f0, f1;
-        unpair(fma2(q[i], neg, r), f0, f1);
-        far = fmaxf(far, fmaxf(fabsf(f0), fabsf(f1)));
-    }
-    if (far > 0.5f - 7.62939453125e-6f) {  // 2^-17
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float d0, d1;
-            unpair(d[i], d0, d1);
-            q[i] = pair(rintf(__fdiv_rn(d0, scale)), rintf(__fdiv_rn(d1, scale)));
-        }
+        const uint64_t d = add2(pair(bf16lo(uu[i]), bf16hi(uu[i])), b2), r = mul2(d, i2);
+        q[i] = add2(add2(fma2(fma2(r, s2, d), i2, r), up), down);
     }
     // four codes of 16 bits each side: sums of code * 16^p below 2^16 are exact, the low bits of 2^23 + sum are the half-words
     uint64_t acc = pair(8388608.f, 8388608.f);
@@ -156,7 +145,23 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
             next[g] = t < a.s.T ? *reinterpret_cast<const uint4 *>(src + t * stride + g * (8 * X::LR)) : make_uint4(0, 0, 0, 0);
     };
     fetch(t0);
-    int r0 = 0, r1 = 0, b = -1;
+    // where the rows of the warp's passes go, a lane per row: its position, its page (-1: nowhere)
+    constexpr int WR = 32 / X::LR;  // a warp's rows in a pass
+    const int lane = threadIdx.x & 31;
+    int at = -1, to = -1;
+    {
+        const int t = t0 - lane / X::LR + lane / WR * X::R + lane % WR;
+        if (lane / WR < a.passes && t < a.s.T) {
+            int r0, r1;
+            const int b = kv_seq_of(a.s, t, r0, r1);
+            if (b >= 0) at = a.s.lens[b] - (r1 - t);
+            if (at >= 0) {
+                to = (int)kv_page(a.c, a.s, b, at);
+                if (to < 0 && blockIdx.y == 0) atomicOr(a.c.err, ERR_PAGE);
+            }
+        }
+        __syncwarp();
+    }
 #pragma unroll 1  // once in the instruction cache
     for (int i = 0; i < a.passes; ++i) {
         const int t = t0 + i * X::R;
@@ -164,18 +169,8 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) u[g] = next[g];
         if (i + 1 < a.passes) fetch(t + X::R);
-        long page = -1;
-        int p = -1;
-        if (t < a.s.T) {
-            if (t >= r1 || t < r0) b = kv_seq_of(a.s, t, r0, r1);
-            if (b >= 0) p = a.s.lens[b] - (r1 - t);
-            if (p >= 0) {
-                page = kv_page(a.c, a.s, b, p);
-                if (page < 0 && w == 0) atomicOr(a.c.err, ERR_PAGE);
-            }
-        }
+        const int page = __shfl_sync(0xffffffffu, to, i * WR + lane / X::LR), p = __shfl_sync(0xffffffffu, at, i * WR + lane / X::LR);
         // every lane takes part in the shuffles; a group's lanes are all inside one row
-        __syncwarp();
         uint32_t word[NG], out[NG], par[NG];
         if (FMT == FMT_Q4) {
             __nv_bfloat162 m = kv_q4_range(u[0]);
