@@ -37,8 +37,8 @@ MOEB_DEV void lane_words(const uint32_t (&in)[N], uint32_t (&out)[N], bool to_wo
 // by memory: pairs of values go through packed operations, and where a lane has two groups, four of the eight lanes work
 // out the parameters of one, four those of the other.
 struct Q4Group {
-    float scale, bias, inv;
-    uint32_t par;  // as stored; 0: all zeros
+    float scale, bias, inv;  // inv = 0: all codes are 0
+    uint32_t par;            // as stored; 0: all zeros
 };
 // (largest, -smallest) of the group; a NaN stays
 MOEB_DEV __nv_bfloat162 kv_q4_range(const uint4 u) {
@@ -66,10 +66,10 @@ MOEB_DEV Q4Group kv_q4_group(const __nv_bfloat162 m) {
         g.bias = edge;
     }
     g.scale = scale;
-    g.inv = __frcp_rn(scale);
     // q0 = 0: the largest magnitude is below half the smallest scale, every code is 0 and the values are zeros. The weight
     // quantizer keeps that scale; here it is 0, so that attention, which takes codes less 8, meets nothing to cancel.
     g.par = bad ? 0x7fff7fffu : q0 == 0.0f ? 0u : (uint32_t)f2bf(scale) | ((uint32_t)f2bf(g.bias) << 16);
+    g.inv = bad || q0 == 0.0f ? 0.0f : __frcp_rn(scale);
     return g;
 }
 MOEB_DEV uint32_t kv_quant_q4(const uint4 u, const Q4Group &g) {
@@ -79,27 +79,18 @@ MOEB_DEV uint32_t kv_quant_q4(const uint4 u, const Q4Group &g) {
     // difference exact in a fused product, which is the quotient's rounding when 1 / scale is rounded to nearest (P. Markstein,
     // Computation of elementary functions on the IBM RISC System/6000, 1990). No branch: bf16 values fall on halves so often
     // that half of the warps took one that divided only there.
-    // Adding 1.5 * 2^23 rounds to a whole number, to even as rintf does.
-    const float big = 12582912.f;
-    const uint64_t b2 = pair(-bias, -bias), i2 = pair(inv, inv), s2 = pair(-scale, -scale), up = pair(big, big), down = pair(-big, -big);
+    // Adding 1.5 * 2^23 rounds to a whole number, to even as rintf does, and leaves it in the low bits.
+    const uint64_t b2 = pair(-bias, -bias), i2 = pair(inv, inv), s2 = pair(-scale, -scale), up = pair(12582912.f, 12582912.f);
     const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
-    uint64_t q[4];
+    uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint64_t d = add2(pair(bf16lo(uu[i]), bf16hi(uu[i])), b2), r = mul2(d, i2);
-        q[i] = add2(add2(fma2(fma2(r, s2, d), i2, r), up), down);
+        const uint64_t q = add2(fma2(fma2(r, s2, d), i2, r), up);
+        // value 2 i's code in the low half, 2 i + 1's in the high one: nibbles i and i + 4 of the word
+        word += __vminu2(__byte_perm((uint32_t)q, (uint32_t)(q >> 32), 0x5410), 0x000f000fu) << (4 * i);
     }
-    // four codes of 16 bits each side: sums of code * 16^p below 2^16 are exact, the low bits of 2^23 + sum are the half-words
-    uint64_t acc = pair(8388608.f, 8388608.f);
-#pragma unroll
-    for (int p = 3; p >= 0; --p) {
-        float c0, c1;
-        unpair(q[p], c0, c1);
-        const float w = (float)(1 << (4 * p));
-        acc = fma2(pair(fminf(c0, 15.f), fminf(c1, 15.f)), pair(w, w), acc);
-    }
-    const uint32_t word = __byte_perm((uint32_t)acc, (uint32_t)(acc >> 32), 0x5410);
-    return g.par == 0u || g.par == 0x7fff7fffu ? 0u : word;
+    return inv == 0.f ? 0u : word;
 }
 MOEB_DEV uint32_t kv_quant_fp4(const uint4 u, uint32_t &par) {
     const float v[8] = {bf16lo(u.x), bf16hi(u.x), bf16lo(u.y), bf16hi(u.y), bf16lo(u.z), bf16hi(u.z), bf16lo(u.w), bf16hi(u.w)};
@@ -179,6 +170,7 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
                 if (w & 4) m = m1;
             }
             const Q4Group mine = kv_q4_group(m);
+            par[0] = mine.par;  // of the group whose parameters this lane worked out
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 Q4Group q = mine;
@@ -187,9 +179,7 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
                     q.scale = __shfl_sync(0xffffffffu, mine.scale, from);
                     q.bias = __shfl_sync(0xffffffffu, mine.bias, from);
                     q.inv = __shfl_sync(0xffffffffu, mine.inv, from);
-                    q.par = __shfl_sync(0xffffffffu, mine.par, from);
                 }
-                par[g] = q.par;
                 word[g] = kv_quant_q4(u[g], q);
             }
         } else {
@@ -201,10 +191,10 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
         lane_words<FMT>(word, out, false);
         using T = typename Vec<NG>::T;
         *reinterpret_cast<T *>(codes + row * (D / 8)) = *reinterpret_cast<const T *>(out);
-        if (w == 0) {
-            if (FMT == FMT_Q4) {
-                *reinterpret_cast<T *>(ps + row * (4 * NG)) = *reinterpret_cast<const T *>(par);
-            } else if (NG == 4) {
+        if (FMT == FMT_Q4) {
+            if (w % (8 / NG) == 0) *reinterpret_cast<uint32_t *>(ps + row * (4 * NG) + w / (8 / NG) * 4) = par[0];
+        } else if (w == 0) {
+            if (NG == 4) {
                 *reinterpret_cast<uint32_t *>(ps + row * NG) = par[0] | par[1] << 8 | par[NG - 2] << 16 | par[NG - 1] << 24;
             } else {
                 *reinterpret_cast<uint16_t *>(ps + row * NG) = (uint16_t)(par[0] | par[1 % NG] << 8);
