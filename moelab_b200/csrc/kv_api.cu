@@ -4,8 +4,7 @@
 #include <stdio.h>
 
 #include <algorithm>
-#include <map>
-#include <mutex>
+#include <atomic>
 
 #include "../../include/moelab_b200.h"
 #include "kv.cuh"
@@ -52,36 +51,37 @@ cudaError_t launch(void (*kern)(K...), dim3 grid, int threads, size_t smem, cuda
     return launch_cluster(kern, grid, threads, smem, 1, st, args...);
 }
 
+constexpr int DEVICES = 64;  // whose answers are kept
+
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 int sms() {
-    static std::mutex mu;
-    static std::map<int, int> cache;
-    int dev = 0;
+    static std::atomic<int> cache[DEVICES];
+    int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) {
         cudaGetLastError();
         return 148;
     }
-    std::lock_guard<std::mutex> lk(mu);
-    int &n = cache[dev];
-    if (!n && (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)) n = 148;
+    if (dev < DEVICES && (n = cache[dev].load())) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    if (dev < DEVICES) cache[dev] = n;
     return n;
 }
 
-// Resident CTAs per SM of a kernel on the current device; its dynamic shared memory is allowed on the first call.
-int resident(const void *kern, int threads, size_t smem) {
-    static std::mutex mu;
-    static std::map<std::pair<const void *, int>, int> cache;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lk(mu);
-    int &n = cache[{kern, dev}];
-    if (!n) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n < 1)
-            n = 0;
+// Resident CTAs per SM of a kernel on the current device, 0 if it cannot run; its dynamic shared memory is allowed on the first
+// call. `cache`: the kernel's own.
+int resident(std::atomic<int> (&cache)[DEVICES], const void *kern, int threads, size_t smem) {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess) {
+        if (dev < DEVICES && (n = cache[dev].load())) return n;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess &&
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) == cudaSuccess && n > 0) {
+            if (dev < DEVICES) cache[dev] = n;
+            return n;
+        }
     }
-    return n;
+    cudaGetLastError();
+    return 0;
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -153,7 +153,7 @@ struct Plan {
     long tiles, splits; // row tiles of the kernel for many rows; parts that each one's keys are cut into
     size_t split_bytes;
 };
-constexpr int FEW_RESIDENT = 3;  // CTAs per SM at most (the kernel's launch bound)
+constexpr int FEW_RESIDENT = 3;  // CTAs per SM at most: the workspace has room for their partial results
 
 Plan plan_of(int T, int B, int P, int page_size, int H, int Hkv, int D, int max_q, int window, int sinks, bool cu) {
     Plan p = {};
@@ -204,7 +204,8 @@ Plan plan_of(int T, int B, int P, int page_size, int H, int Hkv, int D, int max_
 template <int FMT, int D, int NT>
 int launch_few(const KvAttnArgs &a, const Plan &p, void *ws, cudaStream_t st) {
     const size_t smem = kv_few_smem<FMT, D, NT>();
-    const int per = resident((const void *)k_kv_attn_few<FMT, D, NT>, 128, smem);
+    static std::atomic<int> cache[DEVICES];
+    const int per = std::min(resident(cache, (const void *)k_kv_attn_few<FMT, D, NT>, 128, smem), FEW_RESIDENT);
     if (!per) return launched(cudaErrorInvalidConfiguration, "kv_attention");
     int *pre = (int *)ws;
     float *part = (float *)((char *)ws + p.part);
@@ -223,7 +224,8 @@ int launch_few(const KvAttnArgs &a, const Plan &p, void *ws, cudaStream_t st) {
 template <int FMT, int D>
 int launch_prompt(const KvAttnArgs &a, const Plan &p, void *ws, cudaStream_t st) {
     const size_t smem = kv_prompt_smem(D);
-    if (!resident((const void *)k_kv_attn_prompt<FMT, D>, KV_PROMPT_THREADS, smem))
+    static std::atomic<int> cache[DEVICES];
+    if (!resident(cache, (const void *)k_kv_attn_prompt<FMT, D>, KV_PROMPT_THREADS, smem))
         return launched(cudaErrorInvalidConfiguration, "kv_attention");
     float *part = p.splits > 1 ? (float *)ws : nullptr;
     cudaError_t e = launch(k_kv_attn_prompt<FMT, D>, dim3((unsigned)(p.tiles * a.c.Hkv), (unsigned)p.splits), KV_PROMPT_THREADS, smem, st, a,
@@ -293,7 +295,7 @@ int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, lon
     if (H > 4096) return bad("at most 4096 query heads");
     if ((long)T * H > 0x7fffffffL) return bad("at most 2^31 - 1 rows times query heads a call");
     if (window < 0 || sinks < 0) return bad("window and sinks must not be negative");
-    if (!isfinite(scale)) return bad("scale must be finite");
+    if (!isfinite(scale * 1.4426950408889634f)) return bad("scale must be finite, and below 2^127");
     // what the page tables cannot hold is beyond any window and any first tokens
     const int all = P << a.c.pshift;
     if (window > all) window = 0;

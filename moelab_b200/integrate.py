@@ -185,6 +185,10 @@ def policy_for(T, block):
 ATTENTION = "moelab_b200_kv4"
 
 
+class _Length(int):
+    """A mask's number of keys that comes from a 4-bit cache."""
+
+
 def _kv_cache_class():
     """The cache class, made on first use (transformers is optional)."""
     global QuantizedKVCache
@@ -194,7 +198,8 @@ def _kv_cache_class():
         class _QuantizedKVCache(DynamicCache):
             """Keys and values of every layer in 4 bits (ops.KVCache), `batch` sequences of equal length, up to `max_len`
             tokens each. Pass as past_key_values to a model patched with patch_hf_attention. Sequences advance together, so
-            padded batches are refused (by the mask function, when a prompt comes)."""
+            padded batches are refused (by the mask function, when a prompt comes), and so is what reorders or repeats them
+            (beam search). crop() and reset() give tokens up."""
 
             def __init__(self, config, batch, max_len, fmt="q4", page_size=64, device="cuda"):
                 super().__init__(config=config)
@@ -215,7 +220,19 @@ def _kv_cache_class():
 
             def get_mask_sizes(self, new, layer_idx=0):
                 n = new if isinstance(new, int) else new.shape[0]
-                return self.get_seq_length(layer_idx) + n, 0
+                return _Length(self.get_seq_length(layer_idx) + n), 0
+
+            def crop(self, max_length):
+                n = max_length if max_length >= 0 else self.get_seq_length() + max_length
+                self.moeb_seen = [max(min(n, s), 0) for s in self.moeb_seen]
+
+            def reset(self):
+                self.crop(0)
+
+            def _refuse(self, *_, **__):
+                raise NotImplementedError("sequences of the 4-bit KV cache are not reordered, repeated or selected")
+
+            reorder_cache = batch_repeat_interleave = batch_select_indices = _refuse
 
             def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
                 B, H, n, D = key_states.shape
@@ -224,7 +241,7 @@ def _kv_cache_class():
                 seen = self.moeb_seen[layer_idx] + n
                 if seen > self.moeb_max:
                     raise ValueError(f"{seen} tokens, the cache holds {self.moeb_max}")
-                if max(self.moeb_seen) < seen:  # the first layer of this step
+                if layer_idx == 0:
                     self.moeb_lens.fill_(seen)
                 self.moeb_seen[layer_idx] = seen
                 ops.kv_write(self.moeb_layers[layer_idx], _rows(key_states), _rows(value_states), self.moeb_table,
@@ -271,28 +288,35 @@ def _rows(t):
 
 def _attention(module, query, key, value, attention_mask=None, scaling=None, sliding_window=None, s_aux=None, **_):
     B, H, n, D = query.shape
-    window = int(sliding_window or 0)
     tag = getattr(key, "_moeb_kv", None)
-    if tag is not None and not module.training:
+    if tag is not None:
+        if module.training:
+            raise ValueError("the 4-bit KV cache has no backward pass: call model.eval() first")
+        if attention_mask is not None:
+            raise ValueError("attention masks of the caller's own are not supported by the 4-bit KV cache attention")
         cache, layer = tag
         y = ops.kv_attention(_rows(query), cache.moeb_layers[layer], cache.moeb_table, cache.moeb_lens, scale=scaling,
-                             window=window, sink_logits=None if s_aux is None else s_aux.detach().float())
+                             window=int(sliding_window or 0), sink_logits=None if s_aux is None else s_aux.detach().float())
         return y.view(B, n, H, D).to(query.dtype), None
-    # no 4-bit cache in this call: the definition, in plain torch
+    # no 4-bit cache in this call: the definition, in plain torch, with the mask that the eager attention gets
     L, G = key.shape[2], H // key.shape[1]
     k, v = (t.repeat_interleave(G, dim=1).float() for t in (key, value))
     s = torch.matmul(query.float(), k.transpose(2, 3)) * (D ** -0.5 if scaling is None else scaling)
-    i, j = torch.arange(L - n, L, device=s.device)[:, None], torch.arange(L, device=s.device)
-    see = j <= i if not window else (j <= i) & (j > i - window)
-    s = s.masked_fill(~see, float("-inf"))
+    if attention_mask is not None:
+        m = attention_mask[..., :L]
+        s = s.masked_fill(~m, torch.finfo(s.dtype).min) if m.dtype == torch.bool else s + m.float()
     if s_aux is not None:
         s = torch.cat([s, s_aux.float().view(1, H, 1, 1).expand(B, H, n, 1)], dim=-1)
     p = torch.softmax(s, dim=-1)[..., :L]
     return torch.matmul(p, v).transpose(1, 2).to(query.dtype).contiguous(), None
 
 
-def _attention_mask(*_, attention_mask=None, q_length=None, **__):
-    """No mask tensor: causality and the window are the kernel's. A prompt of a padded batch is refused here."""
+def _attention_mask(*args, kv_length=None, attention_mask=None, q_length=None, **kw):
+    """With a 4-bit cache no mask tensor: causality and the window are the kernel's; a prompt of a padded batch is refused
+    here. Without one the mask of the eager attention."""
+    if not isinstance(kv_length, _Length):
+        from transformers import AttentionMaskInterface
+        return AttentionMaskInterface()["eager"](*args, kv_length=kv_length, attention_mask=attention_mask, q_length=q_length, **kw)
     if attention_mask is not None and (q_length is None or q_length > 1) and not bool(attention_mask.bool().all()):
         raise ValueError("padded batches are not supported by the 4-bit KV cache attention")
     return None

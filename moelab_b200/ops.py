@@ -465,13 +465,14 @@ def kv_write(cache, k, v, table, lens, cu=None):
 
 def kv_read(cache, table, cu, rows, first=None, out=None):
     """Read rows back as bf16: (k, v), each [rows, kv_heads, head_dim]. Row i of sequence b (rows cu[b] .. cu[b + 1] - 1;
-    cu None: rows / B each) is its position first[b] + i (first None: i). out: (k, v) to fill, whose rows behind the last
+    cu None: rows / B each) is its position first[b] + i (first None: i); without a valid page it is zero and sets
+    DEVERR_PAGE. out: (k, v) to fill, whose rows behind the last
     sequence are left as they were; without it those rows are zero."""
     tp, trow, B, P = _kv_table(table, cache)
     cp, fp = _kv_cu(cu, rows, B, cache), _kv_ints(first, "first", cache, B)
     shape = (rows, cache.kv_heads, cache.head_dim)
     if out is None:
-        new = torch.empty if cu is None else torch.zeros
+        new = torch.empty if cu is None and B else torch.zeros
         k, v = (new(shape, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
     else:
         k, v = (_kv_out(t, "out", shape, cache) for t in out)
@@ -496,6 +497,7 @@ def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=
         raise ValueError(f"{H} query heads over {cache.kv_heads} KV heads")
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
+    window, sinks = min(int(window), 0x7fffffff), min(int(sinks), 0x7fffffff)
     if sink_logits is not None:
         _need(sink_logits, torch.float32, "sink_logits")
         if sink_logits.shape != (H,) or sink_logits.device != cache.device:
@@ -503,7 +505,7 @@ def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=
     max_q = T // max(B, 1) if cu is None else T if max_q is None else min(int(max_q), T)
     if T and max_q <= 0:
         raise ValueError("max_q must be positive")
-    new = torch.empty if cu is None else torch.zeros
+    new = torch.empty if cu is None and B else torch.zeros
     y = new((T, H, D), dtype=_BF16, device=cache.device) if out is None else _kv_out(out, "out", (T, H, D), cache)
     lse = torch.full((T, H), -float("inf"), device=cache.device) if return_lse else None
     key = (T, B, P, H, max_q, window, sinks, cp is None)
@@ -516,7 +518,7 @@ def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=
                 T, B, P, cache.page_size, H, cache.kv_heads, D, max_q, window, sinks, cp is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None  # of this call alone
     _kv_call(cache, "moeb_kv_attention", cache._c, qp, qrow, qhead, T, H, cp, lp, tp, trow, B, P, max_q,
-             D ** -0.5 if scale is None else float(scale), int(window), int(sinks),
+             D ** -0.5 if scale is None else float(scale), window, sinks,
              None if sink_logits is None else sink_logits.data_ptr(), y.data_ptr(), None if lse is None else lse.data_ptr(),
              None if ws is None else ws.data_ptr(), nbytes)
     return (y, lse) if return_lse else y

@@ -51,6 +51,25 @@ def test_extreme_rows(fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+def test_many_rows_are_the_oracles_quantization(fmt):
+    """16,000 groups and more of each kind, from 2^-60 to 2^60: normal, all of one sign, around a large middle, small integers
+    (codes that lie on a half all the time)."""
+    g = torch.Generator().manual_seed(11)
+    w = torch.randn(2048, 8, 128, generator=g)
+    w[1::4] = w[1::4].abs()
+    w[2::4] += 30 * torch.randn(512, 8, 1, generator=g)
+    w[3::4] = torch.randint(-128, 129, (512, 8, 128), generator=g).float()
+    w = (w * torch.exp2(torch.randint(-60, 61, (2048, 8, 1), generator=g).float())).to(torch.bfloat16)
+    c = ops.KVCache(32, 8, 128, page_size=64, fmt=fmt)
+    table = torch.arange(32, dtype=torch.int32, device="cuda").view(1, 32)
+    ops.kv_write(c, w.cuda(), w.flip(0).cuda(), table, torch.tensor([2048], dtype=torch.int32, device="cuda"))
+    k, v = ops.kv_read(c, table, None, 2048)
+    ref = stored(w, fmt).to(torch.bfloat16)
+    assert torch.equal(k.cpu().view(torch.int16), ref.view(torch.int16))
+    assert torch.equal(v.cpu().view(torch.int16), ref.flip(0).view(torch.int16))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 def test_group_with_a_nan_reads_back_as_nan_alone(fmt):
     D, gs = 128, 64 if fmt == "q4" else 32
     w = torch.randn(4, 2, D, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
@@ -126,7 +145,14 @@ def test_no_tokens():
     assert ops.kv_attention(torch.empty(0, 2, 64, dtype=torch.bfloat16, device="cuda"), c, table, lens).shape == (0, 2, 64)
     y = ops.kv_attention(torch.ones(2, 2, 64, dtype=torch.bfloat16, device="cuda"), c, table, lens)
     assert not y.any()  # sequences of length zero: rows before their start see nothing
-    assert c.read_error() == 0
+    # rows, but no sequences: all of them are behind the last one
+    rows, junk = torch.ones(300, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.full((1 << 20,), 7.0, device="cuda")
+    del junk
+    for t, n in ((table[:0], lens[:0]),):
+        assert not ops.kv_attention(rows, c, t, n).any() and not ops.kv_attention(rows, c, t, n, cu=lens[:1]).any()
+        assert not ops.kv_read(c, t, None, 300)[0].any()
+        ops.kv_write(c, rows[:, :1], rows[:, :1], t, n)
+    assert c.read_error() == 0 and not c.kq.any()
 
 
 # ------------------------------------------------------------------ attention
@@ -300,9 +326,27 @@ def test_windows_and_first_tokens_of_any_size(n):
     b = Batch([n + 300], [n], 4, 2, 64, "mxfp4", page=64, seed=41)
     c = b.cache(ops)
     y = attend(b, c)
-    for w, s in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (n + 300, 0), (5, 2 ** 31 - 1), (5, n + 300)):
+    for w, s in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (n + 300, 0), (5, 2 ** 31 - 1), (5, n + 300), (2 ** 32 + 5, 0),
+                 (5, 2 ** 32 + 5)):
         assert torch.equal(attend(b, c, window=w, sinks=s), y) or torch.allclose(
             attend(b, c, window=w, sinks=s).float(), y.float(), rtol=2 ** -7, atol=1e-3), (w, s)
+
+
+@pytest.mark.parametrize("n", (1, 60))
+def test_pages_that_sequences_share(n):
+    """Two sequences with the same first pages, and one that has a page twice: read as if each had its own."""
+    b = Batch([300, 300], [n, n], 8, 2, 128, "q4", page=32, seed=43)
+    b.k[1, :192], b.v[1, :192] = b.k[0, :192], b.v[0, :192]
+    for t in (b.k, b.v):
+        t[:, 32:64] = t[:, :32]
+    c = b.cache(ops)
+    table = b.table.clone()
+    table[1, :6] = table[0, :6]
+    table[:, 1] = table[:, 0]
+    ref, bound, _ = b.reference()
+    check(ops.kv_attention(b.q, c, table, b.lens_t, cu=b.cu, max_q=n), ref, bound)
+    k, _ = ops.kv_read(c, table, None, 600)
+    assert torch.equal(k, ops.kv_read(c, b.table, None, 600)[0])
 
 
 def test_more_rows_than_max_q_says():

@@ -130,6 +130,70 @@ def test_refusals(stand_in):
         integrate._head_dim(wide)
 
 
+@pytest.mark.parametrize("family", ["qwen3", "gptoss"])
+def test_without_the_cache_masks_are_the_stock_models(family):
+    """A patched model called without a 4-bit cache: padded batches, the caller's own mask and a static cache give the eager
+    attention's logits; gradients are its gradients."""
+    m = _sinks(MODELS[family](dtype=torch.float32)).eval()
+    m.set_attn_implementation("eager")
+    ids = torch.randint(0, 512, (2, 12), generator=torch.Generator().manual_seed(5))
+    pad = torch.ones(2, 12, dtype=torch.long)
+    pad[0, :4] = 0
+    own = torch.ones(12, 12, dtype=torch.bool).tril().expand(2, 1, 12, 12).clone()
+    own[:, :, 6:, :6] = False  # two documents in a row
+    first = lambda: transformers.StaticCache(config=m.config, max_cache_len=40)
+
+    def grads():
+        m.zero_grad()
+        m(ids, attention_mask=pad).logits[pad.bool()].square().mean().backward()
+        return [p.grad.clone() for n, p in m.named_parameters() if "q_proj.weight" in n or "k_proj.weight" in n]
+
+    # the eager attention adds whatever mask it is given: a bool one would be 0 and 1 there, so it gets the additive form
+    added = torch.zeros(own.shape).masked_fill(~own, torch.finfo(torch.float32).min)
+
+    def calls(own):
+        with torch.no_grad():
+            yield m(ids, attention_mask=pad).logits[pad.bool()]
+            yield m(ids, attention_mask=own).logits
+            yield m(ids, past_key_values=first()).logits
+
+    want, want_grads = list(calls(added)), grads()
+    integrate.patch_hf_attention(m)
+    for mask in (own, added):
+        for got, ref in zip(calls(mask), want):
+            assert (got - ref).norm() / ref.norm() < 1e-4
+    for got, ref in zip(grads(), want_grads):
+        assert (got - ref).norm() / ref.norm() < 1e-3
+
+
+def test_cache_gives_tokens_up_and_refuses_the_rest(stand_in):
+    m = _qwen3(dtype=torch.float32).eval()
+    integrate.patch_hf_attention(m)
+    ids = torch.randint(0, 512, (2, 20), generator=torch.Generator().manual_seed(6))
+    new = lambda: integrate.quantized_kv_cache(m, 2, 32, page_size=16)
+    with torch.no_grad():
+        want, cache = m(ids, past_key_values=new()).logits, new()
+        m(ids.flip(1), past_key_values=cache)
+        cache.crop(-5)
+        assert cache.get_seq_length() == 15
+        cache.reset()
+        m(ids[:, :17], past_key_values=cache)
+        cache.crop(11)
+        got = m(ids[:, 11:], past_key_values=cache).logits
+        assert (got - want[:, 11:]).norm() / want[:, 11:].norm() < 1e-4
+        with pytest.raises(ValueError, match="own"):
+            m(ids[:, :3], attention_mask=torch.ones(2, 1, 3, 23, dtype=torch.bool), past_key_values=cache)
+        with pytest.raises(NotImplementedError):
+            m.generate(ids[:1], past_key_values=new(), num_beams=2, max_new_tokens=3, do_sample=False, pad_token_id=0,
+                       attention_mask=torch.ones(1, 20, dtype=torch.long))
+        with pytest.raises(ValueError, match="eval"):
+            m.train()(ids, past_key_values=new())
+    for call in (lambda c: c.reorder_cache(torch.tensor([1, 0])), lambda c: c.batch_repeat_interleave(2),
+                 lambda c: c.batch_select_indices(torch.tensor([0]))):
+        with pytest.raises(NotImplementedError):
+            call(new())
+
+
 # ------------------------------------------------------------------ GPU
 class _Stored(transformers.DynamicCache):
     """The stock cache, with every row replaced by what the 4-bit cache stores of it."""

@@ -57,6 +57,7 @@ def test_bad_write_is_refused(kw, match):
 @pytest.mark.parametrize("kw,match", [
     (dict(H=3), "multiple"), (dict(H=0), "multiple"), (dict(H=8192), "4096"), (dict(window=-1), "negative"),
     (dict(sinks=-1), "negative"), (dict(scale=float("inf")), "finite"), (dict(scale=float("nan")), "finite"),
+    (dict(scale=3e38), "finite"), (dict(scale=-3e38), "finite"),
     (dict(max_q=0), "max_q"), (dict(q=4104), "16-byte"), (dict(q_row=4), "16-byte"), (dict(y=None), "aligned"),
     (dict(y=8), "aligned"), (dict(T=-2), "negative"), (dict(T=1 << 22, H=2048), "2\\^31"), (dict(ws_bytes=16, P=512), "small"),
     (dict(ws=None, P=512), "workspace"), (dict(ws=4104, P=512), "workspace")])
