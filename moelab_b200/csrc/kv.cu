@@ -12,6 +12,8 @@ template <int FMT, int D>
 struct Wd {
     static constexpr int LR = FMT == FMT_Q4 ? 8 : 4;  // lanes per row, = words of 8 values in a group
     static constexpr int NG = D / (8 * LR);           // groups in a row, = words per lane
+    static constexpr int A = KV_BOTH(D) ? 2 : 1;      // arrays that a thread has rows of: K or V, or both
+    static constexpr int NW = NG * A;                 // its words
     static constexpr int R = 128 / LR;                // rows per CTA and pass
 };
 template <int N>
@@ -116,24 +118,32 @@ MOEB_DEV uint32_t kv_quant_fp4(const uint4 u, uint32_t &par) {
     return word;
 }
 
-// CTA: R * KV_U tokens of K or V of one head (blockIdx.y = 2 * head + is V)
+// CTA: R * passes tokens of one head, K or V (blockIdx.y = 2 * head + is V) or both (blockIdx.y = head)
 template <int FMT, int D>
 __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
     using X = Wd<FMT, D>;
-    constexpr int NG = X::NG;
-    const int w = threadIdx.x % X::LR, h = blockIdx.y >> 1;
-    const bool isv = blockIdx.y & 1;
-    const uint16_t *src = (isv ? a.v + h * a.v_head : a.k + h * a.k_head) + 8 * w;
-    const long stride = isv ? a.v_row : a.k_row;
-    uint32_t *codes = (isv ? a.c.vq : a.c.kq) + w * NG;
-    unsigned char *ps = static_cast<unsigned char *>(isv ? a.c.vs : a.c.ks);
+    constexpr int NG = X::NG, A = X::A, NW = X::NW;
+    const int w = threadIdx.x % X::LR, h = A == 2 ? blockIdx.y : blockIdx.y >> 1;
+    const bool isv = A == 1 && (blockIdx.y & 1);
+    const uint16_t *src[A];
+    long stride[A];
+    uint32_t *codes[A];
+    unsigned char *ps[A];
+#pragma unroll
+    for (int x = 0; x < A; ++x) {
+        const bool v = isv || x == 1;
+        src[x] = (v ? a.v + h * a.v_head : a.k + h * a.k_head) + 8 * w;
+        stride[x] = v ? a.v_row : a.k_row;
+        codes[x] = (v ? a.c.vq : a.c.kq) + w * NG;
+        ps[x] = static_cast<unsigned char *>(v ? a.c.vs : a.c.ks);
+    }
     const int t0 = (int)blockIdx.x * (X::R * a.passes) + (int)threadIdx.x / X::LR;
     pdl_wait();
-    uint4 next[NG];
+    uint4 next[NW];
     auto fetch = [&](int t) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-            next[g] = t < a.s.T ? *reinterpret_cast<const uint4 *>(src + t * stride + g * (8 * X::LR)) : make_uint4(0, 0, 0, 0);
+        for (int g = 0; g < NW; ++g)
+            next[g] = t < a.s.T ? *reinterpret_cast<const uint4 *>(src[g / NG] + t * stride[g / NG] + g % NG * (8 * X::LR)) : make_uint4(0, 0, 0, 0);
     };
     fetch(t0);
     // where the rows of the warp's passes go, a lane per row: its position, its page (-1: nowhere)
@@ -156,65 +166,73 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
 #pragma unroll 1  // once in the instruction cache
     for (int i = 0; i < a.passes; ++i) {
         const int t = t0 + i * X::R;
-        uint4 u[NG];
+        uint4 u[NW];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) u[g] = next[g];
+        for (int g = 0; g < NW; ++g) u[g] = next[g];
         if (i + 1 < a.passes) fetch(t + X::R);
         const int page = __shfl_sync(0xffffffffu, to, i * WR + lane / X::LR), p = __shfl_sync(0xffffffffu, at, i * WR + lane / X::LR);
         // every lane takes part in the shuffles; a group's lanes are all inside one row
-        uint32_t word[NG], out[NG], par[NG];
-        if (FMT == FMT_Q4) {
+        uint32_t word[NW], par[NW];
+        if (FMT == FMT_Q4) {  // NW == 2
             __nv_bfloat162 m = kv_q4_range(u[0]);
-            if (NG == 2) {
-                const __nv_bfloat162 m1 = kv_q4_range(u[NG - 1]);
-                if (w & 4) m = m1;
-            }
+            const __nv_bfloat162 m1 = kv_q4_range(u[NW - 1]);
+            if (w & 4) m = m1;
             const Q4Group mine = kv_q4_group(m);
             par[0] = mine.par;  // of the group whose parameters this lane worked out
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                Q4Group q = mine;
-                if (NG == 2) {
-                    const int from = ((int)threadIdx.x & 24) | 4 * g;
-                    q.scale = __shfl_sync(0xffffffffu, mine.scale, from);
-                    q.bias = __shfl_sync(0xffffffffu, mine.bias, from);
-                    q.inv = __shfl_sync(0xffffffffu, mine.inv, from);
-                }
+            for (int g = 0; g < NW; ++g) {
+                const int from = ((int)threadIdx.x & 24) | 4 * g;
+                Q4Group q;
+                q.scale = __shfl_sync(0xffffffffu, mine.scale, from);
+                q.bias = __shfl_sync(0xffffffffu, mine.bias, from);
+                q.inv = __shfl_sync(0xffffffffu, mine.inv, from);
                 word[g] = kv_quant_q4(u[g], q);
             }
         } else {
 #pragma unroll
-            for (int g = 0; g < NG; ++g) word[g] = kv_quant_fp4(u[g], par[g]);
+            for (int g = 0; g < NW; ++g) word[g] = kv_quant_fp4(u[g], par[g]);
         }
         if (page < 0) continue;
         const size_t row = kv_row(a.c, page, h, p);
-        lane_words<FMT>(word, out, false);
         using T = typename Vec<NG>::T;
-        *reinterpret_cast<T *>(codes + row * (D / 8)) = *reinterpret_cast<const T *>(out);
-        if (FMT == FMT_Q4) {
-            if (w % (8 / NG) == 0) *reinterpret_cast<uint32_t *>(ps + row * (4 * NG) + w / (8 / NG) * 4) = par[0];
-        } else if (w == 0) {
-            if (NG == 4) {
-                *reinterpret_cast<uint32_t *>(ps + row * NG) = par[0] | par[1] << 8 | par[NG - 2] << 16 | par[NG - 1] << 24;
-            } else {
-                *reinterpret_cast<uint16_t *>(ps + row * NG) = (uint16_t)(par[0] | par[1 % NG] << 8);
+#pragma unroll
+        for (int x = 0; x < A; ++x) {
+            uint32_t in[NG], out[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) in[g] = word[x * NG + g];
+            lane_words<FMT>(in, out, false);
+            *reinterpret_cast<T *>(codes[x] + row * (D / 8)) = *reinterpret_cast<const T *>(out);
+            if (FMT != FMT_Q4 && w == 0) {
+                const uint32_t *e = par + x * NG;
+                if (NG == 4) *reinterpret_cast<uint32_t *>(ps[x] + row * NG) = e[0] | e[1] << 8 | e[NG - 2] << 16 | e[NG - 1] << 24;
+                else *reinterpret_cast<uint16_t *>(ps[x] + row * NG) = (uint16_t)(e[0] | e[1 % NG] << 8);
             }
         }
+        if (FMT == FMT_Q4 && w % 4 == 0)  // lane 0 has the first group's parameters (K's), lane 4 the second's (V's)
+            *reinterpret_cast<uint32_t *>((w == 0 ? ps[0] : ps[A - 1]) + row * (4 * NG) + (A == 2 ? 0 : w)) = par[0];
     }
 }
 
 template <int FMT, int D>
 __global__ void __launch_bounds__(128) k_kv_read(const KvReadArgs a) {
     using X = Wd<FMT, D>;
-    constexpr int NG = X::NG;
+    constexpr int NG = X::NG, A = X::A;
     using T = typename Vec<NG>::T;
-    const int w = threadIdx.x % X::LR, h = blockIdx.y >> 1;
-    const bool isv = blockIdx.y & 1;
+    const int w = threadIdx.x % X::LR, h = A == 2 ? blockIdx.y : blockIdx.y >> 1;
+    const bool isv = A == 1 && (blockIdx.y & 1);
     const int t0 = (int)blockIdx.x * (X::R * a.passes) + (int)threadIdx.x / X::LR;
-    const uint32_t *codes = (isv ? a.c.vq : a.c.kq) + w * NG;
-    const unsigned char *ps = static_cast<const unsigned char *>(isv ? a.c.vs : a.c.ks);
+    const uint32_t *codes[A];
+    const unsigned char *ps[A];
+    uint16_t *dst[A];
+#pragma unroll
+    for (int x = 0; x < A; ++x) {
+        const bool v = isv || x == 1;
+        codes[x] = (v ? a.c.vq : a.c.kq) + w * NG;
+        ps[x] = static_cast<const unsigned char *>(v ? a.c.vs : a.c.ks);
+        dst[x] = (v ? a.v : a.k) + (size_t)h * D + 8 * w;
+    }
     pdl_wait();
-    uint32_t code[KV_U][NG], par[KV_U][FMT == FMT_Q4 ? NG : 1];
+    uint32_t code[KV_U][A][NG], par[KV_U][A][FMT == FMT_Q4 ? NG : 1];
     int has = 0, got = 0;  // bit i: row i is some sequence's, its page is valid
     int r0 = 0, r1 = 0, b = -1;
 #pragma unroll
@@ -232,23 +250,28 @@ __global__ void __launch_bounds__(128) k_kv_read(const KvReadArgs a) {
         }
         got |= 1 << i;
         const size_t row = kv_row(a.c, page, h, (int)p);
-        *reinterpret_cast<T *>(code[i]) = *reinterpret_cast<const T *>(codes + row * (D / 8));
-        if (FMT == FMT_Q4) *reinterpret_cast<T *>(par[i]) = *reinterpret_cast<const T *>(ps + row * (4 * NG));
-        else par[i][0] = NG == 4 ? *reinterpret_cast<const uint32_t *>(ps + row * NG) : *reinterpret_cast<const uint16_t *>(ps + row * NG);
+#pragma unroll
+        for (int x = 0; x < A; ++x) {
+            *reinterpret_cast<T *>(code[i][x]) = *reinterpret_cast<const T *>(codes[x] + row * (D / 8));
+            if (FMT == FMT_Q4) *reinterpret_cast<T *>(par[i][x]) = *reinterpret_cast<const T *>(ps[x] + row * (4 * NG));
+            else par[i][x][0] = NG == 4 ? *reinterpret_cast<const uint32_t *>(ps[x] + row * NG) : *reinterpret_cast<const uint16_t *>(ps[x] + row * NG);
+        }
     }
-    uint16_t *dst = (isv ? a.v : a.k) + (size_t)h * D + 8 * w;
 #pragma unroll
     for (int i = 0; i < KV_U; ++i) {
         if (!((has >> i) & 1)) continue;
-        uint32_t word[NG];
-        lane_words<FMT>(code[i], word, true);
-        uint16_t *to = dst + (size_t)(t0 + i * X::R) * a.c.Hkv * D;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            float x[8];
-            kv_word_values<FMT>(word[g], FMT == FMT_Q4 ? par[i][FMT == FMT_Q4 ? g : 0] : (par[i][0] >> (8 * g)) & 255u, x);
-            const uint4 o = make_uint4(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7]));
-            *reinterpret_cast<uint4 *>(to + g * (8 * X::LR)) = (got >> i) & 1 ? o : make_uint4(0, 0, 0, 0);
+        for (int x = 0; x < A; ++x) {
+            uint32_t word[NG];
+            lane_words<FMT>(code[i][x], word, true);
+            uint16_t *to = dst[x] + (size_t)(t0 + i * X::R) * a.c.Hkv * D;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float y[8];
+                kv_word_values<FMT>(word[g], FMT == FMT_Q4 ? par[i][x][FMT == FMT_Q4 ? g : 0] : (par[i][x][0] >> (8 * g)) & 255u, y);
+                const uint4 o = make_uint4(pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]), pack_bf2(y[4], y[5]), pack_bf2(y[6], y[7]));
+                *reinterpret_cast<uint4 *>(to + g * (8 * X::LR)) = (got >> i) & 1 ? o : make_uint4(0, 0, 0, 0);
+            }
         }
     }
 }

@@ -137,6 +137,9 @@ MOEB_DEV void kv_word_values(uint32_t word, uint32_t par, float (&o)[8]) {
         }
     }
 }
+// Rows of 64 values: a thread of the kernels that write and read rows has both K and V of its (token, head), so that there is as
+// much work per lookup as with 128.
+#define KV_BOTH(D) ((D) == 64)
 struct KvWriteArgs {
     KvCache c;
     KvSeqs s;

@@ -133,15 +133,16 @@ int check_seqs(const KvCache &c, int T, const int *cu, const int *lens, bool nee
     ((c)->format == MOEB_KV_Q4 ? ((c)->head_dim == 64 ? kern<FMT_Q4, 64> : kern<FMT_Q4, 128>) \
                                : ((c)->head_dim == 64 ? kern<FMT_FP4, 64> : kern<FMT_FP4, 128>))
 
-// The kernels that write and read rows: a CTA takes 16 (int4) or 32 (MXFP4) tokens of one head's K or V at a time, 4 times
-// where that still gives every SM eight CTAs.
+// The kernels that write and read rows: a CTA takes 16 (int4) or 32 (MXFP4) tokens of one head at a time, 4 times where that
+// still gives every SM eight CTAs.
+int word_heads(const moeb_kv_cache *c) { return KV_BOTH(c->head_dim) ? c->kv_heads : 2 * c->kv_heads; }
 int word_passes(const moeb_kv_cache *c, int T) {
-    const long ctas = (((long)T + (c->format == MOEB_KV_Q4 ? 15 : 31)) / (c->format == MOEB_KV_Q4 ? 16 : 32)) * 2 * c->kv_heads;
+    const long rows = c->format == MOEB_KV_Q4 ? 16 : 32, ctas = (T + rows - 1) / rows * word_heads(c);
     return ctas >= 32L * sms() ? 4 : 1;
 }
 dim3 word_grid(const moeb_kv_cache *c, int T, int passes) {
     const int tokens = (c->format == MOEB_KV_Q4 ? 16 : 32) * passes;
-    return dim3((unsigned)((T + tokens - 1) / tokens), 2u * c->kv_heads);
+    return dim3((unsigned)((T + tokens - 1) / tokens), (unsigned)word_heads(c));
 }
 
 // What a call of moeb_kv_attention launches, from what the host knows: the rows, the page tables' width and the window.
