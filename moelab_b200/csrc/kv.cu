@@ -1,8 +1,13 @@
-// Writing K and V rows into the 4-bit cache, and reading them back (layout: kv.cuh). Both are one pass over memory. A thread
-// has what one lane of the cache's readers has: the same word of every group of a row (int4: 1 / 8 of the row, MXFP4: 1 / 4),
-// so that its codes are one load or store and the page arithmetic is done once for all of them; and KV_U tokens of one head,
-// so that as many loads are in flight (one token in calls too small to fill the GPU). The lanes of a group reduce its extremes
-// by shuffles.
+// Writing K and V rows into the 4-bit cache, and reading them back (layout: kv.cuh). Both are one pass over memory: per value
+// two bytes of bf16 and 0.56 (int4) or 0.53 (MXFP4) of the cache. A thread has what one lane of the cache's readers has: the
+// same word of every group of a row (int4: 1 / 8 of the row, MXFP4: 1 / 4; rows of 64 values: of K's and V's), so that its codes
+// are one load or store and the page arithmetic is done once for all of them; and KV_U tokens of one head, so that as many loads
+// are in flight (one token in calls too small to fill the GPU). The lanes of a group reduce its extremes by shuffles.
+// Measured with 65,536 tokens of 1,024 values each of K and V (8 heads of 128 / 16 of 64), copies of the same bytes at 6.56
+// TB/s being 52 us:
+//   write  int4 72 / 75 us (4.8 / 4.6 TB/s; bound by instructions), MXFP4 55 / 62 us (6.2 / 5.5 TB/s)
+//   read   int4 62 / 70 us (5.5 / 4.9 TB/s), MXFP4 61 / 67 us (5.6 / 5.1 TB/s)
+// A call of one token is bound by its launch: written and read back, 4.7 us in a graph.
 #include "kv.cuh"
 
 namespace moeb {
@@ -36,8 +41,8 @@ MOEB_DEV void lane_words(const uint32_t (&in)[N], uint32_t (&out)[N], bool to_wo
 // int4: a group's 64 values lie in 8 neighbouring lanes, 8 in each. The operations are those of the weight quantizer
 // (quant.cu), so a cache row equals mx.quantize of it. A group that holds an infinity or a NaN, or whose span passes fp32, is
 // stored with NaN parameters: it reads back as NaN everywhere, and nothing else is touched by it. Bound by its instructions, not
-// by memory: pairs of values go through packed operations, and where a lane has two groups, four of the eight lanes work
-// out the parameters of one, four those of the other.
+// by memory: pairs of values go through packed operations, and each of the eight lanes works out the parameters of one of the
+// eight groups that they have in four tokens (all lanes those of every group: 84 against 72 us).
 struct Q4Group {
     float scale, bias, inv;  // inv = 0: all codes are 0
     uint32_t par;            // as stored; 0: all zeros
@@ -139,13 +144,15 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
     }
     const int t0 = (int)blockIdx.x * (X::R * a.passes) + (int)threadIdx.x / X::LR;
     pdl_wait();
-    uint4 next[NW];
-    auto fetch = [&](int t) {
+    auto fetch = [&](int t, bool any, uint4 (&u)[NW]) {
 #pragma unroll
         for (int g = 0; g < NW; ++g)
-            next[g] = t < a.s.T ? *reinterpret_cast<const uint4 *>(src[g / NG] + t * stride[g / NG] + g % NG * (8 * X::LR)) : make_uint4(0, 0, 0, 0);
+            u[g] = any && t < a.s.T ? *reinterpret_cast<const uint4 *>(src[g / NG] + t * stride[g / NG] + g % NG * (8 * X::LR)) : make_uint4(0, 0, 0, 0);
     };
-    fetch(t0);
+    constexpr int U = FMT == FMT_Q4 ? KV_U : 1;
+    uint4 next[U][NW];
+#pragma unroll
+    for (int i = 0; i < U; ++i) fetch(t0 + i * X::R, i < a.passes, next[i]);
     // where the rows of the warp's passes go, a lane per row: its position, its page (-1: nowhere)
     constexpr int WR = 32 / X::LR;  // a warp's rows in a pass
     const int lane = threadIdx.x & 31;
@@ -163,38 +170,11 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
         }
         __syncwarp();
     }
-#pragma unroll 1  // once in the instruction cache
-    for (int i = 0; i < a.passes; ++i) {
-        const int t = t0 + i * X::R;
-        uint4 u[NW];
-#pragma unroll
-        for (int g = 0; g < NW; ++g) u[g] = next[g];
-        if (i + 1 < a.passes) fetch(t + X::R);
+    using T = typename Vec<NG>::T;
+    auto store = [&](int i, const uint32_t (&word)[NW], const uint32_t *par) {
         const int page = __shfl_sync(0xffffffffu, to, i * WR + lane / X::LR), p = __shfl_sync(0xffffffffu, at, i * WR + lane / X::LR);
-        // every lane takes part in the shuffles; a group's lanes are all inside one row
-        uint32_t word[NW], par[NW];
-        if (FMT == FMT_Q4) {  // NW == 2
-            __nv_bfloat162 m = kv_q4_range(u[0]);
-            const __nv_bfloat162 m1 = kv_q4_range(u[NW - 1]);
-            if (w & 4) m = m1;
-            const Q4Group mine = kv_q4_group(m);
-            par[0] = mine.par;  // of the group whose parameters this lane worked out
-#pragma unroll
-            for (int g = 0; g < NW; ++g) {
-                const int from = ((int)threadIdx.x & 24) | 4 * g;
-                Q4Group q;
-                q.scale = __shfl_sync(0xffffffffu, mine.scale, from);
-                q.bias = __shfl_sync(0xffffffffu, mine.bias, from);
-                q.inv = __shfl_sync(0xffffffffu, mine.inv, from);
-                word[g] = kv_quant_q4(u[g], q);
-            }
-        } else {
-#pragma unroll
-            for (int g = 0; g < NW; ++g) word[g] = kv_quant_fp4(u[g], par[g]);
-        }
-        if (page < 0) continue;
+        if (page < 0) return;
         const size_t row = kv_row(a.c, page, h, p);
-        using T = typename Vec<NG>::T;
 #pragma unroll
         for (int x = 0; x < A; ++x) {
             uint32_t in[NG], out[NG];
@@ -208,8 +188,54 @@ __global__ void __launch_bounds__(128) k_kv_write(const KvWriteArgs a) {
                 else *reinterpret_cast<uint16_t *>(ps[x] + row * NG) = (uint16_t)(e[0] | e[1 % NG] << 8);
             }
         }
-        if (FMT == FMT_Q4 && w % 4 == 0)  // lane 0 has the first group's parameters (K's), lane 4 the second's (V's)
-            *reinterpret_cast<uint32_t *>((w == 0 ? ps[0] : ps[A - 1]) + row * (4 * NG) + (A == 2 ? 0 : w)) = par[0];
+    };
+    // every lane takes part in the shuffles; a group's lanes are all inside one row
+    if constexpr (FMT == FMT_Q4) {
+        static_assert(KV_U * NW == X::LR, "a lane per group of a row's passes");
+        __nv_bfloat162 m;
+#pragma unroll
+        for (int i = 0; i < KV_U; ++i) {
+            if (i >= a.passes) break;
+#pragma unroll
+            for (int g = 0; g < NW; ++g) {
+                const __nv_bfloat162 x = kv_q4_range(next[i][g]);
+                if (i * NW + g == 0 || w == i * NW + g) m = x;
+            }
+        }
+        const Q4Group mine = kv_q4_group(m);
+#pragma unroll
+        for (int i = 0; i < KV_U; ++i) {
+            if (i >= a.passes) break;
+            uint32_t word[NW];
+#pragma unroll
+            for (int g = 0; g < NW; ++g) {
+                const int from = ((int)threadIdx.x & 24) | (i * NW + g);
+                Q4Group q;
+                q.scale = __shfl_sync(0xffffffffu, mine.scale, from);
+                q.bias = __shfl_sync(0xffffffffu, mine.bias, from);
+                q.inv = __shfl_sync(0xffffffffu, mine.inv, from);
+                word[g] = kv_quant_q4(next[i][g], q);
+            }
+            store(i, word, nullptr);
+            __syncwarp();
+        }
+        // lane w has the parameters of pass w / 2, group w % 2 (or K's and V's)
+        const int from = w / NW * WR + lane / X::LR, page = __shfl_sync(0xffffffffu, to, from), p = __shfl_sync(0xffffffffu, at, from);
+        if (page >= 0)
+            *reinterpret_cast<uint32_t *>((w % NW == 0 ? ps[0] : ps[A - 1]) + kv_row(a.c, page, h, p) * (4 * NG) + (A == 2 ? 0 : w % NW * 4)) = mine.par;
+    } else {
+#pragma unroll 1  // once in the instruction cache
+        for (int i = 0; i < a.passes; ++i) {
+            uint4 u[NW];
+#pragma unroll
+            for (int g = 0; g < NW; ++g) u[g] = next[0][g];
+            if (i + 1 < a.passes) fetch(t0 + (i + 1) * X::R, true, next[0]);
+            uint32_t word[NW], par[NW];
+#pragma unroll
+            for (int g = 0; g < NW; ++g) word[g] = kv_quant_fp4(u[g], par[g]);
+            store(i, word, par);
+            __syncwarp();
+        }
     }
 }
 
