@@ -264,7 +264,7 @@ int moeb_probe_mma_sync(int warps_per_sm, int iters, double *tflops);
  * Rows of a call: T rows, B sequences. Sequence b has rows cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1], not decreasing),
  * or T / B rows each where cu is NULL. They are its newest tokens: row i of n sits at position lens[b] - n + i (lens
  * int32 [B] counts them in). Position p is in page table[b * table_row + p / page_size] (int32, P entries per sequence).
- * Rows behind the last sequence, and rows whose position is negative, are passed over. A position outside the table, or
+ * Rows behind the last sequence, and rows whose position is negative, are passed over (as queries the latter see nothing). A position outside the table, or
  * a page id outside [0, pages), sets MOEB_DEVERR_PAGE: nothing is written there and nothing is read from there. */
 #define MOEB_KV_Q4 0
 #define MOEB_KV_MXFP4 1

@@ -164,7 +164,7 @@ Plan plan_of(int T, int B, int P, int page_size, int H, int Hkv, int D, int max_
     auto seen = [&](long rows) { return window ? std::min(all, (long)window + rows + std::min<long>(sinks, all) + 128 + (sinks ? 128 : 0)) : all; };
     // Sequences whose (row, head) columns fit one or two tensor-core tiles go to the kernel for few rows. Without cu all
     // sequences have T / B rows; with it, and more than one sequence, both kinds may be in the call: over up to 1024 keys
-    // the kernel for many rows takes them all (8 key tiles, 16 us at most, against two more launches).
+    // the kernel for many rows takes them all (8 key tiles, 18 to 26 us, against two more launches).
     p.only = cols <= 16;
     p.few = p.only ? (int)cols : cu && B > 1 && seen(max_q) > 1024 ? 16 : 0;
     if (p.few) {
@@ -183,14 +183,15 @@ Plan plan_of(int T, int B, int P, int page_size, int H, int Hkv, int D, int max_
         p.tiles = cu ? (long)T * Gq / KV_PROMPT_ROWS + B : (long)B * (((long)(T / B) * Gq + KV_PROMPT_ROWS - 1) / KV_PROMPT_ROWS);
         const long ctas = p.tiles * Hkv, key_tiles = (seen(KV_PROMPT_ROWS) + 127) / 128;
         // One CTA per SM: where the row tiles alone are less than three waves, their keys are cut into as many parts (8 key tiles
-        // or more each) as make the last wave fullest. A key tile takes about 2 us; a part's sums are written and read once more.
+        // or more each) as make the last wave fullest. A key tile takes 2.2 us with heads of 64 and 3.2 us with 128; a part's sums
+        // are written and read once more.
         p.splits = 1;
         if (ctas < 3L * sms()) {
             double best = 0;
             const long most = std::max(1L, std::min(key_tiles / 8, ctas * 2 <= sms() ? sms() / std::max(ctas, 1L) : 8L));
             for (long n = 1; n <= most; ++n) {
                 const double waves = (double)((ctas * n + sms() - 1) / sms());
-                const double us = waves * ((double)key_tiles / n * 2.0 + 6.0) + (n > 1 ? 3.0 + (double)n * T * H * D * 8 / 5e6 : 0.0);
+                const double us = waves * ((double)key_tiles / n * (D == 64 ? 2.2 : 3.2) + 6.0) + (n > 1 ? 3.0 + (double)n * T * H * D * 8 / 5e6 : 0.0);
                 if (n == 1 || us < best * 0.97) {
                     best = us;
                     p.splits = n;

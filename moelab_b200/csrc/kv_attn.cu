@@ -1,29 +1,43 @@
 // Attention of a few query rows per sequence over the 4-bit cache: decode steps and drafted tokens (layout: kv.cuh).
 //
+// y = sum_j w_j v_j / sum_j w_j, w_j = 2^(score_j - m), score = scale log2(e) q . k: one pass over the keys with a running
+// maximum m (the sums so far are scaled when it grows), statistics and sums in fp32.
+//
 // The rows of a sequence that share a KV head (n tokens x Gq query heads, at most NC = 8 or 16) are the columns of
-// one tensor-core tile, so the cache is read once for all of them. The kernel is bound by the cache's bytes when the
-// caches are long, and by the chain lengths -> page table -> codes -> sums when they are short.
+// one tensor-core tile, so the cache is read once for all of them. Long caches are bound by their bytes, short ones
+// by the chain lengths -> page table -> codes -> sums. Measured:
+//   64 sequences of 1 to 8192 tokens, 32 query heads on 8, int4 (306 MB): 85 us with the join, 3.6 TB/s; in its loop over the
+//     blocks the kernel moves 5.9 TB/s (a copy 6.56), the rest is the 2 us until a CTA knows its run, the 5 us until its first
+//     copies are there, CTAs that end between 59 and 78 us (memory is not equally far from all SMs) and the join. Shares of two
+//     sizes, the small ones for CTAs that end early, cost more than they even out (92 us): new CTAs start slowly under load.
+//   one of 200,001 tokens, 64 heads on 4, MXFP4 (109 MB, two column tiles, 8 warps per SM): 52 us, 2.1 TB/s, bound by the
+//     latencies of one warp's steps: half of the issue slots are taken
+//   one of 1021 tokens, 32 heads on 4, int4: 7.2 us in a graph
 //
 // Work split: the visible keys of every (sequence, KV head) are cut into blocks of 128; all blocks of the call in a row are
 // dealt to the CTAs in equal runs, so uneven lengths cost nothing and the host needs to know none of them (a captured
-// graph replays with other lengths). A run's start and end cost about as much as FR blocks, which each (sequence, head) has in
-// the count before its first one (without them CTAs with many short sequences end last). A CTA that holds all blocks of a (sequence, head) writes y; otherwise it leaves its
-// unnormalised sum, maximum and sum of weights, and k_kv_attn_join joins them. Where the page tables' width or the window bounds
-// the keys to a few blocks there is no second launch: a CTA (a.direct = 1) or a cluster of 8 CTAs, which join through their
-// shared memories, has a (sequence, head).
+// graph replays with other lengths). A run's start and end cost about as much as FR blocks, which each (sequence, head) has
+// in the count before its first one (without them CTAs with many short sequences end last: 106 us for the batch above). A CTA
+// that holds all blocks of a (sequence, head) writes y; otherwise it leaves its unnormalised sum, maximum and sum of weights,
+// and k_kv_attn_join joins them. Where the page tables' width or the window bounds the keys to a few blocks there is no second
+// launch: a CTA (a.direct = 1) or a cluster of 8 CTAs, which join through their shared memories, has a (sequence, head)
+// (1021 tokens: 8.4 us with the second launch; windows of 128: 26 us, 16 without).
 //
 // A warp takes 32 keys of each block, straight from a cp.async ring of its own (no block-wide barrier in the loop; the next
 // run's first copies are on their way while a run's warps join; bulk copies from single lanes cost twice the instructions), and
-// feeds the codes to mma.sync m16n8k16 without dequantizing them:
+// feeds the codes to mma.sync m16n8k16 without dequantizing them. mma.sync and not tcgen05: with 8 or 16 columns the products
+// are a fifth of the time either way, and codes would have to pass through shared or tensor memory once more.
 //   scores^T [16 keys x NC] = K codes . q, q in fp16 after a power of two per row (8 bits of significand fit 11). int4: a
-//     masked code is an fp16 subnormal, code * 2^-24, so that an operand costs one instruction; with group g's scale s and bias
-//     b, score = sum_g s acc_g + b qsum_g in fp32. MXFP4: E2M1 codes convert to fp16, score = sum_g 2^e acc_g.
+//     masked code is an fp16 subnormal, code * 2^-24, so that an operand costs one instruction (converted: 114 us for the batch
+//     above when that was 106); with group g's scale s and bias b, score = sum_g s acc_g + b qsum_g in fp32. MXFP4: E2M1 codes
+//     convert to fp16, score = sum_g 2^e acc_g.
 //   y^T [D x NC] += V^T codes . P, P = fp16(p * scale of the key's group). A running power of two per warp, taken into p's
-//     exponent, keeps the product in fp16's range whatever the values' size; codes as subnormals (int4) or E2M1 in fp16, exact. fp16 and not
-//     bf16: P is the only rounding here, 2^-11 keeps it below the result's own 2^-8. int4's bias term is summed in fp32.
-// Softmax statistics and sums are fp32; a column's maximum is shared by the warp's lanes (three shuffles), warps join at
-// the end of a run of blocks. MMA row r is key r / 2 + 4 (r % 2) of its eight, which makes the four keys of a lane's V
-// operand consecutive rows of shared memory (no bank conflicts) and costs K nothing.
+//     exponent, keeps the product in fp16's range whatever the values' size; codes as subnormals (int4) or E2M1 in fp16 are
+//     exact. fp16 and not bf16: P is the only rounding here, 2^-11 keeps it below the result's own 2^-8. int4's bias term is
+//     summed in fp32.
+// A column's maximum is shared by the warp's lanes (three shuffles), warps join at the end of a run of blocks. MMA row r is key
+// r / 2 + 4 (r % 2) of its eight, which makes the four keys of a lane's V operand consecutive rows of shared memory (no bank
+// conflicts) and costs K nothing.
 #include <type_traits>
 
 #include "kv.cuh"
@@ -33,13 +47,13 @@ namespace moeb {
 namespace {
 
 constexpr int FW = 4, FT = 32 * FW;  // warps per CTA, threads
-constexpr int FS = 3;                // ring stages
+constexpr int FS = 3;                // ring stages (4: two CTAs per SM instead of three, 96 us for the batch above)
 constexpr int FB = 32 * FW;          // keys per block
 constexpr int FR = 2;                // blocks that a run costs besides its own
 
 template <int FMT, int D>
 struct Few {
-    static constexpr int W = D / 8, G = D / 64, NG = FMT == FMT_Q4 ? D / 64 : D / 32;
+    static constexpr int G = D / 64, NG = FMT == FMT_Q4 ? D / 64 : D / 32;
     static constexpr int ROW = D / 2, PROW = FMT == FMT_Q4 ? G * 4 : NG;  // bytes of a row's codes, of its parameters
     static constexpr int O_V = 32 * ROW, O_KP = 2 * O_V, O_VP = O_KP + 32 * PROW, STAGE = O_VP + 32 * PROW;  // 32 rows
 };
