@@ -263,9 +263,10 @@ int moeb_probe_mma_sync(int warps_per_sm, int iters, double *tflops);
  *
  * Rows of a call: T rows, B sequences. Sequence b has rows cu[b] .. cu[b + 1] - 1 (cu int32 [B + 1], not decreasing),
  * or T / B rows each where cu is NULL. They are its newest tokens: row i of n sits at position lens[b] - n + i (lens
- * int32 [B] counts them in). Position p is in page table[b * table_row + p / page_size] (int32, P entries per sequence).
- * Rows behind the last sequence, and rows whose position is negative, are passed over (as queries the latter see nothing). A position outside the table, or
- * a page id outside [0, pages), sets MOEB_DEVERR_PAGE: nothing is written there and nothing is read from there. */
+ * int32 [B] counts them in). Position p is in page table[b * table_row + p / page_size] (int32, P entries per
+ * sequence). Rows behind the last sequence, and rows whose position is negative, are passed over (as queries the
+ * latter see nothing). A position outside the table, or a page id outside [0, pages), sets MOEB_DEVERR_PAGE: nothing
+ * is written there and nothing is read from there. */
 #define MOEB_KV_Q4 0
 #define MOEB_KV_MXFP4 1
 #define MOEB_DEVERR_PAGE 4u
@@ -292,10 +293,10 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
  * staying visible). sink_logits (fp32 [H] or NULL): exp(sink_logits[h]) joins the softmax's sum without a value. A row
  * that sees nothing gives zeros (lse -inf, or the sink logit). Pages that no row of the call sees are not read: their
  * table entries may be anything. q: bf16, strides as moeb_kv_write's k; y: bf16 [T][H][head_dim]; lse: fp32 [T][H], the
- * natural logarithm of the softmax's sum, or NULL. max_q: the most rows that a sequence has in this call (a larger bound
- * costs time only; a sequence with more rows may be passed over, which sets MOEB_DEVERR_ROWS). Scores, statistics and sums are fp32. ws: scratch
- * of moeb_kv_attention_workspace_bytes (for the same arguments; with_cu: cu is given; 0 for many calls), with no first
- * contents and none kept, 16-byte aligned: one call at a time. */
+ * natural logarithm of the softmax's sum, or NULL. max_q: the most rows that a sequence has in this call (a larger
+ * bound costs time only; a sequence with more rows may be passed over, which sets MOEB_DEVERR_ROWS). Scores,
+ * statistics and sums are fp32. ws: scratch of moeb_kv_attention_workspace_bytes (for the same arguments; with_cu: cu
+ * is given; 0 for many calls), with no first contents and none kept, 16-byte aligned: one call at a time. */
 size_t moeb_kv_attention_workspace_bytes(int T, int B, int P, int page_size, int H, int kv_heads, int head_dim, int max_q,
                                          int window, int sinks, int with_cu);
 int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, long q_head, int T, int H, const int *cu,
