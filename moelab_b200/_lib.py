@@ -8,6 +8,7 @@ import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libmoelab_b200.so")
+PYCALL_PATH = os.path.join(HERE, "lib", "moelab_b200_pycall.so")
 
 MOEB_OK, MOEB_EINVAL, MOEB_ELAUNCH, MOEB_ETIMEOUT, MOEB_EUNSUP = 0, 1, 2, 3, 4
 POLICY_AUTO, POLICY_SLOTS, POLICY_TILES8, POLICY_TILES16, POLICY_TILES8_RING, POLICY_TILES16_RING = 0, 1, 2, 3, 4, 5
@@ -101,9 +102,33 @@ def load():
     return _lib
 
 
+_hot = None
+
+
+def hot():
+    """The CPython module over moeb_kv_write, moeb_kv_read and moeb_kv_attention (csrc/pycall.cpp), bound to the library."""
+    global _hot
+    if _hot is None:
+        import importlib.machinery
+        import importlib.util
+        if not os.path.exists(PYCALL_PATH):
+            raise MoebError(f"{PYCALL_PATH} is missing: build it with `python -m moelab_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("moelab_b200_pycall", PYCALL_PATH)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("moelab_b200_pycall", loader))
+        loader.exec_module(mod)
+        lib = load()
+        mod.bind(*(ctypes.cast(getattr(lib, n), _P).value for n in ("moeb_kv_write", "moeb_kv_read", "moeb_kv_attention")))
+        _hot = mod
+    return _hot
+
+
+def failed(name, rc):
+    """Raise for a status that is not MOEB_OK."""
+    raise MoebError(f"{name} failed with status {rc}: {load().moeb_last_error().decode(errors='replace')}")
+
+
 def call(name, *args):
     rc = getattr(load(), name)(*args)
     if rc != MOEB_OK:
-        msg = load().moeb_last_error().decode(errors="replace")
-        raise MoebError(f"{name} failed with status {rc}: {msg}")
+        failed(name, rc)
     return rc

@@ -1,4 +1,4 @@
-"""Build libmoelab_b200.so (all CUDA sources, sm_100a) in-tree with nvcc.
+"""Build libmoelab_b200.so (all CUDA sources, sm_100a) and the CPython module over its hottest calls in-tree with nvcc.
 
     python -m moelab_b200.build [--jobs N] [--verbose]
 
@@ -11,6 +11,7 @@ import glob
 import os
 import shutil
 import subprocess
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -18,6 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 OBJDIR = os.path.join(LIBDIR, "obj")
 LIB = os.path.join(LIBDIR, "libmoelab_b200.so")
+PYCALL = os.path.join(LIBDIR, "moelab_b200_pycall.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
@@ -62,7 +64,18 @@ def build(jobs=None, verbose=False, extra=()):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _pycall()
     return LIB
+
+
+def _pycall():
+    src = os.path.join(CSRC, "pycall.cpp")
+    if os.path.exists(PYCALL) and os.path.getmtime(PYCALL) >= max(os.path.getmtime(src), _headers_mtime()):
+        return
+    cmd = [nvcc(), "-O2", "-std=c++17", "-Xcompiler", "-fPIC", "-I" + sysconfig.get_paths()["include"], "-shared", "-o", PYCALL, src]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"nvcc failed on {src}:\n{r.stdout}\n{r.stderr}")
 
 
 if __name__ == "__main__":

@@ -370,15 +370,16 @@ class KVCache:
         self.ks, self.vs = (torch.zeros(*rows, par[0], dtype=par[1], device=device) for _ in range(2))
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
         self.device, self.index, self._ws_bytes = self.kq.device, self.kq.get_device(), {}
-        self._c = ctypes.pointer(_lib.KvCacheStruct(
+        self._struct = _lib.KvCacheStruct(
             *(t.data_ptr() for t in (self.kq, self.ks, self.vq, self.vs, self.err)), pages, page_size, kv_heads, head_dim,
-            _lib.KV_Q4 if fmt == "q4" else _lib.KV_MXFP4))
+            _lib.KV_Q4 if fmt == "q4" else _lib.KV_MXFP4)
+        self._c = ctypes.addressof(self._struct)
 
     def read_error(self):
         """Sticky device error bits (DEVERR_PAGE, DEVERR_ROWS); synchronises the current stream and clears them."""
         out = ctypes.c_uint(0)
         with torch.cuda.device(self.device):
-            _lib.call("moeb_kv_read_error", self._c, ctypes.byref(out), _stream())
+            _lib.call("moeb_kv_read_error", self._struct, ctypes.byref(out), _stream())
         return out.value
 
 
@@ -435,10 +436,12 @@ def _kv_call(cache, name, *args):
     i = cache.index
     stream = torch._C._cuda_getCurrentRawStream(i)
     if i == torch._C._cuda_getDevice():
-        _lib.call(name, *args, stream)
+        rc = getattr(_lib._hot or _lib.hot(), name)(*args, stream)
     else:
         with torch.cuda.device(i):
-            _lib.call(name, *args, stream)
+            rc = getattr(_lib.hot(), name)(*args, stream)
+    if rc:
+        _lib.failed(name, rc)
 
 
 def _kv_cu(cu, T, B, cache):

@@ -106,3 +106,31 @@ def test_python_checks():
         ops.kv_attention(cpu, Fake, torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32))
     with pytest.raises(ValueError, match="CUDA"):
         ops.kv_read(Fake, torch.zeros(2, 1, dtype=torch.int32), None, 2)
+
+
+def test_calls_from_python_reach_the_same_entries():
+    """The CPython module over the calls: its arguments in the header's order, what does not convert is refused, the status of
+    the entry comes back."""
+    hot, c = _lib.hot(), _cache()
+    a = ctypes.addressof(c.contents)
+    write = (a, 4096, 128, 64, 4096, 128, 64, 0, None, 4096, 4096, 4, 2, 4, None)
+    read = (a, 0, None, None, 4096, 4, 2, 4, 4096, 4096, None)
+    attend = (a, 4096, 256, 64, 0, 4, None, 4096, 4096, 4, 2, 4, 1, 0.125, 0, 0, None, 4096, None, 4096, 0, None)
+    for name, args in (("moeb_kv_write", write), ("moeb_kv_read", read), ("moeb_kv_attention", attend)):
+        f = getattr(hot, name)
+        assert f(*args) == _lib.MOEB_OK
+        assert len(args) == len(_lib.SIGNATURES[name][1])
+        assert f(None, *args[1:]) == _lib.MOEB_EINVAL and b"null" in _lib.load().moeb_last_error()
+        for i, (kind, v) in enumerate(zip(_lib.SIGNATURES[name][1], args)):
+            with pytest.raises(TypeError):
+                f(*args[:i], "x", *args[i + 1:])
+            if kind is ctypes.c_int:
+                with pytest.raises(OverflowError):
+                    f(*args[:i], 2 ** 31, *args[i + 1:])
+                with pytest.raises(OverflowError):
+                    f(*args[:i], 2 ** 70, *args[i + 1:])
+        with pytest.raises(TypeError, match="arguments"):
+            f(*args[1:])
+    assert hot.moeb_kv_attention(*attend[:14], -1, *attend[15:]) == _lib.MOEB_EINVAL  # the window
+    with pytest.raises(_lib.MoebError, match="moeb_kv_read failed with status 1"):
+        _lib.failed("moeb_kv_read", 1)
