@@ -154,7 +154,7 @@ struct Plan {
     long tiles, splits; // row tiles of the kernel for many rows; parts that each one's keys are cut into
     size_t split_bytes;
 };
-constexpr int FEW_RESIDENT = 3;  // CTAs per SM at most: the workspace has room for their partial results
+constexpr int FEW_RESIDENT = 4;  // CTAs per SM at most: the workspace has room for their partial results
 
 Plan plan_of(int T, int B, int P, int page_size, int H, int Hkv, int D, int max_q, int window, int sinks, bool cu) {
     Plan p = {};
