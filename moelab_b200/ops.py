@@ -385,7 +385,9 @@ class KVCache:
 
 # The checks of these calls are written for the good case: a decode step makes them for every layer, so each tensor is asked
 # once for what it has, and the reason is looked for only when something is wrong.
+# A call on another device than the current one is made again with the cache's device current.
 _BF16, _I32 = torch.bfloat16, torch.int32
+_current_device, _raw_stream = (getattr(torch._C, n, None) for n in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
 
 
 def _kv_ints(t, name, cache, size):
@@ -431,19 +433,6 @@ def _kv_out(t, name, shape, cache):
     return t
 
 
-def _kv_call(cache, name, *args):
-    """The call on the cache's device and that device's current stream."""
-    i = cache.index
-    stream = torch._C._cuda_getCurrentRawStream(i)
-    if i == torch._C._cuda_getDevice():
-        rc = getattr(_lib._hot or _lib.hot(), name)(*args, stream)
-    else:
-        with torch.cuda.device(i):
-            rc = getattr(_lib.hot(), name)(*args, stream)
-    if rc:
-        _lib.failed(name, rc)
-
-
 def _kv_cu(cu, T, B, cache):
     if cu is None:
         if B and T % B:
@@ -462,8 +451,14 @@ def kv_write(cache, k, v, table, lens, cu=None):
     if Tv != T:
         raise ValueError(f"k has {T} rows, v {Tv}")
     tp, trow, B, P = _kv_table(table, cache)
-    _kv_call(cache, "moeb_kv_write", cache._c, kp, krow, khead, vp, vrow, vhead, T, _kv_cu(cu, T, B, cache),
-             _kv_ints(lens, "lens", cache, B), tp, trow, B, P)
+    cp, lp, i = _kv_cu(cu, T, B, cache), _kv_ints(lens, "lens", cache, B), cache.index
+    if i != _current_device():
+        with torch.cuda.device(i):
+            return kv_write(cache, k, v, table, lens, cu)
+    rc = (_lib._hot or _lib.hot()).moeb_kv_write(cache._c, kp, krow, khead, vp, vrow, vhead, T, cp, lp, tp, trow, B, P,
+                                                 _raw_stream(i))
+    if rc:
+        _lib.failed("moeb_kv_write", rc)
 
 
 def kv_read(cache, table, cu, rows, first=None, out=None):
@@ -472,14 +467,20 @@ def kv_read(cache, table, cu, rows, first=None, out=None):
     DEVERR_PAGE. out: (k, v) to fill, whose rows behind the last
     sequence are left as they were; without it those rows are zero."""
     tp, trow, B, P = _kv_table(table, cache)
-    cp, fp = _kv_cu(cu, rows, B, cache), _kv_ints(first, "first", cache, B)
+    cp, fp, i = _kv_cu(cu, rows, B, cache), _kv_ints(first, "first", cache, B), cache.index
+    if i != _current_device():
+        with torch.cuda.device(i):
+            return kv_read(cache, table, cu, rows, first, out)
     shape = (rows, cache.kv_heads, cache.head_dim)
     if out is None:
         new = torch.empty if cu is None and B else torch.zeros
         k, v = (new(shape, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
     else:
         k, v = (_kv_out(t, "out", shape, cache) for t in out)
-    _kv_call(cache, "moeb_kv_read", cache._c, rows, cp, fp, tp, trow, B, P, k.data_ptr(), v.data_ptr())
+    rc = (_lib._hot or _lib.hot()).moeb_kv_read(cache._c, rows, cp, fp, tp, trow, B, P, k.data_ptr(), v.data_ptr(),
+                                                _raw_stream(i))
+    if rc:
+        _lib.failed("moeb_kv_read", rc)
     return k, v
 
 
@@ -495,7 +496,10 @@ def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=
     qp, qrow, qhead, T, H = _kv_rows(q, "q", cache)
     D = cache.head_dim
     tp, trow, B, P = _kv_table(table, cache)
-    cp, lp = _kv_cu(cu, T, B, cache), _kv_ints(lens, "lens", cache, B)
+    cp, lp, i = _kv_cu(cu, T, B, cache), _kv_ints(lens, "lens", cache, B), cache.index
+    if i != _current_device():
+        with torch.cuda.device(i):
+            return kv_attention(q, cache, table, lens, cu, max_q, scale, window, sinks, sink_logits, out, return_lse)
     if H == 0 or H % cache.kv_heads:
         raise ValueError(f"{H} query heads over {cache.kv_heads} KV heads")
     if window < 0 or sinks < 0:
@@ -516,12 +520,13 @@ def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=
     if nbytes is None:
         if len(cache._ws_bytes) > 4096:
             cache._ws_bytes.clear()
-        with torch.cuda.device(cache.index):
-            nbytes = cache._ws_bytes[key] = _lib.load().moeb_kv_attention_workspace_bytes(
-                T, B, P, cache.page_size, H, cache.kv_heads, D, max_q, window, sinks, cp is not None)
+        nbytes = cache._ws_bytes[key] = _lib.load().moeb_kv_attention_workspace_bytes(
+            T, B, P, cache.page_size, H, cache.kv_heads, D, max_q, window, sinks, cp is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None  # of this call alone
-    _kv_call(cache, "moeb_kv_attention", cache._c, qp, qrow, qhead, T, H, cp, lp, tp, trow, B, P, max_q,
-             D ** -0.5 if scale is None else float(scale), window, sinks,
-             None if sink_logits is None else sink_logits.data_ptr(), y.data_ptr(), None if lse is None else lse.data_ptr(),
-             None if ws is None else ws.data_ptr(), nbytes)
+    rc = (_lib._hot or _lib.hot()).moeb_kv_attention(
+        cache._c, qp, qrow, qhead, T, H, cp, lp, tp, trow, B, P, max_q, D ** -0.5 if scale is None else float(scale), window,
+        sinks, None if sink_logits is None else sink_logits.data_ptr(), y.data_ptr(), None if lse is None else lse.data_ptr(),
+        None if ws is None else ws.data_ptr(), nbytes, _raw_stream(i))
+    if rc:
+        _lib.failed("moeb_kv_attention", rc)
     return (y, lse) if return_lse else y

@@ -502,6 +502,26 @@ def test_calls_on_two_streams():
         assert all(torch.equal(y, want[i]) for y in got[i])
 
 
+def test_another_current_device(monkeypatch):
+    """Calls made while another device is current are made again with the cache's: here the first look says so."""
+    b = Batch([70, 33], [1, 1], 8, 2, 128, "q4", page=16, seed=44)
+    c = b.cache(ops)
+    want, rows = attend(b, c, return_lse=True), ops.kv_read(c, b.table, None, 2)
+    fresh = b.cache(ops, fill=False)
+    looks = []
+    monkeypatch.setattr(ops, "_current_device", lambda: 0 if len(looks) % 2 else 1)
+    real = torch.cuda.device
+    monkeypatch.setattr(torch.cuda, "device", lambda i: (looks.append(i), real(i))[1])
+    cu = torch.tensor([0, 70, 103], dtype=torch.int32, device="cuda")
+    ops.kv_write(fresh, b.flat(b.k), b.flat(b.v), b.table, b.lens_t, cu=cu)
+    looks.append(None)
+    got = ops.kv_attention(b.q, fresh, b.table, b.lens_t, cu=b.cu, max_q=1, return_lse=True)
+    looks.append(None)
+    back = ops.kv_read(fresh, b.table, None, 2)
+    assert looks == [0, None, 0, None, 0]
+    assert all(torch.equal(x, y) for x, y in zip((*got, *back), (*want, *rows)))
+
+
 def test_refusals():
     b = Batch([20], [1], 4, 2, 64, "q4", page=16)
     c = b.cache(ops)
