@@ -25,8 +25,8 @@
 //
 // A warp takes 32 keys of each block, straight from a cp.async ring of its own (no block-wide barrier in the loop; the next
 // run's first copies are on their way while a run's warps join; bulk copies from single lanes cost twice the instructions), and
-// feeds the codes to mma.sync m16n8k16 without dequantizing them. mma.sync and not tcgen05: with 8 or 16 columns the products
-// are a fifth of the time either way, and codes would have to pass through shared or tensor memory once more.
+// feeds the codes to mma.sync m16n8k16 without dequantizing them. mma.sync and not tcgen05: its pipe is busy for a fifth of
+// the time, and codes would have to be written to shared or tensor memory once more on their way.
 //   scores^T [16 keys x NC] = K codes . q, q in fp16 after a power of two per row (8 bits of significand fit 11). int4: a
 //     masked code is an fp16 subnormal, code * 2^-24, so that an operand costs one instruction (converted: 114 us for the batch
 //     above when that was 106); with group g's scale s and bias b, score = sum_g s acc_g + b qsum_g in fp32. MXFP4: E2M1 codes
