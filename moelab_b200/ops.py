@@ -5,6 +5,7 @@ CUDA, contiguous, with the dtypes documented in include/moelab_b200.h (packed co
 uint8 tensors).
 """
 import ctypes
+import math
 import threading
 
 import torch
@@ -512,9 +513,16 @@ def kv_attention(q, cache, table, lens, cu=None, max_q=None, scale=None, window=
     max_q = T // max(B, 1) if cu is None else T if max_q is None else min(int(max_q), T)
     if T and max_q <= 0:
         raise ValueError("max_q must be positive")
-    new = torch.empty if cu is None and B else torch.zeros
-    y = new((T, H, D), dtype=_BF16, device=cache.device) if out is None else _kv_out(out, "out", (T, H, D), cache)
-    lse = torch.full((T, H), -float("inf"), device=cache.device) if return_lse else None
+    whole = cp is None and B  # every row is some sequence's: all are written
+    if out is not None:
+        y = _kv_out(out, "out", (T, H, D), cache)
+    elif qrow == H * D and qhead == D:  # twice as fast as naming shape, type and device
+        y = torch.empty_like(q) if whole else torch.zeros_like(q)
+    else:
+        y = (torch.empty if whole else torch.zeros)((T, H, D), dtype=_BF16, device=cache.device)
+    lse = None
+    if return_lse:
+        lse = torch.empty((T, H), device=cache.device) if whole else torch.full((T, H), -math.inf, device=cache.device)
     key = (T, B, P, H, max_q, window, sinks, cp is None)
     nbytes = cache._ws_bytes.get(key)
     if nbytes is None:

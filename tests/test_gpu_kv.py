@@ -502,6 +502,29 @@ def test_calls_on_two_streams():
         assert all(torch.equal(y, want[i]) for y in got[i])
 
 
+@pytest.mark.parametrize("n", (1, 5, 40))
+def test_without_cu_every_row_is_written(n):
+    """Without cu the results are not cleared first: rows before a sequence's start, and their lse, are written all the same.
+    Views of q too."""
+    b = Batch([300, 40, 130], [n, n, n], 8, 2, 128, "q4", page=32, seed=45)
+    c = b.cache(ops)
+    lens = b.lens_t.clone()
+    lens[1] = n - 1
+    want, want_lse = ops.kv_attention(b.q, c, b.table, lens, cu=b.cu, max_q=n, return_lse=True)
+    wide = torch.cat([b.q, b.q], dim=1)
+    for q in (b.q, wide[:, :8]):
+        for shape, dtype in ((b.q.shape, torch.bfloat16), (want_lse.shape, torch.float32)):
+            junk = torch.full(shape, 7.0, dtype=dtype, device="cuda")
+            del junk  # the next tensors of these sizes
+        y, lse = ops.kv_attention(q, c, b.table, lens, return_lse=True)
+        assert y.shape == b.q.shape and y.is_contiguous()
+        # two kernels' results: 2^-8 of each by the last rounding, 2^-10 of the values (below 1 on average) by those inside
+        assert torch.allclose(y.float(), want.float(), rtol=2 ** -7, atol=2e-3)
+        assert not y[n].any() and lse[n].isneginf().all()
+        seen = ~want_lse.isneginf()
+        assert torch.equal(seen, ~lse.isneginf()) and torch.allclose(lse[seen], want_lse[seen], rtol=1e-4, atol=1e-4)
+
+
 def test_another_current_device(monkeypatch):
     """Calls made while another device is current are made again with the cache's: here the first look says so."""
     b = Batch([70, 33], [1, 1], 8, 2, 128, "q4", page=16, seed=44)
