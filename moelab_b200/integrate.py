@@ -28,6 +28,7 @@ dtype, near-ties can pick a different expert. `dequantize_into_stock` writes the
 back into the stock parameters, so a stock model runs on exactly the weights the kernels see; the tests compare
 the two on that basis.
 """
+import sys
 import types
 
 import torch
@@ -182,7 +183,7 @@ def policy_for(T, block):
 
 
 # ------------------------------------------------------------------ attention over the 4-bit KV cache
-ATTENTION = "moelab_b200_kv4"
+ATTENTION, ATTENTION_SDPA = "moelab_b200_kv4", "moelab_b200_kv4_sdpa"
 
 
 class _Length(int):
@@ -286,7 +287,7 @@ def _rows(t):
     return t.detach().to(torch.bfloat16).transpose(1, 2).reshape(B * n, H, D)
 
 
-def _attention(module, query, key, value, attention_mask=None, scaling=None, sliding_window=None, s_aux=None, **_):
+def _attention(module, query, key, value, attention_mask=None, **kw):
     B, H, n, D = query.shape
     tag = getattr(key, "_moeb_kv", None)
     if tag is not None:
@@ -295,44 +296,64 @@ def _attention(module, query, key, value, attention_mask=None, scaling=None, sli
         if attention_mask is not None:
             raise ValueError("attention masks of the caller's own are not supported by the 4-bit KV cache attention")
         cache, layer = tag
-        y = ops.kv_attention(_rows(query), cache.moeb_layers[layer], cache.moeb_table, cache.moeb_lens, scale=scaling,
-                             window=int(sliding_window or 0), sink_logits=None if s_aux is None else s_aux.detach().float())
+        sinks = kw.get("s_aux")
+        y = ops.kv_attention(_rows(query), cache.moeb_layers[layer], cache.moeb_table, cache.moeb_lens, scale=kw.get("scaling"),
+                             window=int(kw.get("sliding_window") or 0), sink_logits=None if sinks is None else sinks.detach().float())
         return y.view(B, n, H, D).to(query.dtype), None
-    # no 4-bit cache in this call: the definition, in plain torch, with the mask that the eager attention gets
-    L, G = key.shape[2], H // key.shape[1]
-    k, v = (t.repeat_interleave(G, dim=1).float() for t in (key, value))
-    s = torch.matmul(query.float(), k.transpose(2, 3)) * (D ** -0.5 if scaling is None else scaling)
-    if attention_mask is not None:
-        m = attention_mask[..., :L]
-        s = s.masked_fill(~m, torch.finfo(s.dtype).min) if m.dtype == torch.bool else s + m.float()
-    if s_aux is not None:
-        s = torch.cat([s, s_aux.float().view(1, H, 1, 1).expand(B, H, n, 1)], dim=-1)
-    p = torch.softmax(s, dim=-1)[..., :L]
-    return torch.matmul(p, v).transpose(1, 2).to(query.dtype).contiguous(), None
+    return _stock_attention(module, query, key, value, attention_mask, **kw)
 
 
-def _attention_mask(*args, kv_length=None, attention_mask=None, q_length=None, **kw):
+def _stock_attention(module, query, key, value, attention_mask, **kw):
+    """A call without the 4-bit cache: the attention that the model ran before the patch (or the nearest, see _without)."""
+    if module.config._attn_implementation == ATTENTION_SDPA:
+        from transformers import AttentionInterface
+        return AttentionInterface()["sdpa"](module, query, key, value, attention_mask, **kw)
+    if attention_mask is not None and attention_mask.dtype == torch.bool:  # the eager attention adds its mask
+        attention_mask = torch.zeros_like(attention_mask, dtype=query.dtype).masked_fill(~attention_mask, torch.finfo(query.dtype).min)
+    for c in type(module).__mro__:  # each model's file has its own
+        eager = getattr(sys.modules.get(c.__module__), "eager_attention_forward", None)
+        if eager is not None:
+            return eager(module, query, key, value, attention_mask, **kw)
+    raise ValueError(f"{type(module).__name__} has no eager attention to run a call without the 4-bit KV cache")
+
+
+def _attention_mask(*args, **kw):
+    return _mask("eager", *args, **kw)
+
+
+def _attention_mask_sdpa(*args, **kw):
+    return _mask("sdpa", *args, **kw)
+
+
+def _mask(stock, *args, kv_length=None, attention_mask=None, q_length=None, **kw):
     """With a 4-bit cache no mask tensor: causality and the window are the kernel's; a prompt of a padded batch is refused
-    here. Without one the mask of the eager attention."""
+    here. Without one the mask of the stock attention."""
     if not isinstance(kv_length, _Length):
         from transformers import AttentionMaskInterface
-        return AttentionMaskInterface()["eager"](*args, kv_length=kv_length, attention_mask=attention_mask, q_length=q_length, **kw)
+        return AttentionMaskInterface()[stock](*args, kv_length=kv_length, attention_mask=attention_mask, q_length=q_length, **kw)
     if attention_mask is not None and (q_length is None or q_length > 1) and not bool(attention_mask.bool().all()):
         raise ValueError("padded batches are not supported by the 4-bit KV cache attention")
     return None
 
 
+def _without(model, stock):
+    """The name under which a model is patched: calls without the 4-bit cache keep its eager or sdpa attention; what ran on
+    another kernel (flash, flex) runs on sdpa where the model has it."""
+    return ATTENTION_SDPA if stock != "eager" and getattr(model, "_supports_sdpa", False) else ATTENTION
+
+
 def patch_hf_attention(model):
-    """Route the model's attention through the library for calls with a quantized_kv_cache (others run the same attention in
-    plain torch). Returns the name of the implementation that unpatch_hf_attention restores."""
+    """Route the model's attention through the library for calls with a quantized_kv_cache (others run the stock attention).
+    Returns the name of the implementation that unpatch_hf_attention restores."""
     from transformers import AttentionInterface, AttentionMaskInterface
     _head_dim(model.config.get_text_config())
-    AttentionInterface.register(ATTENTION, _attention)
-    AttentionMaskInterface.register(ATTENTION, _attention_mask)
+    for name, mask in ((ATTENTION, _attention_mask), (ATTENTION_SDPA, _attention_mask_sdpa)):
+        AttentionInterface.register(name, _attention)
+        AttentionMaskInterface.register(name, mask)
     stock = model.config._attn_implementation
-    if stock != ATTENTION:
+    if stock not in (ATTENTION, ATTENTION_SDPA):
         model._moeb_attention_stock = stock
-        model.set_attn_implementation(ATTENTION)
+        model.set_attn_implementation(_without(model, stock))
     return model._moeb_attention_stock
 
 

@@ -1,0 +1,50 @@
+"""Calls of a model patched for the 4-bit KV cache that are not its ordinary prompt and steps: what the stock attention does in
+calls without the cache, and what is refused with it. On the CPU, with the stand-ins of test_integrate_kv."""
+import pytest
+import torch
+
+from moelab_b200 import integrate
+
+transformers = pytest.importorskip("transformers")
+from test_integrate import _gptoss, _qwen3  # noqa: E402
+from test_integrate_kv import _sinks, stand_in  # noqa: E402, F401
+
+
+def _ids(rows, n, seed=1):
+    return torch.randint(0, 512, (rows, n), generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("family,stock", [(_qwen3, "eager"), (_qwen3, "sdpa"), (_gptoss, "eager")])
+def test_calls_without_the_cache_are_the_stock_attention(family, stock):
+    """Inference, a padded batch, training with dropout on the attention weights, gradients: bit for bit the stock model's, which
+    ran the same function."""
+    m = _sinks(family(dtype=torch.float32))
+    m.config.attention_dropout = 0.5
+    for x in m.modules():
+        if hasattr(x, "attention_dropout"):
+            x.attention_dropout = 0.5
+    m.set_attn_implementation(stock)
+    ids, pad = _ids(2, 12), torch.ones(2, 12, dtype=torch.long)
+    pad[0, :4] = 0
+
+    def calls():
+        m.eval()
+        with torch.no_grad():
+            yield m(ids).logits
+            yield m(ids, attention_mask=pad).logits
+        m.train()
+        torch.manual_seed(5)
+        m.zero_grad()
+        y = m(ids, attention_mask=pad).logits
+        y.square().mean().backward()
+        yield y.detach()
+        yield m.model.layers[0].self_attn.k_proj.weight.grad.clone()
+
+    want = list(calls())
+    assert integrate.patch_hf_attention(m) == stock and integrate.patch_hf_attention(m) == stock
+    for got, ref in zip(calls(), want):
+        assert torch.equal(got, ref)
+    integrate.unpatch_hf_attention(m)
+    assert m.config._attn_implementation == stock
+    for got, ref in zip(calls(), want):
+        assert torch.equal(got, ref)
