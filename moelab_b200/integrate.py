@@ -275,6 +275,8 @@ def quantized_kv_cache(model, batch, max_len, fmt="q4", page_size=64):
 def _head_dim(cfg):
     if getattr(cfg, "kv_lora_rank", None):
         raise ValueError("latent attention (DeepSeek) has no per-head cache: not supported")
+    if getattr(cfg, "attn_logit_softcapping", None) is not None:
+        raise ValueError("capped attention scores (attn_logit_softcapping) are not supported by the 4-bit KV cache attention")
     dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
     if dim not in (64, 128):
         raise ValueError(f"heads of 64 or 128 values are supported, this model has {dim}")
@@ -287,6 +289,12 @@ def _rows(t):
     return t.detach().to(torch.bfloat16).transpose(1, 2).reshape(B * n, H, D)
 
 
+# What models hand to their attention function that the kernel has an argument for, or that changes nothing about a call's result.
+_KNOWN = frozenset(("scaling", "sliding_window", "s_aux", "dropout", "is_causal", "position_ids", "cache_position", "use_cache",
+                    "output_attentions", "output_hidden_states", "output_router_logits", "return_dict", "logits_to_keep",
+                    "num_items_in_batch"))
+
+
 def _attention(module, query, key, value, attention_mask=None, **kw):
     B, H, n, D = query.shape
     tag = getattr(key, "_moeb_kv", None)
@@ -295,6 +303,9 @@ def _attention(module, query, key, value, attention_mask=None, **kw):
             raise ValueError("the 4-bit KV cache has no backward pass: call model.eval() first")
         if attention_mask is not None:
             raise ValueError("attention masks of the caller's own are not supported by the 4-bit KV cache attention")
+        unknown = sorted(k for k, v in kw.items() if k not in _KNOWN and v is not None and v is not False)
+        if unknown or kw.get("dropout") or kw.get("is_causal") is False or getattr(module, "is_causal", True) is False:
+            raise ValueError(f"the 4-bit KV cache attention is causal, without dropout, and does not know {unknown or 'other kinds'}")
         cache, layer = tag
         sinks = kw.get("s_aux")
         y = ops.kv_attention(_rows(query), cache.moeb_layers[layer], cache.moeb_table, cache.moeb_lens, scale=kw.get("scaling"),

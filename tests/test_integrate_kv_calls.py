@@ -48,3 +48,40 @@ def test_calls_without_the_cache_are_the_stock_attention(family, stock):
     assert m.config._attn_implementation == stock
     for got, ref in zip(calls(), want):
         assert torch.equal(got, ref)
+
+
+# ------------------------------------------------------------------ refused with the cache
+BASE = dict(vocab_size=512, hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=2,
+            num_key_value_heads=1, head_dim=64, max_position_embeddings=128)
+
+
+def _keyed(m, batch=1):
+    """Arguments of a call of the attention function as a layer of m makes it, its key marked by a cache."""
+    integrate.patch_hf_attention(m)
+    cache = integrate.quantized_kv_cache(m, batch, 32, page_size=16)
+    k = torch.randn(batch, 2, 3, 64)
+    key, value = cache.update(k, k, 0)
+    return (m.eval().model.layers[0].self_attn, torch.randn(batch, 4, 3, 64), key, value)
+
+
+def test_capped_scores_are_refused(stand_in):
+    m = transformers.Gemma2ForCausalLM(transformers.Gemma2Config(**BASE))
+    with pytest.raises(ValueError, match="capped"):
+        integrate.patch_hf_attention(m)
+    with pytest.raises(ValueError, match="capped"):
+        integrate.quantized_kv_cache(m, 1, 32)
+    m.config.attn_logit_softcapping = None
+    integrate.patch_hf_attention(m)
+
+
+def test_arguments_the_kernel_does_not_know_are_refused(stand_in):
+    call = _keyed(_qwen3(dtype=torch.float32))
+    fine = dict(scaling=0.125, dropout=0.0, sliding_window=None, softcap=None, position_ids=torch.arange(3), use_cache=True)
+    y, _ = integrate._attention(*call, None, **fine)
+    assert y.shape == (1, 3, 4, 64)
+    for kw in (dict(softcap=50.0), dict(cu_seq_lens_q=torch.tensor([0, 3])), dict(dropout=0.1), dict(is_causal=False), dict(bias=1)):
+        with pytest.raises(ValueError, match="causal"):
+            integrate._attention(*call, None, **{**fine, **kw})
+    call[0].is_causal = False
+    with pytest.raises(ValueError, match="causal"):
+        integrate._attention(*call, None, **fine)
