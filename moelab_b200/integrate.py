@@ -190,6 +190,13 @@ class _Length(int):
     """A mask's number of keys that comes from a 4-bit cache."""
 
 
+class _Causal:
+    """What a layer's attention gets in a mask's place with a 4-bit cache: causal, the last `window` keys (0: all)."""
+
+    def __init__(self, window):
+        self.window = window
+
+
 def _kv_cache_class():
     """The cache class, made on first use (transformers is optional)."""
     global QuantizedKVCache
@@ -301,7 +308,12 @@ def _attention(module, query, key, value, attention_mask=None, **kw):
     if tag is not None:
         if module.training:
             raise ValueError("the 4-bit KV cache has no backward pass: call model.eval() first")
-        if attention_mask is not None:
+        window = int(kw.get("sliding_window") or 0)
+        if isinstance(attention_mask, _Causal):
+            if window and window != attention_mask.window:
+                raise ValueError(f"a layer with a window of {window} and a mask with one of {attention_mask.window}")
+            window = attention_mask.window
+        elif attention_mask is not None:
             raise ValueError("attention masks of the caller's own are not supported by the 4-bit KV cache attention")
         unknown = sorted(k for k, v in kw.items() if k not in _KNOWN and v is not None and v is not False)
         if unknown or kw.get("dropout") or kw.get("is_causal") is False or getattr(module, "is_causal", True) is False:
@@ -309,13 +321,15 @@ def _attention(module, query, key, value, attention_mask=None, **kw):
         cache, layer = tag
         sinks = kw.get("s_aux")
         y = ops.kv_attention(_rows(query), cache.moeb_layers[layer], cache.moeb_table, cache.moeb_lens, scale=kw.get("scaling"),
-                             window=int(kw.get("sliding_window") or 0), sink_logits=None if sinks is None else sinks.detach().float())
+                             window=window, sink_logits=None if sinks is None else sinks.detach().float())
         return y.view(B, n, H, D).to(query.dtype), None
     return _stock_attention(module, query, key, value, attention_mask, **kw)
 
 
 def _stock_attention(module, query, key, value, attention_mask, **kw):
     """A call without the 4-bit cache: the attention that the model ran before the patch (or the nearest, see _without)."""
+    if isinstance(attention_mask, _Causal):
+        raise ValueError(f"{type(module).__name__} does not hand the keys of the 4-bit KV cache to its attention as they are")
     if module.config._attn_implementation == ATTENTION_SDPA:
         from transformers import AttentionInterface
         return AttentionInterface()["sdpa"](module, query, key, value, attention_mask, **kw)
@@ -336,15 +350,37 @@ def _attention_mask_sdpa(*args, **kw):
     return _mask("sdpa", *args, **kw)
 
 
+def _same(f, g):
+    """Whether two functions are the same code over equal values."""
+    if not (callable(f) and callable(g)):
+        if isinstance(f, tuple) and isinstance(g, tuple):
+            return len(f) == len(g) and all(_same(x, y) for x, y in zip(f, g))
+        return type(f) is type(g) is int and f == g
+    if f is g:
+        return True
+    cells = [[c.cell_contents for c in getattr(x, "__closure__", None) or ()] for x in (f, g)]
+    return getattr(f, "__code__", f) is getattr(g, "__code__", g) and _same(*map(tuple, cells))
+
+
+def _window(mask_function, local_size):
+    """The window of a mask function (0: plainly causal); any other (chunks, packed sequences, both directions) is refused."""
+    from transformers import masking_utils as m
+    if mask_function is None or _same(mask_function, m.causal_mask_function):
+        return 0
+    if local_size and _same(mask_function, m.sliding_window_causal_mask_function(local_size)):
+        return int(local_size)
+    raise ValueError("masks other than the causal one and its sliding window are not supported by the 4-bit KV cache attention")
+
+
 def _mask(stock, *args, kv_length=None, attention_mask=None, q_length=None, **kw):
-    """With a 4-bit cache no mask tensor: causality and the window are the kernel's; a prompt of a padded batch is refused
-    here. Without one the mask of the stock attention."""
+    """With a 4-bit cache no mask tensor: causality and the window are the kernel's; what it has no argument for and a prompt of
+    a padded batch are refused here. Without one the mask of the stock attention."""
     if not isinstance(kv_length, _Length):
         from transformers import AttentionMaskInterface
         return AttentionMaskInterface()[stock](*args, kv_length=kv_length, attention_mask=attention_mask, q_length=q_length, **kw)
     if attention_mask is not None and (q_length is None or q_length > 1) and not bool(attention_mask.bool().all()):
         raise ValueError("padded batches are not supported by the 4-bit KV cache attention")
-    return None
+    return _Causal(_window(kw.get("mask_function"), kw.get("local_size")))
 
 
 def _without(model, stock):

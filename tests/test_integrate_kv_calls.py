@@ -85,3 +85,34 @@ def test_arguments_the_kernel_does_not_know_are_refused(stand_in):
     call[0].is_causal = False
     with pytest.raises(ValueError, match="causal"):
         integrate._attention(*call, None, **fine)
+
+
+def _llama4(**kw):
+    return transformers.Llama4ForCausalLM(transformers.Llama4TextConfig(**BASE, num_local_experts=2, **kw))
+
+
+def test_masks_that_are_not_causal_or_a_window_are_refused(stand_in):
+    """Chunked attention (stated through the mask alone), packed sequences, both directions. A window that the model states
+    through the mask alone is the kernel's."""
+    from transformers import masking_utils as mu
+    m = _llama4(attention_chunk_size=8).eval()
+    integrate.patch_hf_attention(m)
+    with torch.no_grad(), pytest.raises(ValueError, match="other than the causal"):
+        m(_ids(1, 20), past_key_values=integrate.quantized_kv_cache(m, 1, 32, page_size=16))
+    assert integrate._window(mu.causal_mask_function, None) == 0
+    assert integrate._window(mu.sliding_window_causal_mask_function(9), 9) == 9
+    packed = mu.and_masks(mu.causal_mask_function, mu.packed_sequence_mask_function(torch.zeros(1, 4, dtype=torch.long)))
+    for f, n in ((mu.sliding_window_causal_mask_function(9), 8), (mu.sliding_window_causal_mask_function(9), None), (packed, None),
+                 (mu.bidirectional_mask_function, None), (mu.chunked_causal_mask_function(8, torch.zeros(1, dtype=torch.int)), 8),
+                 (lambda b, h, q, k: k <= q, None), (mu.sliding_window_bidirectional_mask_function(9), 9)):
+        with pytest.raises(ValueError, match="other than the causal"):
+            integrate._window(f, n)
+
+    call = _keyed(_qwen3(dtype=torch.float32))
+    got = [integrate._attention(*call, integrate._Causal(w), scaling=0.125, **kw)[0]
+           for w, kw in ((2, {}), (2, dict(sliding_window=2)), (0, {}))]
+    assert torch.equal(got[0], got[1]) and not torch.equal(got[0], got[2])
+    with pytest.raises(ValueError, match="window"):
+        integrate._attention(*call, integrate._Causal(0), scaling=0.125, sliding_window=2)
+    with pytest.raises(ValueError, match="as they are"):  # the key is not the one that the cache marked
+        integrate._attention(*call[:2], call[2].clone(), call[3], integrate._Causal(0), scaling=0.125)
