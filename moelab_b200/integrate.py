@@ -206,7 +206,7 @@ def _kv_cache_class():
         class _QuantizedKVCache(DynamicCache):
             """Keys and values of every layer in 4 bits (ops.KVCache), `batch` sequences of equal length, up to `max_len`
             tokens each. Pass as past_key_values to a model patched with patch_hf_attention. Sequences advance together, so
-            padded batches are refused (by the mask function, when a prompt comes), and so is what reorders or repeats them
+            padded batches are refused (by the mask function), and so is what reorders or repeats them
             (beam search). crop() and reset() give tokens up."""
 
             def __init__(self, config, batch, max_len, fmt="q4", page_size=64, device="cuda"):
@@ -372,13 +372,13 @@ def _window(mask_function, local_size):
     raise ValueError("masks other than the causal one and its sliding window are not supported by the 4-bit KV cache attention")
 
 
-def _mask(stock, *args, kv_length=None, attention_mask=None, q_length=None, **kw):
-    """With a 4-bit cache no mask tensor: causality and the window are the kernel's; what it has no argument for and a prompt of
-    a padded batch are refused here. Without one the mask of the stock attention."""
+def _mask(stock, *args, kv_length=None, attention_mask=None, **kw):
+    """With a 4-bit cache no mask tensor: causality and the window are the kernel's; what it has no argument for and padded
+    batches are refused here, in every call: a mask may come with single tokens too. Without one the mask of the stock attention."""
     if not isinstance(kv_length, _Length):
         from transformers import AttentionMaskInterface
-        return AttentionMaskInterface()[stock](*args, kv_length=kv_length, attention_mask=attention_mask, q_length=q_length, **kw)
-    if attention_mask is not None and (q_length is None or q_length > 1) and not bool(attention_mask.bool().all()):
+        return AttentionMaskInterface()[stock](*args, kv_length=kv_length, attention_mask=attention_mask, **kw)
+    if attention_mask is not None and not bool(attention_mask.bool().all()):  # waits for the device, as generate() does per token
         raise ValueError("padded batches are not supported by the 4-bit KV cache attention")
     return _Causal(_window(kw.get("mask_function"), kw.get("local_size")))
 

@@ -116,3 +116,22 @@ def test_masks_that_are_not_causal_or_a_window_are_refused(stand_in):
         integrate._attention(*call, integrate._Causal(0), scaling=0.125, sliding_window=2)
     with pytest.raises(ValueError, match="as they are"):  # the key is not the one that the cache marked
         integrate._attention(*call[:2], call[2].clone(), call[3], integrate._Causal(0), scaling=0.125)
+
+
+def test_padded_batches_are_refused_token_by_token(stand_in):
+    m = _qwen3(dtype=torch.float32).eval()
+    integrate.patch_hf_attention(m)
+    ids = _ids(2, 4)
+    cache = integrate.quantized_kv_cache(m, 2, 32, page_size=16)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="padded"):
+            m(ids[:, :1], attention_mask=torch.tensor([[1], [0]]), past_key_values=cache)
+        assert cache.get_seq_length() == 0
+        for i in range(3):
+            m(ids[:, i:i + 1], attention_mask=torch.ones(2, i + 1, dtype=torch.long), past_key_values=cache)
+        for late in (0, 3):
+            mask = torch.ones(2, 4, dtype=torch.long)
+            mask[1, late] = 0
+            with pytest.raises(ValueError, match="padded"):
+                m(ids[:, 3:], attention_mask=mask, past_key_values=cache)
+    assert cache.get_seq_length() == 3
