@@ -296,6 +296,18 @@ def _rows(t):
     return t.detach().to(torch.bfloat16).transpose(1, 2).reshape(B * n, H, D)
 
 
+class _NoBackward(torch.autograd.Function):
+    """The first argument, as a function of the others whose backward pass is an error and not a missing term."""
+
+    @staticmethod
+    def forward(ctx, y, *inputs):
+        return y.view_as(y)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise NotImplementedError("the 4-bit KV cache has no backward pass: call the model without it, or under torch.no_grad()")
+
+
 # What models hand to their attention function that the kernel has an argument for, or that changes nothing about a call's result.
 _KNOWN = frozenset(("scaling", "sliding_window", "s_aux", "dropout", "is_causal", "position_ids", "cache_position", "use_cache",
                     "output_attentions", "output_hidden_states", "output_router_logits", "return_dict", "logits_to_keep",
@@ -322,7 +334,10 @@ def _attention(module, query, key, value, attention_mask=None, **kw):
         sinks = kw.get("s_aux")
         y = ops.kv_attention(_rows(query), cache.moeb_layers[layer], cache.moeb_table, cache.moeb_lens, scale=kw.get("scaling"),
                              window=window, sink_logits=None if sinks is None else sinks.detach().float())
-        return y.view(B, n, H, D).to(query.dtype), None
+        y = y.view(B, n, H, D).to(query.dtype)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (query, key, value, sinks)):
+            y = _NoBackward.apply(y, query, key, value, sinks)
+        return y, None
     return _stock_attention(module, query, key, value, attention_mask, **kw)
 
 

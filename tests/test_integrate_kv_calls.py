@@ -135,3 +135,24 @@ def test_padded_batches_are_refused_token_by_token(stand_in):
             with pytest.raises(ValueError, match="padded"):
                 m(ids[:, 3:], attention_mask=mask, past_key_values=cache)
     assert cache.get_seq_length() == 3
+
+
+@pytest.mark.parametrize("frozen", [(), ("q_proj",), ("q_proj", "k_proj"), ("k_proj", "v_proj")])
+def test_gradients_through_the_cache_are_an_error(stand_in, frozen):
+    """In eval mode with gradients on the logits are those without, and a backward pass through the cached attention is refused,
+    whichever of its inputs needs one. Where none does the rest of the model has its gradients."""
+    m = _qwen3(dtype=torch.float32).eval()
+    integrate.patch_hf_attention(m)
+    ids = _ids(1, 5)
+    with torch.no_grad():
+        want = m(ids, past_key_values=integrate.quantized_kv_cache(m, 1, 32, page_size=16)).logits
+    for n, p in m.named_parameters():
+        p.requires_grad_("lm_head" in n or ("_proj" in n and "self_attn" in n and not any(f in n for f in frozen)))
+    y = m(ids, past_key_values=integrate.quantized_kv_cache(m, 1, 32, page_size=16)).logits
+    assert torch.equal(y.detach(), want)
+    with pytest.raises(NotImplementedError, match="backward"):
+        y.sum().backward()
+    for n, p in m.named_parameters():
+        p.requires_grad_("lm_head" in n)
+    m(ids, past_key_values=integrate.quantized_kv_cache(m, 1, 32, page_size=16)).logits.sum().backward()
+    assert m.lm_head.weight.grad.any()
