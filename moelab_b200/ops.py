@@ -386,6 +386,7 @@ class KVCache:
 
 # The checks of these calls are written for the good case: a decode step makes them for every layer, so each tensor is asked
 # once for what it has, and the reason is looked for only when something is wrong.
+# There is no backward pass: a tensor that needs a gradient is refused where one would be recorded.
 # A call on another device than the current one is made again with the cache's device current.
 _BF16, _I32 = torch.bfloat16, torch.int32
 _current_device, _raw_stream = (getattr(torch._C, n, None) for n in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
@@ -412,6 +413,9 @@ def _kv_table(table, cache):
 
 
 def _kv_rows(t, name, cache, heads=None):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} needs a gradient, and the 4-bit KV cache has no backward pass: detach it, or call under "
+                         f"torch.no_grad()")
     if t.dtype != _BF16 or t.get_device() != cache.index or t.dim() != 3:
         raise ValueError(f"{name} must be a bfloat16 [rows, heads, {cache.head_dim}] tensor on {cache.device} (a CUDA device), "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
