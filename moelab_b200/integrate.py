@@ -221,7 +221,7 @@ def _kv_cache_class():
                 dev = self.moeb_layers[0].device
                 self.moeb_table = torch.arange(batch * per, dtype=torch.int32, device=dev).view(batch, per)
                 self.moeb_lens = torch.zeros(batch, dtype=torch.int32, device=dev)
-                self.moeb_seen = [0] * cfg.num_hidden_layers
+                self.moeb_seen, self.moeb_filled = [0] * cfg.num_hidden_layers, 0  # tokens of each layer; what moeb_lens holds
 
             def get_seq_length(self, layer_idx=0):
                 return self.moeb_seen[layer_idx or 0]
@@ -249,8 +249,9 @@ def _kv_cache_class():
                 seen = self.moeb_seen[layer_idx] + n
                 if seen > self.moeb_max:
                     raise ValueError(f"{seen} tokens, the cache holds {self.moeb_max}")
-                if layer_idx == 0:
+                if seen != self.moeb_filled:  # by the first layer of a call that has attention
                     self.moeb_lens.fill_(seen)
+                    self.moeb_filled = seen
                 self.moeb_seen[layer_idx] = seen
                 ops.kv_write(self.moeb_layers[layer_idx], _rows(key_states), _rows(value_states), self.moeb_table,
                              self.moeb_lens)

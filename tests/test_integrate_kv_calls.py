@@ -96,9 +96,12 @@ def test_masks_that_are_not_causal_or_a_window_are_refused(stand_in):
     through the mask alone is the kernel's."""
     from transformers import masking_utils as mu
     m = _llama4(attention_chunk_size=8).eval()
+    m.config.layer_types, types = None, m.config.layer_types  # the patch refuses them: here the calls
     integrate.patch_hf_attention(m)
+    cache = integrate.quantized_kv_cache(m, 1, 32, page_size=16)
+    m.config.layer_types = types
     with torch.no_grad(), pytest.raises(ValueError, match="other than the causal"):
-        m(_ids(1, 20), past_key_values=integrate.quantized_kv_cache(m, 1, 32, page_size=16))
+        m(_ids(1, 20), past_key_values=cache)
     assert integrate._window(mu.causal_mask_function, None) == 0
     assert integrate._window(mu.sliding_window_causal_mask_function(9), 9) == 9
     packed = mu.and_masks(mu.causal_mask_function, mu.packed_sequence_mask_function(torch.zeros(1, 4, dtype=torch.long)))
@@ -156,3 +159,21 @@ def test_gradients_through_the_cache_are_an_error(stand_in, frozen):
         p.requires_grad_("lm_head" in n)
     m(ids, past_key_values=integrate.quantized_kv_cache(m, 1, 32, page_size=16)).logits.sum().backward()
     assert m.lm_head.weight.grad.any()
+
+
+def test_lengths_follow_the_layer_that_calls(stand_in):
+    """A model whose first layer does not write keys: the rows of the next one are where its own count says, and read back."""
+    m = _qwen3(dtype=torch.float32)
+    integrate.patch_hf_attention(m)
+    cache = integrate.quantized_kv_cache(m, 2, 32, page_size=16)
+    k = torch.randn(2, 2, 5, 64)
+    for a, b in ((0, 3), (3, 4), (4, 5)):
+        cache.update(k[:, :, a:b], -k[:, :, a:b], 1)
+        assert cache.moeb_lens.tolist() == [b, b] and cache.moeb_seen == [0, b]
+    stored = cache.moeb_layers[1]
+    assert torch.equal(stored.k[:5], k[0].transpose(0, 1)) and torch.equal(stored.v[32:37], -k[1].transpose(0, 1))
+    cache.crop(0)
+    cache.update(k, k, 0)
+    assert cache.moeb_lens.tolist() == [5, 5]
+    cache.update(k[:, :, :2], k[:, :, :2], 1)
+    assert cache.moeb_lens.tolist() == [2, 2]
