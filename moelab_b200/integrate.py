@@ -283,6 +283,9 @@ def quantized_kv_cache(model, batch, max_len, fmt="q4", page_size=64):
 def _head_dim(cfg):
     if getattr(cfg, "kv_lora_rank", None):
         raise ValueError("latent attention (DeepSeek) has no per-head cache: not supported")
+    other = set(getattr(cfg, "layer_types", None) or ()) - {"full_attention", "sliding_attention"}
+    if other:
+        raise ValueError(f"layers of full and sliding attention are supported, this model has {', '.join(sorted(other))}")
     if getattr(cfg, "attn_logit_softcapping", None) is not None:
         raise ValueError("capped attention scores (attn_logit_softcapping) are not supported by the 4-bit KV cache attention")
     dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads

@@ -177,3 +177,11 @@ def test_lengths_follow_the_layer_that_calls(stand_in):
     assert cache.moeb_lens.tolist() == [5, 5]
     cache.update(k[:, :, :2], k[:, :, :2], 1)
     assert cache.moeb_lens.tolist() == [2, 2]
+
+
+def test_models_with_other_layers_are_refused():
+    linear = transformers.Qwen3NextConfig(**{**BASE, "num_hidden_layers": 4})
+    with pytest.raises(ValueError, match="linear_attention"):
+        integrate._head_dim(linear)
+    with pytest.raises(ValueError, match="chunked_attention"):
+        integrate.patch_hf_attention(_llama4())
