@@ -211,7 +211,7 @@ def _kv_cache_class():
 
             def __init__(self, config, batch, max_len, fmt="q4", page_size=64, device="cuda"):
                 super().__init__(config=config)
-                cfg = config.get_text_config()
+                cfg = self.moeb_config = config.get_text_config()
                 dim = _head_dim(cfg)
                 heads = getattr(cfg, "num_key_value_heads", None) or cfg.num_attention_heads
                 per = -(-max_len // page_size)
@@ -243,6 +243,9 @@ def _kv_cache_class():
             reorder_cache = batch_repeat_interleave = batch_select_indices = _refuse
 
             def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
+                if self.moeb_config._attn_implementation not in (ATTENTION, ATTENTION_SDPA):
+                    raise ValueError("the model's attention does not read the 4-bit KV cache: call patch_hf_attention(model) first, "
+                                     "or go on with to_stock()")
                 B, H, n, D = key_states.shape
                 if B != self.moeb_batch:
                     raise ValueError(f"a batch of {B} sequences, the cache is for {self.moeb_batch}")

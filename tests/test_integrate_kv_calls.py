@@ -185,3 +185,23 @@ def test_models_with_other_layers_are_refused():
         integrate._head_dim(linear)
     with pytest.raises(ValueError, match="chunked_attention"):
         integrate.patch_hf_attention(_llama4())
+
+
+def test_models_that_are_not_patched_refuse_the_cache(stand_in):
+    """Their attention would see the newest keys alone. After unpatching, to_stock() goes on."""
+    m = _qwen3(dtype=torch.float32).eval()
+    ids = _ids(1, 9)
+    cache = integrate.quantized_kv_cache(m, 1, 32, page_size=16)
+    with torch.no_grad():
+        want = m(ids).logits
+        with pytest.raises(ValueError, match="patch_hf_attention"):
+            m(ids[:, :5], past_key_values=cache)
+        assert cache.get_seq_length() == 0
+        integrate.patch_hf_attention(m)
+        m(ids[:, :5], past_key_values=cache)
+        integrate.unpatch_hf_attention(m)
+        with pytest.raises(ValueError, match="to_stock"):
+            m(ids[:, 5:6], past_key_values=cache)
+        assert cache.get_seq_length() == 5
+        got = m(ids[:, 5:], past_key_values=cache.to_stock()).logits
+    assert (got - want[:, 5:]).norm() / want[:, 5:].norm() < 2e-2  # the stand-in's rows come back in bfloat16
