@@ -246,6 +246,9 @@ def _kv_cache_class():
                 if self.moeb_config._attn_implementation not in (ATTENTION, ATTENTION_SDPA):
                     raise ValueError("the model's attention does not read the 4-bit KV cache: call patch_hf_attention(model) first, "
                                      "or go on with to_stock()")
+                if _capturing(key_states):
+                    raise RuntimeError("the 4-bit cache of a model counts its tokens on the host: a captured call would write the "
+                                       "same places in every replay. Capture ops.kv_write and ops.kv_attention, which read lens")
                 B, H, n, D = key_states.shape
                 if B != self.moeb_batch:
                     raise ValueError(f"a batch of {B} sequences, the cache is for {self.moeb_batch}")
@@ -295,6 +298,10 @@ def _head_dim(cfg):
     if dim not in (64, 128):
         raise ValueError(f"heads of 64 or 128 values are supported, this model has {dim}")
     return dim
+
+
+def _capturing(t):
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
 
 
 def _rows(t):

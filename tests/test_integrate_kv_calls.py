@@ -205,3 +205,14 @@ def test_models_that_are_not_patched_refuse_the_cache(stand_in):
         assert cache.get_seq_length() == 5
         got = m(ids[:, 5:], past_key_values=cache.to_stock()).logits
     assert (got - want[:, 5:]).norm() / want[:, 5:].norm() < 2e-2  # the stand-in's rows come back in bfloat16
+
+
+def test_captured_calls_are_refused(stand_in, monkeypatch):
+    m = _qwen3(dtype=torch.float32).eval()
+    integrate.patch_hf_attention(m)
+    cache = integrate.quantized_kv_cache(m, 1, 32, page_size=16)
+    assert not integrate._capturing(torch.zeros(1))
+    monkeypatch.setattr(integrate, "_capturing", lambda t: True)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="captured"):
+        m(_ids(1, 5), past_key_values=cache)
+    assert cache.moeb_seen == [0, 0]
