@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             const float mine = la + lb, o = other(mine);
             l = sub ? o + mine : mine + o;
         }
-        if (poison >> 31) l = __uint_as_float(0x7fffffffu);
+        if (poison >> 31 && (qmul >= 0.f || l != 0.f)) l = __uint_as_float(0x7fffffffu);  // a query that sees nothing is not looked at
         // ---- the rows' results (m is off by P_OFF against the weights' sum: undone here)
         const float M = l == 0.f ? -INFINITY : m - P_OFF;
         float mul = nk > 0 ? sh.vun : 0.f, Ls = l, sum_m = M;
