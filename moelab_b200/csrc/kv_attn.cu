@@ -404,7 +404,8 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
                 t16 = max(t16, __shfl_xor_sync(0xffffffffu, t16, 1));
                 t16 = max(t16, __shfl_xor_sync(0xffffffffu, t16, 2));
                 const int e = min(max((int)(t16 >> 7), UP + 1), 254);  // biased exponent of the largest value
-                const float down = __uint_as_float((uint32_t)(254 + UP - e) << 23);  // 2^(UP - (e - 127))
+                // 2^(UP - (e - 127)); a row that is not finite becomes NaN, as infinities would not where all scores are -inf
+                const float down = t16 < 0x7f80u ? __uint_as_float((uint32_t)(254 + UP - e) << 23) : __uint_as_float(0x7fffffffu);
                 // what undoes it; int4: and 2^24 for the codes, taken out of qsum below
                 mul *= __uint_as_float((uint32_t)(e - UP) << 23) * (FMT == FMT_Q4 ? 16777216.f : 1.f);
 #pragma unroll

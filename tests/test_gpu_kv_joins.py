@@ -39,3 +39,19 @@ def test_queries_that_see_nothing_are_not_looked_at(fmt, n, split):
         assert (lse[:2] == (-math.inf if sink is None else 0.5)).all()
         if sink is None:
             check(y[2:], ref, bound)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n,L", [(1, 1), (1, 3), (3, 300), (2, 9000), (150, 300)])
+@pytest.mark.parametrize("bad", (math.inf, -math.inf, math.nan))
+def test_queries_that_are_not_finite_give_nan_and_touch_no_other_row(fmt, n, L, bad):
+    """inf - inf is in every softmax of such a row, over one key as well, whatever the sign of its scores."""
+    b = Batch([L, L + 5], [n, n], 4, 2, 64, fmt, page=16, seed=52)
+    c = b.cache(ops)
+    ref, bound, _ = b.reference()
+    b.q[n - 1, 1, 7] = bad
+    y, lse = attend(b, c, return_lse=True)
+    assert y[n - 1, 1].isnan().all() and lse[n - 1, 1].isnan()
+    rest = torch.ones(2 * n, 4, dtype=torch.bool)
+    rest[n - 1, 1] = False
+    check(y.cpu()[rest], ref[rest], bound[rest])
