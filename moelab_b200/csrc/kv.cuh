@@ -190,6 +190,84 @@ MOEB_DEV void kv_finish(const KvAttnArgs &a, int t, int head, int d4, float4 v, 
     *reinterpret_cast<uint2 *>(a.y + row * D + 4 * d4) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
     if (a.lse && d4 == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
+// first value of the 4 that physical half-word u of a row holds
+template <int FMT, int D>
+MOEB_DEV int kv_dim(int u) {
+    return FMT == FMT_Q4 ? 64 * ((u >> 1) % (D / 64)) + 8 * ((u >> 1) / (D / 64)) + 4 * (u & 1) : 32 * (u % (D / 32)) + 4 * (u / (D / 32));
+}
+// its values in row `row` of an array
+template <int FMT, int D>
+MOEB_DEV float4 kv_four(const void *codes, const void *pars, size_t row, int u) {
+    // MXFP4: a 32-bit load and a shift; from a 16-bit load nvcc 12.9 made zeros of the conversions' bytes
+    const uint32_t word = static_cast<const uint32_t *>(codes)[row * (D / 8) + (u >> 1)] >> ((FMT == FMT_Q4 ? 8 : 16) * (u & 1));
+    const uint32_t par = FMT == FMT_Q4 ? static_cast<const uint32_t *>(pars)[row * (D / 64) + (u >> 1) % (D / 64)]
+                                       : static_cast<const uint8_t *>(pars)[row * (D / 32) + u % (D / 32)];
+    float y[8];
+    kv_word_values<FMT>(word, par, y);
+    return make_float4(y[0], y[1], y[2], y[3]);
+}
+// A row's attention in fp32 throughout, by one warp: its keys in blocks [k0, k1) of 128, block k from token 128 k on for k < ns
+// and 128 (k + skip) for the others. For keys and values whose sizes are too far apart for the tensor cores' fp16 operands (see
+// KV_SPREAD); ordinary ones never come here, so it is written to be short and every key's score is a sum over the lanes. v: values kv_dim(lane) .. + 3 of the sum of weights 2^(score - M) times
+// values, L: the sum of the weights, in every lane.
+struct KvSum {
+    float4 v;
+    float M, L;
+};
+template <int FMT, int D>
+MOEB_DEV KvSum kv_exact(const KvAttnArgs &a, int b, int h, const uint16_t *q, int pos, int k0, int k1, int ns, int skip) {
+    const int lane = threadIdx.x & 31, u = lane % (D / 4);
+    const uint2 w = *reinterpret_cast<const uint2 *>(q + kv_dim<FMT, D>(u));
+    float4 x = make_float4(bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y));
+    const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+    const bool bad = __any_sync(0xffffffffu, !(top < INFINITY) || x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w);
+    if (bad) x = make_float4(__uint_as_float(0x7fffffffu), 0.f, 0.f, 0.f);  // NaN, whatever it meets
+    if (lane >= D / 4 || (a.scale == 0.f && !bad)) x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -INFINITY, L = 0.f;
+#pragma unroll 1
+    for (int k = k0; k < k1; ++k) {
+#pragma unroll 1
+        for (int j0 = 128 * (k < ns ? k : k + skip), end = min(j0 + 128, pos + 1); j0 < end; j0 += 16) {
+            const long page = kv_page(a.c, a.s, b, j0);
+            if (page < 0 || (a.window && j0 + 15 <= pos - a.window && j0 >= a.sinks)) continue;
+            const size_t row = kv_row(a.c, page, h, j0);
+#pragma unroll 1
+            for (int i = 0; i < 16; i += 4) {
+                float s[4];
+                float4 y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 c = kv_four<FMT, D>(a.c.kq, a.c.ks, row + i + e, u);
+                    y[e] = kv_four<FMT, D>(a.c.vq, a.c.vs, row + i + e, u);
+                    s[e] = fmaf(x.x, c.x, fmaf(x.y, c.y, fmaf(x.z, c.z, x.w * c.w)));
+                    if (lane >= D / 4) s[e] = 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) s[e] += __shfl_xor_sync(0xffffffffu, s[e], o);
+                    const int j = j0 + i + e;
+                    if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) continue;
+                    const float t = s[e] * a.scale, N = fmaxf(M, t), use = N == -INFINITY ? 0.f : N, f = exp2f(M - use), p = exp2f(t - use);
+                    M = N;
+                    L = fmaf(L, f, p);
+                    v.x = fmaf(v.x, f, p * y[e].x);
+                    v.y = fmaf(v.y, f, p * y[e].y);
+                    v.z = fmaf(v.z, f, p * y[e].z);
+                    v.w = fmaf(v.w, f, p * y[e].w);
+                }
+            }
+        }
+    }
+    return {v, M, L};
+}
+// The tensor cores' fp16 operands hold groups of values up to 2^KV_SPREAD apart without loss: the largest is put near 2^8, one
+// 2^14 smaller is near 2^-6 and rounds to 2^-25, 2^-19 of it. Groups further below the largest, but not below 2^-120 (those may
+// count as zeros), make a run of keys uneven: kv_exact has it. The largest may be a key's that the row does not see, or hardly
+// looks at, so that what it would round away can be all of the row's result.
+constexpr int KV_SPREAD = 14;
+constexpr uint32_t KV_ZERO = 7u << 23;  // bits of 2^-120
 template <int FMT, int D>
 __global__ void k_kv_write(const KvWriteArgs a);
 template <int FMT, int D>

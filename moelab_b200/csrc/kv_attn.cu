@@ -6,7 +6,7 @@
 // The rows of a sequence that share a KV head (n tokens x Gq query heads, at most NC = 8 or 16) are the columns of
 // one tensor-core tile, so the cache is read once for all of them. Long caches are bound by their bytes, short ones
 // by the chain lengths -> page table -> codes -> sums. Measured:
-//   64 sequences of 1 to 8192 tokens, 32 query heads on 8, int4 (306 MB): 85 us with the join, 3.6 TB/s; in its loop over the
+//   64 sequences of 1 to 8192 tokens, 32 query heads on 8, int4 (306 MB): 86 us with the join, 3.6 TB/s; in its loop over the
 //     blocks the kernel moves 5.9 TB/s (a copy 6.56), the rest is the 2 us until a CTA knows its run, the 5 us until its first
 //     copies are there, CTAs that end between 59 and 78 us (memory is not equally far from all SMs) and the join. Shares of two
 //     sizes, the small ones for CTAs that end early, cost more than they even out (92 us): new CTAs start slowly under load.
@@ -482,6 +482,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
                 for (int g = 0; g < (FMT == FMT_Q4 ? NG : 1); ++g) bs[nt][g][e] = 0.f;
             }
         }
+        uint32_t low = ~0u;  // the smallest group of values among this lane's keys, less what counts as zero (which wraps)
         uint32_t vlim = 0;  // bits of the largest value scale that the running power of two takes
         float vexp = 0.f;   // its exponent: weights are 2^(score - m + vexp), and o, l and bs are sums of them
 
@@ -564,6 +565,22 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
                                 s[x][nt][e] = fmaf(xa[g], acc[nt][e], s[x][nt][e]);
                                 s[x][nt][2 + e] = fmaf(xb[g], acc[nt][2 + e], s[x][nt][2 + e]);
                             }
+                        }
+                    }
+                }
+                {  // The smallest group of values, by its largest magnitude (int4: |bias|, 7.5 scales or more; the bits doubled to drop
+                   // its sign) or its power of two. The four lanes that have the same keys below take one of the four keys each (all
+                   // four in every lane: 88 us for the batch above; nothing looked at: 85)
+                    const int j = 16 * (c >> 1) + 8 * (c & 1) + ta;
+                    const unsigned char *par = st + F::O_VP + j * F::PROW;
+                    if (full32 || (((has >> (c >> 1)) & 1u) && tok + j <= plast && (tok + j >= qr.lo || tok + j < a.sinks))) {
+                        if (FMT == FMT_Q4) {
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) low = min(low, 2u * reinterpret_cast<const uint32_t *>(par)[g] - 2u * KV_ZERO);
+                        } else {
+                            const uint32_t w = NG == 4 ? *reinterpret_cast<const uint32_t *>(par) : *reinterpret_cast<const uint16_t *>(par);
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) low = min(low, __byte_perm(w, 0, 0x4440 + g) - (KV_ZERO >> 23));
                         }
                     }
                 }
@@ -772,50 +789,12 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
                 }
             }
         }
-        __syncthreads();
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int col = nt * 8 + 2 * c + e;
-                float M = s_m[0][col];
-#pragma unroll
-                for (int i = 1; i < FW; ++i) M = fmaxf(M, s_m[i][col]);
-                const float fm = ex2(m[nt][e] - (M == -INFINITY ? 0.f : M));
-                float *dst = so + (warp * NC + col) * D;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    // int4: tile 4 g + p is elements 2 p, 2 p + 1 of words r of group g; MXFP4: tile 2 g + x is elements
-                    // 4 r + 2 x, 4 r + 2 x + 1 of group g (of 32)
-                    const int dim = FMT == FMT_Q4 ? 64 * (i >> 2) + 8 * r + 2 * (i & 3) : 32 * (i >> 1) + 4 * r + 2 * (i & 1);
-                    const float add = FMT == FMT_Q4 ? bs[nt][i >> 2 < NG ? i >> 2 : 0][e] : 0.f;
-                    float2 v;
-                    const float up = FMT == FMT_FP4 ? 1.f : i & 1 ? 1048576.f : 16777216.f;  // codes were * 2^-20, 2^-24
-                    v.x = fmaf(o[nt][i][e], up, add) * fm;
-                    v.y = fmaf(o[nt][i][2 + e], up, add) * fm;
-                    *reinterpret_cast<float2 *>(dst + dim) = v;
-                }
-            }
-        }
-        __syncthreads();
+        // a group of values too far below the largest for fp16? int4: scales of 2^-11 of the largest have a bias of 2^-14 of its 15
+        const int under = (int)(vlim >> 23) - (KV_SPREAD + 6 - (FMT == FMT_Q4 ? 3 : 0)) - (int)(KV_ZERO >> 23);
+        const bool uneven = __syncthreads_or(under > 0 && low < (FMT == FMT_Q4 ? (uint32_t)under << 24 : (uint32_t)under));
         const bool whole = kr0 == 0 && kr1 == qr.nb;
         float *pt = part + ((size_t)blockIdx.x * 2 + (us >= segr ? 0 : 1)) * (NC * (D + 2));
-        for (int i = threadIdx.x; i < qr.n * a.Gq * (D / 4); i += FT) {
-            const int col = i / (D / 4), d4 = i % (D / 4);
-            float M = s_m[0][col], L = 0.f;
-#pragma unroll
-            for (int x = 1; x < FW; ++x) M = fmaxf(M, s_m[x][col]);
-            const float use = M == -INFINITY ? 0.f : M;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int x = 0; x < FW; ++x) {
-                const float4 w = *reinterpret_cast<const float4 *>(so + (x * NC + col) * D + 4 * d4);
-                v.x += w.x;
-                v.y += w.y;
-                v.z += w.z;
-                v.w += w.w;
-                L += s_l[x][col] * ex2(s_m[x][col] - use);
-            }
+        auto put = [&](int col, int d4, float4 v, float M, float L) {  // the run's sums of 4 values of a column
             if (a.direct > 1) {  // to the front of the rings, which are empty now
                 float *mine = reinterpret_cast<float *>(sm);
                 *reinterpret_cast<float4 *>(mine + col * D + 4 * d4) = v;
@@ -826,6 +805,59 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
             } else {
                 *reinterpret_cast<float4 *>(pt + col * D + 4 * d4) = v;
                 if (d4 == 0) *reinterpret_cast<float2 *>(pt + NC * D + 2 * col) = make_float2(M, L);
+            }
+        };
+        if (uneven) {  // a warp per column, in fp32 from the cache
+#pragma unroll 1
+            for (int col = warp; col < qr.n * a.Gq; col += FW) {
+                const int ri = kv_div(col, a.Gdiv);
+                const KvSum x = kv_exact<FMT, D>(a, br, hr, a.q + (qr.r0 + ri) * a.q_row + (hr * a.Gq + col - ri * a.Gq) * a.q_head, p0 + ri, kr0,
+                                                 kr1, qr.ns, qr.lo / FB - qr.ns);
+                if (lane < D / 4) put(col, kv_dim<FMT, D>(lane) / 4, x.v, x.M, x.L);
+            }
+        } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int col = nt * 8 + 2 * c + e;
+                    float M = s_m[0][col];
+#pragma unroll
+                    for (int i = 1; i < FW; ++i) M = fmaxf(M, s_m[i][col]);
+                    const float fm = ex2(m[nt][e] - (M == -INFINITY ? 0.f : M));
+                    float *dst = so + (warp * NC + col) * D;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        // int4: tile 4 g + p is elements 2 p, 2 p + 1 of words r of group g; MXFP4: tile 2 g + x is elements
+                        // 4 r + 2 x, 4 r + 2 x + 1 of group g (of 32)
+                        const int dim = FMT == FMT_Q4 ? 64 * (i >> 2) + 8 * r + 2 * (i & 3) : 32 * (i >> 1) + 4 * r + 2 * (i & 1);
+                        const float add = FMT == FMT_Q4 ? bs[nt][i >> 2 < NG ? i >> 2 : 0][e] : 0.f;
+                        float2 v;
+                        const float up = FMT == FMT_FP4 ? 1.f : i & 1 ? 1048576.f : 16777216.f;  // codes were * 2^-20, 2^-24
+                        v.x = fmaf(o[nt][i][e], up, add) * fm;
+                        v.y = fmaf(o[nt][i][2 + e], up, add) * fm;
+                        *reinterpret_cast<float2 *>(dst + dim) = v;
+                    }
+                }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < qr.n * a.Gq * (D / 4); i += FT) {
+                const int col = i / (D / 4), d4 = i % (D / 4);
+                float M = s_m[0][col], L = 0.f;
+#pragma unroll
+                for (int x = 1; x < FW; ++x) M = fmaxf(M, s_m[x][col]);
+                const float use = M == -INFINITY ? 0.f : M;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int x = 0; x < FW; ++x) {
+                    const float4 w = *reinterpret_cast<const float4 *>(so + (x * NC + col) * D + 4 * d4);
+                    v.x += w.x;
+                    v.y += w.y;
+                    v.z += w.z;
+                    v.w += w.w;
+                    L += s_l[x][col] * ex2(s_m[x][col] - use);
+                }
+                put(col, d4, v, M, L);
             }
         }
         if (a.direct > 1) {

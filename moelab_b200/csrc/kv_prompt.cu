@@ -29,6 +29,10 @@
 // product: such a group enters as zeros, and the rows that see its key are marked and written as NaN. Likewise keys and
 // queries, so that no score is NaN.
 //
+// Keys or values too far apart for the tile's power of two (KV_SPREAD) make the CTA's rows go through kv_exact as well, in fp32:
+// the large ones may be later tokens', or have no weight, and would round the others away. Finding out costs 1% (4096 tokens 181
+// -> 183 us); with values of ordinary models it does not happen.
+//
 // Every wait is bounded: after its limit the kernel records MOEB_DEVERR_TIMEOUT, its roles stop, TMEM is released.
 #include "kv.cuh"
 
@@ -69,6 +73,7 @@ struct PrShared {
     float vun;                 // 2^e of O at the end
     uint32_t tmem;
     int b, tile, fail;
+    int uneven;                // a group of K or V too far below the largest for fp16
 };
 
 MOEB_DEV float ex2p(float x) {
@@ -190,12 +195,6 @@ MOEB_DEV PrKeys pr_keys(const KvAttnArgs &a, int pmin, int pmax) {
 }
 MOEB_DEV int pr_tok(const PrKeys &k, int i) { return (i < k.ns ? i : (k.lo >> 7) + i - k.ns) << 7; }
 
-// first value of the 4 that physical half-word u of a row holds (K, and Q with it, and V's columns of O keep this order)
-template <int FMT, int D>
-MOEB_DEV int pr_dim(int u) {
-    return FMT == FMT_Q4 ? 64 * ((u >> 1) % (D / 64)) + 8 * ((u >> 1) / (D / 64)) + 4 * (u & 1) : 32 * (u % (D / 32)) + 4 * (u / (D / 32));
-}
-
 // a code word of 8 values to fp16, in the word's order; q4: s2 / b2 scale and bias, MXFP4: s2 / b2 the scales of the word's
 // two half-words
 template <int FMT>
@@ -240,17 +239,23 @@ MOEB_DEV unsigned pr_byte(unsigned x) {
     return (x | x >> 12) & 0xFFu;
 }
 
-// Largest magnitude (bits) that a row's parameters allow, NaN groups apart; nan: which groups are NaN.
+// Largest magnitude (bits) that a row's parameters allow, NaN groups apart; nan: which groups are NaN; low: the smallest group's
+// less KV_ZERO, groups below that wrapping to the top (they count as zeros).
 template <int FMT, int NG>
-MOEB_DEV uint32_t pr_top(const float (&s)[NG], const float (&b)[NG], unsigned &nan) {
+MOEB_DEV uint32_t pr_top(const float (&s)[NG], const float (&b)[NG], unsigned &nan, uint32_t &low) {
     uint32_t top = 0;
     nan = 0;
+    low = ~0u;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         const float x = FMT == FMT_Q4 ? fmaxf(fabsf(b[g]), fabsf(fmaf(15.f, s[g], b[g]))) : 6.f * s[g];
         const uint32_t u = __float_as_uint(x);
-        if (u < 0x7f800000u && s[g] == s[g]) top = max(top, u);
-        else nan |= 1u << g;
+        if (u < 0x7f800000u && s[g] == s[g]) {
+            top = max(top, u);
+            low = min(low, u - KV_ZERO);
+        } else {
+            nan |= 1u << g;
+        }
     }
     return top;
 }
@@ -331,8 +336,8 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
             bb[g] = FMT == FMT_Q4 ? bf16hi(par[FMT == FMT_Q4 ? g : 0]) : 0.f;
         }
         unsigned nan;
-        uint32_t top = pr_top<FMT, NG>(s, bb, nan);
-        if (id < 0) top = 0;  // zeros (MXFP4: codes of zero)
+        uint32_t low, top = pr_top<FMT, NG>(s, bb, nan, low);
+        if (id < 0) top = 0, low = ~0u;  // zeros (MXFP4: codes of zero)
         const unsigned hole = __ballot_sync(0xffffffffu, id == -2);
         id = id1;
         fetch_par(j + 1, id);  // of the next tile; what this one needs is in s and bb
@@ -355,6 +360,7 @@ MOEB_DEV void pr_feed(const KvAttnArgs &a, PrShared &sh, unsigned char *sm, cons
                 vlim = (e + 6u) << 23;
             }
             mul = vmul;
+            if (low < (uint32_t)max((int)vlim - ((KV_SPREAD + 6) << 23) - (int)KV_ZERO, 0)) sh.uneven = 1;
             uint32_t s2[NG], b2[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
@@ -528,7 +534,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         if (lane == 0) {
             sh.b = b;
             sh.tile = at;
-            sh.fail = 0;
+            sh.fail = sh.uneven = 0;
         }
     }
     __syncthreads();
@@ -566,7 +572,8 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // ---- queries: fp16 after a power of two per row (the largest value near 2^8), K's order of words, swizzled. D / 8
+    // ---- queries: fp16 after a power of two per row (the largest value near 2^8), K's order of values (kv_dim; V's columns of O
+    // keep it too), swizzled. D / 8
     // lanes have a row (one word of 8 values each), so that the loads are whole lines.
     if (warp < 16) {
         constexpr int LR = D / 8, RW = 32 / LR;  // lanes per row, rows per load
@@ -579,8 +586,8 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             if (R < NR) {
                 const int ri = R / a.Gq;
                 const uint16_t *src = a.q + (r0 + ri) * a.q_row + (h * a.Gq + R - ri * a.Gq) * a.q_head;
-                const uint2 lo = *reinterpret_cast<const uint2 *>(src + pr_dim<FMT, D>(2 * x));
-                const uint2 hi = *reinterpret_cast<const uint2 *>(src + pr_dim<FMT, D>(2 * x + 1));
+                const uint2 lo = *reinterpret_cast<const uint2 *>(src + kv_dim<FMT, D>(2 * x));
+                const uint2 hi = *reinterpret_cast<const uint2 *>(src + kv_dim<FMT, D>(2 * x + 1));
                 w[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
             }
         }
@@ -795,7 +802,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             }
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-                const int d = sub ? pr_dim<FMT, D>((D / 2 + x + i) / 4) : pr_dim<FMT, D>((x + i) / 4), g = d / (FMT == FMT_Q4 ? 64 : 32);
+                const int d = sub ? kv_dim<FMT, D>((D / 2 + x + i) / 4) : kv_dim<FMT, D>((x + i) / 4), g = d / (FMT == FMT_Q4 ? 64 : 32);
                 float y[4];
                 const bool nanv = (poison >> g) & 1u;
 #pragma unroll
@@ -827,6 +834,26 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             else if (a.lse) a.lse[orow] = Ls == 0.f ? -INFINITY : (sum_m + log2f(Ls)) * 0.6931471805599453f;
         }
         fence_before();
+        // ---- a tile with groups too far apart for fp16: the rows that this warp stored once more, in fp32. The feeders set the
+        // mark before their tiles were full. No barrier below: after a timeout the warps may find it set or not
+        asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
+        if (*reinterpret_cast<volatile int *>(&sh.uneven)) {
+            const int Ru = R0 + t * 128 + (warp & 3) * 32 + 16 * sub;
+#pragma unroll 1
+            for (int i = 0; i < 16 && Ru + i < NR; ++i) {
+                const int xi = (Ru + i) / a.Gq, xh = h * a.Gq + Ru + i - xi * a.Gq;
+                const KvSum x = kv_exact<FMT, D>(a, b, h, a.q + (r0 + xi) * a.q_row + xh * a.q_head, p0 + xi, k0, k1, keys.ns, (keys.lo >> 7) - keys.ns);
+                if (lane >= D / 4) continue;
+                const size_t xrow = (size_t)(r0 + xi) * a.H + xh;
+                if (!part) {
+                    kv_finish<D>(a, r0 + xi, xh, kv_dim<FMT, D>(lane) / 4, x.v, x.M, x.L);
+                    continue;
+                }
+                *reinterpret_cast<float4 *>(part + ((size_t)sp * a.s.T * a.H + xrow) * D + kv_dim<FMT, D>(lane)) = x.v;
+                if (lane == 0)
+                    reinterpret_cast<float2 *>(part + (size_t)ns * a.s.T * a.H * D)[(size_t)sp * a.s.T * a.H + xrow] = make_float2(x.M, x.L);
+            }
+        }
     }
     __syncthreads();
     if (threadIdx.x == 0 && sh.fail) atomicOr(a.c.err, ERR_TIMEOUT);

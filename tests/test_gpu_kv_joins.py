@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from kv_helpers import Batch, check
+from kv_helpers import U_BF16, U_FP16, Batch, check, stored
 from moelab_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
@@ -18,6 +18,59 @@ FMTS = ("q4", "mxfp4")
 def attend(b, c, **kw):
     kw.setdefault("max_q", max([1] + list(b.rows)))
     return ops.kv_attention(b.q, c, b.table, b.lens_t, cu=b.cu, **kw)
+
+
+def reference(b, scale=None, window=0, sinks=0, sink_logits=None):
+    """(y, bound, lse) in float64, and per row only from what the row sees.
+
+    The bound, with A = sum_j p_j |v_j| over the softmax's weights p: the result is rounded to bf16 (2^-8 of it). Values may be
+    rounded to fp16 (2^-11 of A); so may weights, times A again with MXFP4 (codes are exact), and for int4 times
+    sum_j p_j 2 max_group |v_j|, as a weight scales s code <= 15 s and s <= 2 / 15 of the group's largest magnitude. A key may be
+    rounded to fp16, which moves its score by 2^-11 |scale| sum |q| |k|; the score's own sums are fp32, for int4 over terms as
+    large as the group's largest |k| (2^-20 of sum_g |q|_1 2 max_group |k|, two dozen roundings of 2^-24). A score moved by e
+    moves the weighted mean by 2 e A at most. fp32 sums and exponentials: 2^-15 of A."""
+    scale = b.D ** -0.5 if scale is None else scale
+    G = b.H // b.Hkv
+    y = torch.zeros(b.T, b.H, b.D, dtype=torch.float64)
+    bound, lse = torch.zeros_like(y), torch.full((b.T, b.H), -math.inf, dtype=torch.float64)
+    ks, vs = (stored(x, b.fmt).double().to(b.device) for x in (b.k, b.v))
+    gs = 64 if b.fmt == "q4" else 32
+    group = lambda x: x.abs().nan_to_num().unflatten(-1, (-1, gs)).amax(-1, keepdim=True).expand(-1, -1, gs).flatten(1)
+    q, at = b.q.double(), 0
+    for s, (L, n) in enumerate(zip(b.lens, b.rows)):
+        pos, key = torch.arange(L - n, L, device=b.device), torch.arange(max(L, 0), device=b.device)
+        see = key[None] <= pos[:, None]
+        if window:
+            see &= (key[None] > pos[:, None] - window) | (key[None] < sinks)
+        for h in range(b.H):
+            kk, vv, qq = ks[s, :L, h // G], vs[s, :L, h // G], q[at:at + n, h]
+            e = (U_FP16 * qq.abs() @ kk.abs().nan_to_num().T + 2.0 ** -19 * qq.abs() @ group(kk).T) * abs(scale)
+            e = e.masked_fill(~see, 0.0).amax(-1, keepdim=True) if L else torch.zeros(n, 1, device=b.device, dtype=torch.float64)
+            x = (qq @ kk.T * scale).masked_fill(~see, -math.inf)
+            if sink_logits is not None:
+                x = torch.cat([x, sink_logits[h].double().to(b.device).expand(n, 1)], -1)
+            if x.shape[1] == 0:
+                continue
+            m = x.amax(-1, keepdim=True)
+            m = torch.where(m == -math.inf, 0.0, m)
+            p = torch.exp(x - m)
+            tot = p.sum(-1, keepdim=True)
+            p = (p / torch.where(tot == 0, 1.0, tot))[:, :L]
+            seen = lambda v: torch.where((p != 0)[:, :, None], p[:, :, None] * v[None], 0.0).sum(1) if v.isnan().any() else p @ v
+            out, A = seen(vv), p @ vv.abs().nan_to_num()
+            Ap = p @ group(vv) * 2 if b.fmt == "q4" else A
+            y[at:at + n, h] = out.cpu()
+            bound[at:at + n, h] = (U_BF16 * out.abs() + ((2 * e + U_FP16 + 2.0 ** -15) * A + U_FP16 * Ap) * (1 + U_BF16)).cpu() + 1e-36
+            lse[at:at + n, h] = (m + torch.log(tot)).squeeze(-1).cpu()
+        at += n
+    return y, bound, lse
+
+
+def within(y, ref, bound, what=""):
+    y = y.double().cpu()
+    assert torch.isfinite(y).all(), what
+    off = (y - ref).abs() - bound
+    assert (off <= 0).all(), (what, int((off > 0).sum()), (off / bound).max().item(), (off > 0).nonzero()[:4].tolist())
 
 
 # ------------------------------------------------------------------ queries that are not finite
@@ -55,3 +108,58 @@ def test_queries_that_are_not_finite_give_nan_and_touch_no_other_row(fmt, n, L, 
     rest = torch.ones(2 * n, 4, dtype=torch.bool)
     rest[n - 1, 1] = False
     check(y.cpu()[rest], ref[rest], bound[rest])
+
+
+# ------------------------------------------------------------------ keys and values of sizes far apart
+@pytest.mark.parametrize("fmt,D", [("q4", 64), ("q4", 128), ("mxfp4", 64), ("mxfp4", 128)])
+@pytest.mark.parametrize("n,L", [(1, 300), (3, 300), (3, 9000), (150, 300), (150, 9000)])
+@pytest.mark.parametrize("what", ("key", "value", "unattended", "first"))
+@pytest.mark.parametrize("power", (13, 30, 60))
+def test_sizes_far_apart(fmt, D, n, L, what, power):
+    """A key or value 2^power times the others' size that some rows do not see (the last token's) or give no weight (a token with
+    a score far below the rest), or others that are that much larger than the first token's, the only one that row 0 sees: the
+    other rows' results are as accurate as without it."""
+    if what == "first":
+        L = n
+    b = Batch([L], [n], 4, 1, D, fmt, page=32, seed=53)
+    far = 2.0 ** power
+    rows = torch.arange(n)
+    if what == "key":
+        b.k[0, L - 1] = (b.k[0, L - 1].float() * far).to(torch.bfloat16)
+        rows = rows[:-1]  # the last row's scores are that large too
+    elif what == "value":
+        b.v[0, L - 1] = (b.v[0, L - 1].float() * far).to(torch.bfloat16)
+    elif what == "unattended":
+        b.q = b.q.abs()
+        b.k[0, 5] = -14.0 * (128 / D) ** 0.5  # weight below 2^-100
+        b.v[0, 5] = (b.v[0, 5].float() * far).to(torch.bfloat16)
+    else:
+        b.v[0, 0] = (b.v[0, 0].float() / far).to(torch.bfloat16)
+        b.k[0, 0] = (b.k[0, 0].float() / far).to(torch.bfloat16)
+    c = b.cache(ops)
+    y, lse = attend(b, c, return_lse=True)
+    ref, bound, lref = reference(b)
+    if len(rows):
+        within(y[rows], ref[rows], bound[rows])
+        assert (lse[rows].double().cpu() - lref[rows]).abs().max() < 5e-3
+    assert c.read_error() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n", (1, 3, 150))
+def test_sizes_far_apart_in_window_and_batch(fmt, n):
+    """The same beside windows, first tokens, sink logits and ordinary sequences, NaN where no row looks; the calls repeat."""
+    b = Batch([700, 9000, 431], [n, n, n], 8, 2, 64, fmt, page=16, seed=54, pad=2)
+    b.v[1, 8990, 0] = (b.v[1, 8990, 0].float() * 2.0 ** 40).to(torch.bfloat16)
+    b.v[2, 0] = (b.v[2, 0].float() * 2.0 ** -30).to(torch.bfloat16)
+    b.k[0, 690, 1] = 0.0
+    b.v[0, 100] = math.nan  # out of the window of every row
+    logits = torch.linspace(-3, 3, 8, device="cuda")
+    c = b.cache(ops)
+    ref, bound, lref = reference(b, window=380, sinks=3, sink_logits=logits)
+    out = torch.full((b.T, 8, 64), 9.0, dtype=torch.bfloat16, device="cuda")
+    y, lse = attend(b, c, window=380, sinks=3, sink_logits=logits, return_lse=True, out=out)
+    within(y[:-2], ref[:-2], bound[:-2])
+    assert (y[-2:] == 9).all()
+    assert (lse[:-2].double().cpu() - lref[:-2]).abs().max() < 5e-3
+    assert torch.equal(attend(b, c, window=380, sinks=3, sink_logits=logits)[:-2], y[:-2])
