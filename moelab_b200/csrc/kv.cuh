@@ -208,7 +208,8 @@ MOEB_DEV float4 kv_four(const void *codes, const void *pars, size_t row, int u) 
 }
 // A row's attention in fp32 throughout, by one warp: its keys in blocks [k0, k1) of 128, block k from token 128 k on for k < ns
 // and 128 (k + skip) for the others. For keys and values whose sizes are too far apart for the tensor cores' fp16 operands (see
-// KV_SPREAD); ordinary ones never come here, so it is written to be short and every key's score is a sum over the lanes. v: values kv_dim(lane) .. + 3 of the sum of weights 2^(score - M) times
+// KV_SPREAD) and for scores of sizes that no softmax has (KV_FAR); ordinary ones never come here, so it is written to be short
+// and every key's score is a sum over the lanes. v: values kv_dim(lane) .. + 3 of the sum of weights 2^(score - M) times
 // values, L: the sum of the weights, in every lane.
 struct KvSum {
     float4 v;
@@ -267,6 +268,10 @@ MOEB_DEV KvSum kv_exact(const KvAttnArgs &a, int b, int h, const uint16_t *q, in
 // count as zeros), make a run of keys uneven: kv_exact has it. The largest may be a key's that the row does not see, or hardly
 // looks at, so that what it would round away can be all of the row's result.
 constexpr int KV_SPREAD = 14;
+// A weight is 2^(score * scale - m) in one fused product, m being a score * scale that was rounded: off by 2^-8 at this size of m
+// (in powers of two, as the fp32 score itself), and by whole powers above 2^24, where the largest weight could pass any range.
+// kv_exact subtracts what it has rounded.
+constexpr float KV_FAR = 65536.f;
 constexpr uint32_t KV_ZERO = 7u << 23;  // bits of 2^-120
 template <int FMT, int D>
 __global__ void k_kv_write(const KvWriteArgs a);

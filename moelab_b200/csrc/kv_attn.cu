@@ -770,10 +770,12 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
         }
 
         // ---- the warps' sums join in shared memory; m becomes what the weights are relative to
+        bool far = false;  // scores so large that the product's rounding in m is one of whole powers of two in the weights
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                far |= fabsf(m[nt][e]) > KV_FAR && m[nt][e] != -INFINITY;
                 m[nt][e] -= vexp;
 #pragma unroll
                 for (int x = 4; x <= 16; x <<= 1) {
@@ -791,7 +793,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
         }
         // a group of values too far below the largest for fp16? int4: scales of 2^-11 of the largest have a bias of 2^-14 of its 15
         const int under = (int)(vlim >> 23) - (KV_SPREAD + 6 - (FMT == FMT_Q4 ? 3 : 0)) - (int)(KV_ZERO >> 23);
-        const bool uneven = __syncthreads_or(under > 0 && low < (FMT == FMT_Q4 ? (uint32_t)under << 24 : (uint32_t)under));
+        const bool uneven = __syncthreads_or(far || (under > 0 && low < (FMT == FMT_Q4 ? (uint32_t)under << 24 : (uint32_t)under)));
         const bool whole = kr0 == 0 && kr1 == qr.nb;
         float *pt = part + ((size_t)blockIdx.x * 2 + (us >= segr ? 0 : 1)) * (NC * (D + 2));
         auto put = [&](int col, int d4, float4 v, float M, float L) {  // the run's sums of 4 values of a column

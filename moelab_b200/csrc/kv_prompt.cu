@@ -775,6 +775,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         if (poison >> 31 && (qmul >= 0.f || l != 0.f)) l = __uint_as_float(0x7fffffffu);  // a query that sees nothing is not looked at
         // ---- the rows' results (m is off by P_OFF against the weights' sum: undone here)
         const float M = l == 0.f ? -INFINITY : m - P_OFF;
+        const bool far = __any_sync(0xffffffffu, fabsf(m) > KV_FAR && m != LOW);  // the same for both warps of the rows
         float mul = nk > 0 ? sh.vun : 0.f, Ls = l, sum_m = M;
         if (!part) {
             if (a.sink_logits && have) {
@@ -834,10 +835,10 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             else if (a.lse) a.lse[orow] = Ls == 0.f ? -INFINITY : (sum_m + log2f(Ls)) * 0.6931471805599453f;
         }
         fence_before();
-        // ---- a tile with groups too far apart for fp16: the rows that this warp stored once more, in fp32. The feeders set the
+        // ---- a tile with groups too far apart for fp16, or scores that are too large: the rows that this warp stored once more, in fp32. The feeders set the
         // mark before their tiles were full. No barrier below: after a timeout the warps may find it set or not
         asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
-        if (*reinterpret_cast<volatile int *>(&sh.uneven)) {
+        if (far || *reinterpret_cast<volatile int *>(&sh.uneven)) {
             const int Ru = R0 + t * 128 + (warp & 3) * 32 + 16 * sub;
 #pragma unroll 1
             for (int i = 0; i < 16 && Ru + i < NR; ++i) {

@@ -163,3 +163,26 @@ def test_sizes_far_apart_in_window_and_batch(fmt, n):
     assert (y[-2:] == 9).all()
     assert (lse[:-2].double().cpu() - lref[:-2]).abs().max() < 5e-3
     assert torch.equal(attend(b, c, window=380, sinks=3, sink_logits=logits)[:-2], y[:-2])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("n,L", [(1, 300), (3, 9000), (150, 300), (150, 9000)])
+@pytest.mark.parametrize("size", (2.0 ** 10, -2.0 ** 16, 2.0 ** 20, -2.0 ** 60, 2.0 ** 100))
+def test_scores_of_any_size_pick_the_largest(fmt, D, n, L, size):
+    """Keys of one value each, from 1 to 8 or -1 to -8, one of them larger: the scores differ by at least `size` and more than
+    their rounding, so the result is that key's value."""
+    b = Batch([L], [n], 4, 1, D, fmt, page=32, seed=55)
+    g = torch.Generator().manual_seed(7)
+    best = min(L - n, 130)
+    k = torch.randint(1, 9, (L,), generator=g).float()
+    k[best] = 12.0
+    b.k[0, :, 0] = (k * (1 if size > 0 else -1))[:, None].to(torch.bfloat16)
+    b.q[:] = size
+    c = b.cache(ops)
+    y, lse = attend(b, c, return_lse=True)
+    want = stored(b.v, fmt)[0, best, 0].double()
+    assert torch.isfinite(y).all()
+    assert ((y.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -11 * want.abs().max()).all()
+    top = 12.0 * abs(size) * D ** 0.5
+    assert ((lse.double() - top).abs() <= 2.0 ** -20 * top).all()
