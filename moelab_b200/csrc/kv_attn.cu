@@ -50,6 +50,7 @@ constexpr int FW = 4, FT = 32 * FW;  // warps per CTA, threads
 constexpr int FS = 3;                // ring stages (4: two CTAs per SM instead of three, 96 us for the batch above)
 constexpr int FB = 32 * FW;          // keys per block
 constexpr int FR = 2;                // blocks that a run costs besides its own
+constexpr float LEAST = 1.2e-38f;    // a column's scale at least
 
 template <int FMT, int D>
 struct Few {
@@ -408,6 +409,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
                 const float down = t16 < 0x7f80u ? __uint_as_float((uint32_t)(254 + UP - e) << 23) : __uint_as_float(0x7fffffffu);
                 // what undoes it; int4: and 2^24 for the codes, taken out of qsum below
                 mul *= __uint_as_float((uint32_t)(e - UP) << 23) * (FMT == FMT_Q4 ? 16777216.f : 1.f);
+                if (t16 == 0) mul = 1.f;
 #pragma unroll
                 for (int j = 0; j < D / 32; ++j) {
                     uint32_t ww[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                cs[nt][e] = fmaxf(__shfl_sync(0xffffffffu, mul, 8 * c + 4 * e), 1.2e-38f);  // above zero: a hidden -inf stays -inf
+                cs[nt][e] = fmaxf(__shfl_sync(0xffffffffu, mul, 8 * c + 4 * e), LEAST);  // above zero: a hidden -inf stays -inf
                 const int ce = nt * 8 + 2 * c + e, ie = kv_div(ce, a.Gdiv);
                 pos[nt][e] = ie < qr.n ? p0 + ie : -1;  // a column without a row sees nothing
             }
@@ -775,7 +777,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                far |= fabsf(m[nt][e]) > KV_FAR && m[nt][e] != -INFINITY;
+                far |= (fabsf(m[nt][e]) > KV_FAR && m[nt][e] != -INFINITY) || cs[nt][e] == LEAST || cs[nt][e] > 1e38f;  // or no such power for q
                 m[nt][e] -= vexp;
 #pragma unroll
                 for (int x = 4; x <= 16; x <<= 1) {

@@ -186,3 +186,28 @@ def test_scores_of_any_size_pick_the_largest(fmt, D, n, L, size):
     assert ((y.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -11 * want.abs().max()).all()
     top = 12.0 * abs(size) * D ** 0.5
     assert ((lse.double() - top).abs() <= 2.0 ** -20 * top).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n", (1, 3, 150))
+@pytest.mark.parametrize("power", (121, 126, -119, -124))
+def test_queries_at_the_ends_of_the_range(fmt, n, power):
+    """Queries of 2^power and keys that make ordinary scores of them, where the cache has such keys (int4's are zero below 2^-24,
+    then all weights are the same); rows of zeros beside them, and with 2^126 times more than 4 an infinite query, whose row is NaN.
+    The scale's half of the exponents is a user's to choose too."""
+    b = Batch([300], [n], 4, 2, 64, fmt, page=32, seed=56)
+    b.k = (b.k.float() * 2.0 ** -power).to(torch.bfloat16)
+    b.q = (b.q.float() * 2.0 ** power).to(torch.bfloat16)
+    b.q[0, 0] = 0.0
+    c = b.cache(ops)
+    ref, bound, lref = reference(b)
+    y, lse = attend(b, c, return_lse=True)
+    fine = torch.isfinite(b.q).all(-1).cpu()
+    within(y.cpu()[fine], ref[fine], bound[fine])
+    assert (lse.double().cpu() - lref)[fine].abs().max() < 5e-3
+    assert y.cpu()[~fine].isnan().all() and lse.cpu()[~fine].isnan().all()
+    b.k = (b.k.float() * 2.0 ** power).to(torch.bfloat16)
+    c = b.cache(ops)
+    if abs(power) < 120:  # the scale is a normal fp32 number
+        ref, bound, lref = reference(b, scale=2.0 ** -power / 8)
+        within(attend(b, c, scale=2.0 ** -power / 8), ref, bound)
