@@ -166,7 +166,8 @@ Plan plan_of(int T, int B, int P, int page_size, int H, int Hkv, int D, int max_
     // sequences have T / B rows; with it, and more than one sequence, both kinds may be in the call: over up to 1024 keys
     // the kernel for many rows takes them all (8 key tiles, 18 to 26 us, against two more launches).
     p.only = cols <= 16;
-    p.few = p.only ? (int)cols : cu && B > 1 && seen(max_q) > 1024 ? 16 : 0;
+    // With more than 16 query heads per KV head no row fits them: one launch, no workspace for the other kernel.
+    p.few = p.only ? (int)cols : cu && B > 1 && Gq <= 16 && seen(max_q) > 1024 ? 16 : 0;
     if (p.few) {
         p.nc = cols <= 8 ? 8 : 16;
         // Up to 4 blocks of 128 keys one after the other cost as much as a second launch to join parts of them: one CTA has

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from moelab_b200 import ops
+from moelab_b200 import _lib, ops
 
 
 class Fake:
@@ -21,3 +21,12 @@ def test_tensors_that_need_gradients_are_refused():
             call(grad.detach())
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
             call(grad)
+
+
+def test_no_kernel_for_few_rows_where_no_row_fits_it():
+    """More than 16 query heads per KV head: a call whose row tiles fill the GPU needs no workspace, with cu or without."""
+    size = _lib.load().moeb_kv_attention_workspace_bytes  # T, B, P, page_size, H, kv_heads, head_dim, max_q, window, sinks, with_cu
+    for cu in (0, 1):
+        assert size(64, 64, 512, 64, 8 * 20, 8, 128, 1, 0, 0, cu) == 0
+    assert size(128, 64, 512, 64, 8 * 16, 8, 128, 2, 0, 0, 0) == 0
+    assert size(128, 64, 512, 64, 8 * 16, 8, 128, 2, 0, 0, 1) > 0  # some sequences may have one row: they fit
