@@ -20,7 +20,7 @@ def attend(b, c, **kw):
     return ops.kv_attention(b.q, c, b.table, b.lens_t, cu=b.cu, **kw)
 
 
-def reference(b, scale=None, window=0, sinks=0, sink_logits=None):
+def reference(b, scale=None, window=0, sinks=0, sink_logits=None, steep=False):
     """(y, bound, lse) in float64, and per row only from what the row sees.
 
     The bound, with A = sum_j p_j |v_j| over the softmax's weights p: the result is rounded to bf16 (2^-8 of it). Values may be
@@ -28,7 +28,13 @@ def reference(b, scale=None, window=0, sinks=0, sink_logits=None):
     sum_j p_j 2 max_group |v_j|, as a weight scales s code <= 15 s and s <= 2 / 15 of the group's largest magnitude. A key may be
     rounded to fp16, which moves its score by 2^-11 |scale| sum |q| |k|; the score's own sums are fp32, for int4 over terms as
     large as the group's largest |k| (2^-20 of sum_g |q|_1 2 max_group |k|, two dozen roundings of 2^-24). A score moved by e
-    moves the weighted mean by 2 e A at most. fp32 sums and exponentials: 2^-15 of A."""
+    moves the weighted mean by 2 e A at most. fp32 sums and exponentials: 2^-15 of A.
+
+    steep: scores so far apart that weights become fp16 subnormals, whose roundings are 2^-25 and not relative. With many rows the
+    weights are 2^6 times p / max p or more, so a key's is off by 2^-31 max p; with few they are scaled by the values' power of
+    two, which puts the largest scale so far at 2^8 or more, so weight times value is off by 2^-33 max p max |v| 6 at most (codes
+    of E2M1 up to 6; int4's are 15 times their scale and those 2 / 15 max |v|). Over n keys: n 2^-30 max p max |v| covers both.
+    It shows in values that the row's heaviest keys have as zero."""
     scale = b.D ** -0.5 if scale is None else scale
     G = b.H // b.Hkv
     y = torch.zeros(b.T, b.H, b.D, dtype=torch.float64)
@@ -59,6 +65,8 @@ def reference(b, scale=None, window=0, sinks=0, sink_logits=None):
             seen = lambda v: torch.where((p != 0)[:, :, None], p[:, :, None] * v[None], 0.0).sum(1) if v.isnan().any() else p @ v
             out, A = seen(vv), p @ vv.abs().nan_to_num()
             Ap = p @ group(vv) * 2 if b.fmt == "q4" else A
+            if steep:
+                Ap = Ap + see.sum(-1, keepdim=True) * 2.0 ** -30 / U_FP16 * p.amax(-1, keepdim=True) * vv.abs().max()
             y[at:at + n, h] = out.cpu()
             bound[at:at + n, h] = (U_BF16 * out.abs() + ((2 * e + U_FP16 + 2.0 ** -15) * A + U_FP16 * Ap) * (1 + U_BF16)).cpu() + 1e-36
             lse[at:at + n, h] = (m + torch.log(tot)).squeeze(-1).cpu()
@@ -211,3 +219,76 @@ def test_queries_at_the_ends_of_the_range(fmt, n, power):
     if abs(power) < 120:  # the scale is a normal fp32 number
         ref, bound, lref = reference(b, scale=2.0 ** -power / 8)
         within(attend(b, c, scale=2.0 ** -power / 8), ref, bound)
+
+
+# ------------------------------------------------------------------ joined parts
+def joined(b, **kw):
+    """The call's workspace: parts are joined where it is not empty."""
+    return _lib.load().moeb_kv_attention_workspace_bytes(b.T, len(b.lens), b.table.shape[1], b.page, b.H, b.Hkv, b.D, max(b.rows),
+                                                        kw.get("window", 0), kw.get("sinks", 0), 1) > 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("n", (1, 4, 90))
+@pytest.mark.parametrize("kw", [dict(), dict(window=5000), dict(window=5000, sinks=4), dict(window=5003, sinks=300),
+                                dict(window=4700, sinks=4000)])
+def test_joined_parts(fmt, D, n, kw):
+    """Long caches, whose keys several CTAs share: windows and first tokens (a part may end or begin between them), sink logits, lse,
+    a sequence that begins inside the call's rows."""
+    b = Batch([9100, n, 12007], [n] * 3, 8, 1 if n == 90 else 2, D, fmt, page=64, seed=60, peak=2.0)
+    c = b.cache(ops)
+    assert joined(b, **kw)
+    ref, bound, lref = reference(b, **kw)
+    y, lse = attend(b, c, return_lse=True, **kw)
+    within(y, ref, bound)
+    assert (lse.double().cpu() - lref).abs().max() < 5e-3
+    logits = torch.linspace(-4, 9, 8, device="cuda")
+    logits[2] = -math.inf
+    ref, bound, lref = reference(b, sink_logits=logits, **kw)
+    y, lse = attend(b, c, return_lse=True, sink_logits=logits, **kw)
+    within(y, ref, bound)
+    assert (lse.double().cpu() - lref).abs().max() < 5e-3
+    if n > 1:  # rows before the second sequence's start
+        lens = b.lens_t.clone()
+        lens[1] = n - 2
+        y2, lse2 = ops.kv_attention(b.q, c, b.table, lens, cu=b.cu, max_q=n, return_lse=True, sink_logits=logits, **kw)
+        assert torch.equal(y2[:n], y[:n]) and torch.equal(y2[2 * n:], y[2 * n:]) and torch.equal(lse2[2 * n:], lse[2 * n:])
+        # lse is the logit times log2(e) and back times ln(2): two rounded constants and two rounded products, 2^-24 each
+        assert not y2[n:n + 2].any() and torch.allclose(lse2[n:n + 2], logits.expand(2, 8), rtol=2 ** -22, atol=0)
+    assert c.read_error() == 0
+
+
+@pytest.mark.parametrize("fmt,D", [("q4", 128), ("mxfp4", 64), ("mxfp4", 128)])  # rows of more than one group
+@pytest.mark.parametrize("n", (1, 3, 130))
+def test_nan_through_joined_parts(fmt, D, n):
+    """A NaN value makes its group NaN in the rows that see it, a NaN key the whole row, through the joins; other rows, heads and
+    groups are as without."""
+    gs = 64 if fmt == "q4" else 32
+    b = Batch([9000, 8200], [n, n], 4, 2, D, fmt, page=64, seed=61)
+    assert joined(b)
+    ref, bound, _ = reference(b)
+    b.v[0, 4000, 0, 3] = math.nan             # every row of the first sequence, heads 0 and 1
+    b.v[1, 8200 - 1, 1, gs] = math.inf        # the last row of the second, heads 2 and 3
+    b.k[1, 8200 - 1, 0, 1] = math.nan         # the last row, heads 0 and 1
+    c = b.cache(ops)
+    y = attend(b, c).cpu()
+    nan = torch.zeros(2 * n, 4, D, dtype=torch.bool)
+    nan[:n, :2, :gs] = True
+    nan[2 * n - 1, 2:, gs:2 * gs] = True
+    nan[2 * n - 1, :2] = True
+    assert torch.equal(y.isnan(), nan)
+    within(y[~nan], ref[~nan], bound[~nan])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("n,L", [(1, 300), (3, 9000), (150, 300), (90, 9000)])
+@pytest.mark.parametrize("scale", (-0.2, 0.0, -1e-3, 1.5))
+def test_scales_of_any_sign(fmt, D, n, L, scale):
+    b = Batch([L, n], [n, n], 4, 1, D, fmt, page=32, seed=62, peak=0.5)
+    c = b.cache(ops)
+    ref, bound, lref = reference(b, scale=scale, steep=True)
+    y, lse = attend(b, c, scale=scale, return_lse=True)
+    within(y, ref, bound)
+    assert (lse.double().cpu() - lref).abs().max() < 5e-3
