@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
                 }
             }
         }
-        // a group of values too far below the largest for fp16? int4: scales of 2^-11 of the largest have a bias of 2^-14 of its 15
+        // a group of values too far below the largest for fp16? int4: |bias| is compared with the largest scale, an eighth of its own
         const int under = (int)(vlim >> 23) - (KV_SPREAD + 6 - (FMT == FMT_Q4 ? 3 : 0)) - (int)(KV_ZERO >> 23);
         const bool uneven = __syncthreads_or(far || (under > 0 && low < (FMT == FMT_Q4 ? (uint32_t)under << 24 : (uint32_t)under)));
         const bool whole = kr0 == 0 && kr1 == qr.nb;
