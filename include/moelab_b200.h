@@ -257,7 +257,8 @@ int moeb_probe_mma_sync(int warps_per_sm, int iters, double *tflops);
  *   kq, vq  uint32 [pages][kv_heads][page_size][head_dim / 8]   codes, the word order of csrc/kv.cuh
  *   ks, vs  int4: uint32 [pages][kv_heads][page_size][head_dim / 64] (scale | bias << 16)
  *           MXFP4: uint8 [pages][kv_heads][page_size][head_dim / 32] (E8M0)
- *   err     uint32, zero at first: the sticky error word (MOEB_DEVERR_PAGE, MOEB_DEVERR_ROWS)
+ *   err     uint32, zero at first: the sticky error word (MOEB_DEVERR_PAGE, MOEB_DEVERR_ROWS; MOEB_DEVERR_TIMEOUT where a
+ *           wait inside the kernel for many rows ran out: that call's results are not valid)
  * All arrays are device memory, 16-byte aligned; their first contents do not matter (rows that were never written read
  * back as what they hold). The struct itself is host memory and read during the call only.
  *
@@ -295,7 +296,8 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
  * table entries may be anything. q: bf16, strides as moeb_kv_write's k; y: bf16 [T][H][head_dim]; lse: fp32 [T][H], the
  * natural logarithm of the softmax's sum, or NULL. max_q: the most rows that a sequence has in this call (a larger
  * bound costs time only; a sequence with more rows may be passed over, which sets MOEB_DEVERR_ROWS). Scores,
- * statistics and sums are fp32. Keys and values may be any finite bf16, of any sizes beside one another (groups of a
+ * statistics and sums are fp32; the tensor cores take queries, weights and (for many rows) keys and values in fp16 after powers of
+ * two (2^-11 of each). Keys and values may be any finite bf16, of any sizes beside one another (groups of a
  * head more than 2^18 apart take a path that is 20 to 200 times slower; groups below 2^-120 may count as zeros). ws: scratch of moeb_kv_attention_workspace_bytes (for the same arguments; with_cu: cu
  * is given; 0 for many calls), with no first contents and none kept, 16-byte aligned: one call at a time. */
 size_t moeb_kv_attention_workspace_bytes(int T, int B, int P, int page_size, int H, int kv_heads, int head_dim, int max_q,

@@ -74,7 +74,8 @@ MOEB_DEV Q4Group kv_q4_group(const __nv_bfloat162 m) {
     }
     g.scale = scale;
     // q0 = 0: the largest magnitude is below half the smallest scale, every code is 0 and the values are zeros. The weight
-    // quantizer keeps that scale; here it is 0, so that attention, which takes codes less 8, meets nothing to cancel.
+    // quantizer keeps that scale; here it is 0, so that attention, which goes by the parameters where it weighs values' sizes
+    // against one another, meets no scale of 2^-23 that belongs to nothing.
     g.par = bad ? 0x7fff7fffu : q0 == 0.0f ? 0u : (uint32_t)f2bf(scale) | ((uint32_t)f2bf(g.bias) << 16);
     g.inv = bad || q0 == 0.0f ? 0.0f : __frcp_rn(scale);
     return g;

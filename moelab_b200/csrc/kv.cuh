@@ -264,9 +264,9 @@ MOEB_DEV KvSum kv_exact(const KvAttnArgs &a, int b, int h, const uint16_t *q, in
     return {v, M, L};
 }
 // The tensor cores' fp16 operands hold groups of values up to 2^KV_SPREAD apart: the largest is put near 2^8, one 2^18 smaller is
-// near 2^-10 and rounds by 2^-25, 2^-15 of it (fp16's own rounding: 2^-11 of each value). Groups further below the largest, but not below 2^-120 (those may
-// count as zeros), make a run of keys uneven: kv_exact has it. The largest may be a key's that the row does not see, or hardly
-// looks at, so that what it would round away can be all of the row's result.
+// near 2^-10 and rounds by 2^-25, 2^-15 of it (fp16's own rounding: 2^-11 of each value). Groups further below the largest, but
+// not below 2^-120 (those may count as zeros), make a run of keys uneven: kv_exact has it. The largest may be a key's that the
+// row does not see, or hardly looks at, so that what it would round away can be all of the row's result.
 constexpr int KV_SPREAD = 18;
 // A weight is 2^(score * scale - m) in one fused product, m being a score * scale that was rounded: off by 2^-8 at this size of m
 // (in powers of two, as the fp32 score itself), and by whole powers above 2^24, where the largest weight could pass any range.

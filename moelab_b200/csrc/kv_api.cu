@@ -164,7 +164,10 @@ Plan plan_of(int T, int B, int P, int page_size, int H, int Hkv, int D, int max_
     auto seen = [&](long rows) { return window ? std::min(all, (long)window + rows + std::min<long>(sinks, all) + 128 + (sinks ? 128 : 0)) : all; };
     // Sequences whose (row, head) columns fit one or two tensor-core tiles go to the kernel for few rows. Without cu all
     // sequences have T / B rows; with it, and more than one sequence, both kinds may be in the call: over up to 1024 keys
-    // the kernel for many rows takes them all (8 key tiles, 18 to 26 us, against two more launches).
+    // the kernel for many rows takes them all (at most 9 key tiles each, against up to two more launches). Single tokens beside
+    // one piece of 256 rows, 32 heads on 8, D = 128, this against both kernels: 4 in windows of 128 24 / 34 us, 16 36 / 37, 16 over
+    // 1000 keys 59 / 56. It pays while the tiles are about one round of CTAs and loses beyond: 96 over 1000 keys 194 / 125, 96 in
+    // windows of 128 with 64 heads on 8, D = 64, 86 / 42.
     p.only = cols <= 16;
     // With more than 16 query heads per KV head no row fits them: one launch, no workspace for the other kernel.
     p.few = p.only ? (int)cols : cu && B > 1 && Gq <= 16 && seen(max_q) > 1024 ? 16 : 0;

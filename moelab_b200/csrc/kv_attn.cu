@@ -9,10 +9,12 @@
 //   64 sequences of 1 to 8192 tokens, 32 query heads on 8, int4 (306 MB): 86 us with the join, 3.6 TB/s; in its loop over the
 //     blocks the kernel moves 5.9 TB/s (a copy 6.56), the rest is the 2 us until a CTA knows its run, the 5 us until its first
 //     copies are there, CTAs that end between 59 and 78 us (memory is not equally far from all SMs) and the join. Shares of two
-//     sizes, the small ones for CTAs that end early, cost more than they even out (92 us): new CTAs start slowly under load.
-//   one of 200,001 tokens, 64 heads on 4, MXFP4 (109 MB, two column tiles, 8 warps per SM): 52 us, 2.1 TB/s, bound by the
+//     sizes, the small ones for CTAs that end early, cost more than they even out (92 against 85 us): new CTAs start slowly
+//     under load. MXFP4: 88 us
+//   one of 200,001 tokens, 64 heads on 4, MXFP4 (109 MB, two column tiles, 8 warps per SM): 53 us, 2.1 TB/s, bound by the
 //     latencies of one warp's steps: half of the issue slots are taken
-//   one of 1021 tokens, 32 heads on 4, int4: 7.2 us in a graph
+//   one of 1021 tokens, 32 heads on 4, int4: 7.4 us in a graph
+//   16 of 8192 with 4 drafted rows each, 32 heads on 8 (two column tiles), int4: 70 us, 2.2 TB/s
 //
 // Work split: the visible keys of every (sequence, KV head) are cut into blocks of 128; all blocks of the call in a row are
 // dealt to the CTAs in equal runs, so uneven lengths cost nothing and the host needs to know none of them (a captured
@@ -194,8 +196,8 @@ MOEB_DEV long few_start(long W, unsigned c, unsigned n) {
 
 }  // namespace
 
-// CTAs per SM: as many as registers allow without spills. Heads of 64 with one column tile: four (126 registers) and not three
-// make many short windows faster (512 tokens in windows of 128, 64 heads on 8: 50 -> 42 us) and cost long caches nothing.
+// CTAs per SM: as many as registers allow without spills in the loop. Heads of 64 with one column tile: four (126 registers) and not three
+// make many short windows faster (512 tokens in windows of 128, 64 heads on 8: 50 -> 42 us, 44 since values are looked over) and cost long caches nothing.
 // ws: prefix[B + 1] int32 (blocks before each sequence), then 2 partials per CTA: NC rows of D sums, NC (max, sum).
 template <int FMT, int D, int NT>
 __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 : 2) k_kv_attn_few(const KvAttnArgs a, int *pre, float *part) {

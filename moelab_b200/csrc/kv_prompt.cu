@@ -16,14 +16,14 @@
 //     swizzle
 //   warps 24, 25: issue the products of row tile 0, 1 (26, 27 fill the warpgroup)
 // Registers: 896 x 72 at launch; the softmax warpgroups go to 80, those of the products to 40 (64512 in all).
-// Measured (int4 or MXFP4 within 2%; causal products counted once): 4096 tokens of 32 heads on 4, D = 128: 185 us, 740 TFLOP/s;
-// 1000 rows of 64 heads on 32,001 keys of 8, D = 64: 943 us, 550 TFLOP/s, where the exponentials' unit alone takes 620 us (16 per
-// SM and cycle; a quarter of them as polynomials on the FMA units gave nothing once the loop was lean); 8191 tokens of 32 heads
-// on 8 in a window of 2048 and 4 first tokens: 356 us. Bound by the softmax warps: two thirds of the issue slots are taken, 55%
-// of the exponentials' unit (D = 64), and four such warps per scheduler do not cover all waits between a half's steps. Neither
-// the products (a fourth of them left out: no change) nor dequantizing (1%) are what limits.
-// fp16 and not bf16 operands: both formats' values, and P, would lose 2^-9 to bf16, as much as the result's own rounding;
-// fp16 keeps 2^-12. Its range is kept by powers of two: one per query row, one per K tile (both go into the softmax's
+// Measured (int4 or MXFP4 within 2%; causal products counted once; calls in a row in a graph, call by call in brackets): 4096
+// tokens of 32 heads on 4, D = 128: 183 (194) us, 750 TFLOP/s; 1000 rows of 64 heads on 32,001 keys of 8, D = 64: 955 (959) us,
+// 540 TFLOP/s (its 2.0e9 exponentials need 433 us of their unit at 1965 MHz, 16 per SM and cycle; a quarter of them as
+// polynomials on the FMA units gave nothing); 8191 tokens of 32 heads on 8 in a window of 2048 and 4 first tokens: 358 (366) us.
+// Bound by the softmax warps: 65% to 67% of the issue slots are taken, 43% (D = 128) to 55% (D = 64) of the exponentials' unit, 39%
+// to 27% of the tensor cores, and four such warps per scheduler do not cover all waits between a half's steps.
+// fp16 and not bf16 operands: both formats' values, and P, would lose 2^-8 to bf16, as much as the result's own rounding;
+// fp16 keeps 2^-11. Its range is kept by powers of two: one per query row, one per K tile (both go into the softmax's
 // scale), and a running one for V (a change rescales O; it leaves room for 2^6 of growth, so that it hardly happens).
 // A value that is NaN (a group that held one) must not reach rows that do not see its key, and 0 x NaN is NaN in a
 // product: such a group enters as zeros, and the rows that see its key are marked and written as NaN. Likewise keys and
@@ -31,7 +31,7 @@
 //
 // Keys or values too far apart for the tile's power of two (KV_SPREAD) make the CTA's rows go through kv_exact as well, in fp32:
 // the large ones may be later tokens', or have no weight, and would round the others away. Finding out costs 1% (4096 tokens 181
-// -> 183 us); with values of ordinary models it does not happen.
+// -> 183 us); with values of ordinary models it does not happen (that prompt with such a token in every page: 41 ms).
 //
 // Every wait is bounded: after its limit the kernel records MOEB_DEVERR_TIMEOUT, its roles stop, TMEM is released.
 #include "kv.cuh"

@@ -377,7 +377,7 @@ class KVCache:
         self._c = ctypes.addressof(self._struct)
 
     def read_error(self):
-        """Sticky device error bits (DEVERR_PAGE, DEVERR_ROWS); synchronises the current stream and clears them."""
+        """Sticky device error bits (DEVERR_PAGE, DEVERR_ROWS, DEVERR_TIMEOUT); synchronises the current stream and clears them."""
         out = ctypes.c_uint(0)
         with torch.cuda.device(self.device):
             _lib.call("moeb_kv_read_error", self._struct, ctypes.byref(out), _stream())
