@@ -258,12 +258,20 @@ def _kv_cache_class():
                 if seen != self.moeb_filled:  # by the first layer of a call that has attention
                     self.moeb_lens.fill_(seen)
                     self.moeb_filled = seen
+                try:
+                    ops.kv_write(self.moeb_layers[layer_idx], _rows(key_states), _rows(value_states), self.moeb_table,
+                                 self.moeb_lens)
+                except Exception:
+                    self.moeb_undo(n)
+                    raise
                 self.moeb_seen[layer_idx] = seen
-                ops.kv_write(self.moeb_layers[layer_idx], _rows(key_states), _rows(value_states), self.moeb_table,
-                             self.moeb_lens)
                 key = key_states.view_as(key_states)  # a tensor of its own to mark
                 key._moeb_kv = (self, layer_idx)
                 return key, value_states
+
+            def moeb_undo(self, n):
+                """A call of n tokens ended early: the layers that had taken them give them up."""
+                self.moeb_seen = [s - n if s == self.moeb_filled else s for s in self.moeb_seen]
 
             def to_stock(self):
                 """A DynamicCache with the stored values in bf16, to continue on the stock attention."""
@@ -328,23 +336,33 @@ _KNOWN = frozenset(("scaling", "sliding_window", "s_aux", "dropout", "is_causal"
                     "num_items_in_batch"))
 
 
+def _cached_window(module, attention_mask, kw):
+    """The window of a layer's call with a 4-bit cache; refuses what the kernel has no argument for."""
+    if module.training:
+        raise ValueError("the 4-bit KV cache has no backward pass: call model.eval() first")
+    unknown = sorted(k for k, v in kw.items() if k not in _KNOWN and v is not None and v is not False)
+    if unknown or kw.get("dropout") or kw.get("is_causal") is False or getattr(module, "is_causal", True) is False:
+        raise ValueError(f"the 4-bit KV cache attention is causal, without dropout, and does not know {unknown or 'other kinds'}")
+    window = int(kw.get("sliding_window") or 0)
+    if isinstance(attention_mask, _Causal):
+        if window and window != attention_mask.window:
+            raise ValueError(f"a layer with a window of {window} and a mask with one of {attention_mask.window}")
+        return attention_mask.window
+    if attention_mask is not None:
+        raise ValueError("attention masks of the caller's own are not supported by the 4-bit KV cache attention")
+    return window
+
+
 def _attention(module, query, key, value, attention_mask=None, **kw):
     B, H, n, D = query.shape
     tag = getattr(key, "_moeb_kv", None)
     if tag is not None:
-        if module.training:
-            raise ValueError("the 4-bit KV cache has no backward pass: call model.eval() first")
-        window = int(kw.get("sliding_window") or 0)
-        if isinstance(attention_mask, _Causal):
-            if window and window != attention_mask.window:
-                raise ValueError(f"a layer with a window of {window} and a mask with one of {attention_mask.window}")
-            window = attention_mask.window
-        elif attention_mask is not None:
-            raise ValueError("attention masks of the caller's own are not supported by the 4-bit KV cache attention")
-        unknown = sorted(k for k, v in kw.items() if k not in _KNOWN and v is not None and v is not False)
-        if unknown or kw.get("dropout") or kw.get("is_causal") is False or getattr(module, "is_causal", True) is False:
-            raise ValueError(f"the 4-bit KV cache attention is causal, without dropout, and does not know {unknown or 'other kinds'}")
         cache, layer = tag
+        try:
+            window = _cached_window(module, attention_mask, kw)
+        except ValueError:
+            cache.moeb_undo(n)  # a refused call leaves the cache as it was
+            raise
         sinks = kw.get("s_aux")
         y = ops.kv_attention(_rows(query), cache.moeb_layers[layer], cache.moeb_table, cache.moeb_lens, scale=kw.get("scaling"),
                              window=window, sink_logits=None if sinks is None else sinks.detach().float())

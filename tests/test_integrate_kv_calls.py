@@ -7,7 +7,7 @@ from moelab_b200 import integrate
 
 transformers = pytest.importorskip("transformers")
 from test_integrate import _gptoss, _qwen3  # noqa: E402
-from test_integrate_kv import _sinks, stand_in  # noqa: E402, F401
+from test_integrate_kv import _sinks, _write, stand_in  # noqa: E402, F401
 
 
 def _ids(rows, n, seed=1):
@@ -216,3 +216,37 @@ def test_captured_calls_are_refused(stand_in, monkeypatch):
     with torch.no_grad(), pytest.raises(RuntimeError, match="captured"):
         m(_ids(1, 5), past_key_values=cache)
     assert cache.moeb_seen == [0, 0]
+
+
+def test_refused_calls_leave_the_cache_as_it_was(stand_in, monkeypatch):
+    """A call in training mode, one with a mask of its own, one whose write fails: the next call goes on where the last good one
+    ended."""
+    m = _qwen3(dtype=torch.float32).eval()
+    integrate.patch_hf_attention(m)
+    ids = _ids(2, 12)
+    with torch.no_grad():
+        want = m(ids).logits
+        cache = integrate.quantized_kv_cache(m, 2, 32, page_size=16)
+
+        def no_launch():
+            raise RuntimeError("no launch")
+
+        def refused(n, error, **kw):
+            seen = list(cache.moeb_seen)
+            with pytest.raises(error):
+                m(ids[:, :n], past_key_values=cache, **kw)
+            assert cache.moeb_seen == seen
+
+        for a, b in ((0, 5), (5, 11), (11, 12)):
+            m.train()
+            refused(4, ValueError)
+            m.eval()
+            refused(3, ValueError, attention_mask=torch.ones(2, 1, 3, a + 3, dtype=torch.bool))
+            with monkeypatch.context() as patch:
+                patch.setattr(integrate.ops, "kv_write", lambda *_: no_launch())
+                refused(2, RuntimeError)
+                left = [1]
+                patch.setattr(integrate.ops, "kv_write", lambda *a: _write(*a) if left and left.pop() else no_launch())
+                refused(2, RuntimeError)  # in the second layer
+            got = m(ids[:, a:b], past_key_values=cache).logits
+            assert (got - want[:, a:b]).norm() / want[:, a:b].norm() < 1e-4, (a, b)
