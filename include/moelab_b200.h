@@ -296,10 +296,11 @@ int moeb_kv_read(const moeb_kv_cache *cache, int T, const int *cu, const int *fi
  * table entries may be anything. q: bf16, strides as moeb_kv_write's k; y: bf16 [T][H][head_dim]; lse: fp32 [T][H], the
  * natural logarithm of the softmax's sum, or NULL. max_q: the most rows that a sequence has in this call (a larger
  * bound costs time only; a sequence with more rows may be passed over, which sets MOEB_DEVERR_ROWS). Scores,
- * statistics and sums are fp32; the tensor cores take queries, weights and (for many rows) keys and values in fp16 after powers of
- * two (2^-11 of each). Keys and values may be any finite bf16, of any sizes beside one another (groups of a
- * head more than 2^18 apart take a path that is 20 to 200 times slower; groups below 2^-120 may count as zeros). ws: scratch of moeb_kv_attention_workspace_bytes (for the same arguments; with_cu: cu
- * is given; 0 for many calls), with no first contents and none kept, 16-byte aligned: one call at a time. */
+ * statistics and sums are fp32; the tensor cores take queries, weights and (for many rows) keys and values in fp16 after
+ * powers of two (2^-11 of each). Sizes of keys and values in a call may be up to 2^96 apart: groups of a head that are more
+ * than 2^18 apart take a path 20 to 200 times slower, groups below 2^-120 may count as zeros. ws: scratch of
+ * moeb_kv_attention_workspace_bytes (for the same arguments; with_cu: cu is given; 0 for many calls), with no first
+ * contents and none kept, 16-byte aligned: one call at a time. */
 size_t moeb_kv_attention_workspace_bytes(int T, int B, int P, int page_size, int H, int kv_heads, int head_dim, int max_q,
                                          int window, int sinks, int with_cu);
 int moeb_kv_attention(const moeb_kv_cache *cache, const void *q, long q_row, long q_head, int T, int H, const int *cu,

@@ -120,9 +120,9 @@ def test_queries_that_are_not_finite_give_nan_and_touch_no_other_row(fmt, n, L, 
 
 # ------------------------------------------------------------------ keys and values of sizes far apart
 @pytest.mark.parametrize("fmt,D", [("q4", 64), ("q4", 128), ("mxfp4", 64), ("mxfp4", 128)])
-@pytest.mark.parametrize("n,L", [(1, 300), (3, 300), (3, 9000), (150, 300), (150, 9000)])
+@pytest.mark.parametrize("n,L", [(1, 300), (3, 300), (3, 9000), (150, 257), (150, 300), (150, 9000)])
 @pytest.mark.parametrize("what", ("key", "value", "unattended", "first"))
-@pytest.mark.parametrize("power", (13, 17, 19, 30, 60))
+@pytest.mark.parametrize("power", (13, 17, 19, 30, 60, 96))
 def test_sizes_far_apart(fmt, D, n, L, what, power):
     """A key or value 2^power times the others' size that some rows do not see (the last token's) or give no weight (a token with
     a score far below the rest), or others that are that much larger than the first token's, the only one that row 0 sees: the
