@@ -775,7 +775,9 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
         if (poison >> 31 && (qmul >= 0.f || l != 0.f)) l = __uint_as_float(0x7fffffffu);  // a query that sees nothing is not looked at
         // ---- the rows' results (m is off by P_OFF against the weights' sum: undone here)
         const float M = l == 0.f ? -INFINITY : m - P_OFF;
-        const bool far = __any_sync(0xffffffffu, fabsf(m) > KV_FAR && m != LOW);  // the same for both warps of the rows
+        // a tile with groups too far apart for fp16 (the feeders set the mark before their tiles were full), or scores that are too
+        // large, the same for both warps of the rows: these go through kv_exact below
+        const bool again = *reinterpret_cast<volatile int *>(&sh.uneven) || __any_sync(0xffffffffu, fabsf(m) > KV_FAR && m != LOW);
         float mul = nk > 0 ? sh.vun : 0.f, Ls = l, sum_m = M;
         if (!part) {
             if (a.sink_logits && have) {
@@ -823,7 +825,7 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
 #pragma unroll 4
             for (int i = 16 * sub; i < 16 * sub + 16; i += RW) {
                 const int rr = i + lane / LR, x = lane % LR, Rr = R0 + t * 128 + (warp & 3) * 32 + rr;
-                if (Rr < NR) {
+                if (Rr < NR && !again) {  // y may lie where q does, which kv_exact reads
                     const int ri2 = Rr / a.Gq;
                     const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * (D * 2) + ((x ^ (rr & 7)) << 4));
                     *reinterpret_cast<uint4 *>(a.y + ((size_t)(r0 + ri2) * a.H + h * a.Gq + Rr - ri2 * a.Gq) * D + 8 * x) = v;
@@ -835,10 +837,10 @@ __global__ void __launch_bounds__(PT, 1) k_kv_attn_prompt(const KvAttnArgs a, in
             else if (a.lse) a.lse[orow] = Ls == 0.f ? -INFINITY : (sum_m + log2f(Ls)) * 0.6931471805599453f;
         }
         fence_before();
-        // ---- a tile with groups too far apart for fp16, or scores that are too large: the rows that this warp stored once more, in fp32. The feeders set the
-        // mark before their tiles were full. No barrier below: after a timeout the warps may find it set or not
+        // ---- the rows that are this warp's to store once more, in fp32. No barrier below: after a timeout one warp of the rows may
+        // have found the mark and the other not
         asm volatile("bar.sync %0, 64;" ::"r"(meet) : "memory");
-        if (far || *reinterpret_cast<volatile int *>(&sh.uneven)) {
+        if (again) {
             const int Ru = R0 + t * 128 + (warp & 3) * 32 + 16 * sub;
 #pragma unroll 1
             for (int i = 0; i < 16 && Ru + i < NR; ++i) {

@@ -292,3 +292,42 @@ def test_scales_of_any_sign(fmt, D, n, L, scale):
     y, lse = attend(b, c, scale=scale, return_lse=True)
     within(y, ref, bound)
     assert (lse.double().cpu() - lref).abs().max() < 5e-3
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("far", (False, True))
+@pytest.mark.parametrize("n,L", [(1, 300), (3, 300), (3, 9000), (150, 300), (150, 9000)])
+def test_results_over_the_queries(fmt, far, n, L):
+    """out may be q itself."""
+    b = Batch([L, L + 70], [n, n], 4, 1, 128, fmt, page=32, seed=63)
+    if far:
+        b.v[:, 40] = (b.v[:, 40].float() * 2.0 ** 40).to(torch.bfloat16)
+    c = b.cache(ops)
+    want = attend(b, c)
+    q = b.q.clone()
+    y = ops.kv_attention(q, c, b.table, b.lens_t, cu=b.cu, max_q=n, out=q)
+    assert y is q and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n", (1, 150))
+def test_a_captured_call_follows_values_that_come_to_be_far_apart(fmt, n):
+    b = Batch([9000, 300], [n, n], 4, 1, 64, fmt, page=32, seed=64)
+    c = b.cache(ops)
+    attend(b, c)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = attend(b, c)
+    for power in (0, 50, 0):
+        k, v = b.k.clone(), b.v.clone()
+        b.v[:, 290] = (b.v[:, 290].float() * 2.0 ** power).to(torch.bfloat16)
+        fresh = b.cache(ops)
+        for name in ("kq", "ks", "vq", "vs"):
+            getattr(c, name).copy_(getattr(fresh, name))
+        g.replay()
+        torch.cuda.synchronize()
+        ref, bound, _ = reference(b)
+        within(y, ref, bound, power)
+        assert torch.equal(y, attend(b, fresh))
+        b.k, b.v = k, v
