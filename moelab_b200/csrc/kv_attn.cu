@@ -196,8 +196,9 @@ MOEB_DEV long few_start(long W, unsigned c, unsigned n) {
 
 }  // namespace
 
-// CTAs per SM: as many as registers allow without spills in the loop. Heads of 64 with one column tile: four (126 registers) and not three
-// make many short windows faster (512 tokens in windows of 128, 64 heads on 8: 50 -> 42 us, 44 since values are looked over) and cost long caches nothing.
+// CTAs per SM: as many as registers allow without spills in the loop. Heads of 64 with one column tile: four (126 registers) and
+// not three make many short windows faster (512 tokens in windows of 128, 64 heads on 8: 50 -> 42 us, 44 since values' sizes are
+// looked at) and cost long caches nothing.
 // ws: prefix[B + 1] int32 (blocks before each sequence), then 2 partials per CTA: NC rows of D sums, NC (max, sum).
 template <int FMT, int D, int NT>
 __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 : 2) k_kv_attn_few(const KvAttnArgs a, int *pre, float *part) {
@@ -779,7 +780,8 @@ __global__ void __launch_bounds__(FT, NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                far |= (fabsf(m[nt][e]) > KV_FAR && m[nt][e] != -INFINITY) || cs[nt][e] == LEAST || cs[nt][e] > 1e38f;  // or no such power for q
+                // or a query whose power of two and scale pass fp32
+                far |= (fabsf(m[nt][e]) > KV_FAR && m[nt][e] != -INFINITY) || cs[nt][e] == LEAST || cs[nt][e] > 1e38f;
                 m[nt][e] -= vexp;
 #pragma unroll
                 for (int x = 4; x <= 16; x <<= 1) {
